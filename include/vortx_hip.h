@@ -408,6 +408,120 @@ int vx_quantize(vx_ctx ctx, vx_stream stream, const vx_qweight* out,
 int vx_contiguous(vx_ctx ctx, vx_stream stream, const vx_mview* out,
                   const vx_cview* src, const uint32_t* dev_offset);
 
+/* ------------------------------------------------------------------ */
+/* Quantized key/value cache, and attention over it                    */
+/* (no reference counterpart)                                          */
+/* ------------------------------------------------------------------ */
+
+/* Keys and values of a model layer in pages of page_tokens tokens (a power of
+ * two from 16 to 65536), `heads` key/value heads of `dim` values (64, 96, 128
+ * or 256) each, quantized in blocks of 32 along the head: VX_Q8_0 or VX_Q4_0,
+ * K and V each their own. A block x is held as an f16 scale d and whole
+ * numbers q, for the values d q:
+ *   VX_Q8_0  d = f16(max|x| / 127), q = clamp(rint(x r), -127, 127)
+ *   VX_Q4_0  d = f16(m / -8), m the value of the largest magnitude (the
+ *            positive one of two), q = clamp(rint(x r), -8, 7)
+ * with r = 1 / d (0 where d is 0), each operation one f32 rounding. A block
+ * with a NaN or an infinity, or one that d cannot hold, reads as NaN.
+ * Slot page * page_tokens + i is token i of a page. The arrangement inside a
+ * page is the library's own (vx_kv.hpp); pages need no initial contents, and a
+ * slot's contents are undefined until it is written. base: device memory,
+ * 16-byte aligned, of at least vx_kv_cache_size bytes. */
+typedef struct vx_kv_cache {
+    void* base;
+    uint64_t bytes;
+    uint32_t pages, page_tokens;
+    uint32_t heads, dim;
+    uint32_t k_type, v_type;
+} vx_kv_cache;
+
+/* Bytes of a cache (its `base` and `bytes` are not looked at). */
+int vx_kv_cache_size(const vx_kv_cache* cache, uint64_t* bytes);
+
+/* Quantize k and v, [tokens, heads, dim] f32 views of any strides, into the
+ * slots of the device array slots[tokens] (one launch). A slot outside the
+ * cache leaves its token out; the slots of one call differ. */
+int vx_kv_write(vx_ctx ctx, vx_stream stream, const vx_kv_cache* cache, const vx_cview* k, const vx_cview* v,
+                const int32_t* slots);
+
+/* The values that slots[tokens] hold, into k and v ([tokens, heads, dim], any
+ * strides); NULL k or v: not that one. A slot outside the cache gives zeros. */
+int vx_kv_read(vx_ctx ctx, vx_stream stream, const vx_mview* k, const vx_mview* v, const vx_kv_cache* cache,
+               const int32_t* slots);
+
+/* A batch of sequences. Device arrays, read when the kernels run, so they may
+ * change between calls (and between replays of a captured graph):
+ *   table [seqs][table_stride]  page of each page_tokens keys of a sequence
+ *                               (table_cols of them; a page outside the cache
+ *                               is never read, another is in its place)
+ *   lens [seqs]                 keys of a sequence, those of its queries
+ *                               among them
+ *   starts [seqs + 1]           first query token of each sequence, and the
+ *                               end: query j of sequence s is token
+ *                               starts[s] + j of q and out, at position
+ *                               lens[s] - n + j (n its queries)
+ * max_queries and max_len are upper bounds that the launch is laid out by;
+ * keys past max_len are not seen, queries past max_queries not computed. */
+typedef struct vx_attn_batch {
+    const int32_t* table;
+    const int32_t* lens;
+    const int32_t* starts;
+    uint32_t seqs;
+    uint32_t table_cols, table_stride;
+    uint32_t max_queries, max_len;
+    uint32_t reserved; /* must be 0 */
+} vx_attn_batch;
+
+typedef enum vx_attn_flags {
+    VX_ATTN_CAUSAL = 1 /* a query sees keys up to its own position */
+} vx_attn_flags;
+
+/* Options of vx_attention. Zeros: no option; the arrays are device memory. */
+typedef struct vx_attn_opts {
+    float scale;           /* of q k^T; 0: 1 / sqrt(dim) */
+    float softcap;         /* c > 0: c tanh(score / c) */
+    const float* slopes;   /* [query heads]: score -= slope |position - key position| */
+    const int32_t* prefix; /* [seqs]: keys before it are seen by every query of the sequence, causal or not */
+    const int32_t* first;  /* [tokens]: first key that a query sees (where its document begins) */
+    uint32_t flags;        /* bitwise OR of vx_attn_flags */
+    uint32_t window;       /* > 0: keys less than window positions away only (the prefix too) */
+} vx_attn_opts;
+
+/* out = softmax(score) V for each query token and head: q and out are
+ * [tokens, query heads, dim] f32 views of any strides, query heads a multiple
+ * of the cache's heads (query head h reads head h / (query heads / heads)).
+ * q is taken as two f16 terms per value (22 bits, scaled by a power of two per
+ * row), scores, softmax and sums are f32, products of the exactly decoded
+ * cache on the f16 matrix cores. A query that sees no key gives zeros. Keys
+ * that a query does not see never reach its result, whatever they hold; a NaN
+ * that it sees in K makes its whole row NaN, one in V the 32 values of that
+ * block. opts NULL: scale 1 / sqrt(dim) and no mask.
+ * workspace: device memory, 16-byte aligned, at least vx_attention_ws_size
+ * bytes (a smaller one is VX_ERR_INVALID), for calls whose keys are split over
+ * workgroups and joined by a second launch. With NULL they are not split,
+ * which is slower where there are few queries. Its contents need not start at
+ * zero; calls that share one must be ordered. The library never allocates,
+ * frees or retains it. */
+int vx_attention(vx_ctx ctx, vx_stream stream, const vx_mview* out, const vx_cview* q, const vx_kv_cache* cache,
+                 const vx_attn_batch* batch, const vx_attn_opts* opts, void* workspace, uint64_t workspace_bytes);
+
+/* The same for a tree of drafted tokens: the queries of a sequence are its n
+ * drafts, whose keys are its last n. Draft j sees the cached keys before them
+ * (opts' first and window applied; causal and prefix have nothing to do) and
+ * draft i where bit i % 32 of tree[token j][i / 32] is set: its ancestors and
+ * itself. tree: device array [tokens][tree_stride] of 32-bit words, of which
+ * tree_words are read (32 tree_words >= max_queries, else VX_ERR_SHAPE). A
+ * draft that sees c drafts is at position lens[s] - n + c - 1, its depth in
+ * the tree, for slopes and window. */
+int vx_attention_tree(vx_ctx ctx, vx_stream stream, const vx_mview* out, const vx_cview* q, const vx_kv_cache* cache,
+                      const vx_attn_batch* batch, const vx_attn_opts* opts, const uint32_t* tree, uint32_t tree_words,
+                      uint32_t tree_stride, void* workspace, uint64_t workspace_bytes);
+
+/* Bytes of workspace that either of them may use for `tokens` query tokens of
+ * `q_heads` heads (0: none). */
+int vx_attention_ws_size(vx_ctx ctx, const vx_kv_cache* cache, const vx_attn_batch* batch, const vx_attn_opts* opts,
+                         uint32_t tokens, uint32_t q_heads, uint64_t* bytes);
+
 /* Block geometry of a vx_qtype: weights per block and bytes per block. */
 int vx_qtype_info(uint32_t qtype, uint32_t* block_weights,
                   uint32_t* block_bytes);

@@ -10,6 +10,8 @@ Python-side mirror of the reference interface for this path:
   dequantize, which the reference does not have;
 * :class:`Contiguous` — ``Contiguous::launch`` (src/linalg/contiguous.rs:22-119),
   the strided -> contiguous copy of 4-byte elements;
+* :class:`KvCache` / :class:`KvAttention` — a quantized key/value cache and the
+  attention over it (vortx_amd.attention), which the reference does not have;
 * :class:`GGUFFile` — GGUF model files (vortx_amd.gguf), which feed real
   quantized weights to :class:`QuantGemv`.
 
@@ -29,7 +31,7 @@ from . import _ffi
 from ._ffi import (NONE_STRIDE, ROUTE_EMPTY, ROUTE_GEMV, ROUTE_NAIVE, ROUTE_TILED, VX_Q4_0, VX_Q4_K, VX_Q8_0,
                    VortxError, check, lib)
 
-__all__ = ["TensorLayout", "layout_extent", "XQ", "xq_size", "Gemm", "QuantGemv", "QWeight", "Contiguous", "GGUFFile", "VortxError", "VX_Q4_0", "VX_Q8_0", "VX_Q4_K",
+__all__ = ["TensorLayout", "layout_extent", "XQ", "xq_size", "Gemm", "QuantGemv", "QWeight", "Contiguous", "KvCache", "KvAttention", "AttentionPlan", "kv_cache_size", "tree_mask", "GGUFFile", "VortxError", "VX_Q4_0", "VX_Q8_0", "VX_Q4_K",
            "ROUTE_NAIVE", "ROUTE_TILED", "ROUTE_GEMV", "ROUTE_EMPTY", "qtype_info", "lib"]
 
 # Load eagerly: a missing library must fail at import, not at first call.
@@ -474,3 +476,4 @@ class Contiguous(_Context):
 
 
 from .gguf import GGUFFile  # noqa: E402  (needs QWeight and TensorLayout above)
+from .attention import AttentionPlan, KvAttention, KvCache, kv_cache_size, tree_mask  # noqa: E402

@@ -44,6 +44,23 @@ class VxGemmOpts(C.Structure):
     _fields_ = [("alpha", C.c_float), ("beta", C.c_float), ("flags", C.c_uint32), ("reserved", C.c_uint32)]
 
 
+class VxKvCache(C.Structure):
+    _fields_ = [("base", C.c_void_p), ("bytes", C.c_uint64), ("pages", C.c_uint32), ("page_tokens", C.c_uint32),
+                ("heads", C.c_uint32), ("dim", C.c_uint32), ("k_type", C.c_uint32), ("v_type", C.c_uint32)]
+
+
+class VxAttnBatch(C.Structure):
+    _fields_ = [("table", C.c_void_p), ("lens", C.c_void_p), ("starts", C.c_void_p), ("seqs", C.c_uint32),
+                ("table_cols", C.c_uint32), ("table_stride", C.c_uint32), ("max_queries", C.c_uint32),
+                ("max_len", C.c_uint32), ("reserved", C.c_uint32)]
+
+
+class VxAttnOpts(C.Structure):
+    _fields_ = [("scale", C.c_float), ("softcap", C.c_float), ("slopes", C.c_void_p), ("prefix", C.c_void_p),
+                ("first", C.c_void_p), ("flags", C.c_uint32), ("window", C.c_uint32)]
+
+
+VX_ATTN_CAUSAL = 1
 VX_GEMM_BROADCAST, VX_GEMM_TILE_NARROW, VX_GEMM_TILE_WIDE, VX_GEMM_TILE_SMALL = 1, 2, 4, 8
 
 
@@ -89,6 +106,15 @@ SIGNATURES = [
     ("vx_gemv_q_noalloc", C.c_int, [C.c_void_p, C.c_void_p, _P(VxMView), _P(VxQWeight), _P(VxCView), C.c_uint32]),
     ("vx_quantize", C.c_int, [C.c_void_p, C.c_void_p, _P(VxQWeight), _P(VxCView)]),
     ("vx_contiguous", C.c_int, [C.c_void_p, C.c_void_p, _P(VxMView), _P(VxCView), C.c_void_p]),
+    ("vx_kv_cache_size", C.c_int, [_P(VxKvCache), _P(C.c_uint64)]),
+    ("vx_kv_write", C.c_int, [C.c_void_p, C.c_void_p, _P(VxKvCache), _P(VxCView), _P(VxCView), C.c_void_p]),
+    ("vx_kv_read", C.c_int, [C.c_void_p, C.c_void_p, _P(VxMView), _P(VxMView), _P(VxKvCache), C.c_void_p]),
+    ("vx_attention", C.c_int, [C.c_void_p, C.c_void_p, _P(VxMView), _P(VxCView), _P(VxKvCache), _P(VxAttnBatch),
+                               _P(VxAttnOpts), C.c_void_p, C.c_uint64]),
+    ("vx_attention_tree", C.c_int, [C.c_void_p, C.c_void_p, _P(VxMView), _P(VxCView), _P(VxKvCache), _P(VxAttnBatch),
+                                    _P(VxAttnOpts), C.c_void_p, C.c_uint32, C.c_uint32, C.c_void_p, C.c_uint64]),
+    ("vx_attention_ws_size", C.c_int, [C.c_void_p, _P(VxKvCache), _P(VxAttnBatch), _P(VxAttnOpts), C.c_uint32,
+                                       C.c_uint32, _P(C.c_uint64)]),
     ("vx_qtype_info", C.c_int, [C.c_uint32, _P(C.c_uint32), _P(C.c_uint32)]),
     ("vx_layout_contiguous", C.c_int, [_P(C.c_uint32), C.c_uint32, _P(VxLayout)]),
     ("vx_layout_canonicalize", C.c_int, [_P(VxLayout), _P(VxLayout)]),

@@ -1,0 +1,4 @@
+// attn_d128.hip — the quantized cache and the attention over it, heads of 128.
+#define VX_NB 4
+#define VX_NAME(f, types) vx_##f##_d128_##types
+#include "vx_attn_kernels.hpp"

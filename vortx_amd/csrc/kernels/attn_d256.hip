@@ -1,0 +1,4 @@
+// attn_d256.hip — the quantized cache and the attention over it, heads of 256.
+#define VX_NB 8
+#define VX_NAME(f, types) vx_##f##_d256_##types
+#include "vx_attn_kernels.hpp"

@@ -1,0 +1,4 @@
+// attn_d64.hip — the quantized cache and the attention over it, heads of 64.
+#define VX_NB 2
+#define VX_NAME(f, types) vx_##f##_d64_##types
+#include "vx_attn_kernels.hpp"

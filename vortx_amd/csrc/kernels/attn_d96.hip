@@ -1,0 +1,4 @@
+// attn_d96.hip — the quantized cache and the attention over it, heads of 96.
+#define VX_NB 3
+#define VX_NAME(f, types) vx_##f##_d96_##types
+#include "vx_attn_kernels.hpp"

@@ -1,0 +1,107 @@
+// vx_attn.hpp — what the attention kernels share: a query row's bounds and
+// masks, scores and their cap, and the order of the workgroups.
+#pragma once
+#include "vx_dpp.hpp"
+#include "vx_kv.hpp"
+
+constexpr float VX_LOG2E = 1.44269504088896340736f;
+
+// tanh to about two units in the last place: a minimax polynomial below 0.65,
+// 1 - 2 / (1 + e^2|t|) above (which would cancel below).
+__device__ __forceinline__ float vx_tanh(float t) {
+    const float a = fabsf(t), z = t * t;
+    float p = __builtin_fmaf(z, -0.005468255840241909f, 0.020415181294083595f);
+    p = __builtin_fmaf(z, p, -0.05366527661681175f);
+    p = __builtin_fmaf(z, p, 0.1333041489124298f);
+    p = __builtin_fmaf(z, p, -0.3333323001861572f);
+    p = __builtin_fmaf(z * t, p, t);
+    const float e = __builtin_amdgcn_exp2f(a * (2.f * VX_LOG2E));
+    const float q = __builtin_fmaf(-2.f, __builtin_amdgcn_rcpf(1.f + e), 1.f);
+    return a < 0.65f ? p : __builtin_copysignf(q, t);  // (NaN: q, which is NaN)
+}
+
+// Maximum / sum over the four 16-lane rows, in every lane.
+__device__ __forceinline__ float vx_max_rows4(float v) {
+    uint32_t a = __builtin_bit_cast(uint32_t, v), b = a;
+    vx_swap16(a, b);
+    v = fmaxf(__builtin_bit_cast(float, a), __builtin_bit_cast(float, b));
+    a = b = __builtin_bit_cast(uint32_t, v);
+    vx_swap32(a, b);
+    return fmaxf(__builtin_bit_cast(float, a), __builtin_bit_cast(float, b));
+}
+
+// A sequence of the batch: queries, keys and where they lie.
+struct vx_attn_seq {
+    int start, n, len;  // first query token, query tokens, keys
+    uint32_t rows;      // query rows that are computed
+};
+__device__ __forceinline__ vx_attn_seq vx_attn_sequence(const vx_attn_args& a, uint32_t s) {
+    vx_attn_seq q;
+    const int T = (int)a.tokens;
+    q.start = min(max(a.starts[s], 0), T);
+    q.n = min(max(a.starts[s + 1], q.start), T) - q.start;
+    q.len = min(max(a.lens[s], 0), (int)a.max_len);
+    q.rows = min((uint32_t)q.n, a.max_queries) * a.group;
+    return q;
+}
+
+// What a query row sees: the keys of [lo, hi), and for a tree of drafts those
+// of [tail, len) whose bit is set.
+struct vx_attn_row {
+    bool valid;
+    int token, head;  // of q and out
+    int pos, lo, hi;
+    float slope;      // times log2 e
+};
+
+// Number of drafts that a token's row of the tree sees.
+__device__ __forceinline__ int vx_tree_count(const vx_attn_args& a, int token) {
+    const uint32_t* w = a.tree + (uint64_t)token * a.tree_stride;
+    int n = 0;
+    for (uint32_t i = 0; i < a.tree_words; ++i) n += __builtin_popcount(w[i]);
+    return n;
+}
+
+__device__ __forceinline__ vx_attn_row vx_attn_row_of(const vx_attn_args& a, const vx_attn_seq& q, uint32_t s, uint32_t kvh, uint32_t r) {
+    vx_attn_row w;
+    w.valid = r < q.rows;
+    const uint32_t j = w.valid ? r / a.group : 0u;
+    w.token = q.start + (int)j;
+    w.head = (int)(kvh * a.group + (w.valid ? r - j * a.group : 0u));
+    const int tail = q.len - q.n;
+    if (!w.valid) {
+        w.pos = w.lo = w.hi = 0;
+        w.slope = 0.f;
+        return w;
+    }
+    w.lo = 0;
+    if (a.tree) {
+        w.pos = tail + vx_tree_count(a, w.token) - 1;
+        w.hi = max(tail, 0);
+    } else {
+        w.pos = tail + (int)j;
+        w.hi = q.len;
+        if (a.causal) w.hi = min(w.hi, max(w.pos + 1, a.prefix ? a.prefix[s] : 0));
+    }
+    if (a.first) w.lo = max(w.lo, a.first[w.token]);
+    if (a.window) {
+        w.lo = (int)max((int64_t)w.lo, (int64_t)w.pos - a.window + 1);
+        w.hi = (int)min((int64_t)w.hi, (int64_t)w.pos + a.window);
+    }
+    w.hi = max(w.hi, w.lo);
+    w.slope = a.slopes ? a.slopes[w.head] * VX_LOG2E : 0.f;
+    return w;
+}
+
+// Tree: whether the row sees key (a draft, or past the end), and its distance.
+__device__ __forceinline__ bool vx_tree_sees(const vx_attn_args& a, const vx_attn_seq& q, const vx_attn_row& w, int key, float& dist) {
+    const int j = key - (q.len - q.n);
+    if (!w.valid || key >= q.len || j < 0 || (uint32_t)j >= a.tree_words * 32u) return false;
+    if (!(a.tree[(uint64_t)w.token * a.tree_stride + ((uint32_t)j >> 5)] >> (j & 31) & 1u)) return false;
+    if (a.slopes || a.window) {
+        const int d = abs(w.pos - (q.len - q.n + vx_tree_count(a, q.start + j) - 1));
+        dist = (float)d;
+        if (a.window && (uint32_t)d >= a.window) return false;
+    }
+    return true;
+}

@@ -1,0 +1,24 @@
+// vx_attn_kernels.hpp — the kernels of one head size (VX_NB blocks of 32), for
+// each pair of cache types (k8v8: 8 bits for K and V, and so on).
+#include "vx_attn_rows16.hpp"
+#include "vx_kv_rows.hpp"
+
+#define VX_CAT(f, types) VX_NAME(f, types)
+#define VX_KERNELS(types, KB, VB)                                                                              \
+    extern "C" __global__ __launch_bounds__(256) void VX_CAT(kv_write, types)(vx_kv_rows_args a) {             \
+        vx_kv_write_rows<VX_NB, KB, VB>(a);                                                                    \
+    }                                                                                                          \
+    extern "C" __global__ __launch_bounds__(256) void VX_CAT(kv_read, types)(vx_kv_rows_args a) {              \
+        vx_kv_read_rows<VX_NB, KB, VB>(a);                                                                     \
+    }                                                                                                          \
+    extern "C" __global__ __launch_bounds__(256, 2) void VX_CAT(attn_rows16, types)(vx_attn_args a) {          \
+        vx_rows16<VX_NB, KB, VB>::run(a);                                                                      \
+    }
+VX_KERNELS(k8v8, 8, 8)
+VX_KERNELS(k8v4, 8, 4)
+VX_KERNELS(k4v8, 4, 8)
+VX_KERNELS(k4v4, 4, 4)
+
+#if VX_NB == 4
+extern "C" __global__ __launch_bounds__(256) void vx_attn_join(vx_attn_args a) { vx_attn_join_rows(a); }
+#endif

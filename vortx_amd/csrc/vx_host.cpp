@@ -35,6 +35,14 @@ extern const unsigned char vx_co_gemm_q[];
 extern const unsigned char vx_co_gemm_q_end[];
 extern const unsigned char vx_co_gemm_bf[];
 extern const unsigned char vx_co_gemm_bf_end[];
+extern const unsigned char vx_co_attn_d64[];
+extern const unsigned char vx_co_attn_d64_end[];
+extern const unsigned char vx_co_attn_d96[];
+extern const unsigned char vx_co_attn_d96_end[];
+extern const unsigned char vx_co_attn_d128[];
+extern const unsigned char vx_co_attn_d128_end[];
+extern const unsigned char vx_co_attn_d256[];
+extern const unsigned char vx_co_attn_d256_end[];
 }
 
 namespace vx {
@@ -60,21 +68,15 @@ void clear_error() {
 }
 
 // -------------------------------------------------------------- kernels
-// Every kernel the library launches; resolved by name at vx_init.
-enum Kernel : int {
-#define K(name) K_##name,
-#include "vx_kernel_list.inc"
-#undef K
-    K_COUNT
-};
 static const char* const kKernelNames[K_COUNT] = {
 #define K(name) #name,
 #include "vx_kernel_list.inc"
 #undef K
 };
 // The embedded code objects; every kernel name is unique across them.
-static const unsigned char* const kModules[] = {vx_co_gemm, vx_co_gemv_q, vx_co_copy, vx_co_quantize, vx_co_gemm_q, vx_co_gemm_bf};
-constexpr int kNumModules = 6;
+static const unsigned char* const kModules[] = {vx_co_gemm, vx_co_gemv_q, vx_co_copy, vx_co_quantize, vx_co_gemm_q, vx_co_gemm_bf,
+                                               vx_co_attn_d64, vx_co_attn_d96, vx_co_attn_d128, vx_co_attn_d256};
+constexpr int kNumModules = 10;
 constexpr int kModGemv = 1;  // the module holding vx_scratch
 
 }  // namespace vx
@@ -136,6 +138,17 @@ static int launch_b1(vx_ctx ctx, int k, uint32_t grid, size_t lds, vx_stream str
     void* params[] = {&w, &x, &rs, &M, &nu, &G, &xv, &copy};
     const hipError_t e = hipModuleLaunchKernel(ctx->fn[k], grid, 1, 1, 1024, 1, 1, (unsigned)lds, (hipStream_t)stream,
                                                params, nullptr);
+    if (e != hipSuccess) return fail_hip(e, kKernelNames[k]);
+    return VX_OK;
+}
+
+int ctx_cus(vx_ctx ctx) { return ctx->num_cus; }
+
+int launch_struct(vx_ctx ctx, int k, uint32_t grid, uint32_t block, vx_stream stream, const void* args) {
+    if (grid == 0) return VX_OK;
+    DeviceGuard guard(ctx->device);
+    void* params[] = {const_cast<void*>(args)};
+    const hipError_t e = hipModuleLaunchKernel(ctx->fn[k], grid, 1, 1, block, 1, 1, 0, (hipStream_t)stream, params, nullptr);
     if (e != hipSuccess) return fail_hip(e, kKernelNames[k]);
     return VX_OK;
 }
@@ -223,12 +236,7 @@ static int init(int device, vx_ctx* out) {
 }
 
 // ------------------------------------------------------------ view math
-struct Canon {
-    vx_layout l;      // canonical rank-4 layout (offset applied to ptr)
-    uintptr_t ptr;    // base + original offset, in bytes
-};
-
-static int canon_view(const void* base, const vx_layout* in, Canon* c, const char* name) {
+int canon_view(const void* base, const vx_layout* in, Canon* c, const char* name) {
     if (!in) return fail(VX_ERR_INVALID, "null view");
     if (in->rank > 4) return fail(VX_ERR_UNSUPPORTED, "tensors of ranks > 4 not supported");
     int s = layout_canonicalize(in, &c->l);

@@ -9,6 +9,25 @@
 
 namespace vx {
 
+// Every kernel the library launches; resolved by name at vx_init.
+enum Kernel : int {
+#define K(name) K_##name,
+#include "vx_kernel_list.inc"
+#undef K
+    K_COUNT
+};
+
+// A canonicalized view (rank 4; offset applied to ptr).
+struct Canon {
+    vx_layout l;
+    uintptr_t ptr;
+};
+int canon_view(const void* base, const vx_layout* in, Canon* c, const char* name);
+
+int ctx_cus(vx_ctx ctx);
+// Launches kernel k on the context's device; `args` is its one struct argument.
+int launch_struct(vx_ctx ctx, int k, uint32_t grid, uint32_t block, vx_stream stream, const void* args);
+
 // Records `msg` as this thread's last error and returns `status`.
 int fail(int status, const char* msg);
 int fail_hip(int hip_error, const char* what);

@@ -121,6 +121,54 @@ typedef struct vx_gemv_xq_args {
     int64_t xs_b;
 } vx_gemv_xq_args;
 
+/* Paged key/value cache (the layout of vx_attn.hpp). */
+typedef struct vx_kv_geom {
+    uint8_t* base;
+    uint64_t page_bytes;
+    uint32_t pages;
+    uint32_t page_shift;   /* log2 of the tokens of a page, >= 4 */
+    uint32_t heads;        /* key/value heads */
+    uint32_t dim;
+} vx_kv_geom;
+
+/* Rows into the cache, and out of it. k / v of vx_kv_read may be null. */
+typedef struct vx_kv_rows_args {
+    vx_kv_geom c;
+    float* k;              /* element (t, h, d) at k[t*ks[0] + h*ks[1] + d*ks[2]]; read only by vx_kv_write */
+    float* v;
+    int64_t ks[3], vs[3];
+    const int32_t* slots;  /* [tokens]; one outside the cache is left out (write) or gives zeros (read) */
+    uint32_t tokens;
+    uint32_t vec;          /* 1: k and v have stride 1 along the dim and 16-byte aligned rows */
+} vx_kv_rows_args;
+
+/* Attention over the cache. Query row r = j * group + i of a sequence is its
+ * j-th query token, i-th query head of the key/value head. */
+typedef struct vx_attn_args {
+    vx_kv_geom c;
+    const float* q;        /* element (t, head, d) at q[t*qs[0] + head*qs[1] + d*qs[2]] */
+    float* out;
+    int64_t qs[3], os[3];
+    const int32_t* table;  /* [seqs][table_stride]: page of each page_tokens keys */
+    const int32_t* lens;   /* [seqs] */
+    const int32_t* starts; /* [seqs + 1] */
+    const float* slopes;   /* [query heads] or null */
+    const int32_t* prefix; /* [seqs] or null */
+    const int32_t* first;  /* [tokens] or null */
+    const uint32_t* tree;  /* [tokens][tree_stride] or null */
+    float* part_o;         /* partial sums [split][token][head][dim] (splits > 1) */
+    float* part_ml;        /* [split][token][head][2] */
+    uint32_t table_stride, table_cols;
+    uint32_t seqs, tokens, group;
+    uint32_t max_queries, max_len;
+    uint32_t splits, chunk; /* keys of a split, a multiple of 32 */
+    uint32_t row_blocks;
+    uint32_t causal, window;
+    uint32_t tree_stride, tree_words;
+    float scale, cap;      /* cap 0: none */
+    uint32_t vec;          /* 1: q and out have stride 1 along the dim and 16-byte aligned rows */
+} vx_attn_args;
+
 /* Bytes of the device scratch array of vx_gemv_q_noalloc (vx_scratch in
  * the GEMV code object): the largest activation split it can hold. */
 #define VX_SCRATCH_BYTES (4u << 20)
