@@ -290,7 +290,8 @@ def test_long_history_is_split_and_joined(kv):
     assert plan.ws_bytes > 16
     split = b.out.clone()
     plan.ws = None  # without a workspace the keys are not split
-    kv.attend(b.out, _gpu(b.q), plan)
+    q = _gpu(b.q)
+    kv.attend(b.out, (q.flatten(), vx.TensorLayout(tuple(q.shape), tuple(q.stride()), 3)), plan)
     assert (split - b.out).abs().max() < 2e-6
     b.check(kv, window=1000, slopes=rng.uniform(0, 0.01, 4).astype(np.float32))
     b.check(kv, window=3000, causal=False, first=[8100, 0, 5000])

@@ -133,3 +133,33 @@ def test_unusual_operands_take_the_other_path(ops):
     closed.close()
     with pytest.raises(vx.VortxError):
         closed.dispatch(out, a, a)
+
+
+def test_cache_and_attention_same_bits_both_ways():
+    kv = vx.KvAttention(0)
+    i32 = lambda v: torch.tensor(v, dtype=torch.int32, device="cuda")  # noqa: E731
+    k, v, q = torch.randn(20, 2, 64, device="cuda"), torch.randn(20, 2, 64, device="cuda"), torch.randn(20, 4, 64, device="cuda")
+    slots = i32(list(range(5, 25)))
+    caches = [vx.KvCache(2, 16, 2, 64), vx.KvCache(2, 16, 2, 64)]
+    for c in caches:
+        c.data.zero_()
+    kv.write(caches[0], k, v, slots)
+    kv.write(caches[1], _pair(k), _pair(v), slots)
+    assert torch.equal(caches[0].data, caches[1].data)
+    rows = [torch.empty_like(k) for _ in range(4)]
+    kv.read(rows[0], rows[1], caches[0], slots)
+    kv.read(_pair(rows[2]), _pair(rows[3]), caches[0], slots)
+    assert torch.equal(rows[0], rows[2]) and torch.equal(rows[1], rows[3])
+    plan = kv.plan(caches[0], i32([[0, 1]]), i32([25]), i32([0, 20]), q_heads=4, max_queries=20, max_len=25, first=i32([5] * 20))
+    tree = vx.tree_mask([list(range(-1, 19))])
+    out = [torch.empty_like(q) for _ in range(4)]
+    kv.attend(out[0], q, plan)
+    kv.attend(_pair(out[1]), _pair(q), plan)
+    kv.attend_tree(out[2], q, plan, tree)
+    kv.attend_tree(_pair(out[3]), _pair(q), plan, tree)
+    assert torch.equal(out[0], out[1]) and torch.equal(out[2], out[3])
+    assert torch.allclose(out[0], out[2], rtol=0, atol=2e-6)  # (a chain of drafts)
+    other = torch.randn(21, 4, 64, device="cuda")
+    for a, b in [(other, other), (_pair(other), _pair(other))]:
+        with pytest.raises(vx.VortxError, match="first"):
+            kv.attend(a, b, plan)

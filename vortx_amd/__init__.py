@@ -50,10 +50,11 @@ except ImportError:
 
     class _pycall:
         gemm = gemv = quantize = dequantize = contiguous = setup = staticmethod(lambda *args: None)
+        kv_write = kv_read = attend = setup
 
 _ADDR = {name: C.cast(getattr(lib(), name), C.c_void_p).value
          for name in ("vx_gemm_f32", "vx_gemm_f32_ex", "vx_gemv_q_ex", "vx_gemv_q_ws", "vx_dequantize", "vx_quantize",
-                      "vx_contiguous")}
+                      "vx_contiguous", "vx_kv_write", "vx_kv_read", "vx_attention", "vx_attention_tree")}
 _GEMM, _GEMM_EX = _ADDR["vx_gemm_f32"], _ADDR["vx_gemm_f32_ex"]
 _GEMV_EX, _GEMV_WS = _ADDR["vx_gemv_q_ex"], _ADDR["vx_gemv_q_ws"]
 
@@ -302,7 +303,7 @@ class QWeight:
 def _setup_pycall():
     import torch
     _pycall.setup(QWeight, torch.Tensor, torch.float32, getattr(torch._C, "_cuda_getCurrentRawStream", None),
-                  getattr(torch._C, "_cuda_getDevice", None))
+                  getattr(torch._C, "_cuda_getDevice", None), torch.int32)
 
 
 _setup_pycall()

@@ -19,8 +19,12 @@ from __future__ import annotations
 import ctypes as C
 from dataclasses import dataclass
 
-from . import _Context, _ffi, _stream, _view_of
+import vortx_amd as _vx
+
+from . import _ADDR, _Context, _ffi, _stream, _view_of
 from ._ffi import VX_Q8_0, VortxError, check, lib
+
+_WRITE, _READ, _ATTEND, _TREE = (_ADDR[n] for n in ("vx_kv_write", "vx_kv_read", "vx_attention", "vx_attention_tree"))
 
 
 def kv_cache_size(pages: int, page_tokens: int, heads: int, dim: int, k_type: int = VX_Q8_0, v_type: int = VX_Q8_0) -> int:
@@ -51,6 +55,7 @@ class KvCache:
         self.pages, self.page_tokens, self.heads, self.dim = pages, page_tokens, heads, dim
         self.k_type, self.v_type, self.data = k_type, v_type, data
         self._c = _ffi.VxKvCache(data.data_ptr(), have, pages, page_tokens, heads, dim, k_type, v_type)
+        self._addr = C.addressof(self._c)
 
 
 def _array(t, name: str, shape, dtype="int32"):
@@ -90,6 +95,9 @@ class AttentionPlan:
 
     def __post_init__(self):
         self.ws, self.ws_bytes = self.workspace.data_ptr(), self.workspace.numel()
+        # what _pycall.attend takes: the structs' addresses, the workspace, and what q may be
+        self.call = (self.cache._addr, C.addressof(self.batch), C.addressof(self.opts), self.ws, self.ws_bytes, self.q_heads,
+                     2 ** 32 - 1 if self.first_tokens is None else self.first_tokens)
 
 
 def tree_mask(parents, device="cuda:0"):
@@ -117,6 +125,11 @@ class KvAttention(_Context):
         """Quantize ``k`` and ``v`` ([tokens, heads, dim] f32 views) into the
         cache's ``slots`` (int32 [tokens]; one outside the cache leaves its
         token out; no slot twice)."""
+        st = _vx._pycall.kv_write(_WRITE, self._ctx, stream, cache._addr, k, v, slots)
+        if st is not None:
+            if st:
+                check(st)
+            return
         kv, vv = _view_of(k, False), _view_of(v, False)
         check(lib().vx_kv_write(self._h, _stream(stream), C.byref(cache._c), C.byref(kv), C.byref(vv), self._slots(slots, k, v)))
 
@@ -124,6 +137,11 @@ class KvAttention(_Context):
         """The values of the cache's ``slots`` into ``k`` and ``v`` ([tokens,
         heads, dim] f32 views; None: not that one); zeros for a slot outside
         the cache."""
+        st = _vx._pycall.kv_read(_READ, self._ctx, stream, cache._addr, k, v, slots)
+        if st is not None:
+            if st:
+                check(st)
+            return
         kv, vv = (None if t is None else C.byref(_view_of(t, True)) for t in (k, v))
         check(lib().vx_kv_read(self._h, _stream(stream), kv, vv, C.byref(cache._c), self._slots(slots, k, v)))
 
@@ -178,6 +196,11 @@ class KvAttention(_Context):
     def attend(self, out, q, plan: AttentionPlan, stream=None) -> None:
         """out = softmax(q k^T) v over each sequence's cache; ``q`` and ``out``
         are [tokens, q_heads, dim] f32 views. A query that sees no key gives zeros."""
+        st = _vx._pycall.attend(_ATTEND, _TREE, self._ctx, stream, out, q, None, *plan.call)
+        if st is not None:
+            if st:
+                check(st)
+            return
         ov, qv = self._views(out, q, plan)
         check(lib().vx_attention(self._h, _stream(stream), C.byref(ov), C.byref(qv), C.byref(plan.cache._c), C.byref(plan.batch),
                                  C.byref(plan.opts), plan.ws, plan.ws_bytes))
@@ -187,6 +210,12 @@ class KvAttention(_Context):
         sequence: a draft sees the cached keys and the drafts whose bits are
         set in its row of ``tree`` (int32 [tokens, words], :func:`tree_mask`).
         ``causal`` and ``prefix`` of the plan do not apply."""
+        if tree is not None:
+            st = _vx._pycall.attend(_ATTEND, _TREE, self._ctx, stream, out, q, tree, *plan.call)
+            if st is not None:
+                if st:
+                    check(st)
+                return
         ov, qv = self._views(out, q, plan)
         tokens = qv.layout.size[qv.layout.rank - 3] if qv.layout.rank >= 3 else None
         at = _array(tree, "tree", (tokens, None))

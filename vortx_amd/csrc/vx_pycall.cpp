@@ -21,7 +21,7 @@
 
 namespace {
 
-PyObject *g_qweight, *g_tensor, *g_f32, *g_raw_stream, *g_get_device;  // setup()
+PyObject *g_qweight, *g_tensor, *g_f32, *g_i32, *g_raw_stream, *g_get_device;  // setup()
 PyObject *s_dtype, *s_is_cuda, *s_shape, *s_stride, *s_data_ptr, *s_element_size, *s_cuda_stream, *s_data, *s_qtype, *s_rows,
     *s_cols, *s_row_stride, *s_is_contiguous, *s_nbytes;
 
@@ -87,6 +87,31 @@ bool view_of(PyObject* v, bool any4, View* out) {
     return true;
 }
 
+// A [tokens, heads, dim] view of f32.
+template <class View>
+bool rows_of(PyObject* v, View* out) {
+    return view_of(v, false, out) && out->layout.rank == 3;
+}
+
+// An int32 GPU tensor of n x cols elements, rows in order: [n] with cols 0, else [n, cols] of any row stride.
+bool ints_of(PyObject* v, uint32_t n, bool matrix, const int32_t** at, uint32_t* cols, uint32_t* row_stride) {
+    if (!is_gpu_tensor(v)) return false;
+    Ref d(PyObject_GetAttr(v, s_dtype)), shape(PyObject_GetAttr(v, s_shape)), stride(PyObject_CallMethodNoArgs(v, s_stride));
+    const Py_ssize_t rank = matrix ? 2 : 1;
+    if (d.o != g_i32 || !shape.o || !stride.o || !PyTuple_Check(shape.o) || !PyTuple_Check(stride.o) ||
+        PyTuple_GET_SIZE(shape.o) != rank || PyTuple_GET_SIZE(stride.o) != rank)
+        return false;
+    uint64_t sz[2] = {0, 0}, st[2] = {0, 0}, p = 0;
+    for (Py_ssize_t i = 0; i < rank; ++i)
+        if (!as_u64(PyTuple_GET_ITEM(shape.o, i), UINT32_MAX, &sz[i]) || !as_u64(PyTuple_GET_ITEM(stride.o, i), UINT32_MAX, &st[i]))
+            return false;
+    if (sz[0] != n || st[rank - 1] != 1 || (matrix && n > 1 && st[0] < sz[1])) return false;
+    if (!call_u64(v, s_data_ptr, UINT64_MAX, &p) || !p) return false;
+    *at = (const int32_t*)(uintptr_t)p;
+    if (matrix) *cols = (uint32_t)sz[1], *row_stride = n > 1 ? (uint32_t)st[0] : (uint32_t)sz[1];
+    return true;
+}
+
 bool weight_of(PyObject* w, vx_qweight* out) {
     if ((PyObject*)Py_TYPE(w) != g_qweight) return false;
     Ref data(PyObject_GetAttr(w, s_data));
@@ -134,11 +159,11 @@ PyObject* run(F f) {
     return PyLong_FromLong(s);
 }
 
-// setup(QWeight, torch.Tensor, torch.float32, raw stream of a device | None, current device | None)
+// setup(QWeight, torch.Tensor, torch.float32, raw stream of a device | None, current device | None, torch.int32)
 PyObject* py_setup(PyObject*, PyObject* const* a, Py_ssize_t n) {
-    PyObject** g[] = {&g_qweight, &g_tensor, &g_f32, &g_raw_stream, &g_get_device};
-    if (n != 5) return PyErr_Format(PyExc_TypeError, "setup takes 5 arguments");
-    for (int i = 0; i < 5; ++i) {
+    PyObject** g[] = {&g_qweight, &g_tensor, &g_f32, &g_raw_stream, &g_get_device, &g_i32};
+    if (n != 6) return PyErr_Format(PyExc_TypeError, "setup takes 6 arguments");
+    for (int i = 0; i < 6; ++i) {
         Py_INCREF(a[i]);
         Py_XSETREF(*g[i], a[i]);
     }
@@ -229,11 +254,64 @@ PyObject* py_contiguous(PyObject*, PyObject* const* a, Py_ssize_t n) {
     return run([&] { return f(ctx, st, &o, &v, nullptr); });
 }
 
+// kv_write(fn, ctx, stream, cache, k, v, slots), cache the address of a vx_kv_cache; kv_read the same
+template <class View, class F>
+PyObject* kv_rows(PyObject* const* a, Py_ssize_t n, F call) {
+    if (n != 7) return other_path();
+    void* fn = addr(a[0]);
+    vx_ctx ctx = (vx_ctx)addr(a[1]);
+    const vx_kv_cache* cache = (const vx_kv_cache*)addr(a[3]);
+    vx_stream st;
+    View k, v;
+    const int32_t* slots = nullptr;
+    if (!fn || !cache || PyErr_Occurred() || !rows_of(a[4], &k) || !rows_of(a[5], &v) ||
+        !ints_of(a[6], k.layout.size[0], false, &slots, nullptr, nullptr) || !stream_of(a[2], &st))
+        return other_path();
+    return run([&] { return call(fn, ctx, st, cache, &k, &v, slots); });
+}
+PyObject* py_kv_write(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    return kv_rows<vx_cview>(a, n, [](void* fn, vx_ctx ctx, vx_stream st, const vx_kv_cache* c, const vx_cview* k, const vx_cview* v,
+                                      const int32_t* slots) { return ((decltype(&vx_kv_write))fn)(ctx, st, c, k, v, slots); });
+}
+PyObject* py_kv_read(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    return kv_rows<vx_mview>(a, n, [](void* fn, vx_ctx ctx, vx_stream st, const vx_kv_cache* c, const vx_mview* k, const vx_mview* v,
+                                      const int32_t* slots) { return ((decltype(&vx_kv_read))fn)(ctx, st, k, v, c, slots); });
+}
+
+// attend(vx_attention, vx_attention_tree, ctx, stream, out, q, tree | None, cache, batch, opts, workspace, its bytes,
+//        query heads, tokens at most), the plan's structs by their addresses
+PyObject* py_attend(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    if (n != 14) return other_path();
+    void *fn = addr(a[0]), *ft = addr(a[1]);
+    vx_ctx ctx = (vx_ctx)addr(a[2]);
+    const vx_kv_cache* cache = (const vx_kv_cache*)addr(a[7]);
+    const vx_attn_batch* batch = (const vx_attn_batch*)addr(a[8]);
+    const vx_attn_opts* opts = (const vx_attn_opts*)addr(a[9]);
+    vx_stream st;
+    vx_mview o;
+    vx_cview q;
+    uint64_t ws = 0, bytes = 0, heads = 0, most = 0;
+    if (!fn || !ft || !cache || !batch || !opts || PyErr_Occurred() || !rows_of(a[4], &o) || !rows_of(a[5], &q) ||
+        !as_u64(a[10], UINT64_MAX, &ws) || !as_u64(a[11], UINT64_MAX, &bytes) || !as_u64(a[12], UINT32_MAX, &heads) ||
+        !as_u64(a[13], UINT32_MAX, &most) || q.layout.size[1] != heads || q.layout.size[0] > most || !stream_of(a[3], &st))
+        return other_path();
+    if (a[6] == Py_None)
+        return run([&] { return ((decltype(&vx_attention))fn)(ctx, st, &o, &q, cache, batch, opts, (void*)(uintptr_t)ws, bytes); });
+    const int32_t* tree = nullptr;
+    uint32_t words = 0, stride = 0;
+    if (!ints_of(a[6], q.layout.size[0], true, &tree, &words, &stride)) return other_path();
+    return run([&] {
+        return ((decltype(&vx_attention_tree))ft)(ctx, st, &o, &q, cache, batch, opts, (const uint32_t*)tree, words, stride,
+                                                  (void*)(uintptr_t)ws, bytes);
+    });
+}
+
 #define FAST(f) (PyCFunction)(void (*)(void))f, METH_FASTCALL, nullptr
 PyMethodDef methods[] = {{"setup", FAST(py_setup)},           {"gemm", FAST(py_gemm)},
                          {"gemv", FAST(py_gemv)},             {"dequantize", FAST(py_dequantize)},
                          {"quantize", FAST(py_quantize)},     {"contiguous", FAST(py_contiguous)},
-                         {nullptr, nullptr, 0, nullptr}};
+                         {"kv_write", FAST(py_kv_write)},     {"kv_read", FAST(py_kv_read)},
+                         {"attend", FAST(py_attend)},         {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_pycall", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace
@@ -249,7 +327,7 @@ PyMODINIT_FUNC PyInit__pycall(void) {
                  {&s_is_contiguous, "is_contiguous"}, {&s_nbytes, "nbytes"}};
     for (auto& e : names)
         if (!(*e.s = PyUnicode_InternFromString(e.n))) return nullptr;
-    for (PyObject** g : {&g_qweight, &g_tensor, &g_f32, &g_raw_stream, &g_get_device}) {  // nothing matches before setup()
+    for (PyObject** g : {&g_qweight, &g_tensor, &g_f32, &g_i32, &g_raw_stream, &g_get_device}) {  // nothing matches before setup()
         Py_INCREF(Py_None);
         *g = Py_None;
     }
