@@ -42,6 +42,19 @@ struct vx_rows16 {
         for (int b = 0; b < NB; ++b) s[b] = ((const h4*)p)[g * NB + b];
     }
 
+    static __device__ __forceinline__ void load(const uint8_t* const (&at)[2], uint32_t lane, uint32_t g, raw_k& k, raw_v& v) {
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+            vx_kv_load<NB, KB>(at[t], lane, k.w[t]);
+            load_scales(at[t] + PK::VALS, g, k.s[t]);
+        }
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+            vx_kv_load<NB, VB>(at[t] + PK::BYTES, lane, v.w[t]);
+            load_scales(at[t] + PK::BYTES + PV::VALS, g, v.s[t]);
+        }
+    }
+
     static __device__ void run(const vx_attn_args& a) {
         __shared__ float sh_o[4][16][NB * 32 + 4];
         __shared__ float sh_ml[4][16][2];
@@ -129,17 +142,29 @@ struct vx_rows16 {
         const int last = min(q.len, (int)(a.table_cols << a.c.page_shift)) - 1;
         const float capl = a.cap * VX_LOG2E;
 
-        for (int k0 = kbeg + 32 * (int)wave; k0 < kend; k0 += 128) {
-            raw_k rk;
-            raw_v rv;
+        // records of the next keys are requested while these are computed, and
+        // the page of the ones after those
+        constexpr bool AHEAD = NB <= 4;  // (registers: larger heads fill them)
+        raw_k rk;
+        raw_v rv;
+        const uint8_t* at[2];
+        const int kfirst = kbeg + 32 * (int)wave;
+        if (kfirst < kend) {
 #pragma unroll
-            for (int t = 0; t < 2; ++t) {
-                const uint8_t* rec = record(a, table, base, k0 + 16 * t, last);
-                vx_kv_load<NB, KB>(rec, lane, rk.w[t]);
-                load_scales(rec + PK::VALS, g, rk.s[t]);
-                vx_kv_load<NB, VB>(rec + PK::BYTES, lane, rv.w[t]);
-                load_scales(rec + PK::BYTES + PV::VALS, g, rv.s[t]);
+            for (int t = 0; t < 2; ++t) at[t] = record(a, table, base, kfirst + 16 * t, last);
+            if (AHEAD) {
+                load(at, lane, g, rk, rv);
+#pragma unroll
+                for (int t = 0; t < 2; ++t) at[t] = record(a, table, base, kfirst + 128 + 16 * t, last);
             }
+        }
+        for (int k0 = kfirst; k0 < kend; k0 += 128) {
+            raw_k nk;
+            raw_v nv;
+            if (AHEAD) load(at, lane, g, nk, nv);
+            else load(at, lane, g, rk, rv);
+#pragma unroll
+            for (int t = 0; t < 2; ++t) at[t] = record(a, table, base, k0 + (AHEAD ? 256 : 128) + 16 * t, last);
             float x[2][4];
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
@@ -242,6 +267,10 @@ struct vx_rows16 {
                     o[b][v] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, pl, o[b][v], 0, 0, 0);
                 }
             }
+            if (AHEAD) {
+                rk = nk;
+                rv = nv;
+            }
         }
 
         // the four waves' sums: lane (m, g) holds dims 32 b + 2 (4 g + i) + v of query m
@@ -292,40 +321,62 @@ struct vx_rows16 {
     }
 };
 
-// Joins the splits of 16 rows: the same row blocks as above, a row's dims over
-// a quarter of the threads to an eighth of a wave.
+// Joins the splits of a query row: 16 to 64 lanes take its dims, four at a
+// time, and the splits go over the groups of lanes, of a wave where there are
+// up to 8 splits (four rows a workgroup) and of the workgroup above (one row).
+// One group a row took 90 us for 64 rows of 128 splits, this 4.
 __device__ __forceinline__ void vx_attn_join_rows(const vx_attn_args& a) {
-    uint32_t id = blockIdx.x;
+    __shared__ f4 sh_t[256];
+    __shared__ f2 sh_ml[64];
+    const uint32_t D = a.c.dim, lanes = D <= 64 ? 16 : D <= 128 ? 32 : 64;  // of a group
+    const uint32_t span = a.splits > 8 ? 256 : 64;                         // threads of a row
+    const uint32_t in = threadIdx.x % span, group = in / lanes, groups = span / lanes, d = 4 * (in % lanes);
+    uint32_t id = blockIdx.x * (256 / span) + threadIdx.x / span;
     const uint32_t kvh = id % a.c.heads;
     id /= a.c.heads;
-    const uint32_t s = id % a.seqs, r0 = id / a.seqs * 16;
+    const uint32_t s = id % a.seqs, r = id / a.seqs;
     const vx_attn_seq q = vx_attn_sequence(a, s);
-    const uint32_t rows = q.rows, D = a.c.dim, heads = a.c.heads * a.group;
-    const uint64_t stride = (uint64_t)a.tokens * heads;
-    for (uint32_t at = threadIdx.x; at < 16 * (D / 4); at += 256) {
-        const uint32_t r = r0 + at / (D / 4), d = 4 * (at % (D / 4));
-        if (r >= rows) break;
-        const uint32_t j = r / a.group, token = (uint32_t)q.start + j, head = kvh * a.group + (r - j * a.group);
-        const uint64_t row = (uint64_t)token * heads + head;
-        float M = -__builtin_inff();
-        for (uint32_t i = 0; i < a.splits; ++i) M = fmaxf(M, a.part_ml[(i * stride + row) * 2]);
-        const float Mr = M == -__builtin_inff() ? 0.f : M;
-        f4 t = {};
-        float l = 0.f;
-        for (uint32_t i = 0; i < a.splits; ++i) {
+    const bool valid = r < q.rows && d < D;
+    const uint32_t heads = a.c.heads * a.group, j = r / a.group, head = kvh * a.group + (r - j * a.group);
+    const uint64_t stride = (uint64_t)a.tokens * heads, row = ((uint64_t)q.start + j) * heads + head;
+    float M = -__builtin_inff(), l = 0.f;
+    f4 t = {};
+    if (valid) {
+#pragma unroll 4
+        for (uint32_t i = group; i < a.splits; i += groups) {
             const f2 ml = *(const f2*)(a.part_ml + (i * stride + row) * 2);
             if (ml.y == 0.f) continue;  // nothing seen there, and nothing written (not so for a NaN)
-            const float c = __builtin_amdgcn_exp2f(ml.x - Mr);
-            l = __builtin_fmaf(c, ml.y, l);
-            t += c * *(const f4*)(a.part_o + (i * stride + row) * D + d);
+            const f4 o = *(const f4*)(a.part_o + (i * stride + row) * D + d);
+            const float Mn = fmaxf(M, ml.x), c = __builtin_amdgcn_exp2f(M - Mn), k = __builtin_amdgcn_exp2f(ml.x - Mn);
+            // (M is -inf before the first; a NaN in y may have -inf beside it, and stays)
+            l = __builtin_fmaf(k, ml.y, c * l);
+            t = c * t + k * o;
+            M = Mn;
         }
-        const float k = l == 0.f ? 0.f : 1.f / l;
-        float* op = a.out + (int64_t)token * a.os[0] + (int64_t)head * a.os[1];
-        if (a.vec) {
-            *(f4*)(op + d) = t * k;
-        } else {
+    }
+    sh_t[threadIdx.x] = t;
+    if (in % lanes == 0) sh_ml[threadIdx.x / 16] = f2{M, l};
+    __syncthreads();
+    if (!valid || group) return;
+    const uint32_t first = threadIdx.x;  // this row's first group is this thread's
+    float Mt = M;
+    for (uint32_t i = 1; i < groups; ++i) Mt = fmaxf(Mt, sh_ml[(first - in % lanes + i * lanes) / 16].x);
+    const float Mr = Mt == -__builtin_inff() ? 0.f : Mt;
+    const float c0 = __builtin_amdgcn_exp2f(M - Mr);
+    t *= c0;
+    l *= c0;
+    for (uint32_t i = 1; i < groups; ++i) {
+        const f2 ml = sh_ml[(first - in % lanes + i * lanes) / 16];
+        const float c = __builtin_amdgcn_exp2f(ml.x - Mr);
+        t += c * sh_t[first + i * lanes];
+        l = __builtin_fmaf(c, ml.y, l);
+    }
+    const float k = l == 0.f ? 0.f : 1.f / l;
+    float* op = a.out + (int64_t)(q.start + j) * a.os[0] + (int64_t)head * a.os[1];
+    if (a.vec) {
+        *(f4*)(op + d) = t * k;
+    } else {
 #pragma unroll
-            for (uint32_t i = 0; i < 4; ++i) op[(int64_t)(d + i) * a.os[2]] = t[i] * k;
-        }
+        for (uint32_t i = 0; i < 4; ++i) op[(int64_t)(d + i) * a.os[2]] = t[i] * k;
     }
 }

@@ -216,7 +216,10 @@ static int run_attention(vx_ctx ctx, vx_stream stream, const vx_mview* out, cons
     a.part_ml = (float*)ws + p.splits * rows * cache->dim;
     const uint32_t grid = p.row_blocks * p.splits * batch->seqs * cache->heads;
     if ((s = launch_struct(ctx, kernel_of(cache, kRows16), grid, 256, stream, &a))) return s;
-    if (p.splits > 1) return launch_struct(ctx, K_vx_attn_join, grid / p.splits, 256, stream, &a);
+    if (p.splits > 1) {
+        const uint64_t jobs = (uint64_t)batch->max_queries * a.group * batch->seqs * cache->heads;
+        return launch_struct(ctx, K_vx_attn_join, (uint32_t)(p.splits > 8 ? jobs : (jobs + 3) / 4), 256, stream, &a);
+    }
     return VX_OK;
 }
 
