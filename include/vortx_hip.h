@@ -498,10 +498,9 @@ typedef struct vx_attn_opts {
  * block. opts NULL: scale 1 / sqrt(dim) and no mask.
  * workspace: device memory, 16-byte aligned, at least vx_attention_ws_size
  * bytes (a smaller one is VX_ERR_INVALID), for calls whose keys are split over
- * workgroups and joined by a second launch. With NULL they are not split,
- * which is slower where there are few queries. Its contents need not start at
- * zero; calls that share one must be ordered. The library never allocates,
- * frees or retains it. */
+ * workgroups. With NULL they are not, which is slower where there are few
+ * queries. Its contents need not start at zero; calls that share one must be
+ * ordered. The library never allocates, frees or retains it. */
 int vx_attention(vx_ctx ctx, vx_stream stream, const vx_mview* out, const vx_cview* q, const vx_kv_cache* cache,
                  const vx_attn_batch* batch, const vx_attn_opts* opts, void* workspace, uint64_t workspace_bytes);
 

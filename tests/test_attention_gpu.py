@@ -540,10 +540,12 @@ def test_refusals(kv):
         kv.attend_tree(f(3, 4, 64), q, plan, _i32(np.zeros((2, 1))))
     with pytest.raises(vx.VortxError, match="first"):
         kv.attend(f(3, 4, 64), q, kv.plan(*args, **fine, first=_i32([0, 0])))
-    long = kv.plan(cache, _i32([[0, 1]]), _i32([20]), _i32([0, 3]), q_heads=4, max_queries=1, max_len=4096, tokens=1)
-    long.batch.table_cols = 2  # (as it is)
-    with pytest.raises(vx.VortxError) as e:
-        small = kv.plan(vx.KvCache(64, 64, 2, 64), _i32([list(range(64))]), _i32([20]), _i32([0, 3]), q_heads=4, max_queries=1,
-                        max_len=4096, tokens=1)
-        kv.attend(f(3, 4, 64), q, small)  # a workspace for one token
-    assert status(e) == _ffi.VX_ERR_INVALID
+    for queries, tokens in [(1, 1), (40, 40)]:  # a workspace that is a byte short
+        many = kv.plan(vx.KvCache(64, 64, 2, 64), _i32([list(range(64))]), _i32([20]), _i32([0, tokens]), q_heads=4,
+                       max_queries=queries, max_len=4096)
+        assert many.ws_bytes > 16
+        many.ws_bytes -= 1
+        q = f(tokens, 4, 64)
+        with pytest.raises(vx.VortxError, match="workspace") as e:
+            kv.attend((q.flatten(), vx.TensorLayout(tuple(q.shape), tuple(q.stride()), 3)), q, many)
+        assert status(e) == _ffi.VX_ERR_INVALID

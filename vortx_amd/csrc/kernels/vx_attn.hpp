@@ -4,6 +4,9 @@
 #include "vx_dpp.hpp"
 #include "vx_kv.hpp"
 
+// What is the same for a whole wave and no kernel writes comes by scalar loads.
+typedef const __attribute__((address_space(4))) int32_t* vx_scalar_i32;
+
 constexpr float VX_LOG2E = 1.44269504088896340736f;
 
 // tanh to about two units in the last place: a minimax polynomial below 0.65,
@@ -104,4 +107,16 @@ __device__ __forceinline__ bool vx_tree_sees(const vx_attn_args& a, const vx_att
         if (a.window && (uint32_t)d >= a.window) return false;
     }
     return true;
+}
+
+// Four dims of a row's result: its sums over its weights' sum. Nothing seen: zeros.
+__device__ __forceinline__ void vx_attn_put(const vx_attn_args& a, uint32_t token, uint32_t head, uint32_t d, f4 t, float l) {
+    const float k = l == 0.f ? 0.f : 1.f / l;
+    float* op = a.out + (int64_t)token * a.os[0] + (int64_t)head * a.os[1];
+    if (a.vec) {
+        *(f4*)(op + d) = t * k;
+    } else {
+#pragma unroll
+        for (uint32_t i = 0; i < 4; ++i) op[(int64_t)(d + i) * a.os[2]] = t[i] * k;
+    }
 }

@@ -11,8 +11,11 @@
     extern "C" __global__ __launch_bounds__(256) void VX_CAT(kv_read, types)(vx_kv_rows_args a) {              \
         vx_kv_read_rows<VX_NB, KB, VB>(a);                                                                     \
     }                                                                                                          \
-    extern "C" __global__ __launch_bounds__(256, 2) void VX_CAT(attn_rows16, types)(vx_attn_args a) {          \
-        vx_rows16<VX_NB, KB, VB>::run(a);                                                                      \
+    extern "C" __global__ __launch_bounds__(256, VX_NB <= 4 ? 2 : 1) void VX_CAT(attn_rows16, types)(vx_attn_args a) {          \
+        vx_rows16<VX_NB, KB, VB>::grid(a);                                                                     \
+    }                                                                                                          \
+    extern "C" __global__ __launch_bounds__(256, VX_NB <= 4 ? 2 : 1) void VX_CAT(attn_even16, types)(vx_attn_args a) {          \
+        vx_rows16<VX_NB, KB, VB>::even(a);                                                                     \
     }
 VX_KERNELS(k8v8, 8, 8)
 VX_KERNELS(k8v4, 8, 4)

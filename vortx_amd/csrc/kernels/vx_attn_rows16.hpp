@@ -23,31 +23,41 @@ struct vx_rows16 {
 
     struct raw_k {
         uint32_t w[2][KW];
-        h4 s[2][NB];
+        uint32_t s[2][NB][2];  // f16 pairs: keys 4 g, + 1; + 2, + 3
     };
     struct raw_v {
         uint32_t w[2][VW];
-        h4 s[2][NB];
+        uint32_t s[2][NB][2];
     };
 
     // the record of the 16 keys from key on; past the end the last one
-    static __device__ __forceinline__ const uint8_t* record(const vx_attn_args& a, const int32_t* table, const uint8_t* base, int key, int last) {
+    static __device__ __forceinline__ const uint8_t* record(const vx_attn_args& a, vx_scalar_i32 table, const uint8_t* base, int key, int last) {
         key = min(key, last);
         const uint32_t page = min((uint32_t)table[(uint32_t)key >> a.c.page_shift], a.c.pages - 1u);
         return base + page * a.c.page_bytes + (((uint32_t)key & ((1u << a.c.page_shift) - 1u)) >> 4) * REC;
     }
 
-    static __device__ __forceinline__ void load_scales(const uint8_t* p, uint32_t g, h4 (&s)[NB]) {
+    static __device__ __forceinline__ void load_scales(const uint8_t* p, uint32_t g, uint32_t (&s)[NB][2]) {
+        p += g * (8 * NB);
 #pragma unroll
-        for (int b = 0; b < NB; ++b) s[b] = ((const h4*)p)[g * NB + b];
+        for (int b = 0; b + 1 < NB; b += 2) {
+            const u4 v = *(const u4*)(p + 8 * b);
+            s[b][0] = v.x, s[b][1] = v.y, s[b + 1][0] = v.z, s[b + 1][1] = v.w;
+        }
+        if constexpr (NB % 2 != 0) {
+            const u2 v = *(const u2*)(p + 8 * (NB - 1));
+            s[NB - 1][0] = v.x, s[NB - 1][1] = v.y;
+        }
     }
 
-    static __device__ __forceinline__ void load(const uint8_t* const (&at)[2], uint32_t lane, uint32_t g, raw_k& k, raw_v& v) {
+    static __device__ __forceinline__ void load(const uint8_t* const (&at)[2], uint32_t lane, uint32_t g, raw_k& k) {
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
             vx_kv_load<NB, KB>(at[t], lane, k.w[t]);
             load_scales(at[t] + PK::VALS, g, k.s[t]);
         }
+    }
+    static __device__ __forceinline__ void load(const uint8_t* const (&at)[2], uint32_t lane, uint32_t g, raw_v& v) {
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
             vx_kv_load<NB, VB>(at[t] + PK::BYTES, lane, v.w[t]);
@@ -55,21 +65,18 @@ struct vx_rows16 {
         }
     }
 
-    static __device__ void run(const vx_attn_args& a) {
-        __shared__ float sh_o[4][16][NB * 32 + 4];
-        __shared__ float sh_ml[4][16][2];
+    struct shared {
+        float o[4][16][NB * 32 + 4];
+        float ml[4][16][2];
+    };
+
+    // Rows r0.. of sequence s and key/value head kvh over the keys that
+    // range(lo, hi) gives for those that its rows see; the four waves' sums go to sh.
+    template <class Range>
+    static __device__ __forceinline__ bool unit(const vx_attn_args& a, shared& sh, const vx_attn_seq& q, uint32_t s, uint32_t kvh,
+                                                uint32_t r0, Range range) {
         const uint32_t lane = threadIdx.x & 63, m = lane & 15, g = lane >> 4;
         const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-        // workgroup -> (row block, split, sequence, key/value head), heads fastest
-        uint32_t id = blockIdx.x;
-        const uint32_t kvh = id % a.c.heads;
-        id /= a.c.heads;
-        const uint32_t s = id % a.seqs;
-        id /= a.seqs;
-        const uint32_t split = id % a.splits, rb = id / a.splits;
-        const vx_attn_seq q = vx_attn_sequence(a, s);
-        const uint32_t rows = q.rows, r0 = rb * 16;
-        if (r0 >= rows) return;
         const vx_attn_row w = vx_attn_row_of(a, q, s, kvh, r0 + m);
         const int tail = a.tree ? max(q.len - q.n, 0) : q.len;  // keys from here on: by the tree's bits
         int lo = w.valid && w.hi > w.lo ? w.lo : 0x7FFFFFFF, hi = w.valid && w.hi > w.lo ? w.hi : 0;
@@ -89,10 +96,10 @@ struct vx_rows16 {
         hi = min(__builtin_amdgcn_readfirstlane(hi), min(q.len, (int)(a.table_cols << a.c.page_shift)));
         lo_all = __builtin_amdgcn_readfirstlane(lo_all);
         hi_all = __builtin_amdgcn_readfirstlane(hi_all);
-        // this split's keys; the last one takes what is left
-        const int64_t c0 = (int64_t)(lo & ~31) + (int64_t)split * a.chunk;
-        const int kbeg = (int)min(c0, (int64_t)hi);
-        const int kend = split + 1 == a.splits ? hi : (int)min((int64_t)hi, c0 + a.chunk);
+        if (lo >= hi) lo = hi = 0;  // (lo of rows that see nothing is the largest int: 32 more would be negative)
+        int kbeg = lo, kend = hi;
+        range(kbeg, kend);
+        if (kbeg >= kend) kbeg = kend = 0;
 
         // q: 8 dims of each block, two f16 terms
         h8 qh[NB], ql[NB];
@@ -100,6 +107,8 @@ struct vx_rows16 {
         {
             float x[NB][8];
             const float* qp = a.q + (int64_t)w.token * a.qs[0] + (int64_t)w.head * a.qs[1];
+            int64_t sd = a.qs[2];
+            asm volatile("" : "+s"(sd));  // (else every address of the strided case is kept over all units)
             float top = 0.f;
             bool fine = true;
 #pragma unroll
@@ -110,8 +119,9 @@ struct vx_rows16 {
 #pragma unroll
                     for (int i = 0; i < 4; ++i) x[b][i] = u[i], x[b][4 + i] = v[i];
                 } else {
+                    const float* p = qp + (int64_t)d * sd;
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) x[b][i] = qp[(int64_t)(d + i) * a.qs[2]];
+                    for (int i = 0; i < 8; ++i, p += sd) x[b][i] = *p;
                 }
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
@@ -128,7 +138,7 @@ struct vx_rows16 {
 #pragma unroll
                 for (int i = 0; i < 8; i += 2) {
                     h2 hi, lo;  // (below 2^15)
-                    vx_two_terms(__builtin_ldexpf(x[b][i], 15 - e) + bad, 1.f, __builtin_ldexpf(x[b][i + 1], 15 - e) + bad, 1.f, hi, lo);
+                    vx_two_terms(__builtin_ldexpf(x[b][i], 15 - e) + bad, __builtin_ldexpf(x[b][i + 1], 15 - e) + bad, hi, lo);
                     qh[b][i] = hi.x, qh[b][i + 1] = hi.y, ql[b][i] = lo.x, ql[b][i + 1] = lo.y;
                 }
             // score = product * fq in units of log2 (capped: as the argument of tanh)
@@ -137,34 +147,34 @@ struct vx_rows16 {
 
         f4 o[NB][2] = {};
         float M = -__builtin_inff(), l = 0.f;
-        const int32_t* table = a.table + (uint64_t)s * a.table_stride;
+        const vx_scalar_i32 table = (vx_scalar_i32)(a.table + (uint64_t)s * a.table_stride);
         const uint8_t* base = a.c.base + (uint64_t)(kvh << (a.c.page_shift - 4)) * REC;
         const int last = min(q.len, (int)(a.table_cols << a.c.page_shift)) - 1;
         const float capl = a.cap * VX_LOG2E;
 
-        // records of the next keys are requested while these are computed, and
-        // the page of the ones after those
-        constexpr bool AHEAD = NB <= 4;  // (registers: larger heads fill them)
+        // K of the next keys is requested when these keys' registers are free,
+        // V while the scores are computed
         raw_k rk;
         raw_v rv;
-        const uint8_t* at[2];
+        const uint8_t *at[2], *next[2];
         const int kfirst = kbeg + 32 * (int)wave;
         if (kfirst < kend) {
 #pragma unroll
-            for (int t = 0; t < 2; ++t) at[t] = record(a, table, base, kfirst + 16 * t, last);
-            if (AHEAD) {
-                load(at, lane, g, rk, rv);
-#pragma unroll
-                for (int t = 0; t < 2; ++t) at[t] = record(a, table, base, kfirst + 128 + 16 * t, last);
+            for (int t = 0; t < 2; ++t) {
+                at[t] = record(a, table, base, kfirst + 16 * t, last);
+                next[t] = record(a, table, base, kfirst + 128 + 16 * t, last);
             }
+            load(at, lane, g, rk);
         }
+        float zero = -0.f;
+        asm("" : "+s"(zero));
         for (int k0 = kfirst; k0 < kend; k0 += 128) {
-            raw_k nk;
-            raw_v nv;
-            if (AHEAD) load(at, lane, g, nk, nv);
-            else load(at, lane, g, rk, rv);
+            load(at, lane, g, rv);
 #pragma unroll
-            for (int t = 0; t < 2; ++t) at[t] = record(a, table, base, k0 + (AHEAD ? 256 : 128) + 16 * t, last);
+            for (int t = 0; t < 2; ++t) {
+                at[t] = next[t];
+                next[t] = record(a, table, base, k0 + 256 + 16 * t, last);
+            }
             float x[2][4];
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
@@ -175,11 +185,15 @@ struct vx_rows16 {
                     f4 acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qh[b], f4{}, 0, 0, 0);
                     acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, ql[b], acc, 0, 0, 0);
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) sum[i] = __builtin_fmaf(acc[i], (float)rk.s[t][b][i], sum[i]);
+                    for (int i = 0; i < 4; ++i) {
+                        const h2 d = __builtin_bit_cast(h2, rk.s[t][b][i >> 1]);
+                        sum[i] = __builtin_fmaf(acc[i], (float)(i & 1 ? d.y : d.x), sum[i]);
+                    }
                 }
 #pragma unroll
                 for (int i = 0; i < 4; ++i) x[t][i] = sum[i] * fq;
             }
+            load(at, lane, g, rk);
             if (a.cap > 0.f) {
 #pragma unroll
                 for (int t = 0; t < 2; ++t)
@@ -209,7 +223,7 @@ struct vx_rows16 {
                         // a lane's scales are of its own row: what the row does not see, which
                         // may be anything, counts nowhere
 #pragma unroll
-                        for (int b = 0; b < NB; ++b) rv.s[t][b][i] = v ? rv.s[t][b][i] : (_Float16)0.f;
+                        for (int b = 0; b < NB; ++b) rv.s[t][b][i >> 1] &= v ? 0xFFFFFFFFu : i & 1 ? 0x0000FFFFu : 0xFFFF0000u;
                     }
             }
             // running maximum of score + exponent of V's scales
@@ -220,11 +234,13 @@ struct vx_rows16 {
 #pragma unroll
                 for (int t = 0; t < 2; ++t)
 #pragma unroll
-                    for (int b = 0; b < NB; ++b) {
-                        typedef uint16_t us4 __attribute__((ext_vector_type(4)));
-                        const us4 d = __builtin_bit_cast(us4, rv.s[t][b]) & (uint16_t)0x7FFF;
-                        big = __builtin_elementwise_max(__builtin_elementwise_max(big, d.xy), d.zw);
-                    }
+                    for (int b = 0; b < NB; ++b)
+#pragma unroll
+                        for (int i = 0; i < 2; ++i) {
+                            uint32_t d = rv.s[t][b][i];
+                            if (VB == 4) d &= 0x7FFF7FFFu;  // (8 bits: never negative)
+                            big = __builtin_elementwise_max(big, __builtin_bit_cast(us2, d));
+                        }
                 const int e = (int)(max(big.x, big.y) >> 10) - 15;
                 top = vx_max_rows4(top + (float)(e - 13));  // P times scale below 2^14
             }
@@ -253,7 +269,7 @@ struct vx_rows16 {
 #pragma unroll
                     for (int i = 0; i < 4; i += 2) {
                         h2 hi, lo;
-                        vx_two_terms(x[t][i], (float)rv.s[t][b][i], x[t][i + 1], (float)rv.s[t][b][i + 1], hi, lo);
+                        vx_two_terms(x[t][i], x[t][i + 1], __builtin_bit_cast(h2, rv.s[t][b][i >> 1]), zero, hi, lo);
                         const int n = 4 * t + i;
                         ph[n] = hi.x, ph[n + 1] = hi.y, pl[n] = lo.x, pl[n + 1] = lo.y;
                     }
@@ -267,64 +283,175 @@ struct vx_rows16 {
                     o[b][v] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, pl, o[b][v], 0, 0, 0);
                 }
             }
-            if (AHEAD) {
-                rk = nk;
-                rv = nv;
-            }
         }
 
-        // the four waves' sums: lane (m, g) holds dims 32 b + 2 (4 g + i) + v of query m
+        // lane (m, g) holds dims 32 b + 2 (4 g + i) + v of query m
         l = vx_sum_rows4(l);
         if (g == 0) {
-            sh_ml[wave][m][0] = M;
-            sh_ml[wave][m][1] = l;
+            sh.ml[wave][m][0] = M;
+            sh.ml[wave][m][1] = l;
         }
 #pragma unroll
         for (int b = 0; b < NB; ++b)
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-                *(f2*)&sh_o[wave][m][32 * b + 8 * g + 2 * i] = f2{o[b][0][i], o[b][1][i]};
+            for (int i = 0; i < 4; ++i) *(f2*)&sh.o[wave][m][32 * b + 8 * g + 2 * i] = f2{o[b][0][i], o[b][1][i]};
         __syncthreads();
-        const uint32_t D = 32 * NB;
-        const bool parts = a.splits > 1;
+        return kbeg < kend;
+    }
+
+    // The four waves' sums of a row, 4 dims.
+    static __device__ __forceinline__ f4 total(const shared& sh, uint32_t row, uint32_t d, float& M, float& l) {
+        M = -__builtin_inff();
+#pragma unroll
+        for (int i = 0; i < 4; ++i) M = fmaxf(M, sh.ml[i][row][0]);
+        const float Mr = M == -__builtin_inff() ? 0.f : M;
+        f4 t = {};
+        l = 0.f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float c = __builtin_amdgcn_exp2f(sh.ml[i][row][0] - Mr);
+            t += c * *(const f4*)&sh.o[i][row][d];
+            l = __builtin_fmaf(c, sh.ml[i][row][1], l);
+        }
+        return t;
+    }
+
+    // Row blocks and splits of their keys over the grid, heads fastest.
+    static __device__ void grid(const vx_attn_args& a) {
+        __shared__ shared sh;
+        uint32_t id = blockIdx.x;
+        const uint32_t kvh = id % a.c.heads;
+        id /= a.c.heads;
+        const uint32_t s = id % a.seqs;
+        id /= a.seqs;
+        const uint32_t split = id % a.splits, r0 = id / a.splits * 16;
+        const vx_attn_seq q = vx_attn_sequence(a, s);
+        if (r0 >= q.rows) return;
+        const bool any = unit(a, sh, q, s, kvh, r0, [&](int& lo, int& hi) {
+            // this split's keys; the last one takes what is left
+            const int64_t c0 = (int64_t)(lo & ~31) + (int64_t)split * a.chunk;
+            lo = (int)min(c0, (int64_t)hi);
+            if (split + 1 < a.splits) hi = (int)min((int64_t)hi, c0 + a.chunk);
+        });
+        constexpr uint32_t D = 32 * NB;
         for (uint32_t at = threadIdx.x; at < 16 * (D / 4); at += 256) {
-            const uint32_t row = at / (D / 4), d = 4 * (at % (D / 4));
-            if (r0 + row >= rows) break;  // (rows grow with at)
-            float Mt = -__builtin_inff();
-#pragma unroll
-            for (int i = 0; i < 4; ++i) Mt = fmaxf(Mt, sh_ml[i][row][0]);
-            const float Mr = Mt == -__builtin_inff() ? 0.f : Mt;
-            f4 t = {};
-            float lt = 0.f;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const float c = __builtin_amdgcn_exp2f(sh_ml[i][row][0] - Mr);
-                t += c * *(const f4*)&sh_o[i][row][d];
-                lt = __builtin_fmaf(c, sh_ml[i][row][1], lt);
-            }
-            const uint32_t j = (r0 + row) / a.group, token = (uint32_t)q.start + j, head = kvh * a.group + (r0 + row - j * a.group);
-            if (parts) {
-                const uint64_t at_row = ((uint64_t)split * a.tokens + token) * (a.c.heads * a.group) + head;
-                if (kbeg < kend) *(f4*)(a.part_o + at_row * D + d) = t;
-                if (d == 0) *(f2*)(a.part_ml + at_row * 2) = f2{Mt, lt};
+            const uint32_t r = r0 + at / (D / 4), d = 4 * (at % (D / 4));
+            if (r >= q.rows) break;  // (rows grow with at)
+            float M, l;
+            const f4 t = total(sh, r - r0, d, M, l);
+            const uint32_t j = r / a.group, token = (uint32_t)q.start + j, head = kvh * a.group + (r - j * a.group);
+            if (a.splits > 1) {
+                const uint64_t row = ((uint64_t)split * a.tokens + token) * (a.c.heads * a.group) + head;
+                if (any) *(f4*)(a.part_o + row * D + d) = t;
+                if (d == 0) *(f2*)(a.part_ml + row * 2) = f2{M, l};
             } else {
-                const float r = lt == 0.f ? 0.f : 1.f / lt;  // nothing seen: zeros
-                float* op = a.out + (int64_t)token * a.os[0] + (int64_t)head * a.os[1];
-                if (a.vec) {
-                    *(f4*)(op + d) = t * r;
-                } else {
+                vx_attn_put(a, token, head, d, t, l);
+            }
+        }
+    }
+
+    // One row block a sequence (single tokens, small trees): the key steps of
+    // all sequences and heads, 128 keys each, dealt out evenly, a run of them to
+    // each workgroup, whatever the lengths. Sequence s has cs steps a head (at
+    // least one if it has a query); unit (s, head) begins at step heads * (sum
+    // of c before s) + head * cs. Workgroup w's part of unit u is partial w + u
+    // (no two have the same one); which partials are a unit's goes to info, for
+    // the join.
+    // Against equal splits of every sequence: 32 sequences of 2400 to 8000 keys
+    // 91 -> 72 us.
+    static __device__ __forceinline__ uint32_t steps(const vx_attn_args& a, const vx_attn_seq& q, int& lo) {
+        const int len = min(q.len, (int)(a.table_cols << a.c.page_shift));
+        lo = 0;
+        if (a.window) lo = (int)max((int64_t)0, (int64_t)q.len - q.n - (int64_t)a.window) & ~31;
+        return q.n ? (uint32_t)max(1, (len - lo + 127) / 128) : 0u;
+    }
+
+    static __device__ void even(const vx_attn_args& a) {
+        __shared__ shared sh;
+        __shared__ uint32_t sh_sum[4], sh_at[2];
+        const uint32_t t = threadIdx.x, H = a.c.heads;
+        constexpr uint32_t D = 32 * NB;
+        // sums of steps over the sequences
+        const uint32_t per = (a.seqs + 255) / 256;
+        uint32_t mine = 0;
+        for (uint32_t s = t * per; s < min((t + 1) * per, a.seqs); ++s) {
+            int lo;
+            mine += steps(a, vx_attn_sequence(a, s), lo);
+        }
+        uint32_t upto = mine;
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) op[(int64_t)(d + i) * a.os[2]] = t[i] * r;
+        for (int o = 1; o < 64; o <<= 1) {
+            const uint32_t v = __shfl_up(upto, o);
+            if ((t & 63) >= (uint32_t)o) upto += v;
+        }
+        if ((t & 63) == 63) sh_sum[t >> 6] = upto;
+        __syncthreads();
+        uint32_t before = upto - mine, all = 0;
+#pragma unroll
+        for (uint32_t i = 0; i < 4; ++i) {
+            if (i < t >> 6) before += sh_sum[i];
+            all += sh_sum[i];
+        }
+        const uint64_t total_steps = (uint64_t)all * H, each = (total_steps + gridDim.x - 1) / gridDim.x;
+        uint64_t p = blockIdx.x * each;
+        const uint64_t end = min(p + each, total_steps);
+        if (p >= end) return;
+        if (p >= (uint64_t)before * H && p < (uint64_t)(before + mine) * H) {
+            uint32_t s = t * per, sum = before;
+            for (;; ++s) {
+                int lo;
+                const uint32_t c = steps(a, vx_attn_sequence(a, s), lo);
+                if (p < (uint64_t)(sum + c) * H) break;
+                sum += c;
+            }
+            sh_at[0] = s;
+            sh_at[1] = sum;
+        }
+        __syncthreads();
+        uint32_t s = __builtin_amdgcn_readfirstlane(sh_at[0]);
+        uint64_t begin = (uint64_t)__builtin_amdgcn_readfirstlane(sh_at[1]) * H;  // first step of sequence s
+        while (p < end) {
+            const vx_attn_seq q = vx_attn_sequence(a, s);
+            int klo;
+            const uint32_t c = steps(a, q, klo);
+            if (p >= begin + (uint64_t)c * H) {
+                begin += (uint64_t)c * H;
+                ++s;
+                continue;
+            }
+            const uint32_t kvh = (uint32_t)((p - begin) / c);
+            const uint64_t u0 = begin + (uint64_t)kvh * c;                       // the unit's first step
+            const uint32_t c0 = (uint32_t)(p - u0), c1 = (uint32_t)min((uint64_t)c, end - u0);
+            const uint32_t w0 = (uint32_t)(u0 / each), parts = (uint32_t)((u0 + c - 1) / each) - w0 + 1;
+            unit(a, sh, q, s, kvh, 0, [&](int& lo, int& hi) {
+                lo = max(lo & ~31, klo + (int)c0 * 128);
+                if (c1 < c) hi = min(hi, klo + (int)c1 * 128);
+            });
+            const uint32_t un = s * H + kvh;
+            const uint64_t pitch = (uint64_t)a.max_queries * a.group;  // rows of a partial
+            if (c0 == 0 && t == 0) *(u2*)(a.info + 2 * un) = u2{w0 + un, parts};
+            for (uint32_t at = t; at < q.rows * (D / 4); at += 256) {
+                const uint32_t r = at / (D / 4), d = 4 * (at % (D / 4));
+                float M, l;
+                const f4 v = total(sh, r, d, M, l);
+                if (parts == 1) {
+                    vx_attn_put(a, (uint32_t)q.start + r / a.group, kvh * a.group + r % a.group, d, v, l);
+                } else {
+                    const uint64_t row = ((uint64_t)blockIdx.x + un) * pitch + r;
+                    *(f4*)(a.part_o + row * D + d) = v;
+                    if (d == 0) *(f2*)(a.part_ml + row * 2) = f2{M, l};
                 }
             }
+            p = u0 + c1;
+            __syncthreads();  // sh is the next unit's
         }
     }
 };
 
-// Joins the splits of a query row: 16 to 64 lanes take its dims, four at a
-// time, and the splits go over the groups of lanes, of a wave where there are
-// up to 8 splits (four rows a workgroup) and of the workgroup above (one row).
-// One group a row took 90 us for 64 rows of 128 splits, this 4.
+// Joins the partial sums of a query row: 16 to 64 lanes take its dims, four at
+// a time, and the partials go over the groups of lanes, of a wave where a row
+// has up to 8 of them (four rows a workgroup) and of the workgroup above (one
+// row). One group a row took 90 us for 64 rows of 128 partials, this 4.
 __device__ __forceinline__ void vx_attn_join_rows(const vx_attn_args& a) {
     __shared__ f4 sh_t[256];
     __shared__ f2 sh_ml[64];
@@ -336,16 +463,24 @@ __device__ __forceinline__ void vx_attn_join_rows(const vx_attn_args& a) {
     id /= a.c.heads;
     const uint32_t s = id % a.seqs, r = id / a.seqs;
     const vx_attn_seq q = vx_attn_sequence(a, s);
-    const bool valid = r < q.rows && d < D;
     const uint32_t heads = a.c.heads * a.group, j = r / a.group, head = kvh * a.group + (r - j * a.group);
-    const uint64_t stride = (uint64_t)a.tokens * heads, row = ((uint64_t)q.start + j) * heads + head;
+    uint32_t parts = a.splits;
+    uint64_t stride = (uint64_t)a.tokens * heads, row = ((uint64_t)q.start + j) * heads + head;
+    bool valid = r < q.rows && d < D;
+    if (a.info) {
+        const u2 i = q.n ? *(const u2*)(a.info + 2 * (s * a.c.heads + kvh)) : u2{0, 1};
+        parts = i.y;
+        stride = (uint64_t)a.max_queries * a.group;
+        row = i.x * stride + r;
+        valid = valid && parts > 1;  // (else the result is there)
+    }
     float M = -__builtin_inff(), l = 0.f;
     f4 t = {};
     if (valid) {
 #pragma unroll 4
-        for (uint32_t i = group; i < a.splits; i += groups) {
+        for (uint32_t i = group; i < parts; i += groups) {
             const f2 ml = *(const f2*)(a.part_ml + (i * stride + row) * 2);
-            if (ml.y == 0.f) continue;  // nothing seen there, and nothing written (not so for a NaN)
+            if (ml.y == 0.f) continue;  // nothing seen there, perhaps nothing written (not so for a NaN)
             const f4 o = *(const f4*)(a.part_o + (i * stride + row) * D + d);
             const float Mn = fmaxf(M, ml.x), c = __builtin_amdgcn_exp2f(M - Mn), k = __builtin_amdgcn_exp2f(ml.x - Mn);
             // (M is -inf before the first; a NaN in y may have -inf beside it, and stays)
@@ -371,12 +506,5 @@ __device__ __forceinline__ void vx_attn_join_rows(const vx_attn_args& a) {
         t += c * sh_t[first + i * lanes];
         l = __builtin_fmaf(c, ml.y, l);
     }
-    const float k = l == 0.f ? 0.f : 1.f / l;
-    float* op = a.out + (int64_t)(q.start + j) * a.os[0] + (int64_t)head * a.os[1];
-    if (a.vec) {
-        *(f4*)(op + d) = t * k;
-    } else {
-#pragma unroll
-        for (uint32_t i = 0; i < 4; ++i) op[(int64_t)(d + i) * a.os[2]] = t[i] * k;
-    }
+    vx_attn_put(a, (uint32_t)q.start + j, head, d, t, l);
 }

@@ -34,15 +34,26 @@ typedef float f4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u2 __attribute__((ext_vector_type(2)));
 typedef uint32_t u4 __attribute__((ext_vector_type(4)));
 
-// a * c and b * d as two f16 terms each: hi rounds the product, lo what that
-// left out (exactly formed). The empty asm keeps one rounding for both uses of
-// hi: the compiler otherwise takes v_fma_mixlo for one of them, which rounds
-// the product once instead of twice, and lo is then off by hi's last place.
-__device__ __forceinline__ void vx_two_terms(float a, float c, float b, float d, h2& hi, h2& lo) {
-    uint32_t u = __builtin_bit_cast(uint32_t, __builtin_convertvector((f2{a * c, b * d}), h2));
+// a and b as two f16 terms each: hi rounds, lo what that left out. The empty
+// asm keeps one rounding for both uses of hi: the compiler otherwise folds a
+// multiply before it into v_fma_mixlo for one of them, which rounds once
+// instead of twice, and lo is then off by hi's last place.
+__device__ __forceinline__ void vx_two_terms(float a, float b, h2& hi, h2& lo) {
+    uint32_t u = __builtin_bit_cast(uint32_t, __builtin_convertvector((f2{a, b}), h2));
     asm("" : "+v"(u));
     hi = __builtin_bit_cast(h2, u);
-    lo = __builtin_convertvector((f2{__builtin_fmaf(a, c, -(float)hi.x), __builtin_fmaf(b, d, -(float)hi.y)}), h2);
+    lo = __builtin_convertvector((f2{a - (float)hi.x, b - (float)hi.y}), h2);
+}
+
+// w0 * d.x and w1 * d.y as two f16 terms each, lo from the exact product. `zero`
+// is -0.0 in a register: a product written as a multiply-add takes the f16
+// operand as it is (v_fma_mix), a multiplication would convert it first.
+__device__ __forceinline__ void vx_two_terms(float w0, float w1, h2 d, float zero, h2& hi, h2& lo) {
+    uint32_t u = __builtin_bit_cast(uint32_t, __builtin_convertvector((f2{__builtin_fmaf(w0, (float)d.x, zero),
+                                                                         __builtin_fmaf(w1, (float)d.y, zero)}), h2));
+    asm("" : "+v"(u));
+    hi = __builtin_bit_cast(h2, u);
+    lo = __builtin_convertvector((f2{__builtin_fmaf(w0, (float)d.x, -(float)hi.x), __builtin_fmaf(w1, (float)d.y, -(float)hi.y)}), h2);
 }
 
 // Bytes of a record's parts.

@@ -48,7 +48,8 @@ static int kernel_of(const vx_kv_cache* c, const int (&d)[4]) {
     return d[dim_index(c->dim)] + (c->k_type == VX_Q4_0 ? 2 : 0) + (c->v_type == VX_Q4_0 ? 1 : 0);
 }
 #define VX_DIMS(f) {K_vx_##f##_d64_k8v8, K_vx_##f##_d96_k8v8, K_vx_##f##_d128_k8v8, K_vx_##f##_d256_k8v8}
-static const int kWrite[4] = VX_DIMS(kv_write), kRead[4] = VX_DIMS(kv_read), kRows16[4] = VX_DIMS(attn_rows16);
+static const int kWrite[4] = VX_DIMS(kv_write), kRead[4] = VX_DIMS(kv_read), kRows16[4] = VX_DIMS(attn_rows16),
+                 kEven16[4] = VX_DIMS(attn_even16);
 #undef VX_DIMS
 
 // A [tokens, heads, dim] view.
@@ -112,32 +113,45 @@ static int run_rows(vx_ctx ctx, vx_stream stream, const vx_kv_cache* cache, cons
     return launch_struct(ctx, kernel_of(cache, write ? kWrite : kRead), grid, 256, stream, &a);
 }
 
-// How a call is laid out: row blocks of 16 query rows, and the keys of a block
-// split where there are fewer workgroups than the card takes.
+// How a call is laid out. Up to 16 query rows a sequence and head: `even`, a
+// workgroup on every place of the card, the keys of the whole batch dealt out
+// evenly. More: row blocks of 16, and their keys split where there are fewer
+// workgroups than the card takes.
 struct AttnPlan {
+    bool even;
     uint32_t row_blocks, splits, chunk;
+    uint32_t grid;
+    uint64_t info, rows;  // of the workspace: bytes before, and rows of partial sums
+    uint64_t bytes(uint32_t dim) const { return info + rows * (dim + 2) * 4; }
 };
 
 static int plan_attention(int num_cus, const vx_kv_cache* c, const vx_attn_batch* b, const vx_attn_opts* o, uint32_t q_heads,
-                          AttnPlan* p) {
+                          uint64_t tokens, bool ws, AttnPlan* p) {
     const uint32_t group = q_heads / c->heads;
     const uint64_t queries = b->max_queries;
-    const uint64_t rb = (queries * group + 15) / 16;
+    const uint64_t rb = (queries * group + 15) / 16, units = (uint64_t)b->seqs * c->heads;
     uint64_t span = std::min<uint64_t>(b->max_len, (uint64_t)b->table_cols * c->page_tokens);
     if (o && o->window) span = std::min<uint64_t>(span, 2ull * o->window + queries + 64);
-    const uint64_t wgs = std::max<uint64_t>(1, rb * b->seqs * c->heads), want = 4ull * (uint64_t)num_cus;
-    const uint64_t splits = std::max<uint64_t>(1, std::min<uint64_t>((want + wgs - 1) / wgs, (span + 255) / 256));
-    const uint64_t chunk = std::max<uint64_t>(128, ((span + splits - 1) / splits + 127) / 128 * 128);
+    *p = AttnPlan{};
     p->row_blocks = (uint32_t)rb;
+    if (units * rb >= (1ull << 24)) return fail(VX_ERR_UNSUPPORTED, "attention: too many workgroups (split the batch)");
+    const uint64_t steps = units * ((span + 127) / 128 + 1), places = 2ull * (uint64_t)num_cus;
+    if (rb == 1 && ws) {
+        p->even = true;
+        p->grid = (uint32_t)std::max<uint64_t>(1, std::min(steps, places));
+        p->splits = 16;  // (partials of a unit, for the join)
+        p->info = (units * 8 + 15) / 16 * 16;
+        p->rows = (p->grid + units) * queries * group;
+        return VX_OK;
+    }
+    const uint64_t wgs = std::max<uint64_t>(1, rb * units);
+    const uint64_t splits = ws ? std::max<uint64_t>(1, std::min<uint64_t>((places + wgs - 1) / wgs, (span + 255) / 256)) : 1;
+    const uint64_t chunk = std::max<uint64_t>(128, ((span + splits - 1) / splits + 127) / 128 * 128);
     p->chunk = (uint32_t)std::min<uint64_t>(chunk, 1u << 31);
-    p->splits = (uint32_t)std::max<uint64_t>(1, (span + chunk - 1) / chunk);
-    if (rb * b->seqs * c->heads * p->splits >= (1ull << 24))  // a grid has fewer than 2^32 threads
-        return fail(VX_ERR_UNSUPPORTED, "attention: too many workgroups (split the batch)");
+    p->splits = (uint32_t)(ws ? std::max<uint64_t>(1, (span + chunk - 1) / chunk) : 1);
+    p->grid = (uint32_t)(rb * units * p->splits);
+    if (p->splits > 1) p->rows = p->splits * tokens * q_heads;
     return VX_OK;
-}
-
-static uint64_t ws_bytes(const AttnPlan& p, uint64_t rows, uint32_t dim) {
-    return p.splits > 1 ? p.splits * rows * (dim + 2) * 4 : 0;
 }
 
 static int check_batch(const vx_kv_cache* c, const vx_attn_batch* b, const vx_attn_opts* o, uint32_t q_heads) {
@@ -174,10 +188,8 @@ static int run_attention(vx_ctx ctx, vx_stream stream, const vx_mview* out, cons
     if (rq.tokens > (1u << 30)) return fail(VX_ERR_UNSUPPORTED, "more than 2^30 query tokens");
     if (rq.tokens == 0 || batch->seqs == 0 || batch->max_queries == 0) return VX_OK;
     AttnPlan p;
-    if ((s = plan_attention(ctx_cus(ctx), cache, batch, opts, rq.heads, &p))) return s;
-    const uint64_t rows = (uint64_t)rq.tokens * rq.heads, need = ws_bytes(p, rows, cache->dim);
-    if (need && !ws) p.splits = 1;
-    if (need && ws && ws_size < need) return fail(VX_ERR_INVALID, "workspace smaller than vx_attention_ws_size");
+    if ((s = plan_attention(ctx_cus(ctx), cache, batch, opts, rq.heads, rq.tokens, ws != nullptr, &p))) return s;
+    if (ws_size < p.bytes(cache->dim)) return fail(VX_ERR_INVALID, "workspace smaller than vx_attention_ws_size");
     a.q = (const float*)rq.ptr;
     a.out = (float*)ro.ptr;
     for (int i = 0; i < 3; ++i) {
@@ -212,10 +224,10 @@ static int run_attention(vx_ctx ctx, vx_stream stream, const vx_mview* out, cons
     a.row_blocks = p.row_blocks;
     a.splits = p.splits;
     a.chunk = p.chunk;
-    a.part_o = (float*)ws;
-    a.part_ml = (float*)ws + p.splits * rows * cache->dim;
-    const uint32_t grid = p.row_blocks * p.splits * batch->seqs * cache->heads;
-    if ((s = launch_struct(ctx, kernel_of(cache, kRows16), grid, 256, stream, &a))) return s;
+    a.info = p.even ? (uint32_t*)ws : nullptr;
+    a.part_o = (float*)((char*)ws + p.info);
+    a.part_ml = a.part_o + p.rows * cache->dim;
+    if ((s = launch_struct(ctx, kernel_of(cache, p.even ? kEven16 : kRows16), p.grid, 256, stream, &a))) return s;
     if (p.splits > 1) {
         const uint64_t jobs = (uint64_t)batch->max_queries * a.group * batch->seqs * cache->heads;
         return launch_struct(ctx, K_vx_attn_join, (uint32_t)(p.splits > 8 ? jobs : (jobs + 3) / 4), 256, stream, &a);
@@ -276,8 +288,8 @@ int vx_attention_ws_size(vx_ctx ctx, const vx_kv_cache* cache, const vx_attn_bat
     if ((s = vx::check_batch(cache, batch, opts, q_heads))) return s;
     if (!tokens || !batch->seqs || !batch->max_queries) return VX_OK;
     vx::AttnPlan p;
-    if ((s = vx::plan_attention(vx::ctx_cus(ctx), cache, batch, opts, q_heads, &p))) return s;
-    *bytes = vx::ws_bytes(p, (uint64_t)tokens * q_heads, cache->dim);
+    if ((s = vx::plan_attention(vx::ctx_cus(ctx), cache, batch, opts, q_heads, tokens, true, &p))) return s;
+    *bytes = p.bytes(cache->dim);
     return VX_OK;
 }
 

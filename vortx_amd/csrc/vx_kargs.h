@@ -156,8 +156,9 @@ typedef struct vx_attn_args {
     const int32_t* prefix; /* [seqs] or null */
     const int32_t* first;  /* [tokens] or null */
     const uint32_t* tree;  /* [tokens][tree_stride] or null */
-    float* part_o;         /* partial sums [split][token][head][dim] (splits > 1) */
-    float* part_ml;        /* [split][token][head][2] */
+    uint32_t* info;        /* even split: [seqs][heads] first partial and their number; else null */
+    float* part_o;         /* partial sums [split][token][head][dim] (splits > 1), or [partial][row][dim] */
+    float* part_ml;        /* [split][token][head][2], or [partial][row][2] */
     uint32_t table_stride, table_cols;
     uint32_t seqs, tokens, group;
     uint32_t max_queries, max_len;
