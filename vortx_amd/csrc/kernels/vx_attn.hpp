@@ -9,18 +9,20 @@ typedef const __attribute__((address_space(4))) int32_t* vx_scalar_i32;
 
 constexpr float VX_LOG2E = 1.44269504088896340736f;
 
-// tanh to about two units in the last place: a minimax polynomial below 0.65,
-// 1 - 2 / (1 + e^2|t|) above (which would cancel below).
-__device__ __forceinline__ float vx_tanh(float t) {
-    const float a = fabsf(t), z = t * t;
+// tanh to about two units in the last place: below 0.65 a minimax polynomial,
+// above 1 - 2 / (1 + e^2|t|), which would cancel below.
+__device__ __forceinline__ float vx_tanh_small(float t) {
+    const float z = t * t;
     float p = __builtin_fmaf(z, -0.005468255840241909f, 0.020415181294083595f);
     p = __builtin_fmaf(z, p, -0.05366527661681175f);
     p = __builtin_fmaf(z, p, 0.1333041489124298f);
     p = __builtin_fmaf(z, p, -0.3333323001861572f);
-    p = __builtin_fmaf(z * t, p, t);
-    const float e = __builtin_amdgcn_exp2f(a * (2.f * VX_LOG2E));
+    return __builtin_fmaf(z * t, p, t);
+}
+__device__ __forceinline__ float vx_tanh(float t) {
+    const float a = fabsf(t), e = __builtin_amdgcn_exp2f(a * (2.f * VX_LOG2E));
     const float q = __builtin_fmaf(-2.f, __builtin_amdgcn_rcpf(1.f + e), 1.f);
-    return a < 0.65f ? p : __builtin_copysignf(q, t);  // (NaN: q, which is NaN)
+    return a < 0.65f ? vx_tanh_small(t) : __builtin_copysignf(q, t);  // (NaN: q, which is NaN)
 }
 
 // Maximum / sum over the four 16-lane rows, in every lane.
@@ -43,7 +45,7 @@ __device__ __forceinline__ vx_attn_seq vx_attn_sequence(const vx_attn_args& a, u
     const int T = (int)a.tokens;
     q.start = min(max(a.starts[s], 0), T);
     q.n = min(max(a.starts[s + 1], q.start), T) - q.start;
-    q.len = min(max(a.lens[s], 0), (int)a.max_len);
+    q.len = min(max(a.lens[s], 0), (int)min(a.max_len, a.table_cols << a.c.page_shift));
     q.rows = min((uint32_t)q.n, a.max_queries) * a.group;
     return q;
 }
@@ -96,17 +98,39 @@ __device__ __forceinline__ vx_attn_row vx_attn_row_of(const vx_attn_args& a, con
     return w;
 }
 
-// Tree: whether the row sees key (a draft, or past the end), and its distance.
-__device__ __forceinline__ bool vx_tree_sees(const vx_attn_args& a, const vx_attn_seq& q, const vx_attn_row& w, int key, float& dist) {
-    const int j = key - (q.len - q.n);
-    if (!w.valid || key >= q.len || j < 0 || (uint32_t)j >= a.tree_words * 32u) return false;
-    if (!(a.tree[(uint64_t)w.token * a.tree_stride + ((uint32_t)j >> 5)] >> (j & 31) & 1u)) return false;
-    if (a.slopes || a.window) {
-        const int d = abs(w.pos - (q.len - q.n + vx_tree_count(a, q.start + j) - 1));
-        dist = (float)d;
-        if (a.window && (uint32_t)d >= a.window) return false;
+// Which of the 32 keys from k0 on a row sees, a bit each: those of its
+// interval before `tail`, and the drafts from there on by the tree's bits.
+// at[i] becomes the position of key k0 + i where that is not k0 + i for all of
+// them (slopes or a window over a tree; the wave's own 32 words of LDS).
+__device__ __forceinline__ uint32_t vx_attn_sees(const vx_attn_args& a, const vx_attn_seq& q, const vx_attn_row& w, int tail, int k0, int* at) {
+    auto from = [&](int key) { return key <= k0 ? 0xFFFFFFFFu : key - k0 > 31 ? 0u : 0xFFFFFFFFu << (key - k0); };  // keys >= key
+    uint32_t see = from(w.lo) & ~from(min(w.hi, tail));
+    if (a.tree && k0 + 32 > tail) {
+        const int j0 = k0 - tail;  // first draft of the tile (above -32)
+        uint32_t bits = 0;
+        if (w.valid) {
+            const uint32_t* row = a.tree + (uint64_t)w.token * a.tree_stride;
+            const int i = j0 >> 5, sh = j0 & 31;
+            const uint32_t w0 = i >= 0 && (uint32_t)i < a.tree_words ? row[i] : 0u;
+            const uint32_t w1 = (uint32_t)(i + 1) < a.tree_words ? row[i + 1] : 0u;
+            bits = (uint32_t)(((uint64_t)w1 << 32 | w0) >> sh);
+        }
+        bits &= from(tail) & ~from(q.len);
+        if (a.slopes || a.window) {
+            const int lane = threadIdx.x & 31, key = k0 + lane;
+            int p = key;
+            if (key >= tail && key < q.len) p = q.len - q.n + vx_tree_count(a, q.start + key - (q.len - q.n)) - 1;
+            at[lane] = p;  // (both halves of the wave the same)
+            __builtin_amdgcn_wave_barrier();
+            if (a.window) {
+#pragma unroll 1
+                for (int i = 0; i < 32; ++i)
+                    if ((uint32_t)abs(w.pos - at[i]) >= a.window) bits &= ~(1u << i);
+            }
+        }
+        see |= bits;
     }
-    return true;
+    return see;
 }
 
 // Four dims of a row's result: its sums over its weights' sum. Nothing seen: zeros.

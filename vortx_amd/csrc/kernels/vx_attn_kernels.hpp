@@ -1,6 +1,7 @@
 // vx_attn_kernels.hpp — the kernels of one head size (VX_NB blocks of 32), for
 // each pair of cache types (k8v8: 8 bits for K and V, and so on).
 #include "vx_attn_rows16.hpp"
+#include "vx_attn_tile.hpp"
 #include "vx_kv_rows.hpp"
 
 #define VX_CAT(f, types) VX_NAME(f, types)
@@ -16,6 +17,9 @@
     }                                                                                                          \
     extern "C" __global__ __launch_bounds__(256, VX_NB <= 4 ? 2 : 1) void VX_CAT(attn_even16, types)(vx_attn_args a) {          \
         vx_rows16<VX_NB, KB, VB>::even(a);                                                                     \
+    }                                                                                                          \
+    extern "C" __global__ __launch_bounds__(256, VX_NB <= 4 ? 2 : 1) void VX_CAT(attn_tile, types)(vx_attn_args a) { \
+        vx_tile<VX_NB, KB, VB>::run(a);                                                                        \
     }
 VX_KERNELS(k8v8, 8, 8)
 VX_KERNELS(k8v4, 8, 4)

@@ -68,6 +68,7 @@ struct vx_rows16 {
     struct shared {
         float o[4][16][NB * 32 + 4];
         float ml[4][16][2];
+        int at[4][32];
     };
 
     // Rows r0.. of sequence s and key/value head kvh over the keys that
@@ -93,7 +94,7 @@ struct vx_rows16 {
             hi = q.len;
         }
         lo = __builtin_amdgcn_readfirstlane(lo);
-        hi = min(__builtin_amdgcn_readfirstlane(hi), min(q.len, (int)(a.table_cols << a.c.page_shift)));
+        hi = __builtin_amdgcn_readfirstlane(hi);
         lo_all = __builtin_amdgcn_readfirstlane(lo_all);
         hi_all = __builtin_amdgcn_readfirstlane(hi_all);
         if (lo >= hi) lo = hi = 0;  // (lo of rows that see nothing is the largest int: 32 more would be negative)
@@ -149,7 +150,7 @@ struct vx_rows16 {
         float M = -__builtin_inff(), l = 0.f;
         const vx_scalar_i32 table = (vx_scalar_i32)(a.table + (uint64_t)s * a.table_stride);
         const uint8_t* base = a.c.base + (uint64_t)(kvh << (a.c.page_shift - 4)) * REC;
-        const int last = min(q.len, (int)(a.table_cols << a.c.page_shift)) - 1;
+        const int last = q.len - 1;
         const float capl = a.cap * VX_LOG2E;
 
         // K of the next keys is requested when these keys' registers are free,
@@ -210,20 +211,22 @@ struct vx_rows16 {
                         for (int i = 0; i < 4; ++i) x[t][i] = __builtin_fmaf(-w.slope, fabsf(d0 - (float)(16 * t + i)), x[t][i]);
                 }
             } else {
+                const uint32_t see = vx_attn_sees(a, q, w, tail, k0, sh.at[wave]) >> (4 * g);
+                const bool drafts = a.tree && k0 + 32 > tail;
 #pragma unroll
                 for (int t = 0; t < 2; ++t)
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        const int key = k0 + 16 * t + 4 * (int)g + i;
-                        float dist = fabsf((float)(w.pos - key));
-                        bool v;
-                        if (key < tail) v = key >= w.lo && key < w.hi;
-                        else v = a.tree && vx_tree_sees(a, q, w, key, dist);
-                        x[t][i] = v ? __builtin_fmaf(-w.slope, dist, x[t][i]) : -__builtin_inff();
+                        if (a.slopes) {
+                            const int key = 16 * t + 4 * (int)g + i;
+                            x[t][i] = __builtin_fmaf(-w.slope, fabsf((float)(w.pos - (drafts ? sh.at[wave][key] : k0 + key))), x[t][i]);
+                        }
+                        const uint32_t v = 0u - (see >> (16 * t + i) & 1u);
+                        x[t][i] = v ? x[t][i] : -__builtin_inff();
                         // a lane's scales are of its own row: what the row does not see, which
                         // may be anything, counts nowhere
 #pragma unroll
-                        for (int b = 0; b < NB; ++b) rv.s[t][b][i >> 1] &= v ? 0xFFFFFFFFu : i & 1 ? 0x0000FFFFu : 0xFFFF0000u;
+                        for (int b = 0; b < NB; ++b) rv.s[t][b][i >> 1] &= v | (i & 1 ? 0x0000FFFFu : 0xFFFF0000u);
                     }
             }
             // running maximum of score + exponent of V's scales
@@ -317,7 +320,7 @@ struct vx_rows16 {
     }
 
     // Row blocks and splits of their keys over the grid, heads fastest.
-    static __device__ void grid(const vx_attn_args& a) {
+    static __device__ __forceinline__ void grid(const vx_attn_args& a) {
         __shared__ shared sh;
         uint32_t id = blockIdx.x;
         const uint32_t kvh = id % a.c.heads;
@@ -360,13 +363,12 @@ struct vx_rows16 {
     // Against equal splits of every sequence: 32 sequences of 2400 to 8000 keys
     // 91 -> 72 us.
     static __device__ __forceinline__ uint32_t steps(const vx_attn_args& a, const vx_attn_seq& q, int& lo) {
-        const int len = min(q.len, (int)(a.table_cols << a.c.page_shift));
         lo = 0;
         if (a.window) lo = (int)max((int64_t)0, (int64_t)q.len - q.n - (int64_t)a.window) & ~31;
-        return q.n ? (uint32_t)max(1, (len - lo + 127) / 128) : 0u;
+        return q.n ? (uint32_t)max(1, (q.len - lo + 127) / 128) : 0u;
     }
 
-    static __device__ void even(const vx_attn_args& a) {
+    static __device__ __forceinline__ void even(const vx_attn_args& a) {
         __shared__ shared sh;
         __shared__ uint32_t sh_sum[4], sh_at[2];
         const uint32_t t = threadIdx.x, H = a.c.heads;

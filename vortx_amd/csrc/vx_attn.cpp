@@ -44,12 +44,13 @@ static int check_cache(const vx_kv_cache* c, vx_kv_geom* g) {
 }
 
 // Kernel of this cache's head size and types: the lists go d64 k8v8, k8v4, k4v8, k4v4, d96 ...
-static int kernel_of(const vx_kv_cache* c, const int (&d)[4]) {
+static int kernel_of(const vx_kv_cache* c, const int* d) {
     return d[dim_index(c->dim)] + (c->k_type == VX_Q4_0 ? 2 : 0) + (c->v_type == VX_Q4_0 ? 1 : 0);
 }
 #define VX_DIMS(f) {K_vx_##f##_d64_k8v8, K_vx_##f##_d96_k8v8, K_vx_##f##_d128_k8v8, K_vx_##f##_d256_k8v8}
 static const int kWrite[4] = VX_DIMS(kv_write), kRead[4] = VX_DIMS(kv_read), kRows16[4] = VX_DIMS(attn_rows16),
-                 kEven16[4] = VX_DIMS(attn_even16);
+                 kEven16[4] = VX_DIMS(attn_even16), kTile[4] = VX_DIMS(attn_tile);
+constexpr uint32_t VX_EVEN_ROWS = 16;  // query rows of a workgroup of kEven16
 #undef VX_DIMS
 
 // A [tokens, heads, dim] view.
@@ -113,11 +114,8 @@ static int run_rows(vx_ctx ctx, vx_stream stream, const vx_kv_cache* cache, cons
     return launch_struct(ctx, kernel_of(cache, write ? kWrite : kRead), grid, 256, stream, &a);
 }
 
-// How a call is laid out. Up to 16 query rows a sequence and head: `even`, a
-// workgroup on every place of the card, the keys of the whole batch dealt out
-// evenly. More: row blocks of 16, and their keys split where there are fewer
-// workgroups than the card takes.
 struct AttnPlan {
+    const int* kernel;
     bool even;
     uint32_t row_blocks, splits, chunk;
     uint32_t grid;
@@ -127,29 +125,32 @@ struct AttnPlan {
 
 static int plan_attention(int num_cus, const vx_kv_cache* c, const vx_attn_batch* b, const vx_attn_opts* o, uint32_t q_heads,
                           uint64_t tokens, bool ws, AttnPlan* p) {
-    const uint32_t group = q_heads / c->heads;
-    const uint64_t queries = b->max_queries;
-    const uint64_t rb = (queries * group + 15) / 16, units = (uint64_t)b->seqs * c->heads;
+    const uint64_t group = q_heads / c->heads, queries = b->max_queries, units = (uint64_t)b->seqs * c->heads;
     uint64_t span = std::min<uint64_t>(b->max_len, (uint64_t)b->table_cols * c->page_tokens);
     if (o && o->window) span = std::min<uint64_t>(span, 2ull * o->window + queries + 64);
+    const uint64_t places = (c->dim > 128 ? 1ull : 2ull) * (uint64_t)num_cus;  // workgroups that the card holds
     *p = AttnPlan{};
-    p->row_blocks = (uint32_t)rb;
-    if (units * rb >= (1ull << 24)) return fail(VX_ERR_UNSUPPORTED, "attention: too many workgroups (split the batch)");
-    const uint64_t steps = units * ((span + 127) / 128 + 1), places = 2ull * (uint64_t)num_cus;
-    if (rb == 1 && ws) {
+    if (queries * group <= VX_EVEN_ROWS && ws) {
+        p->kernel = kEven16;
         p->even = true;
-        p->grid = (uint32_t)std::max<uint64_t>(1, std::min(steps, places));
+        p->row_blocks = 1;
+        p->grid = (uint32_t)std::max<uint64_t>(1, std::min(units * ((span + 127) / 128 + 1), places));
         p->splits = 16;  // (partials of a unit, for the join)
         p->info = (units * 8 + 15) / 16 * 16;
         p->rows = (p->grid + units) * queries * group;
+        if (units * queries * group >= (1ull << 24)) return fail(VX_ERR_UNSUPPORTED, "attention: too many rows (split the batch)");
         return VX_OK;
     }
-    const uint64_t wgs = std::max<uint64_t>(1, rb * units);
-    const uint64_t splits = ws ? std::max<uint64_t>(1, std::min<uint64_t>((places + wgs - 1) / wgs, (span + 255) / 256)) : 1;
-    const uint64_t chunk = std::max<uint64_t>(128, ((span + splits - 1) / splits + 127) / 128 * 128);
+    p->kernel = kTile;
+    const uint64_t rb = (queries * group + 127) / 128, wgs = rb * units;
+    uint64_t splits = 1;
+    if (ws && wgs < places) splits = std::max<uint64_t>(1, std::min<uint64_t>(places / wgs, (span + 127) / 128));
+    const uint64_t chunk = std::max<uint64_t>(32, ((span + splits - 1) / splits + 31) / 32 * 32);
+    p->row_blocks = (uint32_t)rb;
     p->chunk = (uint32_t)std::min<uint64_t>(chunk, 1u << 31);
-    p->splits = (uint32_t)(ws ? std::max<uint64_t>(1, (span + chunk - 1) / chunk) : 1);
-    p->grid = (uint32_t)(rb * units * p->splits);
+    p->splits = (uint32_t)(splits > 1 ? std::max<uint64_t>(1, (span + chunk - 1) / chunk) : 1);
+    if (wgs * p->splits >= (1ull << 24)) return fail(VX_ERR_UNSUPPORTED, "attention: too many workgroups (split the batch)");
+    p->grid = (uint32_t)(wgs * p->splits);
     if (p->splits > 1) p->rows = p->splits * tokens * q_heads;
     return VX_OK;
 }
@@ -227,7 +228,7 @@ static int run_attention(vx_ctx ctx, vx_stream stream, const vx_mview* out, cons
     a.info = p.even ? (uint32_t*)ws : nullptr;
     a.part_o = (float*)((char*)ws + p.info);
     a.part_ml = a.part_o + p.rows * cache->dim;
-    if ((s = launch_struct(ctx, kernel_of(cache, p.even ? kEven16 : kRows16), p.grid, 256, stream, &a))) return s;
+    if ((s = launch_struct(ctx, kernel_of(cache, p.kernel), p.grid, 256, stream, &a))) return s;
     if (p.splits > 1) {
         const uint64_t jobs = (uint64_t)batch->max_queries * a.group * batch->seqs * cache->heads;
         return launch_struct(ctx, K_vx_attn_join, (uint32_t)(p.splits > 8 ? jobs : (jobs + 3) / 4), 256, stream, &a);
