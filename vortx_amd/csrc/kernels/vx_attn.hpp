@@ -11,12 +11,13 @@ constexpr float VX_LOG2E = 1.44269504088896340736f;
 
 // tanh to about two units in the last place: below 0.65 a minimax polynomial,
 // above 1 - 2 / (1 + e^2|t|), which would cancel below.
+constexpr float VX_TANH[5] = {-0.3333323001861572f, 0.1333041489124298f, -0.05366527661681175f, 0.020415181294083595f, -0.005468255840241909f};
 __device__ __forceinline__ float vx_tanh_small(float t) {
     const float z = t * t;
-    float p = __builtin_fmaf(z, -0.005468255840241909f, 0.020415181294083595f);
-    p = __builtin_fmaf(z, p, -0.05366527661681175f);
-    p = __builtin_fmaf(z, p, 0.1333041489124298f);
-    p = __builtin_fmaf(z, p, -0.3333323001861572f);
+    float p = __builtin_fmaf(z, VX_TANH[4], VX_TANH[3]);
+    p = __builtin_fmaf(z, p, VX_TANH[2]);
+    p = __builtin_fmaf(z, p, VX_TANH[1]);
+    p = __builtin_fmaf(z, p, VX_TANH[0]);
     return __builtin_fmaf(z * t, p, t);
 }
 __device__ __forceinline__ float vx_tanh(float t) {

@@ -18,13 +18,26 @@
     extern "C" __global__ __launch_bounds__(256, VX_NB <= 4 ? 2 : 1) void VX_CAT(attn_even16, types)(vx_attn_args a) {          \
         vx_rows16<VX_NB, KB, VB>::even(a);                                                                     \
     }                                                                                                          \
-    extern "C" __global__ __launch_bounds__(256, VX_NB <= 4 ? 2 : 1) void VX_CAT(attn_tile, types)(vx_attn_args a) { \
-        vx_tile<VX_NB, KB, VB>::run(a);                                                                        \
+    extern "C" __global__ __launch_bounds__(256, VX_NB <= 4 ? 2 : 1) void VX_CAT(attn_tile4, types)(vx_attn_args a) { \
+        vx_tile<VX_NB, KB, VB, 4>::run(a);                                                                     \
     }
+// (256: eight waves' registers do not hold its sums)
+#if VX_NB <= 4
+#define VX_WIDE(types, KB, VB)                                                                                 \
+    extern "C" __global__ __launch_bounds__(512, 2) void VX_CAT(attn_tile8, types)(vx_attn_args a) {           \
+        vx_tile<VX_NB, KB, VB, 8>::run(a);                                                                     \
+    }
+#else
+#define VX_WIDE(types, KB, VB)
+#endif
 VX_KERNELS(k8v8, 8, 8)
 VX_KERNELS(k8v4, 8, 4)
 VX_KERNELS(k4v8, 4, 8)
 VX_KERNELS(k4v4, 4, 4)
+VX_WIDE(k8v8, 8, 8)
+VX_WIDE(k8v4, 8, 4)
+VX_WIDE(k4v8, 4, 8)
+VX_WIDE(k4v4, 4, 4)
 
 #if VX_NB == 4
 extern "C" __global__ __launch_bounds__(256) void vx_attn_join(vx_attn_args a) { vx_attn_join_rows(a); }

@@ -1,7 +1,7 @@
 // vx_attn_tile.hpp — attention of many query rows over the quantized cache.
 //
-// A workgroup takes 128 query rows of a sequence and key/value head, 32 to a
-// wave, and goes over their keys 32 at a time. The four waves decode a tile of
+// A workgroup takes 128 or 256 query rows of a sequence and key/value head, 32
+// to a wave, and goes over their keys 32 at a time. The waves decode a tile of
 // keys once into LDS, as operands of the 32 x 32 x 16 matrix instructions, while
 // the tile before is computed from the other buffer:
 //   K   the whole numbers, exact in f16; a block's scale is applied to its
@@ -24,14 +24,13 @@
 
 typedef float f16v __attribute__((ext_vector_type(16)));
 
-template <int NB, int KB, int VB>
+template <int NB, int KB, int VB, int WAVES>
 struct vx_tile {
     using PK = vx_kv_part<NB, KB>;
     using PV = vx_kv_part<NB, VB>;
     static constexpr uint32_t REC = PK::BYTES + PV::BYTES;
-    static constexpr int PAIRS = (NB + 1) / 2;               // pairs of blocks
-    static constexpr int ITEMS = (128 * PAIRS + 255) / 256;  // a thread's pieces of a tile: one lane's bytes of a pair
-    static constexpr uint32_t ROWS = 128;
+    static constexpr uint32_t THREADS = 64 * WAVES, ROWS = 32 * WAVES;
+    static constexpr int ITEMS = (128 * NB + THREADS - 1) / THREADS;  // a thread's pieces of a tile: one lane's bytes of a block
 
     struct tile {
         h8 k[NB * 4 * 32];      // [block][8-dim group][key]
@@ -41,136 +40,141 @@ struct vx_tile {
         uint32_t bad[8];        // their V scales that are not finite, bit 4 block + key
     };
 
-    struct raw {  // a thread's piece as loaded
-        uint32_t k[ITEMS][2 * KB / 4], v[ITEMS][2 * VB / 4];
-        uint32_t vs[NB][2];
+    struct raw {  // a thread's pieces as loaded
+        uint32_t k[ITEMS][KB / 4], v[ITEMS][VB / 4], d[ITEMS][2];
+        uint32_t vs[NB][2];  // V scales of its four keys
         uint32_t ks[2];
-        int valid;  // keys of this thread's four that exist
     };
 
     template <int BITS>
-    static __device__ __forceinline__ void load_pair(const uint8_t* p, int c, uint32_t lane, uint32_t (&w)[2 * BITS / 4]) {
-        const uint32_t* q = (const uint32_t*)(p + vx_kv_part<NB, BITS>::at(2 * c, lane));
-        if (NB % 2 == 0 || c + 1 < PAIRS) {
-            if constexpr (BITS == 8) {
-                const u4 v = *(const u4*)q;
-                w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
-            } else {
-                w[0] = q[0], w[1] = q[1];
-            }
+    static __device__ __forceinline__ void load_block(const uint8_t* p, int b, uint32_t lane, uint32_t (&w)[BITS / 4]) {
+        const uint8_t* q = p + vx_kv_part<NB, BITS>::at(b, lane);
+        if constexpr (BITS == 8) {
+            const u2 v = *(const u2*)q;
+            w[0] = v.x, w[1] = v.y;
         } else {
-#pragma unroll
-            for (int i = 0; i < BITS / 4; ++i) w[i] = q[i];
+            w[0] = *(const uint32_t*)q;
         }
     }
 
     // records of the 32 keys from k0 on; past the end the last one
     static __device__ __forceinline__ void load(const vx_attn_args& a, vx_scalar_i32 table, const uint8_t* base, int k0, int last, raw& r) {
-        const uint32_t t = threadIdx.x, rec = __builtin_amdgcn_readfirstlane((t >> 6) & 1), lane = t & 63, g = lane >> 4;
-        const int key0 = k0 + 16 * (int)rec, key = min(key0, last);
+        const uint32_t t = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(t >> 6), rec = wave & 1, lane = t & 63, g = lane >> 4;
+        const int key = min(k0 + 16 * (int)rec, last);
         const uint32_t page = min((uint32_t)table[(uint32_t)key >> a.c.page_shift], a.c.pages - 1u);
         const uint8_t* p = base + page * a.c.page_bytes + (((uint32_t)key & ((1u << a.c.page_shift) - 1u)) >> 4) * REC;
-        r.valid = last + 1 - (key0 + 4 * (int)g);
+        const uint8_t* sc = p + PK::BYTES + PV::VALS + g * (8 * NB);
 #pragma unroll
         for (int i = 0; i < ITEMS; ++i) {
-            const int c = (int)__builtin_amdgcn_readfirstlane(t >> 7) + 2 * i;
-            if (c < PAIRS) {
-                load_pair<KB>(p, c, lane, r.k[i]);
-                load_pair<VB>(p + PK::BYTES, c, lane, r.v[i]);
+            const int b = (int)(wave >> 1) + WAVES / 2 * i;
+            if (NB % (WAVES / 2) == 0 || b < NB) {
+                load_block<KB>(p, b, lane, r.k[i]);
+                load_block<VB>(p + PK::BYTES, b, lane, r.v[i]);
+                const u2 d = *(const u2*)(sc + 8 * b);
+                r.d[i][0] = d.x, r.d[i][1] = d.y;
             }
         }
-        const uint8_t* sc = p + PK::BYTES + PV::VALS + g * (8 * NB);
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
             const u2 v = *(const u2*)(sc + 8 * b);
             r.vs[b][0] = v.x, r.vs[b][1] = v.y;
         }
         // K's scales: lanes 0.. of waves 0 and 1, four keys of a block each
-        if (t < 128 && lane < 4 * NB) {
+        if (wave < 2 && lane < 4 * NB) {
             const u2 v = *(const u2*)(p + PK::VALS + lane * 8);
             r.ks[0] = v.x, r.ks[1] = v.y;
         }
     }
 
-    // decodes a thread's piece into the tile
-    static __device__ __forceinline__ void store(const raw& r, tile& s) {
+    // decodes a thread's pieces into the tile of the keys from k0 on
+    static __device__ __forceinline__ void store(raw& r, tile& s, int k0, int last) {
         typedef uint16_t us2 __attribute__((ext_vector_type(2)));
-        const uint32_t t = threadIdx.x, rec = (t >> 6) & 1, lane = t & 63, m = lane & 15, g = lane >> 4;
-        // V scales of keys that do not exist, which may be anything: 0; of those that are not finite: 0, and noted
-        const uint32_t keep0 = (r.valid > 0 ? 0xFFFFu : 0u) | (r.valid > 1 ? 0xFFFF0000u : 0u);
-        const uint32_t keep1 = (r.valid > 2 ? 0xFFFFu : 0u) | (r.valid > 3 ? 0xFFFF0000u : 0u);
-        uint32_t vs[NB][2], bad = 0, big = 0;
+        const uint32_t t = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(t >> 6), rec = wave & 1, lane = t & 63, m = lane & 15, g = lane >> 4;
+        uint32_t bad = 0;
+        auto largest = [&] {
+            us2 big = {0, 0};
 #pragma unroll
-        for (int b = 0; b < NB; ++b)
+            for (int b = 0; b < NB; ++b)
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                uint32_t d = r.vs[b][i] & (i ? keep1 : keep0);
-                const uint32_t lo = d & 0x7FFFu, hi = d >> 16 & 0x7FFFu;
-                if (lo >= 0x7C00u) d &= 0xFFFF0000u, bad |= 1u << (4 * b + 2 * i);
-                if (hi >= 0x7C00u) d &= 0x0000FFFFu, bad |= 2u << (4 * b + 2 * i);
-                vs[b][i] = d;
-                const uint32_t mag = d & 0x7FFF7FFFu;
-                big = __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(us2, big), __builtin_bit_cast(us2, mag)));
-            }
-        const int e = (int)(max(big & 0xFFFFu, big >> 16) >> 10) - 15;
-        if (t < 128 && m == 0) {
+                for (int i = 0; i < 2; ++i) {
+                    const uint32_t d = VB == 4 ? r.vs[b][i] & 0x7FFF7FFFu : r.vs[b][i];  // (8 bits: never negative)
+                    big = __builtin_elementwise_max(big, __builtin_bit_cast(us2, d));
+                }
+            return (uint32_t)max(big.x, big.y);
+        };
+        uint32_t big = largest();
+        if (k0 + 32 > last + 1 || __any(big >= 0x7C00u)) {
+            // scales of keys that do not exist, which may be anything: 0; those that are not finite: 0, and noted
+            const int valid = last + 1 - (k0 + 16 * (int)rec + 4 * (int)g);
+            auto fix = [&](uint32_t d, int i) {
+                if (valid <= 2 * i || (d & 0x7FFFu) >= 0x7C00u) d &= 0xFFFF0000u;
+                if (valid <= 2 * i + 1 || (d >> 16 & 0x7FFFu) >= 0x7C00u) d &= 0x0000FFFFu;
+                return d;
+            };
+#pragma unroll
+            for (int b = 0; b < NB; ++b)
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const uint32_t d = r.vs[b][i];
+                    if (valid > 2 * i && (d & 0x7FFFu) >= 0x7C00u) bad |= 1u << (4 * b + 2 * i);
+                    if (valid > 2 * i + 1 && (d >> 16 & 0x7FFFu) >= 0x7C00u) bad |= 2u << (4 * b + 2 * i);
+                    r.vs[b][i] = fix(d, i);
+                }
+#pragma unroll
+            for (int n = 0; n < ITEMS; ++n)
+#pragma unroll
+                for (int i = 0; i < 2; ++i) r.d[n][i] = fix(r.d[n][i], i);
+            big = largest();
+        }
+        const int e = (int)(big >> 10) - 15;
+        if (wave < 2 && m == 0) {
             s.e[rec * 4 + g] = (float)e;
             s.bad[rec * 4 + g] = bad;
         }
         const _Float16 f = (_Float16)__builtin_ldexpf(1.f, -e);
         const h2 f2h = {f, f};
-        if (t < 128 && lane < 4 * NB) {  // [g][block] -> [block][pair of keys]
+        if (wave < 2 && lane < 4 * NB) {  // [g][block] -> [block][pair of keys]
             const uint32_t kg = lane / NB, b = lane % NB;
-            s.ks[b][8 * rec + 2 * kg] = r.ks[0];
-            s.ks[b][8 * rec + 2 * kg + 1] = r.ks[1];
+            *(u2*)&s.ks[b][8 * rec + 2 * kg] = u2{r.ks[0], r.ks[1]};
         }
 #pragma unroll
         for (int i = 0; i < ITEMS; ++i) {
-            const int c = (int)__builtin_amdgcn_readfirstlane(t >> 7) + 2 * i;
-            if (c >= PAIRS) break;
+            const int b = (int)(wave >> 1) + WAVES / 2 * i;
+            if (NB % (WAVES / 2) != 0 && b >= NB) break;
+            h2 p[4];
+            if constexpr (KB == 8) {
+                vx_unpack8(r.k[i][0], p[0], p[1]);
+                vx_unpack8(r.k[i][1], p[2], p[3]);
+            } else {
+                const uint32_t w = r.k[i][0];
+                p[0] = vx_unpack4(w), p[1] = vx_unpack4_high(w), p[2] = vx_unpack4(w >> 8), p[3] = vx_unpack4_high(w >> 8);
+            }
+            s.k[(b * 4 + g) * 32 + 16 * rec + m] = h8{p[0].x, p[0].y, p[1].x, p[1].y, p[2].x, p[2].y, p[3].x, p[3].y};
+            const uint32_t d0 = r.d[i][0], d1 = r.d[i][1];
+            const h2 r0 = __builtin_bit_cast(h2, d0) * f2h, r1 = __builtin_bit_cast(h2, d1) * f2h;
 #pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                const int b = 2 * c + u;
-                if (NB % 2 != 0 && b >= NB) break;
-                h2 p[4];
-                if constexpr (KB == 8) {
-                    vx_unpack8(r.k[i][2 * u], p[0], p[1]);
-                    vx_unpack8(r.k[i][2 * u + 1], p[2], p[3]);
+            for (int v = 0; v < 2; ++v) {
+                h2 x0, x1;
+                if constexpr (VB == 8) {
+                    vx_unpack8(r.v[i][v], x0, x1);
                 } else {
-                    const uint32_t w = r.k[i][u];
-                    p[0] = vx_unpack4(w), p[1] = vx_unpack4_high(w), p[2] = vx_unpack4(w >> 8), p[3] = vx_unpack4_high(w >> 8);
+                    const uint32_t w = r.v[i][0];
+                    x0 = v ? vx_unpack4_high(w) : vx_unpack4(w);
+                    x1 = v ? vx_unpack4_high(w >> 8) : vx_unpack4(w >> 8);
                 }
-                s.k[(b * 4 + g) * 32 + 16 * rec + m] = h8{p[0].x, p[0].y, p[1].x, p[1].y, p[2].x, p[2].y, p[3].x, p[3].y};
-                // (b is known to the compiler up to c: select the block's scales without an array index)
-                uint32_t d0 = 0, d1 = 0;
-#pragma unroll
-                for (int q = 0; q < NB; ++q)
-                    if (q == b) d0 = vs[q][0], d1 = vs[q][1];
-                const h2 r0 = __builtin_bit_cast(h2, d0) * f2h, r1 = __builtin_bit_cast(h2, d1) * f2h;
-#pragma unroll
-                for (int v = 0; v < 2; ++v) {
-                    h2 x0, x1;
-                    if constexpr (VB == 8) {
-                        vx_unpack8(r.v[i][2 * u + v], x0, x1);
-                    } else {
-                        const uint32_t w = r.v[i][u];
-                        x0 = v ? vx_unpack4_high(w) : vx_unpack4(w);
-                        x1 = v ? vx_unpack4_high(w >> 8) : vx_unpack4(w >> 8);
-                    }
-                    const h2 a0 = x0 * r0, a1 = x1 * r1;
-                    const h2 b0 = __builtin_elementwise_fma(x0, r0, -a0), b1 = __builtin_elementwise_fma(x1, r1, -a1);
-                    // row 16 v + m of the block's 32 (dim 2 m + v), half g % 2, keys' place g / 2
-                    h4* at = (h4*)&s.v[((b * 2 + rec) * 2) * 64 + (g & 1) * 32 + 16 * v + m] + (g >> 1);
-                    at[0] = h4{a0.x, a0.y, a1.x, a1.y};
-                    at[2 * 64] = h4{b0.x, b0.y, b1.x, b1.y};
-                }
+                const h2 a0 = x0 * r0, a1 = x1 * r1;
+                const h2 b0 = __builtin_elementwise_fma(x0, r0, -a0), b1 = __builtin_elementwise_fma(x1, r1, -a1);
+                // row 16 v + m of the block's 32 (dim 2 m + v), half g % 2, keys' place g / 2
+                h4* at = (h4*)&s.v[((b * 2 + rec) * 2) * 64 + (g & 1) * 32 + 16 * v + m] + (g >> 1);
+                at[0] = h4{a0.x, a0.y, a1.x, a1.y};
+                at[2 * 64] = h4{b0.x, b0.y, b1.x, b1.y};
             }
         }
     }
 
     static __device__ __forceinline__ void run(const vx_attn_args& a) {
         __shared__ tile sh[2];
-        __shared__ int sh_at[4][32];
+        __shared__ int sh_at[WAVES][32];
         const uint32_t lane = threadIdx.x & 63, n = lane & 31, h = lane >> 5;
         const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
         // workgroup -> (row block, split, sequence, head): heads fastest (a head's
@@ -211,10 +215,11 @@ struct vx_tile {
         int wg_lo, wg_hi;
         {
             int* b = (int*)&sh[0];
-            if (lane == 0) b[wave] = lo, b[4 + wave] = hi;
+            if (lane == 0) b[wave] = lo, b[WAVES + wave] = hi;
             __syncthreads();
-            wg_lo = min(min(b[0], b[1]), min(b[2], b[3]));
-            wg_hi = max(max(b[4], b[5]), max(b[6], b[7]));
+            wg_lo = b[0], wg_hi = b[WAVES];
+#pragma unroll
+            for (int i = 1; i < WAVES; ++i) wg_lo = min(wg_lo, b[i]), wg_hi = max(wg_hi, b[WAVES + i]);
             __syncthreads();
         }
         wg_lo = __builtin_amdgcn_readfirstlane(wg_lo);
@@ -274,14 +279,19 @@ struct vx_tile {
         const vx_scalar_i32 table = (vx_scalar_i32)(a.table + (uint64_t)s * a.table_stride);
         const uint8_t* base = a.c.base + (uint64_t)(kvh << (a.c.page_shift - 4)) * REC;
         const float capl = a.cap * VX_LOG2E;
+        float poly[5];
+#pragma unroll
+        for (int i = 0; i < 5; ++i) poly[i] = capl * VX_TANH[i];
 
         if (kbeg < kend) {
             raw r;
             load(a, table, base, kbeg, last, r);
-            store(r, sh[0]);
+            store(r, sh[0], kbeg, last);
         }
         __syncthreads();
         uint32_t buf = 0;
+        float minus = -1.f;
+        asm("" : "+s"(minus));
         for (int k0 = kbeg; k0 < kend; k0 += 32, buf ^= 1) {
             const tile& t = sh[buf];
             raw r;
@@ -320,7 +330,14 @@ struct vx_tile {
                         for (int i = 0; i < 16; ++i) x[i] = capl * vx_tanh(x[i]);
                     } else {
 #pragma unroll
-                        for (int i = 0; i < 16; ++i) x[i] = capl * vx_tanh_small(x[i]);
+                        for (int i = 0; i < 16; ++i) {  // vx_tanh_small times capl
+                            const float z = x[i] * x[i];
+                            float p = __builtin_fmaf(z, poly[4], poly[3]);
+                            p = __builtin_fmaf(z, p, poly[2]);
+                            p = __builtin_fmaf(z, p, poly[1]);
+                            p = __builtin_fmaf(z, p, poly[0]);
+                            x[i] *= __builtin_fmaf(z, p, capl);
+                        }
                     }
                 }
                 const bool whole = k0 >= lo_all && k0 + 32 <= hi_all && k0 + 32 <= tail;
@@ -380,7 +397,7 @@ struct vx_tile {
 #pragma unroll
                     for (int i = 0; i < 4; i += 2) {
                         h2 u, v;
-                        vx_two_terms(x[4 * j + i], x[4 * j + i + 1], u, v);
+                        vx_two_terms(x[4 * j + i], x[4 * j + i + 1], minus, u, v);
                         const int k = 4 * (j % 2) + i;
                         ph[j / 2][k] = u.x, ph[j / 2][k + 1] = u.y, pl[j / 2][k] = v.x, pl[j / 2][k + 1] = v.y;
                     }
@@ -406,7 +423,7 @@ struct vx_tile {
                     }
                 }
             }
-            if (more) store(r, sh[buf ^ 1]);
+            if (more) store(r, sh[buf ^ 1], k0 + 32, last);
             __syncthreads();
         }
 

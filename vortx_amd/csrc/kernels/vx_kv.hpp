@@ -45,6 +45,12 @@ __device__ __forceinline__ void vx_two_terms(float a, float b, h2& hi, h2& lo) {
     lo = __builtin_convertvector((f2{a - (float)hi.x, b - (float)hi.y}), h2);
 }
 
+// The same with -1.0 in a register: a multiply-add takes hi as it is (v_fma_mix).
+__device__ __forceinline__ void vx_two_terms(float a, float b, float minus, h2& hi, h2& lo) {
+    hi = __builtin_convertvector((f2{a, b}), h2);
+    lo = __builtin_convertvector((f2{__builtin_fmaf((float)hi.x, minus, a), __builtin_fmaf((float)hi.y, minus, b)}), h2);
+}
+
 // w0 * d.x and w1 * d.y as two f16 terms each, lo from the exact product. `zero`
 // is -0.0 in a register: a product written as a multiply-add takes the f16
 // operand as it is (v_fma_mix), a multiplication would convert it first.

@@ -49,7 +49,8 @@ static int kernel_of(const vx_kv_cache* c, const int* d) {
 }
 #define VX_DIMS(f) {K_vx_##f##_d64_k8v8, K_vx_##f##_d96_k8v8, K_vx_##f##_d128_k8v8, K_vx_##f##_d256_k8v8}
 static const int kWrite[4] = VX_DIMS(kv_write), kRead[4] = VX_DIMS(kv_read), kRows16[4] = VX_DIMS(attn_rows16),
-                 kEven16[4] = VX_DIMS(attn_even16), kTile[4] = VX_DIMS(attn_tile);
+                 kEven16[4] = VX_DIMS(attn_even16), kTile4[4] = VX_DIMS(attn_tile4),
+                 kTile8[3] = {K_vx_attn_tile8_d64_k8v8, K_vx_attn_tile8_d96_k8v8, K_vx_attn_tile8_d128_k8v8};
 constexpr uint32_t VX_EVEN_ROWS = 16;  // query rows of a workgroup of kEven16
 #undef VX_DIMS
 
@@ -116,6 +117,7 @@ static int run_rows(vx_ctx ctx, vx_stream stream, const vx_kv_cache* cache, cons
 
 struct AttnPlan {
     const int* kernel;
+    uint32_t block = 256;
     bool even;
     uint32_t row_blocks, splits, chunk;
     uint32_t grid;
@@ -128,7 +130,7 @@ static int plan_attention(int num_cus, const vx_kv_cache* c, const vx_attn_batch
     const uint64_t group = q_heads / c->heads, queries = b->max_queries, units = (uint64_t)b->seqs * c->heads;
     uint64_t span = std::min<uint64_t>(b->max_len, (uint64_t)b->table_cols * c->page_tokens);
     if (o && o->window) span = std::min<uint64_t>(span, 2ull * o->window + queries + 64);
-    const uint64_t places = (c->dim > 128 ? 1ull : 2ull) * (uint64_t)num_cus;  // workgroups that the card holds
+    uint64_t places = (c->dim > 128 ? 1ull : 2ull) * (uint64_t)num_cus;  // workgroups that the card holds
     *p = AttnPlan{};
     if (queries * group <= VX_EVEN_ROWS && ws) {
         p->kernel = kEven16;
@@ -141,8 +143,11 @@ static int plan_attention(int num_cus, const vx_kv_cache* c, const vx_attn_batch
         if (units * queries * group >= (1ull << 24)) return fail(VX_ERR_UNSUPPORTED, "attention: too many rows (split the batch)");
         return VX_OK;
     }
-    p->kernel = kTile;
-    const uint64_t rb = (queries * group + 127) / 128, wgs = rb * units;
+    const bool wide = queries * group > 128 && c->dim <= 128;
+    p->kernel = wide ? kTile8 : kTile4;
+    p->block = wide ? 512 : 256;
+    const uint64_t tile = wide ? 256 : 128, rb = (queries * group + tile - 1) / tile, wgs = rb * units;
+    if (wide) places /= 2;
     uint64_t splits = 1;
     if (ws && wgs < places) splits = std::max<uint64_t>(1, std::min<uint64_t>(places / wgs, (span + 127) / 128));
     const uint64_t chunk = std::max<uint64_t>(32, ((span + splits - 1) / splits + 31) / 32 * 32);
@@ -228,7 +233,7 @@ static int run_attention(vx_ctx ctx, vx_stream stream, const vx_mview* out, cons
     a.info = p.even ? (uint32_t*)ws : nullptr;
     a.part_o = (float*)((char*)ws + p.info);
     a.part_ml = a.part_o + p.rows * cache->dim;
-    if ((s = launch_struct(ctx, kernel_of(cache, p.kernel), p.grid, 256, stream, &a))) return s;
+    if ((s = launch_struct(ctx, kernel_of(cache, p.kernel), p.grid, p.block, stream, &a))) return s;
     if (p.splits > 1) {
         const uint64_t jobs = (uint64_t)batch->max_queries * a.group * batch->seqs * cache->heads;
         return launch_struct(ctx, K_vx_attn_join, (uint32_t)(p.splits > 8 ? jobs : (jobs + 3) / 4), 256, stream, &a);
