@@ -10,7 +10,7 @@ from vortx_amd import _ffi
 @pytest.mark.parametrize("k,v,dim,per", [(vx.VX_Q8_0, vx.VX_Q8_0, 128, 272), (vx.VX_Q8_0, vx.VX_Q4_0, 64, 104),
                                          (vx.VX_Q4_0, vx.VX_Q4_0, 96, 108), (vx.VX_Q4_0, vx.VX_Q8_0, 256, 416)])
 def test_cache_size(k, v, dim, per):
-    assert vx.kv_cache_size(3, 32, 5, dim, k, v) == 3 * 32 * 5 * per
+    assert vx.kv_cache_size(3, 32, 5, dim, k, v) == 3 * 32 * 5 * (per + 2)
     assert vx.kv_cache_size(0, 32, 5, dim, k, v) == 0
 
 

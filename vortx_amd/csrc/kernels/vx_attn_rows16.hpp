@@ -18,7 +18,8 @@ template <int NB, int KB, int VB>
 struct vx_rows16 {
     using PK = vx_kv_part<NB, KB>;
     using PV = vx_kv_part<NB, VB>;
-    static constexpr uint32_t REC = PK::BYTES + PV::BYTES;
+    using R = vx_kv_rec<NB, KB, VB>;
+    static constexpr uint32_t REC = R::BYTES;
     static constexpr int KW = NB * KB / 4, VW = NB * VB / 4;
 
     struct raw_k {
@@ -28,6 +29,7 @@ struct vx_rows16 {
     struct raw_v {
         uint32_t w[2][VW];
         uint32_t s[2][NB][2];
+        uint32_t e[2];  // sizes, a byte a key
     };
 
     // the record of the 16 keys from key on; past the end the last one
@@ -62,6 +64,7 @@ struct vx_rows16 {
         for (int t = 0; t < 2; ++t) {
             vx_kv_load<NB, VB>(at[t] + PK::BYTES, lane, v.w[t]);
             load_scales(at[t] + PK::BYTES + PV::VALS, g, v.s[t]);
+            v.e[t] = ((const uint32_t*)(at[t] + R::V_SIZES))[g];
         }
     }
 
@@ -227,25 +230,30 @@ struct vx_rows16 {
                         // may be anything, counts nowhere
 #pragma unroll
                         for (int b = 0; b < NB; ++b) rv.s[t][b][i >> 1] &= v | (i & 1 ? 0x0000FFFFu : 0xFFFF0000u);
+                        rv.e[t] &= v | ~(0xFFu << (8 * i));
                     }
             }
             // running maximum of score + exponent of V's scales
             float top = fmaxf(fmaxf(fmaxf(x[0][0], x[0][1]), fmaxf(x[0][2], x[0][3])), fmaxf(fmaxf(x[1][0], x[1][1]), fmaxf(x[1][2], x[1][3])));
             {
-                typedef uint16_t us2 __attribute__((ext_vector_type(2)));
-                us2 big = {0, 0};
+                uint32_t e = 0;
 #pragma unroll
                 for (int t = 0; t < 2; ++t)
 #pragma unroll
-                    for (int b = 0; b < NB; ++b)
+                    for (int i = 0; i < 4; ++i) e = max(e, rv.e[t] >> (8 * i) & 255u);
+                if (__any(e == 255u)) {  // a scale that is not finite: the largest of the others
+                    e = 0;
 #pragma unroll
-                        for (int i = 0; i < 2; ++i) {
-                            uint32_t d = rv.s[t][b][i];
-                            if (VB == 4) d &= 0x7FFF7FFFu;  // (8 bits: never negative)
-                            big = __builtin_elementwise_max(big, __builtin_bit_cast(us2, d));
-                        }
-                const int e = (int)(max(big.x, big.y) >> 10) - 15;
-                top = vx_max_rows4(top + (float)(e - 13));  // P times scale below 2^14
+                    for (int t = 0; t < 2; ++t)
+#pragma unroll
+                        for (int b = 0; b < NB; ++b)
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) {
+                                const uint32_t d = vx_kv_size(rv.s[t][b][i >> 1] >> (16 * (i & 1)));
+                                e = max(e, d == 255u ? 0u : d);
+                            }
+                }
+                top = vx_max_rows4(top + (float)((int)e - 29));  // P times scale below 2^14
             }
             const float Mn = fmaxf(M, top), Mr = Mn == -__builtin_inff() ? 0.f : Mn;
             if (__any(Mn != M)) {

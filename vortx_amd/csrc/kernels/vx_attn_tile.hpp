@@ -4,13 +4,15 @@
 // to a wave, and goes over their keys 32 at a time. The waves decode a tile of
 // keys once into LDS, as operands of the 32 x 32 x 16 matrix instructions, while
 // the tile before is computed from the other buffer:
-//   K   the whole numbers, exact in f16; a block's scale is applied to its
-//       32-dim product in f32 (S^T = K q^T: rows are keys, columns queries);
-//   V   scale x number, 19 bits, as two f16 terms whose sum is exact: hi rounds
-//       the product, lo = fma(number, scale, -hi). The scales of each four keys
-//       are first brought to [1, 2) by a power of two 2^-e, and 2^e goes to the
-//       weights: w = exp2(score + e - M), so V of any magnitude fills f16's
-//       range, and the weights' sum takes w 2^-e.
+// each value is scale x number, 19 bits, held as two f16 terms whose sum is
+// exact: hi rounds the product, lo = fma(number, scale, -hi). The scales of each
+// four keys are first brought below 2 by a power of two, which K's scores take
+// back as a factor, and V's weights: w = exp2(score + e - M), so V of any
+// magnitude fills f16's range, and the weights' sum takes w 2^-e.
+// (With K as whole numbers, exact in one term, and its scales on the 32-dim
+// products, a tile had 8 matrix instructions fewer and 64 multiply-adds and 32
+// registers a wave more: 430 us where this takes 415, 4096 causal tokens of
+// 32 heads of 128.)
 // q is two f16 terms (22 bits, a power of two per row), and so are the weights;
 // of the product's terms the one of two lows is left out (2^-22). M follows the
 // maximum of score + e by steps of more than 2^8 only: the weights have f16's
@@ -28,22 +30,26 @@ template <int NB, int KB, int VB, int WAVES>
 struct vx_tile {
     using PK = vx_kv_part<NB, KB>;
     using PV = vx_kv_part<NB, VB>;
-    static constexpr uint32_t REC = PK::BYTES + PV::BYTES;
+    using R = vx_kv_rec<NB, KB, VB>;
+    static constexpr uint32_t REC = R::BYTES;
     static constexpr uint32_t THREADS = 64 * WAVES, ROWS = 32 * WAVES;
     static constexpr int ITEMS = (128 * NB + THREADS - 1) / THREADS;  // a thread's pieces of a tile: one lane's bytes of a block
 
+    // tiles between barriers: two where LDS holds them, so that the waves of a
+    // SIMD drift apart and one's matrix instructions run beside the other's softmax
+    static constexpr int PERIOD = WAVES == 8 || NB <= 2 ? 2 : 1;
+
     struct tile {
-        h8 k[NB * 4 * 32];      // [block][8-dim group][key]
+        h8 k[NB * 2 * 2 * 64];  // [block][16 dims][hi, lo][half, key]
         h8 v[NB * 2 * 2 * 64];  // [block][16 keys][hi, lo][half, dim]
-        uint32_t ks[NB][16];    // K scales, f16 pairs of keys
-        float e[8];             // exponents of four keys' V scales
+        f2 e[8];                // of four keys: 2^exponent of K's scales, exponent of V's
         uint32_t bad[8];        // their V scales that are not finite, bit 4 block + key
     };
 
     struct raw {  // a thread's pieces as loaded
         uint32_t k[ITEMS][KB / 4], v[ITEMS][VB / 4], d[ITEMS][2];
-        uint32_t vs[NB][2];  // V scales of its four keys
-        uint32_t ks[2];
+        uint16_t kd[ITEMS];
+        uint32_t ke, e;  // sizes: of K for the four keys of key m, of V for keys 4 g
     };
 
     template <int BITS>
@@ -57,12 +63,16 @@ struct vx_tile {
         }
     }
 
-    // records of the 32 keys from k0 on; past the end the last one
-    static __device__ __forceinline__ void load(const vx_attn_args& a, vx_scalar_i32 table, const uint8_t* base, int k0, int last, raw& r) {
-        const uint32_t t = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(t >> 6), rec = wave & 1, lane = t & 63, g = lane >> 4;
-        const int key = min(k0 + 16 * (int)rec, last);
+    // the record of the 16 keys from key on; past the end the last one
+    static __device__ __forceinline__ const uint8_t* record(const vx_attn_args& a, vx_scalar_i32 table, const uint8_t* base, int key, int last) {
+        key = min(key, last);
         const uint32_t page = min((uint32_t)table[(uint32_t)key >> a.c.page_shift], a.c.pages - 1u);
-        const uint8_t* p = base + page * a.c.page_bytes + (((uint32_t)key & ((1u << a.c.page_shift) - 1u)) >> 4) * REC;
+        return base + page * a.c.page_bytes + (((uint32_t)key & ((1u << a.c.page_shift) - 1u)) >> 4) * REC;
+    }
+
+    static __device__ __forceinline__ void load(const vx_attn_args& a, vx_scalar_i32 table, const uint8_t* base, int k0, int last, raw& r) {
+        const uint32_t t = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(t >> 6), rec = wave & 1, lane = t & 63, m = lane & 15, g = lane >> 4;
+        const uint8_t* p = record(a, table, base, k0 + 16 * (int)rec, last);
         const uint8_t* sc = p + PK::BYTES + PV::VALS + g * (8 * NB);
 #pragma unroll
         for (int i = 0; i < ITEMS; ++i) {
@@ -72,38 +82,20 @@ struct vx_tile {
                 load_block<VB>(p + PK::BYTES, b, lane, r.v[i]);
                 const u2 d = *(const u2*)(sc + 8 * b);
                 r.d[i][0] = d.x, r.d[i][1] = d.y;
+                r.kd[i] = *(const uint16_t*)(p + PK::VALS + ((m >> 2) * NB + b) * 8 + (m & 3) * 2);
             }
         }
-#pragma unroll
-        for (int b = 0; b < NB; ++b) {
-            const u2 v = *(const u2*)(sc + 8 * b);
-            r.vs[b][0] = v.x, r.vs[b][1] = v.y;
-        }
-        // K's scales: lanes 0.. of waves 0 and 1, four keys of a block each
-        if (wave < 2 && lane < 4 * NB) {
-            const u2 v = *(const u2*)(p + PK::VALS + lane * 8);
-            r.ks[0] = v.x, r.ks[1] = v.y;
-        }
+        r.ke = ((const uint32_t*)(p + R::K_SIZES))[m >> 2];
+        r.e = ((const uint32_t*)(p + R::V_SIZES))[g];
     }
 
     // decodes a thread's pieces into the tile of the keys from k0 on
-    static __device__ __forceinline__ void store(raw& r, tile& s, int k0, int last) {
-        typedef uint16_t us2 __attribute__((ext_vector_type(2)));
+    static __device__ __forceinline__ void store(const vx_attn_args& a, vx_scalar_i32 table, const uint8_t* base, raw& r, tile& s, int k0, int last) {
         const uint32_t t = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(t >> 6), rec = wave & 1, lane = t & 63, m = lane & 15, g = lane >> 4;
         uint32_t bad = 0;
-        auto largest = [&] {
-            us2 big = {0, 0};
-#pragma unroll
-            for (int b = 0; b < NB; ++b)
-#pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    const uint32_t d = VB == 4 ? r.vs[b][i] & 0x7FFF7FFFu : r.vs[b][i];  // (8 bits: never negative)
-                    big = __builtin_elementwise_max(big, __builtin_bit_cast(us2, d));
-                }
-            return (uint32_t)max(big.x, big.y);
-        };
-        uint32_t big = largest();
-        if (k0 + 32 > last + 1 || __any(big >= 0x7C00u)) {
+        auto largest = [&](uint32_t e) { return max(max(e & 255u, e >> 8 & 255u), max(e >> 16 & 255u, e >> 24)); };
+        uint32_t size = largest(r.e), ksize = largest(r.ke);
+        if (k0 + 32 > last + 1 || __any(max(size, ksize) == 255u)) {
             // scales of keys that do not exist, which may be anything: 0; those that are not finite: 0, and noted
             const int valid = last + 1 - (k0 + 16 * (int)rec + 4 * (int)g);
             auto fix = [&](uint32_t d, int i) {
@@ -112,31 +104,36 @@ struct vx_tile {
                 return d;
             };
 #pragma unroll
-            for (int b = 0; b < NB; ++b)
-#pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    const uint32_t d = r.vs[b][i];
-                    if (valid > 2 * i && (d & 0x7FFFu) >= 0x7C00u) bad |= 1u << (4 * b + 2 * i);
-                    if (valid > 2 * i + 1 && (d >> 16 & 0x7FFFu) >= 0x7C00u) bad |= 2u << (4 * b + 2 * i);
-                    r.vs[b][i] = fix(d, i);
-                }
-#pragma unroll
             for (int n = 0; n < ITEMS; ++n)
 #pragma unroll
                 for (int i = 0; i < 2; ++i) r.d[n][i] = fix(r.d[n][i], i);
-            big = largest();
+            const uint32_t* sc = (const uint32_t*)(record(a, table, base, k0 + 16 * (int)rec, last) + PK::BYTES + PV::VALS + g * (8 * NB));
+            uint32_t e[4] = {};
+#pragma unroll 1
+            for (int b = 0; b < NB; ++b)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const uint32_t v = vx_kv_size(sc[2 * b + (i >> 1)] >> (16 * (i & 1)));
+                    if (valid <= i) continue;
+                    if (v == 255u) bad |= 1u << (4 * b + i);
+                    else e[i] = max(e[i], v);
+                }
+            size = max(max(e[0], e[1]), max(e[2], e[3]));
+            // K's keys that do not exist or are not finite: the others' exponent
+            const int kvalid = last + 1 - (k0 + 16 * (int)rec + 4 * (int)(m >> 2));
+            ksize = 0;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const uint32_t v = r.ke >> (8 * i) & 255u;
+                if (i < kvalid && v != 255u) ksize = max(ksize, v);
+            }
         }
-        const int e = (int)(big >> 10) - 15;
-        if (wave < 2 && m == 0) {
-            s.e[rec * 4 + g] = (float)e;
-            s.bad[rec * 4 + g] = bad;
-        }
-        const _Float16 f = (_Float16)__builtin_ldexpf(1.f, -e);
+        const int e = max((int)size - 16, -15);  // (of no key: -16)
+        const int ek = max((int)ksize - 16, -15);
+        if (wave < 2 && m == 4 * g) s.e[rec * 4 + g] = f2{__builtin_ldexpf(1.f, ek), (float)e};
+        if (wave < 2 && m == 0) s.bad[rec * 4 + g] = bad;
+        const _Float16 f = (_Float16)__builtin_ldexpf(1.f, -e), fk = (_Float16)__builtin_ldexpf(1.f, -ek);
         const h2 f2h = {f, f};
-        if (wave < 2 && lane < 4 * NB) {  // [g][block] -> [block][pair of keys]
-            const uint32_t kg = lane / NB, b = lane % NB;
-            *(u2*)&s.ks[b][8 * rec + 2 * kg] = u2{r.ks[0], r.ks[1]};
-        }
 #pragma unroll
         for (int i = 0; i < ITEMS; ++i) {
             const int b = (int)(wave >> 1) + WAVES / 2 * i;
@@ -149,7 +146,18 @@ struct vx_tile {
                 const uint32_t w = r.k[i][0];
                 p[0] = vx_unpack4(w), p[1] = vx_unpack4_high(w), p[2] = vx_unpack4(w >> 8), p[3] = vx_unpack4_high(w >> 8);
             }
-            s.k[(b * 4 + g) * 32 + 16 * rec + m] = h8{p[0].x, p[0].y, p[1].x, p[1].y, p[2].x, p[2].y, p[3].x, p[3].y};
+            const _Float16 rk = __builtin_bit_cast(_Float16, r.kd[i]) * fk;
+            const h2 rk2 = {rk, rk};
+            h2 kh[4], kl[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                kh[j] = p[j] * rk2;
+                kl[j] = __builtin_elementwise_fma(p[j], rk2, -kh[j]);
+            }
+            // dims 16 (g / 2) + 8 (g % 2) ..: step g / 2, half g % 2
+            h8* kat = &s.k[((b * 2 + (g >> 1)) * 2) * 64 + (g & 1) * 32 + 16 * rec + m];
+            kat[0] = h8{kh[0].x, kh[0].y, kh[1].x, kh[1].y, kh[2].x, kh[2].y, kh[3].x, kh[3].y};
+            kat[64] = h8{kl[0].x, kl[0].y, kl[1].x, kl[1].y, kl[2].x, kl[2].y, kl[3].x, kl[3].y};
             const uint32_t d0 = r.d[i][0], d1 = r.d[i][1];
             const h2 r0 = __builtin_bit_cast(h2, d0) * f2h, r1 = __builtin_bit_cast(h2, d1) * f2h;
 #pragma unroll
@@ -173,7 +181,7 @@ struct vx_tile {
     }
 
     static __device__ __forceinline__ void run(const vx_attn_args& a) {
-        __shared__ tile sh[2];
+        __shared__ tile sh[2 * PERIOD];
         __shared__ int sh_at[WAVES][32];
         const uint32_t lane = threadIdx.x & 63, n = lane & 31, h = lane >> 5;
         const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -281,46 +289,59 @@ struct vx_tile {
         const float capl = a.cap * VX_LOG2E;
         float poly[5];
 #pragma unroll
-        for (int i = 0; i < 5; ++i) poly[i] = capl * VX_TANH[i];
+        for (int i = 0; i < 5; ++i) poly[i] = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(capl * VX_TANH[i])));
 
-        if (kbeg < kend) {
-            raw r;
-            load(a, table, base, kbeg, last, r);
-            store(r, sh[0], kbeg, last);
-        }
+#pragma unroll
+        for (int i = 0; i < PERIOD; ++i)
+            if (kbeg + 32 * i < kend) {
+                raw r;
+                load(a, table, base, kbeg + 32 * i, last, r);
+                store(a, table, base, r, sh[i], kbeg + 32 * i, last);
+            }
         __syncthreads();
         uint32_t buf = 0;
         float minus = -1.f;
         asm("" : "+s"(minus));
-        for (int k0 = kbeg; k0 < kend; k0 += 32, buf ^= 1) {
-            const tile& t = sh[buf];
+        for (int k0 = kbeg; k0 < kend; k0 += 32, ++buf) {
+            const tile& t = sh[buf % (2 * PERIOD)];
             raw r;
-            const bool more = k0 + 32 < kend;
-            if (more) load(a, table, base, k0 + 32, last, r);
+            const int kn = k0 + 32 * PERIOD;  // the tile that this one's turn decodes
+            const bool more = kn < kend;
+            if (more) load(a, table, base, kn, last, r);
             if (k0 < hi && k0 + 32 > lo) {
+                __builtin_amdgcn_s_setprio(1);
                 // scores: lane (n, h), register i: query n, key 8 (i / 4) + 4 h + i % 4
+                // Operands are read from LDS two steps before the products that take
+                // them; the barriers keep the compiler from moving the reads back
+                // (vector and scalar arithmetic may cross them).
                 f16v x = {};
+                h8 kf[3][2];
+                auto kread = [&](int u) {
+                    kf[u % 3][0] = t.k[2 * u * 64 + lane];
+                    kf[u % 3][1] = t.k[(2 * u + 1) * 64 + lane];
+                };
+                kread(0);
+                kread(1);
 #pragma unroll
-                for (int b = 0; b < NB; ++b) {
-                    f16v acc = {};
-#pragma unroll
-                    for (int j = 0; j < 2; ++j) {
-                        const h8 kf = t.k[(b * 4 + 2 * j + h) * 32 + n];
-                        acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, qh[b][j], acc, 0, 0, 0);
-                        acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, ql[b][j], acc, 0, 0, 0);
-                    }
-#pragma unroll
-                    for (int i = 0; i < 16; i += 4) {
-                        const u2 sc = *(const u2*)&t.ks[b][i + 2 * h];
-                        const uint32_t s0 = sc.x, s1 = sc.y;
-                        const h2 d0 = __builtin_bit_cast(h2, s0), d1 = __builtin_bit_cast(h2, s1);
-                        x[i] = __builtin_fmaf(acc[i], (float)d0.x, x[i]);
-                        x[i + 1] = __builtin_fmaf(acc[i + 1], (float)d0.y, x[i + 1]);
-                        x[i + 2] = __builtin_fmaf(acc[i + 2], (float)d1.x, x[i + 2]);
-                        x[i + 3] = __builtin_fmaf(acc[i + 3], (float)d1.y, x[i + 3]);
-                    }
+                for (int u = 0; u < 2 * NB; ++u) {
+                    const int b = u / 2, j = u % 2;
+                    if (u + 2 < 2 * NB) kread(u + 2);
+                    __builtin_amdgcn_sched_barrier(6);
+                    x = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[u % 3][0], qh[b][j], x, 0, 0, 0);
+                    x = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[u % 3][0], ql[b][j], x, 0, 0, 0);
+                    x = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[u % 3][1], qh[b][j], x, 0, 0, 0);
+                    __builtin_amdgcn_sched_barrier(6);
                 }
-                x *= fq;
+                __builtin_amdgcn_s_setprio(0);
+                float e[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const f2 ke = t.e[4 * (j / 2) + 2 * (j % 2) + (int)h];
+                    const float f = fq * ke.x;
+                    e[j] = ke.y;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) x[4 * j + i] *= f;
+                }
                 if (a.cap > 0.f) {
                     float big = 0.f;
 #pragma unroll
@@ -342,30 +363,31 @@ struct vx_tile {
                 }
                 const bool whole = k0 >= lo_all && k0 + 32 <= hi_all && k0 + 32 <= tail;
                 uint32_t see = 0xFFFFFFFFu;  // bit k: key k0 + 4 h + k
-                if (whole) {
-                    if (a.slopes) {
+                if (!whole) see = vx_attn_sees(a, q, w, tail, k0, sh_at[wave]) >> (4 * h);
+                if (a.slopes) {
+                    if (a.tree && k0 + 32 > tail) {
+#pragma unroll
+                        for (int i = 0; i < 16; ++i)
+                            x[i] = __builtin_fmaf(-w.slope, fabsf((float)(w.pos - sh_at[wave][8 * (i / 4) + i % 4 + 4 * h])), x[i]);
+                    } else {
                         const float d0 = (float)(w.pos - (k0 + 4 * (int)h));
 #pragma unroll
                         for (int i = 0; i < 16; ++i) x[i] = __builtin_fmaf(-w.slope, fabsf(d0 - (float)(8 * (i / 4) + i % 4)), x[i]);
                     }
-                } else {
-                    see = vx_attn_sees(a, q, w, tail, k0, sh_at[wave]) >> (4 * h);
-                    const bool drafts = a.tree && k0 + 32 > tail;
+                }
+                if (!whole) {
 #pragma unroll
                     for (int i = 0; i < 16; ++i) {
-                        const int key = 8 * (i / 4) + i % 4;
-                        if (a.slopes)
-                            x[i] = __builtin_fmaf(-w.slope, fabsf((float)(w.pos - (drafts ? sh_at[wave][key + 4 * h] : k0 + key + 4 * (int)h))), x[i]);
-                        x[i] = see >> key & 1u ? x[i] : -__builtin_inff();
+                        const uint32_t v = (uint32_t)__builtin_amdgcn_sbfe((int)see, 8 * (i / 4) + i % 4, 1);
+                        x[i] = __uint_as_float((v & __float_as_uint(x[i])) | (~v & 0xFF800000u));
                     }
                 }
                 // running maximum of score + e: four keys at a time
-                float e[4], top = -__builtin_inff();
+                float top = -__builtin_inff();
                 uint32_t bad = 0;
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                     const int at = 4 * (j / 2) + 2 * (j % 2) + (int)h;
-                    e[j] = t.e[at];
                     bad |= t.bad[at];
                     top = fmaxf(top, fmaxf(fmaxf(x[4 * j], x[4 * j + 1]), fmaxf(x[4 * j + 2], x[4 * j + 3])) + e[j]);
                 }
@@ -402,15 +424,25 @@ struct vx_tile {
                         ph[j / 2][k] = u.x, ph[j / 2][k + 1] = u.y, pl[j / 2][k] = v.x, pl[j / 2][k + 1] = v.y;
                     }
                 }
+                __builtin_amdgcn_s_setprio(1);
+                h8 vf[3][2];
+                auto vread = [&](int u) {
+                    vf[u % 3][0] = t.v[2 * u * 64 + lane];
+                    vf[u % 3][1] = t.v[(2 * u + 1) * 64 + lane];
+                };
+                vread(0);
+                vread(1);
 #pragma unroll
-                for (int b = 0; b < NB; ++b)
-#pragma unroll
-                    for (int j = 0; j < 2; ++j) {
-                        const h8 vh = t.v[((b * 2 + j) * 2) * 64 + lane], vl = t.v[((b * 2 + j) * 2 + 1) * 64 + lane];
-                        o[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vh, ph[j], o[b], 0, 0, 0);
-                        o[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vh, pl[j], o[b], 0, 0, 0);
-                        o[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vl, ph[j], o[b], 0, 0, 0);
-                    }
+                for (int u = 0; u < 2 * NB; ++u) {
+                    const int b = u / 2, j = u % 2;
+                    if (u + 2 < 2 * NB) vread(u + 2);
+                    __builtin_amdgcn_sched_barrier(6);
+                    o[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf[u % 3][0], ph[j], o[b], 0, 0, 0);
+                    o[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf[u % 3][0], pl[j], o[b], 0, 0, 0);
+                    o[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf[u % 3][1], ph[j], o[b], 0, 0, 0);
+                    __builtin_amdgcn_sched_barrier(6);
+                }
+                __builtin_amdgcn_s_setprio(0);
                 if (__any(bad)) {
                     // values that are not finite, taken as zeros above: NaN for the rows that see their key
 #pragma unroll
@@ -423,8 +455,8 @@ struct vx_tile {
                     }
                 }
             }
-            if (more) store(r, sh[buf ^ 1], k0 + 32, last);
-            __syncthreads();
+            if (more) store(a, table, base, r, sh[(buf + PERIOD) % (2 * PERIOD)], kn, last);
+            if (PERIOD == 1 || buf % PERIOD == PERIOD - 1) __syncthreads();
         }
 
         // both halves' sums; registers 8 v + 4 p + i hold dims 32 b + 16 p + 8 h + 2 i + v

@@ -6,7 +6,7 @@
 // instructions take its parts, so that attention loads fragments without a
 // transpose and single tokens can still be written on their own:
 //
-//   K values | K scales | V values | V scales
+//   K values | K scales | V values | V scales | K sizes | V sizes
 //
 // Values of one kind: "lane" l = 16 g + m (m, g in 0..15, 0..3) owns the
 // values that lane l of a wave feeds to the matrix cores, LB = NB * 8 bytes
@@ -19,7 +19,9 @@
 //      8 bits: byte 4 v + j; 4 bits: nibble v of byte {0,2,1,3}[j]
 // Values are stored with 128 (8 bits) or 8 (4 bits) added. The orders inside
 // a dword are those that masks and byte permutes unpack to pairs of f16.
-// Scales: f16, [g][b][4]: of K for keys 4 g + j, of V the same.
+// Scales: f16, [g][b][4]: of K for keys 4 g + j, of V the same. Sizes: a byte a
+// key, 16 above the exponent of the largest of its scales (1 to 32; an f16
+// below its normal numbers counts as 2^-15), 255 where one is not finite.
 #pragma once
 #include <hip/hip_runtime.h>
 #include <stdint.h>
@@ -76,6 +78,16 @@ struct vx_kv_part {
         return p < FULL ? p * 1024 + l * 16 + o % 16 : FULL * 1024 + l * REST + o % 16;
     }
 };
+
+template <int NB, int KB, int VB>
+struct vx_kv_rec {
+    static constexpr uint32_t V = vx_kv_part<NB, KB>::BYTES, K_SIZES = V + vx_kv_part<NB, VB>::BYTES, V_SIZES = K_SIZES + 16,
+                              BYTES = V_SIZES + 16;
+};
+__device__ __forceinline__ uint32_t vx_kv_size(uint32_t d) {  // of a scale's bits
+    d &= 0x7FFFu;
+    return d >= 0x7C00u ? 255u : (d >> 10) + 1u;
+}
 
 __device__ __forceinline__ uint64_t vx_kv_page(const vx_kv_geom& c, uint32_t page, uint32_t head, uint32_t rec_bytes) {
     return page * c.page_bytes + (uint64_t)(head << (c.page_shift - 4)) * rec_bytes;

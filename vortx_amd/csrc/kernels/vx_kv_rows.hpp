@@ -73,7 +73,7 @@ __device__ __forceinline__ uint32_t vx_kv_codes(f4 x, float r) {
 }
 
 template <int NB, int BITS>
-__device__ __forceinline__ void vx_kv_put_k(uint8_t* rec, uint32_t key, uint32_t b, uint32_t u, f4 x) {
+__device__ __forceinline__ uint32_t vx_kv_put_k(uint8_t* rec, uint32_t key, uint32_t b, uint32_t u, f4 x) {
     using P = vx_kv_part<NB, BITS>;
     float r;
     const _Float16 d = vx_kv_scale<BITS>(x, r);
@@ -88,10 +88,11 @@ __device__ __forceinline__ void vx_kv_put_k(uint8_t* rec, uint32_t key, uint32_t
         if ((u & 1) == 0) *(uint32_t*)p = n | (o << 8);
     }
     if (u == 0) *(_Float16*)(rec + P::VALS + ((key >> 2) * NB + b) * 8 + (key & 3) * 2) = d;
+    return vx_kv_size(__builtin_bit_cast(uint16_t, d));
 }
 
 template <int NB, int BITS>
-__device__ __forceinline__ void vx_kv_put_v(uint8_t* rec, uint32_t key, uint32_t b, uint32_t u, f4 x) {
+__device__ __forceinline__ uint32_t vx_kv_put_v(uint8_t* rec, uint32_t key, uint32_t b, uint32_t u, f4 x) {
     using P = vx_kv_part<NB, BITS>;
     float r;
     const _Float16 d = vx_kv_scale<BITS>(x, r);
@@ -109,26 +110,39 @@ __device__ __forceinline__ void vx_kv_put_v(uint8_t* rec, uint32_t key, uint32_t
         }
     }
     if (u == 0) *(_Float16*)(rec + P::VALS + ((key >> 2) * NB + b) * 8 + (key & 3) * 2) = d;
+    return vx_kv_size(__builtin_bit_cast(uint16_t, d));
 }
 
 template <int NB, int KB, int VB>
 __device__ __forceinline__ void vx_kv_write_rows(const vx_kv_rows_args& a) {
-    constexpr uint32_t KBYTES = vx_kv_part<NB, KB>::BYTES, REC = KBYTES + vx_kv_part<NB, VB>::BYTES;
-    const uint64_t units = (uint64_t)a.tokens * a.c.heads * NB;
-    const uint32_t u = threadIdx.x & 7;
+    using R = vx_kv_rec<NB, KB, VB>;
+    constexpr uint32_t NP = NB == 3 ? 4 : NB;  // lanes of a row: 8 NP, a power of two
+    const uint64_t units = (uint64_t)a.tokens * a.c.heads * NP;
+    const uint32_t u = threadIdx.x & 7, b = (threadIdx.x >> 3) % NP;
     for (uint64_t n = (uint64_t)blockIdx.x * 32 + (threadIdx.x >> 3); n < units; n += (uint64_t)gridDim.x * 32) {
-        const uint32_t b = (uint32_t)(n % NB);
-        const uint64_t th = n / NB;
+        const uint64_t th = n / NP;
         const uint32_t t = (uint32_t)(th / a.c.heads), h = (uint32_t)(th - (uint64_t)t * a.c.heads);
         const uint32_t slot = (uint32_t)a.slots[t];
         const uint32_t page = slot >> a.c.page_shift, key = slot & ((1u << a.c.page_shift) - 1u);
-        if ((int32_t)slot < 0 || page >= a.c.pages) continue;  // (the same for the block's eight lanes)
-        uint8_t* rec = a.c.base + vx_kv_page(a.c, page, h, REC) + (uint64_t)(key >> 4) * REC;
-        const uint32_t d = 32 * b + 4 * u;
-        const f4 k = vx_kv_get4(a.k + (int64_t)t * a.ks[0] + (int64_t)h * a.ks[1], a.ks[2], d, a.vec);
-        const f4 v = vx_kv_get4(a.v + (int64_t)t * a.vs[0] + (int64_t)h * a.vs[1], a.vs[2], d, a.vec);
-        vx_kv_put_k<NB, KB>(rec, key & 15, b, u, k);
-        vx_kv_put_v<NB, VB>(rec + KBYTES, key & 15, b, u, v);
+        if ((int32_t)slot < 0 || page >= a.c.pages) continue;  // (the same for the row's lanes)
+        uint8_t* rec = a.c.base + vx_kv_page(a.c, page, h, R::BYTES) + (uint64_t)(key >> 4) * R::BYTES;
+        uint32_t size = 0;  // of K above, of V below
+        if (b < NB) {
+            const uint32_t d = 32 * b + 4 * u;
+            const f4 k = vx_kv_get4(a.k + (int64_t)t * a.ks[0] + (int64_t)h * a.ks[1], a.ks[2], d, a.vec);
+            const f4 v = vx_kv_get4(a.v + (int64_t)t * a.vs[0] + (int64_t)h * a.vs[1], a.vs[2], d, a.vec);
+            size = vx_kv_put_k<NB, KB>(rec, key & 15, b, u, k) << 16;
+            size |= vx_kv_put_v<NB, VB>(rec + R::V, key & 15, b, u, v);
+        }
+#pragma unroll
+        for (uint32_t o = 8; o < 8 * NP; o <<= 1) {
+            const uint32_t w = (uint32_t)__shfl_xor((int)size, (int)o);
+            size = max(size & 0xFFFF0000u, w & 0xFFFF0000u) | max(size & 255u, w & 255u);
+        }
+        if (u == 0 && b == 0) {
+            rec[R::K_SIZES + (key & 15)] = (uint8_t)(size >> 16);
+            rec[R::V_SIZES + (key & 15)] = (uint8_t)size;
+        }
     }
 }
 
@@ -145,7 +159,7 @@ template <int NB, int KB, int VB>
 __device__ __forceinline__ void vx_kv_read_rows(const vx_kv_rows_args& a) {
     using PK = vx_kv_part<NB, KB>;
     using PV = vx_kv_part<NB, VB>;
-    constexpr uint32_t REC = PK::BYTES + PV::BYTES;
+    constexpr uint32_t REC = vx_kv_rec<NB, KB, VB>::BYTES;
     const uint64_t units = (uint64_t)a.tokens * a.c.heads * NB;
     const uint32_t u = threadIdx.x & 7;
     for (uint64_t n = (uint64_t)blockIdx.x * 32 + (threadIdx.x >> 3); n < units; n += (uint64_t)gridDim.x * 32) {

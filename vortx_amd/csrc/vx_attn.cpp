@@ -22,7 +22,8 @@ static int check_geometry(const vx_kv_cache* c, uint64_t* bytes) {
         return fail(VX_ERR_UNSUPPORTED, "page_tokens is not a power of two from 16 to 65536");
     if (c->heads == 0 || c->heads > 4096) return fail(VX_ERR_UNSUPPORTED, "cache heads are not 1 to 4096");
     if ((uint64_t)c->pages * c->page_tokens > (1ull << 31)) return fail(VX_ERR_UNSUPPORTED, "a cache has at most 2^31 slots");
-    *bytes = (uint64_t)c->pages * c->page_tokens * c->heads * (token_bytes(c->k_type, c->dim) + token_bytes(c->v_type, c->dim));
+    // (a byte more each: how large the scales are, vx_kv.hpp)
+    *bytes = (uint64_t)c->pages * c->page_tokens * c->heads * (token_bytes(c->k_type, c->dim) + token_bytes(c->v_type, c->dim) + 2);
     return VX_OK;
 }
 
@@ -110,7 +111,7 @@ static int run_rows(vx_ctx ctx, vx_stream stream, const vx_kv_cache* cache, cons
         a.ks[i] = r[0].stride[i];
         a.vs[i] = r[1].stride[i];
     }
-    const uint64_t units = (uint64_t)a.tokens * cache->heads * (cache->dim / 32);
+    const uint64_t units = (uint64_t)a.tokens * cache->heads * (cache->dim == 96 ? 4 : cache->dim / 32);
     const uint32_t grid = (uint32_t)std::min<uint64_t>((units + 31) / 32, 1u << 20);
     return launch_struct(ctx, kernel_of(cache, write ? kWrite : kRead), grid, 256, stream, &a);
 }
