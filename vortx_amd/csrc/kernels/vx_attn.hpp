@@ -54,11 +54,18 @@ __device__ __forceinline__ vx_attn_seq vx_attn_sequence(const vx_attn_args& a, u
 // What a query row sees: the keys of [lo, hi), and for a tree of drafts those
 // of [tail, len) whose bit is set.
 struct vx_attn_row {
-    bool valid;
-    int token, head;  // of q and out
     int pos, lo, hi;
-    float slope;      // times log2 e
+    float slope;  // times log2 e
 };
+
+// Token and query head of a unit's row r (below q.rows). Computed again where
+// they are needed: kept over the keys, they are registers that the sums want.
+__device__ __forceinline__ void vx_attn_token(const vx_attn_args& a, const vx_attn_seq& q, uint32_t kvh, uint32_t r, uint32_t& token, uint32_t& head) {
+    asm volatile("" : "+v"(r));
+    const uint32_t j = r / a.group;
+    token = (uint32_t)q.start + j;
+    head = kvh * a.group + (r - j * a.group);
+}
 
 // Number of drafts that a token's row of the tree sees.
 __device__ __forceinline__ int vx_tree_count(const vx_attn_args& a, int token) {
@@ -70,47 +77,47 @@ __device__ __forceinline__ int vx_tree_count(const vx_attn_args& a, int token) {
 
 __device__ __forceinline__ vx_attn_row vx_attn_row_of(const vx_attn_args& a, const vx_attn_seq& q, uint32_t s, uint32_t kvh, uint32_t r) {
     vx_attn_row w;
-    w.valid = r < q.rows;
-    const uint32_t j = w.valid ? r / a.group : 0u;
-    w.token = q.start + (int)j;
-    w.head = (int)(kvh * a.group + (w.valid ? r - j * a.group : 0u));
     const int tail = q.len - q.n;
-    if (!w.valid) {
+    if (r >= q.rows) {
         w.pos = w.lo = w.hi = 0;
         w.slope = 0.f;
         return w;
     }
+    uint32_t token, head;
+    vx_attn_token(a, q, kvh, r, token, head);
     w.lo = 0;
     if (a.tree) {
-        w.pos = tail + vx_tree_count(a, w.token) - 1;
+        w.pos = tail + vx_tree_count(a, (int)token) - 1;
         w.hi = max(tail, 0);
     } else {
-        w.pos = tail + (int)j;
+        w.pos = tail + (int)token - q.start;
         w.hi = q.len;
         if (a.causal) w.hi = min(w.hi, max(w.pos + 1, a.prefix ? a.prefix[s] : 0));
     }
-    if (a.first) w.lo = max(w.lo, a.first[w.token]);
+    if (a.first) w.lo = max(w.lo, a.first[token]);
     if (a.window) {
         w.lo = (int)max((int64_t)w.lo, (int64_t)w.pos - a.window + 1);
         w.hi = (int)min((int64_t)w.hi, (int64_t)w.pos + a.window);
     }
     w.hi = max(w.hi, w.lo);
-    w.slope = a.slopes ? a.slopes[w.head] * VX_LOG2E : 0.f;
+    w.slope = a.slopes ? a.slopes[head] * VX_LOG2E : 0.f;
     return w;
 }
 
-// Which of the 32 keys from k0 on a row sees, a bit each: those of its
+// Which of the 32 keys from k0 on the unit's row r sees, a bit each: those of its
 // interval before `tail`, and the drafts from there on by the tree's bits.
 // at[i] becomes the position of key k0 + i where that is not k0 + i for all of
 // them (slopes or a window over a tree; the wave's own 32 words of LDS).
-__device__ __forceinline__ uint32_t vx_attn_sees(const vx_attn_args& a, const vx_attn_seq& q, const vx_attn_row& w, int tail, int k0, int* at) {
+__device__ __forceinline__ uint32_t vx_attn_sees(const vx_attn_args& a, const vx_attn_seq& q, const vx_attn_row& w, uint32_t kvh, uint32_t r, int tail, int k0, int* at) {
     auto from = [&](int key) { return key <= k0 ? 0xFFFFFFFFu : key - k0 > 31 ? 0u : 0xFFFFFFFFu << (key - k0); };  // keys >= key
     uint32_t see = from(w.lo) & ~from(min(w.hi, tail));
     if (a.tree && k0 + 32 > tail) {
         const int j0 = k0 - tail;  // first draft of the tile (above -32)
         uint32_t bits = 0;
-        if (w.valid) {
-            const uint32_t* row = a.tree + (uint64_t)w.token * a.tree_stride;
+        if (r < q.rows) {
+            uint32_t token, head;
+            vx_attn_token(a, q, kvh, r, token, head);
+            const uint32_t* row = a.tree + (uint64_t)token * a.tree_stride;
             const int i = j0 >> 5, sh = j0 & 31;
             const uint32_t w0 = i >= 0 && (uint32_t)i < a.tree_words ? row[i] : 0u;
             const uint32_t w1 = (uint32_t)(i + 1) < a.tree_words ? row[i + 1] : 0u;
@@ -141,7 +148,104 @@ __device__ __forceinline__ void vx_attn_put(const vx_attn_args& a, uint32_t toke
     if (a.vec) {
         *(f4*)(op + d) = t * k;
     } else {
+        int64_t sd = a.os[2];
+        asm volatile("" : "+s"(sd));  // (else the addresses of all calls are kept over a kernel's units)
+        op += d * sd;
 #pragma unroll
-        for (uint32_t i = 0; i < 4; ++i) op[(int64_t)(d + i) * a.os[2]] = t[i] * k;
+        for (uint32_t i = 0; i < 4; ++i, op += sd) *op = t[i] * k;
+    }
+}
+
+// Keys that the rows of row block rb (ROWS query rows) may see, by their
+// positions alone, and how many steps of STEP keys they are: at least one where
+// there is a row.
+template <uint32_t ROWS, uint32_t STEP>
+__device__ __forceinline__ uint32_t vx_attn_steps(const vx_attn_args& a, const vx_attn_seq& q, uint32_t s, uint32_t rb, int& lo) {
+    const uint32_t r0 = rb * ROWS;
+    lo = 0;
+    if (r0 >= q.rows) return 0u;
+    // (32 bits: lengths and windows are below 2^31 - 2^16, query tokens 2^30 at most)
+    const int tail = q.len - q.n;  // position of the first query
+    int p0 = tail - 1, p1 = q.len, from = 0, to = q.len;  // a tree's drafts are anywhere from there on
+    if (!a.tree) {
+        p0 = tail + (int)(r0 / a.group);
+        p1 = tail + (int)((min(r0 + ROWS, q.rows) - 1) / a.group);
+        if (a.causal) to = min(to, max(p1 + 1, a.prefix ? a.prefix[s] : 0));
+        if (a.window && p1 < 0x7FFFFFFF - (int)a.window) to = min(to, p1 + (int)a.window);
+    }
+    if (a.window && p0 >= (int)a.window) from = p0 - (int)a.window + 1;
+    lo = min(from, q.len) & ~31;
+    return (uint32_t)max(1, (to - lo + (int)STEP - 1) / (int)STEP);
+}
+
+// The key steps of all units (row block, sequence, head) dealt out evenly, a
+// run of them to each workgroup, whatever the lengths. Pair (s, rb) has c steps
+// a head and its heads follow each other; do_unit takes a unit's keys from..to
+// (end: to its end). A unit that several workgroups share goes to partial sums:
+// a workgroup's first unit is partial 2 w, its last, if another, 2 w + 1; info
+// has a unit's first partial and their number, for the join.
+template <uint32_t THREADS, uint32_t ROWS, uint32_t STEP, class Unit>
+__device__ __forceinline__ void vx_attn_deal(const vx_attn_args& a, Unit do_unit) {
+    __shared__ uint32_t sh_sum[THREADS / 64], sh_at[2];
+    const uint32_t t = threadIdx.x, H = a.c.heads, RB = a.row_blocks, pairs = a.seqs * RB;
+    const uint32_t per = (pairs + THREADS - 1) / THREADS;
+    uint32_t mine = 0;
+    for (uint32_t p = t * per; p < min((t + 1) * per, pairs); ++p) {
+        int lo;
+        const uint32_t s = p / RB;
+        mine += vx_attn_steps<ROWS, STEP>(a, vx_attn_sequence(a, s), s, p - s * RB, lo);
+    }
+    uint32_t upto = mine;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const uint32_t v = __shfl_up(upto, o);
+        if ((t & 63) >= (uint32_t)o) upto += v;
+    }
+    if ((t & 63) == 63) sh_sum[t >> 6] = upto;
+    __syncthreads();
+    uint32_t before = upto - mine, all = 0;
+#pragma unroll
+    for (uint32_t i = 0; i < THREADS / 64; ++i) {
+        if (i < t >> 6) before += sh_sum[i];
+        all += sh_sum[i];
+    }
+    const uint64_t total = (uint64_t)all * H, each = (total + gridDim.x - 1) / gridDim.x;
+    uint64_t p = blockIdx.x * each;
+    const uint64_t end = min(p + each, total);
+    if (p >= end) return;
+    if (p >= (uint64_t)before * H && p < (uint64_t)(before + mine) * H) {
+        uint32_t i = t * per, sum = before;
+        for (;; ++i) {
+            int lo;
+            const uint32_t s = i / RB, c = vx_attn_steps<ROWS, STEP>(a, vx_attn_sequence(a, s), s, i - s * RB, lo);
+            if (p < (uint64_t)(sum + c) * H) break;
+            sum += c;
+        }
+        sh_at[0] = i;
+        sh_at[1] = sum;
+    }
+    __syncthreads();
+    uint32_t pair = __builtin_amdgcn_readfirstlane(sh_at[0]);
+    uint64_t begin = (uint64_t)__builtin_amdgcn_readfirstlane(sh_at[1]) * H;  // first step of the pair
+    bool first = true;
+    while (p < end) {
+        const uint32_t s = pair / RB, rb = pair - s * RB;
+        const vx_attn_seq q = vx_attn_sequence(a, s);
+        int klo;
+        const uint32_t c = vx_attn_steps<ROWS, STEP>(a, q, s, rb, klo);
+        if (p >= begin + (uint64_t)c * H) {
+            begin += (uint64_t)c * H;
+            ++pair;
+            continue;
+        }
+        const uint32_t kvh = (uint32_t)((p - begin) / c);
+        const uint64_t u0 = begin + (uint64_t)kvh * c;  // the unit's first step
+        const uint32_t c0 = (uint32_t)(p - u0), c1 = (uint32_t)min((uint64_t)c, end - u0);
+        const uint32_t parts = (uint32_t)((u0 + c - 1) / each - u0 / each) + 1;
+        const uint32_t part = 2 * blockIdx.x + (first ? 0u : 1u);
+        if (c0 == 0 && t == 0) *(u2*)(a.info + 2 * (pair * H + kvh)) = u2{part, parts};
+        do_unit(q, s, kvh, rb, parts == 1, part, klo + (int)(c0 * STEP), klo + (int)(c1 * STEP), c1 == c);
+        p = u0 + c1;
+        first = false;
     }
 }

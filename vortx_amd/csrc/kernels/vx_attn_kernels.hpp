@@ -12,20 +12,23 @@
     extern "C" __global__ __launch_bounds__(256) void VX_CAT(kv_read, types)(vx_kv_rows_args a) {              \
         vx_kv_read_rows<VX_NB, KB, VB>(a);                                                                     \
     }                                                                                                          \
-    extern "C" __global__ __launch_bounds__(256, VX_NB <= 4 ? 2 : 1) void VX_CAT(attn_rows16, types)(vx_attn_args a) {          \
-        vx_rows16<VX_NB, KB, VB>::grid(a);                                                                     \
-    }                                                                                                          \
-    extern "C" __global__ __launch_bounds__(256, VX_NB <= 4 ? 2 : 1) void VX_CAT(attn_even16, types)(vx_attn_args a) {          \
+    extern "C" __global__ __launch_bounds__(256, VX_NB <= 4 ? 2 : 1) void VX_CAT(attn_even16, types)(vx_attn_args a) { \
         vx_rows16<VX_NB, KB, VB>::even(a);                                                                     \
     }                                                                                                          \
-    extern "C" __global__ __launch_bounds__(256, VX_NB <= 4 ? 2 : 1) void VX_CAT(attn_tile4, types)(vx_attn_args a) { \
-        vx_tile<VX_NB, KB, VB, 4>::run(a);                                                                     \
+    extern "C" __global__ __launch_bounds__(256, VX_NB <= 4 ? 2 : 1) void VX_CAT(attn_each128, types)(vx_attn_args a) { \
+        vx_tile<VX_NB, KB, VB, 4>::each(a);                                                                    \
+    }                                                                                                          \
+    extern "C" __global__ __launch_bounds__(256, VX_NB <= 4 ? 2 : 1) void VX_CAT(attn_even128, types)(vx_attn_args a) { \
+        vx_tile<VX_NB, KB, VB, 4>::even(a);                                                                    \
     }
-// (256: eight waves' registers do not hold its sums)
+// (heads of 256: eight waves' registers do not hold the sums)
 #if VX_NB <= 4
 #define VX_WIDE(types, KB, VB)                                                                                 \
-    extern "C" __global__ __launch_bounds__(512, 2) void VX_CAT(attn_tile8, types)(vx_attn_args a) {           \
-        vx_tile<VX_NB, KB, VB, 8>::run(a);                                                                     \
+    extern "C" __global__ __launch_bounds__(512, 2) void VX_CAT(attn_each256, types)(vx_attn_args a) {         \
+        vx_tile<VX_NB, KB, VB, 8>::each(a);                                                                    \
+    }                                                                                                          \
+    extern "C" __global__ __launch_bounds__(512, 2) void VX_CAT(attn_even256, types)(vx_attn_args a) {         \
+        vx_tile<VX_NB, KB, VB, 8>::even(a);                                                                    \
     }
 #else
 #define VX_WIDE(types, KB, VB)

@@ -81,10 +81,11 @@ struct vx_rows16 {
                                                 uint32_t r0, Range range) {
         const uint32_t lane = threadIdx.x & 63, m = lane & 15, g = lane >> 4;
         const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-        const vx_attn_row w = vx_attn_row_of(a, q, s, kvh, r0 + m);
+        const uint32_t row = r0 + m;
+        const vx_attn_row w = vx_attn_row_of(a, q, s, kvh, row);
         const int tail = a.tree ? max(q.len - q.n, 0) : q.len;  // keys from here on: by the tree's bits
-        int lo = w.valid && w.hi > w.lo ? w.lo : 0x7FFFFFFF, hi = w.valid && w.hi > w.lo ? w.hi : 0;
-        int lo_all = w.valid ? w.lo : 0, hi_all = w.valid ? w.hi : 0x7FFFFFFF;
+        int lo = w.hi > w.lo ? w.lo : 0x7FFFFFFF, hi = w.hi > w.lo ? w.hi : 0;
+        int lo_all = row < q.rows ? w.lo : 0, hi_all = row < q.rows ? w.hi : 0x7FFFFFFF;
 #pragma unroll
         for (int o = 1; o < 16; o <<= 1) {
             lo = min(lo, __shfl_xor(lo, o));
@@ -110,7 +111,9 @@ struct vx_rows16 {
         float fq;
         {
             float x[NB][8];
-            const float* qp = a.q + (int64_t)w.token * a.qs[0] + (int64_t)w.head * a.qs[1];
+            uint32_t token, head;
+            vx_attn_token(a, q, kvh, min(row, q.rows - 1u), token, head);  // (a row past the end: another's, never stored)
+            const float* qp = a.q + (int64_t)token * a.qs[0] + (int64_t)head * a.qs[1];
             int64_t sd = a.qs[2];
             asm volatile("" : "+s"(sd));  // (else every address of the strided case is kept over all units)
             float top = 0.f;
@@ -214,7 +217,7 @@ struct vx_rows16 {
                         for (int i = 0; i < 4; ++i) x[t][i] = __builtin_fmaf(-w.slope, fabsf(d0 - (float)(16 * t + i)), x[t][i]);
                 }
             } else {
-                const uint32_t see = vx_attn_sees(a, q, w, tail, k0, sh.at[wave]) >> (4 * g);
+                const uint32_t see = vx_attn_sees(a, q, w, kvh, row, tail, k0, sh.at[wave]) >> (4 * g);
                 const bool drafts = a.tree && k0 + 32 > tail;
 #pragma unroll
                 for (int t = 0; t < 2; ++t)
@@ -327,171 +330,67 @@ struct vx_rows16 {
         return t;
     }
 
-    // Row blocks and splits of their keys over the grid, heads fastest.
-    static __device__ __forceinline__ void grid(const vx_attn_args& a) {
-        __shared__ shared sh;
-        uint32_t id = blockIdx.x;
-        const uint32_t kvh = id % a.c.heads;
-        id /= a.c.heads;
-        const uint32_t s = id % a.seqs;
-        id /= a.seqs;
-        const uint32_t split = id % a.splits, r0 = id / a.splits * 16;
-        const vx_attn_seq q = vx_attn_sequence(a, s);
-        if (r0 >= q.rows) return;
-        const bool any = unit(a, sh, q, s, kvh, r0, [&](int& lo, int& hi) {
-            // this split's keys; the last one takes what is left
-            const int64_t c0 = (int64_t)(lo & ~31) + (int64_t)split * a.chunk;
-            lo = (int)min(c0, (int64_t)hi);
-            if (split + 1 < a.splits) hi = (int)min((int64_t)hi, c0 + a.chunk);
-        });
-        constexpr uint32_t D = 32 * NB;
-        for (uint32_t at = threadIdx.x; at < 16 * (D / 4); at += 256) {
-            const uint32_t r = r0 + at / (D / 4), d = 4 * (at % (D / 4));
-            if (r >= q.rows) break;  // (rows grow with at)
-            float M, l;
-            const f4 t = total(sh, r - r0, d, M, l);
-            const uint32_t j = r / a.group, token = (uint32_t)q.start + j, head = kvh * a.group + (r - j * a.group);
-            if (a.splits > 1) {
-                const uint64_t row = ((uint64_t)split * a.tokens + token) * (a.c.heads * a.group) + head;
-                if (any) *(f4*)(a.part_o + row * D + d) = t;
-                if (d == 0) *(f2*)(a.part_ml + row * 2) = f2{M, l};
-            } else {
-                vx_attn_put(a, token, head, d, t, l);
-            }
-        }
-    }
-
-    // One row block a sequence (single tokens, small trees): the key steps of
-    // all sequences and heads, 128 keys each, dealt out evenly, a run of them to
-    // each workgroup, whatever the lengths. Sequence s has cs steps a head (at
-    // least one if it has a query); unit (s, head) begins at step heads * (sum
-    // of c before s) + head * cs. Workgroup w's part of unit u is partial w + u
-    // (no two have the same one); which partials are a unit's goes to info, for
-    // the join.
-    // Against equal splits of every sequence: 32 sequences of 2400 to 8000 keys
-    // 91 -> 72 us.
-    static __device__ __forceinline__ uint32_t steps(const vx_attn_args& a, const vx_attn_seq& q, int& lo) {
-        lo = 0;
-        if (a.window) lo = (int)max((int64_t)0, (int64_t)q.len - q.n - (int64_t)a.window) & ~31;
-        return q.n ? (uint32_t)max(1, (q.len - lo + 127) / 128) : 0u;
-    }
-
+    // One row block a sequence (single tokens, small trees), the keys of the
+    // batch dealt out evenly. Against equal splits of every sequence: 32
+    // sequences of 2400 to 8000 keys 91 us, now 78.
     static __device__ __forceinline__ void even(const vx_attn_args& a) {
         __shared__ shared sh;
-        __shared__ uint32_t sh_sum[4], sh_at[2];
-        const uint32_t t = threadIdx.x, H = a.c.heads;
         constexpr uint32_t D = 32 * NB;
-        // sums of steps over the sequences
-        const uint32_t per = (a.seqs + 255) / 256;
-        uint32_t mine = 0;
-        for (uint32_t s = t * per; s < min((t + 1) * per, a.seqs); ++s) {
-            int lo;
-            mine += steps(a, vx_attn_sequence(a, s), lo);
-        }
-        uint32_t upto = mine;
-#pragma unroll
-        for (int o = 1; o < 64; o <<= 1) {
-            const uint32_t v = __shfl_up(upto, o);
-            if ((t & 63) >= (uint32_t)o) upto += v;
-        }
-        if ((t & 63) == 63) sh_sum[t >> 6] = upto;
-        __syncthreads();
-        uint32_t before = upto - mine, all = 0;
-#pragma unroll
-        for (uint32_t i = 0; i < 4; ++i) {
-            if (i < t >> 6) before += sh_sum[i];
-            all += sh_sum[i];
-        }
-        const uint64_t total_steps = (uint64_t)all * H, each = (total_steps + gridDim.x - 1) / gridDim.x;
-        uint64_t p = blockIdx.x * each;
-        const uint64_t end = min(p + each, total_steps);
-        if (p >= end) return;
-        if (p >= (uint64_t)before * H && p < (uint64_t)(before + mine) * H) {
-            uint32_t s = t * per, sum = before;
-            for (;; ++s) {
-                int lo;
-                const uint32_t c = steps(a, vx_attn_sequence(a, s), lo);
-                if (p < (uint64_t)(sum + c) * H) break;
-                sum += c;
-            }
-            sh_at[0] = s;
-            sh_at[1] = sum;
-        }
-        __syncthreads();
-        uint32_t s = __builtin_amdgcn_readfirstlane(sh_at[0]);
-        uint64_t begin = (uint64_t)__builtin_amdgcn_readfirstlane(sh_at[1]) * H;  // first step of sequence s
-        while (p < end) {
-            const vx_attn_seq q = vx_attn_sequence(a, s);
-            int klo;
-            const uint32_t c = steps(a, q, klo);
-            if (p >= begin + (uint64_t)c * H) {
-                begin += (uint64_t)c * H;
-                ++s;
-                continue;
-            }
-            const uint32_t kvh = (uint32_t)((p - begin) / c);
-            const uint64_t u0 = begin + (uint64_t)kvh * c;                       // the unit's first step
-            const uint32_t c0 = (uint32_t)(p - u0), c1 = (uint32_t)min((uint64_t)c, end - u0);
-            const uint32_t w0 = (uint32_t)(u0 / each), parts = (uint32_t)((u0 + c - 1) / each) - w0 + 1;
+        vx_attn_deal<256, 16, 128>(a, [&](const vx_attn_seq& q, uint32_t s, uint32_t kvh, uint32_t, bool whole, uint32_t part, int from,
+                                          int to, bool end) {
             unit(a, sh, q, s, kvh, 0, [&](int& lo, int& hi) {
-                lo = max(lo & ~31, klo + (int)c0 * 128);
-                if (c1 < c) hi = min(hi, klo + (int)c1 * 128);
+                lo = max(lo & ~31, from);
+                if (!end) hi = min(hi, to);
             });
-            const uint32_t un = s * H + kvh;
-            const uint64_t pitch = (uint64_t)a.max_queries * a.group;  // rows of a partial
-            if (c0 == 0 && t == 0) *(u2*)(a.info + 2 * un) = u2{w0 + un, parts};
-            for (uint32_t at = t; at < q.rows * (D / 4); at += 256) {
+            for (uint32_t at = threadIdx.x; at < q.rows * (D / 4); at += 256) {
                 const uint32_t r = at / (D / 4), d = 4 * (at % (D / 4));
                 float M, l;
                 const f4 v = total(sh, r, d, M, l);
-                if (parts == 1) {
+                if (whole) {
                     vx_attn_put(a, (uint32_t)q.start + r / a.group, kvh * a.group + r % a.group, d, v, l);
                 } else {
-                    const uint64_t row = ((uint64_t)blockIdx.x + un) * pitch + r;
+                    const uint64_t row = (uint64_t)part * 16 + r;
                     *(f4*)(a.part_o + row * D + d) = v;
                     if (d == 0) *(f2*)(a.part_ml + row * 2) = f2{M, l};
                 }
             }
-            p = u0 + c1;
             __syncthreads();  // sh is the next unit's
-        }
+        });
     }
 };
 
-// Joins the partial sums of a query row: 16 to 64 lanes take its dims, four at
-// a time, and the partials go over the groups of lanes, of a wave where a row
-// has up to 8 of them (four rows a workgroup) and of the workgroup above (one
-// row). One group a row took 90 us for 64 rows of 128 partials, this 4.
+// Joins the partial sums of a query row (vx_attn_deal): 16 to 64 lanes take its
+// dims, four at a time, and the partials go over the groups of lanes, of a wave
+// where a row has up to 8 of them (four rows a workgroup) and of the workgroup
+// above (one row). One group a row took 90 us for 64 rows of 128 partials, this 9.
 __device__ __forceinline__ void vx_attn_join_rows(const vx_attn_args& a) {
     __shared__ f4 sh_t[256];
     __shared__ f2 sh_ml[64];
     const uint32_t D = a.c.dim, lanes = D <= 64 ? 16 : D <= 128 ? 32 : 64;  // of a group
-    const uint32_t span = a.splits > 8 ? 256 : 64;                         // threads of a row
+    const uint32_t span = a.parts > 8 ? 256 : 64;                          // threads of a row
     const uint32_t in = threadIdx.x % span, group = in / lanes, groups = span / lanes, d = 4 * (in % lanes);
     uint32_t id = blockIdx.x * (256 / span) + threadIdx.x / span;
     const uint32_t kvh = id % a.c.heads;
     id /= a.c.heads;
     const uint32_t s = id % a.seqs, r = id / a.seqs;
     const vx_attn_seq q = vx_attn_sequence(a, s);
-    const uint32_t heads = a.c.heads * a.group, j = r / a.group, head = kvh * a.group + (r - j * a.group);
-    uint32_t parts = a.splits;
-    uint64_t stride = (uint64_t)a.tokens * heads, row = ((uint64_t)q.start + j) * heads + head;
+    const uint32_t j = r / a.group, head = kvh * a.group + (r - j * a.group), rb = r / a.part_rows;
     bool valid = r < q.rows && d < D;
-    if (a.info) {
-        const u2 i = q.n ? *(const u2*)(a.info + 2 * (s * a.c.heads + kvh)) : u2{0, 1};
-        parts = i.y;
-        stride = (uint64_t)a.max_queries * a.group;
-        row = i.x * stride + r;
-        valid = valid && parts > 1;  // (else the result is there)
-    }
+    u2 info = {0, 1};
+    if (valid) info = *(const u2*)(a.info + 2 * (((uint64_t)s * a.row_blocks + rb) * a.c.heads + kvh));
+    const uint32_t parts = info.y;
+    valid = valid && parts > 1;  // (else the result is there)
+    // partials 2 w or 2 w + 1, then 2 (w + 1), 2 (w + 2) ..
+    auto row_of = [&](uint32_t i) { return (uint64_t)(i ? (info.x >> 1) * 2 + 2 * i : info.x) * a.part_rows + (r - rb * a.part_rows); };
     float M = -__builtin_inff(), l = 0.f;
     f4 t = {};
     if (valid) {
 #pragma unroll 4
         for (uint32_t i = group; i < parts; i += groups) {
-            const f2 ml = *(const f2*)(a.part_ml + (i * stride + row) * 2);
-            if (ml.y == 0.f) continue;  // nothing seen there, perhaps nothing written (not so for a NaN)
-            const f4 o = *(const f4*)(a.part_o + (i * stride + row) * D + d);
+            const uint64_t row = row_of(i);
+            const f2 ml = *(const f2*)(a.part_ml + row * 2);
+            const f4 o = *(const f4*)(a.part_o + row * D + d);
+            if (ml.y == 0.f) continue;  // nothing seen there (not so for a NaN)
             const float Mn = fmaxf(M, ml.x), c = __builtin_amdgcn_exp2f(M - Mn), k = __builtin_amdgcn_exp2f(ml.x - Mn);
             // (M is -inf before the first; a NaN in y may have -inf beside it, and stays)
             l = __builtin_fmaf(k, ml.y, c * l);

@@ -180,30 +180,28 @@ struct vx_tile {
         }
     }
 
-    static __device__ __forceinline__ void run(const vx_attn_args& a) {
-        __shared__ tile sh[2 * PERIOD];
-        __shared__ int sh_at[WAVES][32];
+    struct shared {
+        tile t[2 * PERIOD];
+        int at[WAVES][32];
+    };
+
+    // Row block rb of sequence s and head kvh over the keys that range(lo, hi)
+    // leaves of those its rows see; whole: the rows' results, else sums to partial `part`.
+    template <class Range>
+    static __device__ __forceinline__ void unit(const vx_attn_args& a, shared& shm, const vx_attn_seq& q, uint32_t s, uint32_t kvh,
+                                                uint32_t rb, bool whole_unit, uint32_t part, Range range) {
+        tile* sh = shm.t;
         const uint32_t lane = threadIdx.x & 63, n = lane & 31, h = lane >> 5;
         const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-        // workgroup -> (row block, split, sequence, head): heads fastest (a head's
-        // row blocks on one XCD where heads are a multiple of 8), late rows first
-        // (causal: they have the most keys)
-        uint32_t id = blockIdx.x;
-        const uint32_t kvh = id % a.c.heads;
-        id /= a.c.heads;
-        const uint32_t s = id % a.seqs;
-        id /= a.seqs;
-        const uint32_t split = id % a.splits;
-        const vx_attn_seq q = vx_attn_sequence(a, s);
-        const uint32_t blocks = (q.rows + ROWS - 1) / ROWS, place = id / a.splits;
-        if (place >= blocks) return;
-        const uint32_t r0 = (blocks - 1 - place) * ROWS, row = r0 + wave * 32 + n;
+        const uint32_t r0 = rb * ROWS;
+        const uint32_t row = r0 + wave * 32 + n;
         const vx_attn_row w = vx_attn_row_of(a, q, s, kvh, row);
         const int tail = a.tree ? max(q.len - q.n, 0) : q.len;  // keys from here on: by the tree's bits
         const int last = q.len - 1;
+        __syncthreads();  // (LDS may be another unit's still)
         // what the wave's rows see, and all of them; and the workgroup's
-        int lo = w.valid && w.hi > w.lo ? w.lo : 0x7FFFFFFF, hi = w.valid && w.hi > w.lo ? w.hi : 0;
-        int lo_all = w.valid ? w.lo : 0, hi_all = w.valid ? w.hi : 0x7FFFFFFF;
+        int lo = w.hi > w.lo ? w.lo : 0x7FFFFFFF, hi = w.hi > w.lo ? w.hi : 0;
+        int lo_all = row < q.rows ? w.lo : 0, hi_all = row < q.rows ? w.hi : 0x7FFFFFFF;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
             lo = min(lo, __shfl_xor(lo, o));
@@ -217,7 +215,7 @@ struct vx_tile {
             hi = q.len;
         }
         lo = __builtin_amdgcn_readfirstlane(lo);
-        hi = min(__builtin_amdgcn_readfirstlane(hi), last + 1);
+        hi = __builtin_amdgcn_readfirstlane(hi);
         lo_all = __builtin_amdgcn_readfirstlane(lo_all);
         hi_all = __builtin_amdgcn_readfirstlane(hi_all);
         int wg_lo, wg_hi;
@@ -233,15 +231,19 @@ struct vx_tile {
         wg_lo = __builtin_amdgcn_readfirstlane(wg_lo);
         wg_hi = __builtin_amdgcn_readfirstlane(wg_hi);
         if (wg_lo >= wg_hi) wg_lo = wg_hi = 0;  // nothing seen
-        // this split's keys; the last one takes what is left
-        const int64_t c0 = (int64_t)(wg_lo & ~31) + (int64_t)split * a.chunk;
-        const int kbeg = (int)min(c0, (int64_t)wg_hi);
-        const int kend = split + 1 == a.splits ? wg_hi : (int)min((int64_t)wg_hi, c0 + a.chunk);
+        int kbeg = wg_lo, kend = wg_hi;
+        range(kbeg, kend);
+        kbeg &= ~31;
+        if (kbeg >= kend) kbeg = kend = 0;
 
         h8 qh[NB][2], ql[NB][2];
         float fq;
         {
-            const float* qp = a.q + (int64_t)w.token * a.qs[0] + (int64_t)w.head * a.qs[1];
+            uint32_t token, head;
+            vx_attn_token(a, q, kvh, min(row, q.rows - 1u), token, head);  // (a row past the end: another's, never stored)
+            const float* qp = a.q + (int64_t)token * a.qs[0] + (int64_t)head * a.qs[1];
+            int64_t sd = a.qs[2];
+            asm volatile("" : "+s"(sd));  // (else every address of the strided case is kept over all units)
             float x[NB][2][8], top = 0.f;
             bool fine = true;
 #pragma unroll
@@ -254,9 +256,9 @@ struct vx_tile {
 #pragma unroll
                         for (int i = 0; i < 4; ++i) x[b][j][i] = u[i], x[b][j][4 + i] = v[i];
                     } else {
-                        const float* p = qp + (int64_t)d * a.qs[2];
+                        const float* p = qp + (int64_t)d * sd;
 #pragma unroll
-                        for (int i = 0; i < 8; ++i, p += a.qs[2]) x[b][j][i] = *p;
+                        for (int i = 0; i < 8; ++i, p += sd) x[b][j][i] = *p;
                     }
 #pragma unroll
                     for (int i = 0; i < 8; ++i) {
@@ -363,12 +365,12 @@ struct vx_tile {
                 }
                 const bool whole = k0 >= lo_all && k0 + 32 <= hi_all && k0 + 32 <= tail;
                 uint32_t see = 0xFFFFFFFFu;  // bit k: key k0 + 4 h + k
-                if (!whole) see = vx_attn_sees(a, q, w, tail, k0, sh_at[wave]) >> (4 * h);
+                if (!whole) see = vx_attn_sees(a, q, w, kvh, row, tail, k0, shm.at[wave]) >> (4 * h);
                 if (a.slopes) {
                     if (a.tree && k0 + 32 > tail) {
 #pragma unroll
                         for (int i = 0; i < 16; ++i)
-                            x[i] = __builtin_fmaf(-w.slope, fabsf((float)(w.pos - sh_at[wave][8 * (i / 4) + i % 4 + 4 * h])), x[i]);
+                            x[i] = __builtin_fmaf(-w.slope, fabsf((float)(w.pos - shm.at[wave][8 * (i / 4) + i % 4 + 4 * h])), x[i]);
                     } else {
                         const float d0 = (float)(w.pos - (k0 + 4 * (int)h));
 #pragma unroll
@@ -461,12 +463,12 @@ struct vx_tile {
 
         // both halves' sums; registers 8 v + 4 p + i hold dims 32 b + 16 p + 8 h + 2 i + v
         l += __shfl_xor(l, 32);
-        if (!w.valid) return;
-        const uint64_t heads = a.c.heads * a.group;
+        uint32_t r = r0 + (threadIdx.x >> 6) * 32 + (threadIdx.x & 31), token, head;
+        if (r >= q.rows) return;
+        vx_attn_token(a, q, kvh, r, token, head);
         constexpr uint32_t D = 32 * NB;
-        const uint64_t part = ((uint64_t)split * a.tokens + w.token) * heads + w.head;
-        if (a.splits > 1 && h == 0) *(f2*)(a.part_ml + part * 2) = f2{M, l};
-        if (a.splits > 1 && kbeg >= kend) return;
+        const uint64_t at = (uint64_t)part * ROWS + wave * 32 + n;
+        if (!whole_unit && h == 0) *(f2*)(a.part_ml + at * 2) = f2{M, l};
 #pragma unroll
         for (int b = 0; b < NB; ++b)
 #pragma unroll
@@ -475,8 +477,34 @@ struct vx_tile {
                 for (int u = 0; u < 2; ++u) {
                     const f4 v = {o[b][4 * p + 2 * u], o[b][8 + 4 * p + 2 * u], o[b][4 * p + 2 * u + 1], o[b][8 + 4 * p + 2 * u + 1]};
                     const uint32_t d = 32 * b + 16 * p + 8 * h + 4 * u;
-                    if (a.splits > 1) *(f4*)(a.part_o + part * D + d) = v;
-                    else vx_attn_put(a, (uint32_t)w.token, (uint32_t)w.head, d, v, l);
+                    if (whole_unit) vx_attn_put(a, token, head, d, v, l);
+                    else *(f4*)(a.part_o + at * D + d) = v;
                 }
+    }
+
+    // A workgroup a unit: heads fastest (a head's row blocks on one XCD where
+    // heads are a multiple of 8), late rows first (causal: they have the most keys).
+    static __device__ __forceinline__ void each(const vx_attn_args& a) {
+        __shared__ shared sh;
+        uint32_t id = blockIdx.x;
+        const uint32_t kvh = id % a.c.heads;
+        id /= a.c.heads;
+        const uint32_t s = id % a.seqs, place = id / a.seqs;
+        const vx_attn_seq q = vx_attn_sequence(a, s);
+        const uint32_t blocks = (q.rows + ROWS - 1) / ROWS;
+        if (place >= blocks) return;
+        unit(a, sh, q, s, kvh, blocks - 1 - place, true, 0, [](int&, int&) {});
+    }
+
+    // Fewer units than the card has places: their keys dealt out evenly.
+    static __device__ __forceinline__ void even(const vx_attn_args& a) {
+        __shared__ shared sh;
+        vx_attn_deal<THREADS, ROWS, 64>(a, [&](const vx_attn_seq& q, uint32_t s, uint32_t kvh, uint32_t rb, bool whole, uint32_t part,
+                                               int from, int to, bool end) {
+            unit(a, sh, q, s, kvh, rb, whole, part, [&](int& lo, int& hi) {
+                lo = max(lo, from);
+                if (!end) hi = min(hi, to);
+            });
+        });
     }
 };

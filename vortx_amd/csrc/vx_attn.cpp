@@ -49,10 +49,11 @@ static int kernel_of(const vx_kv_cache* c, const int* d) {
     return d[dim_index(c->dim)] + (c->k_type == VX_Q4_0 ? 2 : 0) + (c->v_type == VX_Q4_0 ? 1 : 0);
 }
 #define VX_DIMS(f) {K_vx_##f##_d64_k8v8, K_vx_##f##_d96_k8v8, K_vx_##f##_d128_k8v8, K_vx_##f##_d256_k8v8}
-static const int kWrite[4] = VX_DIMS(kv_write), kRead[4] = VX_DIMS(kv_read), kRows16[4] = VX_DIMS(attn_rows16),
-                 kEven16[4] = VX_DIMS(attn_even16), kTile4[4] = VX_DIMS(attn_tile4),
-                 kTile8[3] = {K_vx_attn_tile8_d64_k8v8, K_vx_attn_tile8_d96_k8v8, K_vx_attn_tile8_d128_k8v8};
-constexpr uint32_t VX_EVEN_ROWS = 16;  // query rows of a workgroup of kEven16
+static const int kWrite[4] = VX_DIMS(kv_write), kRead[4] = VX_DIMS(kv_read), kEven16[4] = VX_DIMS(attn_even16),
+                 kEach128[4] = VX_DIMS(attn_each128), kEven128[4] = VX_DIMS(attn_even128);
+#undef VX_DIMS
+#define VX_DIMS(f) {K_vx_##f##_d64_k8v8, K_vx_##f##_d96_k8v8, K_vx_##f##_d128_k8v8}
+static const int kEach256[3] = VX_DIMS(attn_each256), kEven256[3] = VX_DIMS(attn_even256);
 #undef VX_DIMS
 
 // A [tokens, heads, dim] view.
@@ -116,48 +117,45 @@ static int run_rows(vx_ctx ctx, vx_stream stream, const vx_kv_cache* cache, cons
     return launch_struct(ctx, kernel_of(cache, write ? kWrite : kRead), grid, 256, stream, &a);
 }
 
+// How a call is laid out: the kernel by the query rows of a sequence and head
+// (16, 128 or 256 a workgroup), and whether a workgroup takes a unit (row block,
+// sequence, head) each, or the keys of all units are dealt out evenly over the
+// places that the card has for workgroups.
+constexpr uint32_t VX_MOST_KEYS = (1u << 31) - 65536u;  // of a sequence
+constexpr uint64_t VX_EVEN_ROWS = 16, VX_EVEN_UNITS = 1;
 struct AttnPlan {
     const int* kernel;
-    uint32_t block = 256;
+    uint32_t block, rows, row_blocks, grid, parts;
     bool even;
-    uint32_t row_blocks, splits, chunk;
-    uint32_t grid;
-    uint64_t info, rows;  // of the workspace: bytes before, and rows of partial sums
-    uint64_t bytes(uint32_t dim) const { return info + rows * (dim + 2) * 4; }
+    uint64_t units;
+    uint64_t info() const { return (units * 8 + 15) / 16 * 16; }  // bytes of the workspace before the partial sums
+    uint64_t part_rows() const { return 2ull * grid * rows; }
+    uint64_t bytes(uint32_t dim) const { return even ? info() + part_rows() * (dim + 2) * 4 : 0; }
 };
 
 static int plan_attention(int num_cus, const vx_kv_cache* c, const vx_attn_batch* b, const vx_attn_opts* o, uint32_t q_heads,
-                          uint64_t tokens, bool ws, AttnPlan* p) {
-    const uint64_t group = q_heads / c->heads, queries = b->max_queries, units = (uint64_t)b->seqs * c->heads;
-    uint64_t span = std::min<uint64_t>(b->max_len, (uint64_t)b->table_cols * c->page_tokens);
-    if (o && o->window) span = std::min<uint64_t>(span, 2ull * o->window + queries + 64);
-    uint64_t places = (c->dim > 128 ? 1ull : 2ull) * (uint64_t)num_cus;  // workgroups that the card holds
+                          bool ws, AttnPlan* p) {
+    const uint64_t group = q_heads / c->heads, queries = b->max_queries, rows = queries * group;
+    const bool wide = rows > 128 && c->dim <= 128;
     *p = AttnPlan{};
-    if (queries * group <= VX_EVEN_ROWS && ws) {
-        p->kernel = kEven16;
-        p->even = true;
-        p->row_blocks = 1;
-        p->grid = (uint32_t)std::max<uint64_t>(1, std::min(units * ((span + 127) / 128 + 1), places));
-        p->splits = 16;  // (partials of a unit, for the join)
-        p->info = (units * 8 + 15) / 16 * 16;
-        p->rows = (p->grid + units) * queries * group;
-        if (units * queries * group >= (1ull << 24)) return fail(VX_ERR_UNSUPPORTED, "attention: too many rows (split the batch)");
-        return VX_OK;
-    }
-    const bool wide = queries * group > 128 && c->dim <= 128;
-    p->kernel = wide ? kTile8 : kTile4;
-    p->block = wide ? 512 : 256;
-    const uint64_t tile = wide ? 256 : 128, rb = (queries * group + tile - 1) / tile, wgs = rb * units;
-    if (wide) places /= 2;
-    uint64_t splits = 1;
-    if (ws && wgs < places) splits = std::max<uint64_t>(1, std::min<uint64_t>(places / wgs, (span + 127) / 128));
-    const uint64_t chunk = std::max<uint64_t>(32, ((span + splits - 1) / splits + 31) / 32 * 32);
+    p->rows = rows <= VX_EVEN_ROWS && ws ? 16 : wide ? 256 : 128;
+    p->block = p->rows == 256 ? 512 : 256;
+    const uint64_t places = (uint64_t)num_cus * (p->rows == 256 || c->dim > 128 ? 1 : 2);  // workgroups that the card holds
+    const uint64_t rb = (rows + p->rows - 1) / p->rows;
+    p->units = rb * b->seqs * c->heads;
+    if (p->units >= (1ull << 23) || rows * b->seqs * c->heads >= (1ull << 24))
+        return fail(VX_ERR_UNSUPPORTED, "attention: too many query rows (split the batch)");
     p->row_blocks = (uint32_t)rb;
-    p->chunk = (uint32_t)std::min<uint64_t>(chunk, 1u << 31);
-    p->splits = (uint32_t)(splits > 1 ? std::max<uint64_t>(1, (span + chunk - 1) / chunk) : 1);
-    if (wgs * p->splits >= (1ull << 24)) return fail(VX_ERR_UNSUPPORTED, "attention: too many workgroups (split the batch)");
-    p->grid = (uint32_t)(wgs * p->splits);
-    if (p->splits > 1) p->rows = p->splits * tokens * q_heads;
+    p->even = ws && (p->rows == 16 || p->units <= VX_EVEN_UNITS * places);
+    p->kernel = p->rows == 16 ? kEven16 : p->rows == 128 ? (p->even ? kEven128 : kEach128) : (p->even ? kEven256 : kEach256);
+    p->grid = (uint32_t)p->units;
+    if (p->even) {
+        uint64_t span = std::min<uint64_t>(b->max_len, (uint64_t)b->table_cols * c->page_tokens);
+        if (o && o->window) span = std::min<uint64_t>(span, 2ull * o->window + queries + 64);
+        const uint64_t step = p->rows == 16 ? 128 : 64;
+        p->grid = (uint32_t)std::max<uint64_t>(1, std::min(p->units * ((span + step - 1) / step + 1), places));
+        p->parts = (uint32_t)(p->grid / std::max<uint64_t>(1, p->units)) + 2;
+    }
     return VX_OK;
 }
 
@@ -166,7 +164,7 @@ static int check_batch(const vx_kv_cache* c, const vx_attn_batch* b, const vx_at
     if (b->reserved) return fail(VX_ERR_INVALID, "vx_attn_batch.reserved must be 0");
     if (q_heads == 0 || q_heads % c->heads) return fail(VX_ERR_SHAPE, "query heads are not a multiple of the cache's heads");
     if (b->table_stride < b->table_cols) return fail(VX_ERR_INVALID, "table_stride smaller than table_cols");
-    if (b->max_len > (1u << 31) - 65536u) return fail(VX_ERR_UNSUPPORTED, "max_len is 2^31 - 2^16 at most");
+    if (b->max_len > VX_MOST_KEYS) return fail(VX_ERR_UNSUPPORTED, "max_len is 2^31 - 2^16 at most");
     if (b->seqs && (!b->lens || !b->starts || (!b->table && b->table_cols))) return fail(VX_ERR_INVALID, "null batch array");
     if (((uintptr_t)b->lens | (uintptr_t)b->starts | (uintptr_t)b->table) & 3u)
         return fail(VX_ERR_INVALID, "a batch array is not 4-byte aligned");
@@ -195,7 +193,7 @@ static int run_attention(vx_ctx ctx, vx_stream stream, const vx_mview* out, cons
     if (rq.tokens > (1u << 30)) return fail(VX_ERR_UNSUPPORTED, "more than 2^30 query tokens");
     if (rq.tokens == 0 || batch->seqs == 0 || batch->max_queries == 0) return VX_OK;
     AttnPlan p;
-    if ((s = plan_attention(ctx_cus(ctx), cache, batch, opts, rq.heads, rq.tokens, ws != nullptr, &p))) return s;
+    if ((s = plan_attention(ctx_cus(ctx), cache, batch, opts, rq.heads, ws != nullptr, &p))) return s;
     if (ws_size < p.bytes(cache->dim)) return fail(VX_ERR_INVALID, "workspace smaller than vx_attention_ws_size");
     a.q = (const float*)rq.ptr;
     a.out = (float*)ro.ptr;
@@ -219,7 +217,7 @@ static int run_attention(vx_ctx ctx, vx_stream stream, const vx_mview* out, cons
         a.cap = opts->softcap;
         a.slopes = opts->slopes;
         a.first = opts->first;
-        a.window = opts->window;
+        a.window = opts->window >= VX_MOST_KEYS ? 0u : opts->window;  // (none that any key is outside of)
         if (!tree) {
             a.causal = opts->flags & VX_ATTN_CAUSAL;
             a.prefix = opts->prefix;
@@ -229,15 +227,15 @@ static int run_attention(vx_ctx ctx, vx_stream stream, const vx_mview* out, cons
     a.tree_words = tree_words;
     a.tree_stride = tree_stride;
     a.row_blocks = p.row_blocks;
-    a.splits = p.splits;
-    a.chunk = p.chunk;
-    a.info = p.even ? (uint32_t*)ws : nullptr;
-    a.part_o = (float*)((char*)ws + p.info);
-    a.part_ml = a.part_o + p.rows * cache->dim;
+    a.part_rows = p.rows;
+    a.parts = p.parts;
+    a.info = (uint32_t*)ws;
+    a.part_o = (float*)((char*)ws + p.info());
+    a.part_ml = a.part_o + p.part_rows() * cache->dim;
     if ((s = launch_struct(ctx, kernel_of(cache, p.kernel), p.grid, p.block, stream, &a))) return s;
-    if (p.splits > 1) {
+    if (p.even) {
         const uint64_t jobs = (uint64_t)batch->max_queries * a.group * batch->seqs * cache->heads;
-        return launch_struct(ctx, K_vx_attn_join, (uint32_t)(p.splits > 8 ? jobs : (jobs + 3) / 4), 256, stream, &a);
+        return launch_struct(ctx, K_vx_attn_join, (uint32_t)(p.parts > 8 ? jobs : (jobs + 3) / 4), 256, stream, &a);
     }
     return VX_OK;
 }
@@ -295,7 +293,7 @@ int vx_attention_ws_size(vx_ctx ctx, const vx_kv_cache* cache, const vx_attn_bat
     if ((s = vx::check_batch(cache, batch, opts, q_heads))) return s;
     if (!tokens || !batch->seqs || !batch->max_queries) return VX_OK;
     vx::AttnPlan p;
-    if ((s = vx::plan_attention(vx::ctx_cus(ctx), cache, batch, opts, q_heads, tokens, true, &p))) return s;
+    if ((s = vx::plan_attention(vx::ctx_cus(ctx), cache, batch, opts, q_heads, true, &p))) return s;
     *bytes = p.bytes(cache->dim);
     return VX_OK;
 }

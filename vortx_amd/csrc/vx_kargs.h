@@ -156,14 +156,15 @@ typedef struct vx_attn_args {
     const int32_t* prefix; /* [seqs] or null */
     const int32_t* first;  /* [tokens] or null */
     const uint32_t* tree;  /* [tokens][tree_stride] or null */
-    uint32_t* info;        /* even split: [seqs][heads] first partial and their number; else null */
-    float* part_o;         /* partial sums [split][token][head][dim] (splits > 1), or [partial][row][dim] */
-    float* part_ml;        /* [split][token][head][2], or [partial][row][2] */
+    uint32_t* info;        /* [seqs][row blocks][heads] first partial and their number (vx_attn_deal) */
+    float* part_o;         /* partial sums [partial][part_rows][dim] */
+    float* part_ml;        /* [partial][part_rows][2] */
     uint32_t table_stride, table_cols;
     uint32_t seqs, tokens, group;
     uint32_t max_queries, max_len;
-    uint32_t splits, chunk; /* keys of a split, a multiple of 32 */
-    uint32_t row_blocks;
+    uint32_t row_blocks;   /* of a sequence, part_rows query rows each */
+    uint32_t part_rows;
+    uint32_t parts;        /* about how many partials a unit has */
     uint32_t causal, window;
     uint32_t tree_stride, tree_words;
     float scale, cap;      /* cap 0: none */
