@@ -178,13 +178,21 @@ __device__ __forceinline__ uint32_t vx_attn_steps(const vx_attn_args& a, const v
     return (uint32_t)max(1, (to - lo + (int)STEP - 1) / (int)STEP);
 }
 
+// Quotients of numbers that seldom need 64 bits.
+__device__ __forceinline__ uint64_t vx_div(uint64_t a, uint64_t b) {
+    return (a | b) >> 32 ? a / b : (uint64_t)((uint32_t)a / (uint32_t)b);
+}
+
 // The key steps of all units (row block, sequence, head) dealt out evenly, a
 // run of them to each workgroup, whatever the lengths. Pair (s, rb) has c steps
-// a head and its heads follow each other; do_unit takes a unit's keys from..to
-// (end: to its end). A unit that several workgroups share goes to partial sums:
+// a head and its heads follow each other; a unit counts COST steps more, in
+// front, for what it takes to begin and to end (without that the first row
+// blocks of a causal prompt, many short units to a workgroup, took three times
+// the others' time). do_unit takes a unit's keys from..to (end: to its end). A
+// unit that several workgroups share goes to partial sums:
 // a workgroup's first unit is partial 2 w, its last, if another, 2 w + 1; info
 // has a unit's first partial and their number, for the join.
-template <uint32_t THREADS, uint32_t ROWS, uint32_t STEP, class Unit>
+template <uint32_t THREADS, uint32_t ROWS, uint32_t STEP, uint32_t COST, class Unit>
 __device__ __forceinline__ void vx_attn_deal(const vx_attn_args& a, Unit do_unit) {
     __shared__ uint32_t sh_sum[THREADS / 64], sh_at[2];
     const uint32_t t = threadIdx.x, H = a.c.heads, RB = a.row_blocks, pairs = a.seqs * RB;
@@ -193,7 +201,8 @@ __device__ __forceinline__ void vx_attn_deal(const vx_attn_args& a, Unit do_unit
     for (uint32_t p = t * per; p < min((t + 1) * per, pairs); ++p) {
         int lo;
         const uint32_t s = p / RB;
-        mine += vx_attn_steps<ROWS, STEP>(a, vx_attn_sequence(a, s), s, p - s * RB, lo);
+        const uint32_t c = vx_attn_steps<ROWS, STEP>(a, vx_attn_sequence(a, s), s, p - s * RB, lo);
+        mine += c ? c + COST : 0u;
     }
     uint32_t upto = mine;
 #pragma unroll
@@ -209,17 +218,22 @@ __device__ __forceinline__ void vx_attn_deal(const vx_attn_args& a, Unit do_unit
         if (i < t >> 6) before += sh_sum[i];
         all += sh_sum[i];
     }
-    const uint64_t total = (uint64_t)all * H, each = (total + gridDim.x - 1) / gridDim.x;
-    uint64_t p = blockIdx.x * each;
-    const uint64_t end = min(p + each, total);
+    // workgroup w's run is [w total / G, (w + 1) total / G): step k is run (k G + G - 1) / total
+    const uint64_t total = (uint64_t)all * H;
+    const uint32_t G = (uint32_t)min((uint64_t)gridDim.x, total);  // (no run is empty)
+    if (blockIdx.x >= G) return;
+    uint64_t p = vx_div(blockIdx.x * total, G);
+    const uint64_t end = vx_div((blockIdx.x + 1) * total, G);
     if (p >= end) return;
+    auto run_of = [&](uint64_t k) { return vx_div(k * G + G - 1, total); };
     if (p >= (uint64_t)before * H && p < (uint64_t)(before + mine) * H) {
         uint32_t i = t * per, sum = before;
         for (;; ++i) {
             int lo;
             const uint32_t s = i / RB, c = vx_attn_steps<ROWS, STEP>(a, vx_attn_sequence(a, s), s, i - s * RB, lo);
-            if (p < (uint64_t)(sum + c) * H) break;
-            sum += c;
+            const uint32_t all_c = c ? c + COST : 0u;
+            if (p < (uint64_t)(sum + all_c) * H) break;
+            sum += all_c;
         }
         sh_at[0] = i;
         sh_at[1] = sum;
@@ -233,19 +247,20 @@ __device__ __forceinline__ void vx_attn_deal(const vx_attn_args& a, Unit do_unit
         const vx_attn_seq q = vx_attn_sequence(a, s);
         int klo;
         const uint32_t c = vx_attn_steps<ROWS, STEP>(a, q, s, rb, klo);
-        if (p >= begin + (uint64_t)c * H) {
-            begin += (uint64_t)c * H;
+        if (!c || p >= begin + (uint64_t)(c + COST) * H) {
+            begin += c ? (uint64_t)(c + COST) * H : 0u;
             ++pair;
             continue;
         }
-        const uint32_t kvh = (uint32_t)((p - begin) / c);
-        const uint64_t u0 = begin + (uint64_t)kvh * c;  // the unit's first step
-        const uint32_t c0 = (uint32_t)(p - u0), c1 = (uint32_t)min((uint64_t)c, end - u0);
-        const uint32_t parts = (uint32_t)((u0 + c - 1) / each - u0 / each) + 1;
+        const uint32_t kvh = (uint32_t)vx_div(p - begin, c + COST);
+        const uint64_t k0 = begin + (uint64_t)kvh * (c + COST) + COST;  // the unit's first step of keys
+        if (k0 >= end) break;
+        const uint32_t c0 = p > k0 ? (uint32_t)(p - k0) : 0u, c1 = (uint32_t)min((uint64_t)c, end - k0);
+        const uint32_t parts = (uint32_t)(run_of(k0 + c - 1) - run_of(k0)) + 1;
         const uint32_t part = 2 * blockIdx.x + (first ? 0u : 1u);
         if (c0 == 0 && t == 0) *(u2*)(a.info + 2 * (pair * H + kvh)) = u2{part, parts};
         do_unit(q, s, kvh, rb, parts == 1, part, klo + (int)(c0 * STEP), klo + (int)(c1 * STEP), c1 == c);
-        p = u0 + c1;
+        p = k0 + c1;
         first = false;
     }
 }

@@ -330,24 +330,26 @@ struct vx_rows16 {
         return t;
     }
 
-    // One row block a sequence (single tokens, small trees), the keys of the
-    // batch dealt out evenly. Against equal splits of every sequence: 32
-    // sequences of 2400 to 8000 keys 91 us, now 78.
+    // Single tokens, small trees: the keys of the batch dealt out evenly. Against
+    // equal splits of every sequence: 32 sequences of 2400 to 8000 keys 91 us, now 78.
     static __device__ __forceinline__ void even(const vx_attn_args& a) {
         __shared__ shared sh;
         constexpr uint32_t D = 32 * NB;
-        vx_attn_deal<256, 16, 128>(a, [&](const vx_attn_seq& q, uint32_t s, uint32_t kvh, uint32_t, bool whole, uint32_t part, int from,
+        vx_attn_deal<256, 16, 128, 1>(a, [&](const vx_attn_seq& q, uint32_t s, uint32_t kvh, uint32_t rb, bool whole, uint32_t part, int from,
                                           int to, bool end) {
-            unit(a, sh, q, s, kvh, 0, [&](int& lo, int& hi) {
+            const uint32_t r0 = rb * 16, rows = min(q.rows - r0, 16u);
+            unit(a, sh, q, s, kvh, r0, [&](int& lo, int& hi) {
                 lo = max(lo & ~31, from);
                 if (!end) hi = min(hi, to);
             });
-            for (uint32_t at = threadIdx.x; at < q.rows * (D / 4); at += 256) {
+            for (uint32_t at = threadIdx.x; at < rows * (D / 4); at += 256) {
                 const uint32_t r = at / (D / 4), d = 4 * (at % (D / 4));
                 float M, l;
                 const f4 v = total(sh, r, d, M, l);
                 if (whole) {
-                    vx_attn_put(a, (uint32_t)q.start + r / a.group, kvh * a.group + r % a.group, d, v, l);
+                    uint32_t token, head;
+                    vx_attn_token(a, q, kvh, r0 + r, token, head);
+                    vx_attn_put(a, token, head, d, v, l);
                 } else {
                     const uint64_t row = (uint64_t)part * 16 + r;
                     *(f4*)(a.part_o + row * D + d) = v;

@@ -499,7 +499,7 @@ struct vx_tile {
     // Fewer units than the card has places: their keys dealt out evenly.
     static __device__ __forceinline__ void even(const vx_attn_args& a) {
         __shared__ shared sh;
-        vx_attn_deal<THREADS, ROWS, 64>(a, [&](const vx_attn_seq& q, uint32_t s, uint32_t kvh, uint32_t rb, bool whole, uint32_t part,
+        vx_attn_deal<THREADS, ROWS, 64, 4>(a, [&](const vx_attn_seq& q, uint32_t s, uint32_t kvh, uint32_t rb, bool whole, uint32_t part,
                                                int from, int to, bool end) {
             unit(a, sh, q, s, kvh, rb, whole, part, [&](int& lo, int& hi) {
                 lo = max(lo, from);

@@ -122,7 +122,17 @@ static int run_rows(vx_ctx ctx, vx_stream stream, const vx_kv_cache* cache, cons
 // sequence, head) each, or the keys of all units are dealt out evenly over the
 // places that the card has for workgroups.
 constexpr uint32_t VX_MOST_KEYS = (1u << 31) - 65536u;  // of a sequence
-constexpr uint64_t VX_EVEN_ROWS = 16, VX_EVEN_UNITS = 1;
+// Up to so many rows the 16-row kernel, whose row blocks read the keys again, is
+// faster than the tiles of 128 and 256 rows, which decode them once. Trees of
+// drafts, us, 16 rows / tiles:
+//   dim 128, 1 sequence of 1500 keys   96 rows 18.6 / 25.9   128 rows 19.7 / 27.4
+//            1 of 20000                96      56.0 / 63.5   128      67.9 / 71.4   192 rows 93.7 / 86.4
+//            8 of up to 12000          96       114 / 124    128       145 / 134
+//            32 of up to 2000          96      97.9 / 106    128       124 / 112
+//   dim 64,  4 of up to 6000          128      43.0 / 48.1   192      44.1 / 50.5
+//   dim 256, 4 of up to 6000          128      92.3 / 117    192       132 / 149
+static uint64_t rows16_most(uint32_t dim) { return dim == 96 || dim == 128 ? 112 : 192; }
+constexpr uint64_t VX_EVEN_UNITS = 1;
 struct AttnPlan {
     const int* kernel;
     uint32_t block, rows, row_blocks, grid, parts;
@@ -138,7 +148,7 @@ static int plan_attention(int num_cus, const vx_kv_cache* c, const vx_attn_batch
     const uint64_t group = q_heads / c->heads, queries = b->max_queries, rows = queries * group;
     const bool wide = rows > 128 && c->dim <= 128;
     *p = AttnPlan{};
-    p->rows = rows <= VX_EVEN_ROWS && ws ? 16 : wide ? 256 : 128;
+    p->rows = rows <= rows16_most(c->dim) && ws ? 16 : wide ? 256 : 128;
     p->block = p->rows == 256 ? 512 : 256;
     const uint64_t places = (uint64_t)num_cus * (p->rows == 256 || c->dim > 128 ? 1 : 2);  // workgroups that the card holds
     const uint64_t rb = (rows + p->rows - 1) / p->rows;
