@@ -160,6 +160,46 @@ def test_rows_in_order_fill_pages(kv, types):
 
 
 @pytest.mark.parametrize("types", TYPES, ids=["k8v8", "k8v4", "k4v8", "k4v4"])
+@pytest.mark.parametrize("dim", [64, 96, 128, 256])
+@pytest.mark.parametrize("kind", ["aligned", "off_by_one", "off_by_three", "sequences", "shuffled", "gaps"])
+def test_many_rows(kv, types, dim, kind):
+    """Enough tokens to go by fours: runs of slots that begin anywhere, end in a
+    group of four, are broken, or none."""
+    note(f"many rows {types} {dim} {kind}")
+    rng = np.random.default_rng(dim)
+    T, heads = 403, 3
+    slots = {"aligned": np.arange(T), "off_by_one": np.arange(1, T + 1), "off_by_three": np.arange(3, T + 3),
+             "sequences": np.concatenate([np.arange(0, 130), np.arange(146, 146 + 131), np.arange(301, 301 + 142)]),
+             "shuffled": rng.permutation(512)[:T], "gaps": np.arange(T) + np.arange(T) // 7}[kind]
+    outside = rng.choice(T, 9, replace=False) if kind in ("gaps", "sequences") else []
+    slots[outside] = rng.choice([-1, -8, 512, 2 ** 31 - 4], len(outside))
+    cache = vx.KvCache(16, 32, heads, dim, *types)
+    cache.data.fill_(255)
+    k, v = _edge_rows(rng, T, heads, dim), _edge_rows(rng, T, heads, dim)
+    kv.write(cache, _gpu(k), _gpu(v), _i32(slots))
+    ko, vo = (torch.full((T, heads, dim), float("nan"), device=DEV) for _ in range(2))
+    kv.read(ko, vo, cache, _i32(slots))
+    wk, wv = A.values(k, types[0]).astype(np.float32), A.values(v, types[1]).astype(np.float32)
+    wk[outside], wv[outside] = 0, 0
+    assert np.array_equal(ko.cpu().numpy(), wk) and np.array_equal(vo.cpu().numpy(), wv)
+    # attention reads what was written, sizes of the scales among it
+    inside = slots[(slots >= 0) & (slots < 512)]
+    other = vx.KvCache(16, 32, heads, dim, *types)
+    other.data.fill_(255)
+    for i in np.argsort(rng.random(T))[:]:
+        if 0 <= slots[i] < 512 and i % 97 == 0:  # some, one by one
+            kv.write(other, _gpu(k[i:i + 1]), _gpu(v[i:i + 1]), _i32(slots[i:i + 1]))
+            at = int(slots[i])
+            one = [kv.plan(c, _i32([[at // 32]]), _i32([at % 32 + 1]), _i32([0, 1]), q_heads=heads, max_queries=1, max_len=32,
+                           first=_i32([at % 32])) for c in (cache, other)]
+            q, outs = _gpu(_normal(rng, 1, heads, dim)), [torch.empty(1, heads, dim, device=DEV) for _ in range(2)]
+            for plan, out in zip(one, outs):
+                kv.attend(out, q, plan)
+            assert torch.equal(outs[0], outs[1])
+    assert len(inside) >= T - 9
+
+
+@pytest.mark.parametrize("types", TYPES, ids=["k8v8", "k8v4", "k4v8", "k4v4"])
 def test_writing_a_slot_leaves_the_others(kv, types):
     rng = np.random.default_rng(5)
     cache = vx.KvCache(3, 16, 2, 96, *types)

@@ -1,6 +1,10 @@
 // vx_kv_rows.hpp — rows into the quantized cache and out of it.
 //
-// Eight lanes take a block of 32 values of K and of V, four values each.
+// Eight lanes take a block of 32 values of K and of V, four values each, of one
+// token, or of four whose slots are a record's group of four keys: their V bytes
+// make up whole words, where one token's go byte by byte.
+// 8000 tokens of 8 heads of 128 written and read back, K in 8 and V in 4 bits:
+// 49 us token by token, now 42; 51000 tokens read back, both in 4 bits: 99, now 74.
 // Quantization of a block x: d = f16(max|x| / 127) and q = clamp(rint(x r),
 // -127, 127) at 8 bits; d = f16(m / -8) with m the value of the largest
 // magnitude (the positive one of two) and q = clamp(rint(x r), -8, 7) at 4,
@@ -113,35 +117,140 @@ __device__ __forceinline__ uint32_t vx_kv_put_v(uint8_t* rec, uint32_t key, uint
     return vx_kv_size(__builtin_bit_cast(uint16_t, d));
 }
 
+// Tokens that a group of lanes takes: one, or (many tokens) four, cut so that
+// the first token's run of slots begins a group of four keys where it does.
+struct vx_kv_tokens {
+    int64_t first;
+    bool four;  // all there, and their slots are a record's group of four keys
+    __device__ __forceinline__ vx_kv_tokens(const vx_kv_rows_args& a, uint64_t n) {
+        four = false;
+        first = (int64_t)n;
+        if (a.quads) {
+            first = 4 * (int64_t)n - (a.slots[0] & 3);
+            if (first < 0 || first + 3 >= a.tokens) return;
+            const int32_t* s = a.slots + first;
+            const int32_t s0 = s[0];
+            four = (s0 & 3) == 0 && s[1] == s0 + 1 && s[2] == s0 + 2 && s[3] == s0 + 3;
+        }
+    }
+};
+
+// Four tokens' scales, codes and sizes (a byte a token) of a block.
+template <int BITS>
+__device__ __forceinline__ void vx_kv_quantize4(const f4 (&x)[4], uint32_t (&w)[4], u2& d, uint32_t& lo, uint32_t& hi) {
+    uint32_t h[4], e[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        float r;
+        h[i] = __builtin_bit_cast(uint16_t, vx_kv_scale<BITS>(x[i], r));
+        w[i] = vx_kv_codes<BITS>(x[i], r);
+        e[i] = vx_kv_size(h[i]);
+    }
+    d = u2{h[0] | h[1] << 16, h[2] | h[3] << 16};
+    lo = e[0] | e[1] << 16;  // sizes in halves, for packed maxima
+    hi = e[2] | e[3] << 16;
+}
+
+template <int NP>
+__device__ __forceinline__ uint32_t vx_kv_max_halves(uint32_t v) {
+    typedef uint16_t us2 __attribute__((ext_vector_type(2)));
+#pragma unroll
+    for (int o = 8; o < 8 * NP; o <<= 1) {
+        const uint32_t w = (uint32_t)__shfl_xor((int)v, o);
+        v = __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(us2, v), __builtin_bit_cast(us2, w)));
+    }
+    return v;
+}
+__device__ __forceinline__ uint32_t vx_kv_bytes(uint32_t lo, uint32_t hi) { return (lo & 255u) | (lo >> 8 & 0xFF00u) | (hi & 255u) << 16 | (hi >> 16) << 24; }
+
+// The dims 4 u + 2 p, + 1 of four keys (codes w, a byte a dim) as the record has them: V
+template <int BITS>
+__device__ __forceinline__ u2 vx_kv_v4(const uint32_t (&w)[4], int p) {
+    uint32_t c[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) c[i] = w[i] >> (16 * p) & 0xFFFFu;
+    if constexpr (BITS == 8)
+        return u2{(c[0] & 255u) | (c[1] & 255u) << 8 | (c[2] & 255u) << 16 | c[3] << 24,
+                  c[0] >> 8 | (c[1] & 0xFF00u) | (c[2] >> 8) << 16 | (c[3] >> 8) << 24};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) c[i] = (c[i] | c[i] >> 4) & 255u;  // two nibbles
+    return u2{c[0] | c[2] << 8 | c[1] << 16 | c[3] << 24, 0u};
+}
+
 template <int NB, int KB, int VB>
 __device__ __forceinline__ void vx_kv_write_rows(const vx_kv_rows_args& a) {
     using R = vx_kv_rec<NB, KB, VB>;
+    using PK = vx_kv_part<NB, KB>;
+    using PV = vx_kv_part<NB, VB>;
     constexpr uint32_t NP = NB == 3 ? 4 : NB;  // lanes of a row: 8 NP, a power of two
-    const uint64_t units = (uint64_t)a.tokens * a.c.heads * NP;
+    const uint64_t units = (uint64_t)a.groups * a.c.heads * NP;
     const uint32_t u = threadIdx.x & 7, b = (threadIdx.x >> 3) % NP;
     for (uint64_t n = (uint64_t)blockIdx.x * 32 + (threadIdx.x >> 3); n < units; n += (uint64_t)gridDim.x * 32) {
         const uint64_t th = n / NP;
-        const uint32_t t = (uint32_t)(th / a.c.heads), h = (uint32_t)(th - (uint64_t)t * a.c.heads);
+        const uint32_t group = (uint32_t)(th / a.c.heads), h = (uint32_t)(th - (uint64_t)group * a.c.heads);
+        const vx_kv_tokens run(a, group);
+        const uint32_t d = 32 * b + 4 * u;
+#pragma unroll 1
+        for (int64_t t = run.first; t < run.first + (a.quads && !run.four ? 4 : 1); ++t) {  // (the same for the row's lanes)
+        if (t < 0 || t >= a.tokens) continue;
         const uint32_t slot = (uint32_t)a.slots[t];
-        const uint32_t page = slot >> a.c.page_shift, key = slot & ((1u << a.c.page_shift) - 1u);
-        if ((int32_t)slot < 0 || page >= a.c.pages) continue;  // (the same for the row's lanes)
+        const uint32_t page = slot >> a.c.page_shift, key = slot & ((1u << a.c.page_shift) - 1u), m = key & 15;
+        if ((int32_t)slot < 0 || page >= a.c.pages) continue;
         uint8_t* rec = a.c.base + vx_kv_page(a.c, page, h, R::BYTES) + (uint64_t)(key >> 4) * R::BYTES;
+        const float* kp = a.k + t * a.ks[0] + (int64_t)h * a.ks[1];
+        const float* vp = a.v + t * a.vs[0] + (int64_t)h * a.vs[1];
+        if (run.four) {
+            uint32_t klo = 0, khi = 0, vlo = 0, vhi = 0;
+            if (b < NB) {
+                f4 x[4], y[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    x[i] = vx_kv_get4(kp + i * a.ks[0], a.ks[2], d, a.vec);
+                    y[i] = vx_kv_get4(vp + i * a.vs[0], a.vs[2], d, a.vec);
+                }
+                uint32_t w[4];
+                u2 sc;
+                vx_kv_quantize4<KB>(x, w, sc, klo, khi);
+#pragma unroll
+                for (uint32_t i = 0; i < 4; ++i) {
+                    uint8_t* p = rec + PK::at(b, (u >> 1) * 16 + m + i);
+                    if constexpr (KB == 8) *(uint32_t*)(p + 4 * (u & 1)) = w[i];
+                    else {
+                        const uint32_t k4 = (w[i] & 15u) | ((w[i] >> 8 & 15u) << 16) | ((w[i] >> 16 & 15u) << 4) | ((w[i] >> 24) << 20);
+                        const uint32_t o = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)k4, 0xB1, 0xF, 0xF, false);
+                        if ((u & 1) == 0) *(uint32_t*)p = k4 | (o << 8);
+                    }
+                }
+                if (u == 0) *(u2*)(rec + PK::VALS + ((m >> 2) * NB + b) * 8) = sc;
+                vx_kv_quantize4<VB>(y, w, sc, vlo, vhi);
+#pragma unroll
+                for (uint32_t p = 0; p < 2; ++p) {
+                    uint8_t* q = rec + R::V + PV::at(b, (m >> 2) * 16 + 2 * u + p);
+                    const u2 v = vx_kv_v4<VB>(w, p);
+                    if constexpr (VB == 8) *(u2*)q = v;
+                    else *(uint32_t*)q = v.x;
+                }
+                if (u == 0) *(u2*)(rec + R::V + PV::VALS + ((m >> 2) * NB + b) * 8) = sc;
+            }
+            klo = vx_kv_max_halves<NP>(klo), khi = vx_kv_max_halves<NP>(khi);
+            vlo = vx_kv_max_halves<NP>(vlo), vhi = vx_kv_max_halves<NP>(vhi);
+            if (u == 0 && b == 0) {
+                *(uint32_t*)(rec + R::K_SIZES + m) = vx_kv_bytes(klo, khi);
+                *(uint32_t*)(rec + R::V_SIZES + m) = vx_kv_bytes(vlo, vhi);
+            }
+            continue;
+        }
         uint32_t size = 0;  // of K above, of V below
         if (b < NB) {
-            const uint32_t d = 32 * b + 4 * u;
-            const f4 k = vx_kv_get4(a.k + (int64_t)t * a.ks[0] + (int64_t)h * a.ks[1], a.ks[2], d, a.vec);
-            const f4 v = vx_kv_get4(a.v + (int64_t)t * a.vs[0] + (int64_t)h * a.vs[1], a.vs[2], d, a.vec);
-            size = vx_kv_put_k<NB, KB>(rec, key & 15, b, u, k) << 16;
-            size |= vx_kv_put_v<NB, VB>(rec + R::V, key & 15, b, u, v);
+            const f4 k = vx_kv_get4(kp, a.ks[2], d, a.vec), v = vx_kv_get4(vp, a.vs[2], d, a.vec);
+            size = vx_kv_put_k<NB, KB>(rec, m, b, u, k) << 16;
+            size |= vx_kv_put_v<NB, VB>(rec + R::V, m, b, u, v);
         }
-#pragma unroll
-        for (uint32_t o = 8; o < 8 * NP; o <<= 1) {
-            const uint32_t w = (uint32_t)__shfl_xor((int)size, (int)o);
-            size = max(size & 0xFFFF0000u, w & 0xFFFF0000u) | max(size & 255u, w & 255u);
-        }
+        size = vx_kv_max_halves<NP>(size);
         if (u == 0 && b == 0) {
-            rec[R::K_SIZES + (key & 15)] = (uint8_t)(size >> 16);
-            rec[R::V_SIZES + (key & 15)] = (uint8_t)size;
+            rec[R::K_SIZES + m] = (uint8_t)(size >> 16);
+            rec[R::V_SIZES + m] = (uint8_t)size;
+        }
         }
     }
 }
@@ -155,60 +264,86 @@ __device__ __forceinline__ void vx_kv_set4(float* p, int64_t sd, uint32_t d, boo
     for (uint32_t i = 0; i < 4; ++i) p[(d + i) * sd] = x[i];
 }
 
+// Dims 4 u .. of a key: K. One dword holds them (8 bits) or eight (4 bits).
+template <int BITS>
+__device__ __forceinline__ f4 vx_kv_k_values(uint32_t w, uint32_t u, float s) {
+    f4 x;
+    constexpr int at[4] = {0, 16, 4, 20};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = s * (float)(BITS == 8 ? (int)(w >> (8 * i) & 255u) - 128 : (int)(w >> (8 * (u & 1) + at[i]) & 15u) - 8);
+    return x;
+}
+// Dims 4 u .. of key j of four: V, from the words of dims 4 u (+ 1) and 4 u + 2 (+ 1).
+template <int BITS>
+__device__ __forceinline__ f4 vx_kv_v_values(const u2 (&w)[2], uint32_t j, float s) {
+    f4 x;
+    const uint32_t sh = BITS == 8 ? 8 * j : 8 * ((j >> 1) | ((j & 1) << 1));
+#pragma unroll
+    for (int p = 0; p < 2; ++p) {
+        x[2 * p] = s * (float)(BITS == 8 ? (int)(w[p].x >> sh & 255u) - 128 : (int)(w[p].x >> sh & 15u) - 8);
+        x[2 * p + 1] = s * (float)(BITS == 8 ? (int)(w[p].y >> sh & 255u) - 128 : (int)(w[p].x >> (sh + 4) & 15u) - 8);
+    }
+    return x;
+}
+
 template <int NB, int KB, int VB>
 __device__ __forceinline__ void vx_kv_read_rows(const vx_kv_rows_args& a) {
+    using R = vx_kv_rec<NB, KB, VB>;
     using PK = vx_kv_part<NB, KB>;
     using PV = vx_kv_part<NB, VB>;
-    constexpr uint32_t REC = vx_kv_rec<NB, KB, VB>::BYTES;
-    const uint64_t units = (uint64_t)a.tokens * a.c.heads * NB;
+    const uint64_t units = (uint64_t)a.groups * a.c.heads * NB;
     const uint32_t u = threadIdx.x & 7;
     for (uint64_t n = (uint64_t)blockIdx.x * 32 + (threadIdx.x >> 3); n < units; n += (uint64_t)gridDim.x * 32) {
-        const uint32_t b = (uint32_t)(n % NB);
+        const uint32_t b = (uint32_t)(n % NB), d = 32 * b + 4 * u;
         const uint64_t th = n / NB;
-        const uint32_t t = (uint32_t)(th / a.c.heads), h = (uint32_t)(th - (uint64_t)t * a.c.heads);
+        const uint32_t group = (uint32_t)(th / a.c.heads), h = (uint32_t)(th - (uint64_t)group * a.c.heads);
+        const vx_kv_tokens run(a, group);
+#pragma unroll 1
+        for (int64_t t = run.first; t < run.first + (a.quads && !run.four ? 4 : 1); ++t) {
+        if (t < 0 || t >= a.tokens) continue;
         const uint32_t slot = (uint32_t)a.slots[t];
-        const uint32_t page = slot >> a.c.page_shift, key = slot & ((1u << a.c.page_shift) - 1u);
+        const uint32_t page = slot >> a.c.page_shift, key = slot & ((1u << a.c.page_shift) - 1u), m = key & 15;
         const bool in = (int32_t)slot >= 0 && page < a.c.pages;
-        const uint32_t d = 32 * b + 4 * u, m = key & 15, sc = ((m >> 2) * NB + b) * 8 + (m & 3) * 2;
-        const uint8_t* rec = a.c.base + vx_kv_page(a.c, in ? page : 0u, h, REC) + (in ? (uint64_t)(key >> 4) * REC : 0u);
-        if (a.k) {
-            f4 x = {};
-            if (in) {
-                const uint8_t* p = rec + PK::at(b, (u >> 1) * 16 + m);
-                const float s = (float)*(const _Float16*)(rec + PK::VALS + sc);
-                if constexpr (KB == 8) {
-                    const uint32_t w = *(const uint32_t*)(p + 4 * (u & 1));
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) x[i] = s * (float)((int)(w >> (8 * i) & 255u) - 128);
-                } else {
-                    const uint32_t w = *(const uint32_t*)p >> (8 * (u & 1));
-                    constexpr int at[4] = {0, 16, 4, 20};
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) x[i] = s * (float)((int)(w >> at[i] & 15u) - 8);
-                }
-            }
-            vx_kv_set4(a.k + (int64_t)t * a.ks[0] + (int64_t)h * a.ks[1], a.ks[2], d, a.vec, x);
+        float* kp = a.k ? a.k + t * a.ks[0] + (int64_t)h * a.ks[1] : nullptr;
+        float* vp = a.v ? a.v + t * a.vs[0] + (int64_t)h * a.vs[1] : nullptr;
+        if (!in) {
+            if (kp) vx_kv_set4(kp, a.ks[2], d, a.vec, f4{});
+            if (vp) vx_kv_set4(vp, a.vs[2], d, a.vec, f4{});
+            continue;
         }
-        if (a.v) {
-            f4 x = {};
-            if (in) {
-                const uint8_t* vrec = rec + PK::BYTES;
-                const float s = (float)*(const _Float16*)(vrec + PV::VALS + sc);
-                const uint32_t j = m & 3;
+        const uint8_t* rec = a.c.base + vx_kv_page(a.c, page, h, R::BYTES) + (uint64_t)(key >> 4) * R::BYTES;
+        const uint32_t scales = ((m >> 2) * NB + b) * 8;
+        const h4 ks = *(const h4*)(rec + PK::VALS + scales), vs = *(const h4*)(rec + R::V + PV::VALS + scales);
+        u2 vw[2] = {};
+        if (vp) {
 #pragma unroll
-                for (uint32_t i = 0; i < 2; ++i) {
-                    const uint8_t* p = vrec + PV::at(b, (m >> 2) * 16 + 2 * u + i);
-                    if constexpr (VB == 8) {
-                        x[2 * i] = s * (float)((int)p[j] - 128);
-                        x[2 * i + 1] = s * (float)((int)p[4 + j] - 128);
-                    } else {
-                        const uint32_t w = p[(j >> 1) | ((j & 1) << 1)];
-                        x[2 * i] = s * (float)((int)(w & 15u) - 8);
-                        x[2 * i + 1] = s * (float)((int)(w >> 4) - 8);
-                    }
-                }
+            for (uint32_t p = 0; p < 2; ++p) {
+                const uint8_t* q = rec + R::V + PV::at(b, (m >> 2) * 16 + 2 * u + p);
+                if constexpr (VB == 8) vw[p] = *(const u2*)q;
+                else vw[p].x = *(const uint32_t*)q;
             }
-            vx_kv_set4(a.v + (int64_t)t * a.vs[0] + (int64_t)h * a.vs[1], a.vs[2], d, a.vec, x);
+        }
+        if (run.four) {  // (keys 4 g to 4 g + 3: m is the first)
+            if (kp) {
+                uint32_t w[4];
+#pragma unroll
+                for (uint32_t i = 0; i < 4; ++i) w[i] = *(const uint32_t*)(rec + PK::at(b, (u >> 1) * 16 + m + i) + (KB == 8 ? 4 * (u & 1) : 0));
+#pragma unroll
+                for (uint32_t i = 0; i < 4; ++i) vx_kv_set4(kp + i * a.ks[0], a.ks[2], d, a.vec, vx_kv_k_values<KB>(w[i], u, (float)ks[i]));
+            }
+            if (vp) {
+#pragma unroll
+                for (uint32_t i = 0; i < 4; ++i) vx_kv_set4(vp + i * a.vs[0], a.vs[2], d, a.vec, vx_kv_v_values<VB>(vw, i, (float)vs[i]));
+            }
+            continue;
+        }
+        const uint32_t j = m & 3;
+        const float kd = (float)(j & 2 ? (j & 1 ? ks.w : ks.z) : (j & 1 ? ks.y : ks.x)), vd = (float)(j & 2 ? (j & 1 ? vs.w : vs.z) : (j & 1 ? vs.y : vs.x));
+        if (kp) {
+            const uint32_t w = *(const uint32_t*)(rec + PK::at(b, (u >> 1) * 16 + m) + (KB == 8 ? 4 * (u & 1) : 0));
+            vx_kv_set4(kp, a.ks[2], d, a.vec, vx_kv_k_values<KB>(w, u, kd));
+        }
+        if (vp) vx_kv_set4(vp, a.vs[2], d, a.vec, vx_kv_v_values<VB>(vw, j, vd));
         }
     }
 }

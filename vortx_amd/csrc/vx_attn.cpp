@@ -82,6 +82,7 @@ static int rows_view(const void* base, const vx_layout* l, uint32_t dim, Rows* r
     return VX_OK;
 }
 
+constexpr uint32_t VX_QUAD_TOKENS = 256;
 static int run_rows(vx_ctx ctx, vx_stream stream, const vx_kv_cache* cache, const vx_cview* k, const vx_cview* v,
                     const int32_t* slots, bool write) {
     clear_error();
@@ -112,7 +113,9 @@ static int run_rows(vx_ctx ctx, vx_stream stream, const vx_kv_cache* cache, cons
         a.ks[i] = r[0].stride[i];
         a.vs[i] = r[1].stride[i];
     }
-    const uint64_t units = (uint64_t)a.tokens * cache->heads * (cache->dim == 96 ? 4 : cache->dim / 32);
+    a.quads = a.tokens >= VX_QUAD_TOKENS;
+    a.groups = a.quads ? a.tokens / 4 + 2 : a.tokens;  // (the cut may leave a part at both ends)
+    const uint64_t units = (uint64_t)a.groups * cache->heads * (cache->dim == 96 ? 4 : cache->dim / 32);
     const uint32_t grid = (uint32_t)std::min<uint64_t>((units + 31) / 32, 1u << 20);
     return launch_struct(ctx, kernel_of(cache, write ? kWrite : kRead), grid, 256, stream, &a);
 }

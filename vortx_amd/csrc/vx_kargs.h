@@ -140,6 +140,8 @@ typedef struct vx_kv_rows_args {
     const int32_t* slots;  /* [tokens]; one outside the cache is left out (write) or gives zeros (read) */
     uint32_t tokens;
     uint32_t vec;          /* 1: k and v have stride 1 along the dim and 16-byte aligned rows */
+    uint32_t quads;        /* 1: tokens go by fours */
+    uint32_t groups;       /* of tokens: one each, or four */
 } vx_kv_rows_args;
 
 /* Attention over the cache. Query row r = j * group + i of a sequence is its
