@@ -117,21 +117,28 @@ __device__ __forceinline__ uint32_t vx_kv_put_v(uint8_t* rec, uint32_t key, uint
     return vx_kv_size(__builtin_bit_cast(uint16_t, d));
 }
 
-// Tokens that a group of lanes takes: one, or (many tokens) four, cut so that
-// the first token's run of slots begins a group of four keys where it does.
+// What a group of lanes does with its tokens, one or (many tokens) four: a token
+// is taken alone, with the three after it where their slots are a record's group
+// of four keys, or not at all where such a four before it has it.
 struct vx_kv_tokens {
-    int64_t first;
-    bool four;  // all there, and their slots are a record's group of four keys
-    __device__ __forceinline__ vx_kv_tokens(const vx_kv_rows_args& a, uint64_t n) {
-        four = false;
-        first = (int64_t)n;
-        if (a.quads) {
-            first = 4 * (int64_t)n - (a.slots[0] & 3);
-            if (first < 0 || first + 3 >= a.tokens) return;
-            const int32_t* s = a.slots + first;
-            const int32_t s0 = s[0];
-            four = (s0 & 3) == 0 && s[1] == s0 + 1 && s[2] == s0 + 2 && s[3] == s0 + 3;
+    uint32_t first, count;
+    uint32_t fours, ones;  // bit i: token first + i
+    __device__ __forceinline__ vx_kv_tokens(const vx_kv_rows_args& a, uint32_t n) : first(n), count(1), fours(0), ones(1) {
+        if (!a.quads) return;
+        first = 4 * n;
+        count = min(4u, a.tokens - first);
+        int32_t s[10];  // slots of tokens first - 3 to first + 6
+#pragma unroll
+        for (int i = 0; i < 10; ++i) {
+            const int64_t t = (int64_t)first + i - 3;
+            s[i] = t >= 0 && t < a.tokens ? a.slots[t] : -1;
         }
+        uint32_t lead = 0;  // bit i: the tokens from first - 3 + i on are such a four
+#pragma unroll
+        for (int i = 0; i < 7; ++i)
+            if (s[i] >= 0 && (s[i] & 3) == 0 && s[i + 1] == s[i] + 1 && s[i + 2] == s[i] + 2 && s[i + 3] == s[i] + 3) lead |= 1u << i;
+        fours = lead >> 3;
+        ones = ~((lead | lead << 1 | lead << 2 | lead << 3) >> 3) & ((1u << count) - 1u);
     }
 };
 
@@ -191,15 +198,17 @@ __device__ __forceinline__ void vx_kv_write_rows(const vx_kv_rows_args& a) {
         const vx_kv_tokens run(a, group);
         const uint32_t d = 32 * b + 4 * u;
 #pragma unroll 1
-        for (int64_t t = run.first; t < run.first + (a.quads && !run.four ? 4 : 1); ++t) {  // (the same for the row's lanes)
-        if (t < 0 || t >= a.tokens) continue;
+        for (uint32_t i = 0; i < run.count; ++i) {  // (the same for the row's lanes)
+        const bool four = run.fours >> i & 1u;
+        if (!four && !(run.ones >> i & 1u)) continue;
+        const int64_t t = run.first + i;
         const uint32_t slot = (uint32_t)a.slots[t];
         const uint32_t page = slot >> a.c.page_shift, key = slot & ((1u << a.c.page_shift) - 1u), m = key & 15;
         if ((int32_t)slot < 0 || page >= a.c.pages) continue;
         uint8_t* rec = a.c.base + vx_kv_page(a.c, page, h, R::BYTES) + (uint64_t)(key >> 4) * R::BYTES;
         const float* kp = a.k + t * a.ks[0] + (int64_t)h * a.ks[1];
         const float* vp = a.v + t * a.vs[0] + (int64_t)h * a.vs[1];
-        if (run.four) {
+        if (four) {
             uint32_t klo = 0, khi = 0, vlo = 0, vhi = 0;
             if (b < NB) {
                 f4 x[4], y[4];
@@ -299,8 +308,10 @@ __device__ __forceinline__ void vx_kv_read_rows(const vx_kv_rows_args& a) {
         const uint32_t group = (uint32_t)(th / a.c.heads), h = (uint32_t)(th - (uint64_t)group * a.c.heads);
         const vx_kv_tokens run(a, group);
 #pragma unroll 1
-        for (int64_t t = run.first; t < run.first + (a.quads && !run.four ? 4 : 1); ++t) {
-        if (t < 0 || t >= a.tokens) continue;
+        for (uint32_t i = 0; i < run.count; ++i) {
+        const bool four = run.fours >> i & 1u;
+        if (!four && !(run.ones >> i & 1u)) continue;
+        const int64_t t = run.first + i;
         const uint32_t slot = (uint32_t)a.slots[t];
         const uint32_t page = slot >> a.c.page_shift, key = slot & ((1u << a.c.page_shift) - 1u), m = key & 15;
         const bool in = (int32_t)slot >= 0 && page < a.c.pages;
@@ -323,7 +334,7 @@ __device__ __forceinline__ void vx_kv_read_rows(const vx_kv_rows_args& a) {
                 else vw[p].x = *(const uint32_t*)q;
             }
         }
-        if (run.four) {  // (keys 4 g to 4 g + 3: m is the first)
+        if (four) {  // (keys 4 g to 4 g + 3: m is the first)
             if (kp) {
                 uint32_t w[4];
 #pragma unroll
