@@ -186,9 +186,10 @@ __device__ __forceinline__ uint64_t vx_div(uint64_t a, uint64_t b) {
 // The key steps of all units (row block, sequence, head) dealt out evenly, a
 // run of them to each workgroup, whatever the lengths. Pair (s, rb) has c steps
 // a head and its heads follow each other; a unit counts COST steps more, in
-// front, for what it takes to begin and to end (without that the first row
+// front, for what it takes to begin and to end: without that the first row
 // blocks of a causal prompt, many short units to a workgroup, took three times
-// the others' time). do_unit takes a unit's keys from..to (end: to its end). A
+// the others' time (8192 tokens, 8 heads over 2 of 128, 64-key steps: COST 0
+// 577 us, 2 438, 4 417, 8 443). do_unit takes a unit's keys from..to (end: to its end). A
 // unit that several workgroups share goes to partial sums:
 // a workgroup's first unit is partial 2 w, its last, if another, 2 w + 1; info
 // has a unit's first partial and their number, for the join.

@@ -10,7 +10,13 @@
 // scale is two f16 terms again. The running maximum M is of score + e, e the
 // exponent of the largest scale that a lane's keys have for V: then P times
 // a scale fills f16's range whatever the magnitude of V.
-// Each of four waves takes every fourth 32 keys; their sums meet in LDS.
+// Each of four waves takes every fourth 32 keys, straight from memory to the
+// registers that the matrix instructions read; their sums meet in LDS.
+// Bound: memory and vector instructions together. 32 sequences of 2400 to 8000
+// keys, 32 heads over 8 of 128 in 8 bits: 78 us, 4.5 TB/s of the cache (vector
+// issue 38 %, matrix cores 10 %); one of 131000, 64 heads over 8, values in 4
+// bits, scores capped: 60 us, 3.6 TB/s (55 %, 12 %). Two waves a SIMD: a third
+// one spills in the loop (120 us for the 78).
 #pragma once
 #include "vx_attn.hpp"
 

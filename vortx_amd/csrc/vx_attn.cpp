@@ -82,6 +82,8 @@ static int rows_view(const void* base, const vx_layout* l, uint32_t dim, Rows* r
     return VX_OK;
 }
 
+// Tokens by fours from so many on: 333 of 3 heads of 64 read back 3.9 us (one by one 4.3), 8000 of
+// 8 heads of 128 written and read 42 (49). Fewer leave most of the card without work.
 constexpr uint32_t VX_QUAD_TOKENS = 256;
 static int run_rows(vx_ctx ctx, vx_stream stream, const vx_kv_cache* cache, const vx_cview* k, const vx_cview* v,
                     const int32_t* slots, bool write) {
@@ -135,6 +137,12 @@ constexpr uint32_t VX_MOST_KEYS = (1u << 31) - 65536u;  // of a sequence
 //   dim 64,  4 of up to 6000          128      43.0 / 48.1   192      44.1 / 50.5
 //   dim 256, 4 of up to 6000          128      92.3 / 117    192       132 / 149
 static uint64_t rows16_most(uint32_t dim) { return dim == 96 || dim == 128 ? 112 : 192; }
+// More units than places: a workgroup each (units of one length, or many of them,
+// fill the card by themselves, and no partial sums are written). Us, a workgroup
+// each / dealt out evenly: 512 units on 256 places, 4096 causal tokens of 32
+// heads of 128, 415 / 476; 480, packed documents, 78 / 119; but 752 of dim 64,
+// two prompts of 3000, 246 / 217. Up to as many: 256, four chunks behind
+// histories of 900 to 3000, 237 / 206; 256, a prompt of 2000, 152 / 146.
 constexpr uint64_t VX_EVEN_UNITS = 1;
 struct AttnPlan {
     const int* kernel;
@@ -149,6 +157,9 @@ struct AttnPlan {
 static int plan_attention(int num_cus, const vx_kv_cache* c, const vx_attn_batch* b, const vx_attn_opts* o, uint32_t q_heads,
                           bool ws, AttnPlan* p) {
     const uint64_t group = q_heads / c->heads, queries = b->max_queries, rows = queries * group;
+    // 256 rows a workgroup decode a tile of keys once where two of 128 do it twice; us, 256 / 128
+    // rows: 4096 causal tokens, dim 128 416 / 468, dim 64 225 / 252; chunks behind histories 215 / 218;
+    // trees of 244 rows 202 / 203, of 200 rows, 16 sequences, 131 / 113. (256 dims: see the kernels.)
     const bool wide = rows > 128 && c->dim <= 128;
     *p = AttnPlan{};
     p->rows = rows <= rows16_most(c->dim) && ws ? 16 : wide ? 256 : 128;
