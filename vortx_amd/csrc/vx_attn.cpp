@@ -162,7 +162,10 @@ static int plan_attention(int num_cus, const vx_kv_cache* c, const vx_attn_batch
     // trees of 244 rows 202 / 203, of 200 rows, 16 sequences, 131 / 113. (256 dims: see the kernels.)
     const bool wide = rows > 128 && c->dim <= 128;
     *p = AttnPlan{};
-    p->rows = rows <= rows16_most(c->dim) && ws ? 16 : wide ? 256 : 128;
+    // (the keys are dealt out by their number of steps, which is counted in 32 bits)
+    const uint64_t most = std::min<uint64_t>(b->max_len, (uint64_t)b->table_cols * c->page_tokens);
+    const bool deal = ws && ((rows + 15) / 16) * b->seqs * (most / 64 + 8) < (1ull << 32);
+    p->rows = rows <= rows16_most(c->dim) && deal ? 16 : wide ? 256 : 128;
     p->block = p->rows == 256 ? 512 : 256;
     const uint64_t places = (uint64_t)num_cus * (p->rows == 256 || c->dim > 128 ? 1 : 2);  // workgroups that the card holds
     const uint64_t rb = (rows + p->rows - 1) / p->rows;
@@ -170,11 +173,11 @@ static int plan_attention(int num_cus, const vx_kv_cache* c, const vx_attn_batch
     if (p->units >= (1ull << 23) || rows * b->seqs * c->heads >= (1ull << 24))
         return fail(VX_ERR_UNSUPPORTED, "attention: too many query rows (split the batch)");
     p->row_blocks = (uint32_t)rb;
-    p->even = ws && (p->rows == 16 || p->units <= VX_EVEN_UNITS * places);
+    p->even = deal && (p->rows == 16 || p->units <= VX_EVEN_UNITS * places);
     p->kernel = p->rows == 16 ? kEven16 : p->rows == 128 ? (p->even ? kEven128 : kEach128) : (p->even ? kEven256 : kEach256);
     p->grid = (uint32_t)p->units;
     if (p->even) {
-        uint64_t span = std::min<uint64_t>(b->max_len, (uint64_t)b->table_cols * c->page_tokens);
+        uint64_t span = most;
         if (o && o->window) span = std::min<uint64_t>(span, 2ull * o->window + queries + 64);
         const uint64_t step = p->rows == 16 ? 128 : 64;
         p->grid = (uint32_t)std::max<uint64_t>(1, std::min(p->units * ((span + step - 1) / step + 1), places));
