@@ -197,10 +197,12 @@ static int init(int device, vx_ctx* out) {
             return VX_ERR_NO_CODE_OBJECT;
         }
     }
-    for (int k = 0; k < K_COUNT; ++k) {
+    for (int k = 0, at = 0; k < K_COUNT; ++k) {
         e = hipErrorNotFound;
-        for (int i = 0; i < kNumModules && e != hipSuccess; ++i) {
-            e = hipModuleGetFunction(&ctx->fn[k], ctx->mods[i], kKernelNames[k]);
+        for (int i = 0; i < kNumModules && e != hipSuccess; ++i) {  // from the module of the kernel before: the list goes by modules
+            const int mod = (at + i) % kNumModules;
+            e = hipModuleGetFunction(&ctx->fn[k], ctx->mods[mod], kKernelNames[k]);
+            if (e == hipSuccess) at = mod;
             // a miss in one module is expected; do not leave it as the
             // runtime's last error for the caller's next HIP call
             if (e != hipSuccess) (void)hipGetLastError();
