@@ -399,6 +399,45 @@ def test_values_of_all_sizes_in_one_history(kv, queries):
     b.check(kv, first=np.where(np.arange(320 - queries, 320) < 256, 0, 256))
 
 
+@pytest.mark.parametrize("queries,group", [(2, 2), (40, 4), (90, 4)])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("side", ["k", "v", "both"])
+@pytest.mark.parametrize("types,huge", [((Q8, Q8), 1e6), ((Q4, Q8), 5e4)], ids=["k8v8", "k4v8"])
+def test_huge_keys_out_of_sight_cost_the_others_nothing(kv, queries, group, dim, side, types, huge):
+    """Keys before the document and every other draft are 2^15 or 2^20 larger, and no row sees them."""
+    rng = np.random.default_rng(14)
+    L = 200 + queries
+    k, v = [_normal(rng, L, 1, dim)], [_normal(rng, L, 1, dim)]
+    first = 111  # the last of its four keys
+    trees = np.zeros((queries, queries), bool)
+    trees[np.arange(queries), np.arange(queries)] = True
+    trees[:, ::2] = False  # no row sees an even draft
+    for x, on in ((k, side != "v"), (v, side != "k")):
+        if on:
+            x[0][:first] *= np.float32(huge)
+            x[0][L - queries:][::2] *= np.float32(huge)
+    b = Batch(kv, rng, [L], [queries], 1, group, dim, 16, types, k=k, v=v)
+    b.check(kv, trees=[trees], first=np.full(queries, first))
+
+
+@pytest.mark.parametrize("queries", [2, 90])
+def test_a_huge_value_of_no_weight(kv, queries):
+    """A key that every row sees with a score far below the others', its value 2^28 larger than theirs."""
+    rng = np.random.default_rng(15)
+    L = 200 + queries
+    k, v = [_normal(rng, L, 1, 64) * np.float32(0.1)], [_normal(rng, L, 1, 64) * np.float32(0.01)]
+    b = Batch(kv, rng, [L], [queries], 1, 2, 64, 16, (Q8, Q8), k=k, v=v)
+    b.q[..., 0] = 40.0
+    k[0][50], v[0][50] = 0.0, 1e6
+    k[0][50, 0, 0] = -100.0
+    c = Batch(kv, rng, [L], [queries], 1, 2, 64, 16, (Q8, Q8), k=k, v=v)
+    want, _ = A.attend(b.q, c.kd, c.vd, c.starts, c.lens)
+    _, tol = A.attend(b.q, b.kd, [np.clip(x, -1, 1) for x in b.vd], b.starts, b.lens)
+    out = torch.empty(b.q.shape, device=DEV)
+    kv.attend(out, _gpu(b.q), c.plan(kv))
+    assert (np.abs(out.cpu().numpy() - want) <= tol).all()
+
+
 @pytest.mark.parametrize("size", [1e-35, 1e-4, 1e30])
 def test_queries_of_any_size(kv, size):
     rng = np.random.default_rng(4)

@@ -8,8 +8,8 @@
 // power of two per row (22 bits); the cached whole numbers are exact in f16, a
 // block's scale is applied to its 32-dim product in f32. P times a value's
 // scale is two f16 terms again. The running maximum M is of score + e, e the
-// exponent of the largest scale that a lane's keys have for V: then P times
-// a scale fills f16's range whatever the magnitude of V.
+// exponent of the key's largest scale for V: then P times a scale fills f16's
+// range whatever the magnitude of V.
 // Each of four waves takes every fourth 32 keys, straight from memory to the
 // registers that the matrix instructions read; their sums meet in LDS.
 // Bound: memory and vector instructions together. 32 sequences of 2400 to 8000
@@ -243,26 +243,28 @@ struct vx_rows16 {
                     }
             }
             // running maximum of score + exponent of V's scales
-            float top = fmaxf(fmaxf(fmaxf(x[0][0], x[0][1]), fmaxf(x[0][2], x[0][3])), fmaxf(fmaxf(x[1][0], x[1][1]), fmaxf(x[1][2], x[1][3])));
+            float top = -__builtin_inff();
             {
-                uint32_t e = 0;
-#pragma unroll
-                for (int t = 0; t < 2; ++t)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) e = max(e, rv.e[t] >> (8 * i) & 255u);
-                if (__any(e == 255u)) {  // a scale that is not finite: the largest of the others
-                    e = 0;
+                if (__any((rv.e[0] | rv.e[1]) & 0x80808080u)) {  // a scale that is not finite (255): the largest of the others
 #pragma unroll
                     for (int t = 0; t < 2; ++t)
 #pragma unroll
-                        for (int b = 0; b < NB; ++b)
+                        for (int i = 0; i < 4; ++i) {
+                            uint32_t e = 0;
 #pragma unroll
-                            for (int i = 0; i < 4; ++i) {
+                            for (int b = 0; b < NB; ++b) {
                                 const uint32_t d = vx_kv_size(rv.s[t][b][i >> 1] >> (16 * (i & 1)));
                                 e = max(e, d == 255u ? 0u : d);
                             }
+                            top = fmaxf(top, x[t][i] + (float)e);
+                        }
+                } else {
+#pragma unroll
+                    for (int t = 0; t < 2; ++t)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) top = fmaxf(top, x[t][i] + (float)(rv.e[t] >> (8 * i) & 255u));
                 }
-                top = vx_max_rows4(top + (float)((int)e - 29));  // P times scale below 2^14
+                top = vx_max_rows4(top - 29.f);  // P times scale below 2^14
             }
             const float Mn = fmaxf(M, top), Mr = Mn == -__builtin_inff() ? 0.f : Mn;
             if (__any(Mn != M)) {

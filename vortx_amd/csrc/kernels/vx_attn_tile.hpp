@@ -8,7 +8,8 @@
 // exact: hi rounds the product, lo = fma(number, scale, -hi). The scales of each
 // four keys are first brought below 2 by a power of two, which K's scores take
 // back as a factor, and V's weights: w = exp2(score + e - M), so V of any
-// magnitude fills f16's range, and the weights' sum takes w 2^-e.
+// magnitude fills f16's range, and the weights' sum takes w 2^-e. Four keys that
+// are more than 2^10 apart, some of which a row may not see, have a power each.
 // (With K as whole numbers, exact in one term, and its scales on the 32-dim
 // products, a tile had 8 matrix instructions fewer and 64 multiply-adds and 32
 // registers a wave more: 430 us where this takes 415, 4096 causal tokens of
@@ -45,7 +46,8 @@ struct vx_tile {
     struct tile {
         h8 k[NB * 2 * 2 * 64];  // [block][16 dims][hi, lo][half, key]
         h8 v[NB * 2 * 2 * 64];  // [block][16 keys][hi, lo][half, dim]
-        f2 e[8];                // of four keys: 2^exponent of K's scales, exponent of V's
+        f2 e[8];                // of four keys: 2^exponent of K's scales (negative: see key), exponent of V's
+        f2 key[32];             // of keys far apart: what their own powers are to those, factor and difference
         uint32_t bad[8];        // their V scales that are not finite, bit 4 block + key
     };
 
@@ -65,6 +67,9 @@ struct vx_tile {
             w[0] = *(const uint32_t*)q;
         }
     }
+
+    static constexpr uint32_t FAR = 10;  // f16 holds both terms of a key that is 2^10 below to 22 bits
+    static __device__ __forceinline__ int power(uint32_t size) { return max((int)size - 16, -15); }  // (of no key: size 0)
 
     // the record of the 16 keys from key on; past the end the last one
     static __device__ __forceinline__ const uint8_t* record(const vx_attn_args& a, vx_scalar_i32 table, const uint8_t* base, int key, int last) {
@@ -96,9 +101,22 @@ struct vx_tile {
     static __device__ __forceinline__ void store(const vx_attn_args& a, vx_scalar_i32 table, const uint8_t* base, raw& r, tile& s, int k0, int last) {
         const uint32_t t = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(t >> 6), rec = wave & 1, lane = t & 63, m = lane & 15, g = lane >> 4;
         uint32_t bad = 0;
-        auto largest = [&](uint32_t e) { return max(max(e & 255u, e >> 8 & 255u), max(e >> 16 & 255u, e >> 24)); };
-        uint32_t size = largest(r.e), ksize = largest(r.ke);
-        if (k0 + 32 > last + 1 || __any(max(size, ksize) == 255u)) {
+        // largest of four sizes, and whether another is far below it
+        auto largest = [](uint32_t e, bool& far) {
+            typedef uint16_t us2 __attribute__((ext_vector_type(2)));
+            const us2 lo = __builtin_bit_cast(us2, e & 0x00FF00FFu), hi = __builtin_bit_cast(us2, e >> 8 & 0x00FF00FFu);
+            const us2 most = __builtin_elementwise_max(lo, hi), least = __builtin_elementwise_min(lo, hi);
+            const uint32_t top = max((uint32_t)most.x, (uint32_t)most.y);
+            far = top > min((uint32_t)least.x, (uint32_t)least.y) + FAR;
+            return top;
+        };
+        bool far, kfar;
+        uint32_t size = largest(r.e, far), ksize = largest(r.ke, kfar);
+        auto below = [](uint32_t v) { return (_Float16)__builtin_ldexpf(1.f, -power(v)); };
+        h2 f0, f1;  // what V's four keys and K's key are brought down by
+        _Float16 fk;
+        float sign = 1.f;
+        if (k0 + 32 > last + 1 || __any(far | kfar | (max(size, ksize) == 255u))) {
             // scales of keys that do not exist, which may be anything: 0; those that are not finite: 0, and noted
             const int valid = last + 1 - (k0 + 16 * (int)rec + 4 * (int)g);
             auto fix = [&](uint32_t d, int i) {
@@ -122,21 +140,43 @@ struct vx_tile {
                     else e[i] = max(e[i], v);
                 }
             size = max(max(e[0], e[1]), max(e[2], e[3]));
+            uint32_t least = size;
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (valid > i) least = min(least, e[i]);
+            far = size > least + FAR;
+            uint32_t own[4], kown = 0;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) own[i] = far ? e[i] : size;
+            f0 = h2{below(own[0]), below(own[1])}, f1 = h2{below(own[2]), below(own[3])};
             // K's keys that do not exist or are not finite: the others' exponent
             const int kvalid = last + 1 - (k0 + 16 * (int)rec + 4 * (int)(m >> 2));
             ksize = 0;
+            least = 255u;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const uint32_t v = r.ke >> (8 * i) & 255u;
-                if (i < kvalid && v != 255u) ksize = max(ksize, v);
+                if (i < kvalid && v != 255u) {
+                    ksize = max(ksize, v);
+                    least = min(least, v);
+                    if (i == (int)(m & 3)) kown = v;
+                }
             }
+            kfar = ksize > least + FAR;
+            if (!kfar) kown = ksize;
+            fk = below(kown);
+            if (far | kfar) sign = -1.f;
+            if (wave < 2 && (m >> 2) == g) {
+                const uint32_t v = m & 2 ? (m & 1 ? own[3] : own[2]) : (m & 1 ? own[1] : own[0]);
+                s.key[rec * 16 + m] = f2{__builtin_ldexpf(1.f, power(kown) - power(ksize)), (float)(power(v) - power(size))};
+            }
+        } else {
+            const _Float16 f = below(size);
+            f0 = f1 = h2{f, f};
+            fk = below(ksize);
         }
-        const int e = max((int)size - 16, -15);  // (of no key: -16)
-        const int ek = max((int)ksize - 16, -15);
-        if (wave < 2 && m == 4 * g) s.e[rec * 4 + g] = f2{__builtin_ldexpf(1.f, ek), (float)e};
+        if (wave < 2 && m == 4 * g) s.e[rec * 4 + g] = f2{__builtin_ldexpf(sign, power(ksize)), (float)power(size)};
         if (wave < 2 && m == 0) s.bad[rec * 4 + g] = bad;
-        const _Float16 f = (_Float16)__builtin_ldexpf(1.f, -e), fk = (_Float16)__builtin_ldexpf(1.f, -ek);
-        const h2 f2h = {f, f};
 #pragma unroll
         for (int i = 0; i < ITEMS; ++i) {
             const int b = (int)(wave >> 1) + WAVES / 2 * i;
@@ -162,7 +202,7 @@ struct vx_tile {
             kat[0] = h8{kh[0].x, kh[0].y, kh[1].x, kh[1].y, kh[2].x, kh[2].y, kh[3].x, kh[3].y};
             kat[64] = h8{kl[0].x, kl[0].y, kl[1].x, kl[1].y, kl[2].x, kl[2].y, kl[3].x, kl[3].y};
             const uint32_t d0 = r.d[i][0], d1 = r.d[i][1];
-            const h2 r0 = __builtin_bit_cast(h2, d0) * f2h, r1 = __builtin_bit_cast(h2, d1) * f2h;
+            const h2 r0 = __builtin_bit_cast(h2, d0) * f0, r1 = __builtin_bit_cast(h2, d1) * f1;
 #pragma unroll
             for (int v = 0; v < 2; ++v) {
                 h2 x0, x1;
@@ -338,15 +378,27 @@ struct vx_tile {
                     __builtin_amdgcn_sched_barrier(6);
                 }
                 __builtin_amdgcn_s_setprio(0);
-                float e[4];
+                float e[4], apart = 0.f;
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                     const f2 ke = t.e[4 * (j / 2) + 2 * (j % 2) + (int)h];
-                    const float f = fq * ke.x;
+                    const float f = fq * fabsf(ke.x);
                     e[j] = ke.y;
+                    apart = fminf(apart, ke.x);
 #pragma unroll
                     for (int i = 0; i < 4; ++i) x[4 * j + i] *= f;
                 }
+                // keys far apart: own(register, factor and difference)
+                const bool far = __any(apart < 0.f);
+                auto each_own = [&](auto own) {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        if (t.e[2 * j + (int)h].x < 0.f) {
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) own(4 * j + i, t.key[8 * j + 4 * (int)h + i]);
+                        }
+                };
+                if (far) each_own([&](int i, f2 k) { x[i] *= k.x; });
                 if (a.cap > 0.f) {
                     float big = 0.f;
 #pragma unroll
@@ -387,6 +439,7 @@ struct vx_tile {
                         x[i] = __uint_as_float((v & __float_as_uint(x[i])) | (~v & 0xFF800000u));
                     }
                 }
+                if (far) each_own([&](int i, f2 k) { x[i] += k.y; });
                 // running maximum of score + e: four keys at a time
                 float top = -__builtin_inff();
                 uint32_t bad = 0;
@@ -429,6 +482,8 @@ struct vx_tile {
                         ph[j / 2][k] = u.x, ph[j / 2][k + 1] = u.y, pl[j / 2][k] = v.x, pl[j / 2][k + 1] = v.y;
                     }
                 }
+                if (far)  // the weights' sum takes w 2^-e of the key's own e
+                    each_own([&](int i, f2 k) { l += x[i] * __builtin_ldexpf(__builtin_ldexpf(1.f, -(int)k.y) - 1.f, -(int)e[i / 4]); });
                 __builtin_amdgcn_s_setprio(1);
                 h8 vf[3][2];
                 auto vread = [&](int u) {
