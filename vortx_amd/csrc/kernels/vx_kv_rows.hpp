@@ -317,9 +317,11 @@ __device__ __forceinline__ void vx_kv_read_rows(const vx_kv_rows_args& a) {
         const bool in = (int32_t)slot >= 0 && page < a.c.pages;
         float* kp = a.k ? a.k + t * a.ks[0] + (int64_t)h * a.ks[1] : nullptr;
         float* vp = a.v ? a.v + t * a.vs[0] + (int64_t)h * a.vs[1] : nullptr;
-        if (!in) {
-            if (kp) vx_kv_set4(kp, a.ks[2], d, a.vec, f4{});
-            if (vp) vx_kv_set4(vp, a.vs[2], d, a.vec, f4{});
+        if (!in) {  // (a group of four lies outside as a whole: it is in one page)
+            for (uint32_t i = 0; i < (four ? 4u : 1u); ++i) {
+                if (kp) vx_kv_set4(kp + i * a.ks[0], a.ks[2], d, a.vec, f4{});
+                if (vp) vx_kv_set4(vp + i * a.vs[0], a.vs[2], d, a.vec, f4{});
+            }
             continue;
         }
         const uint8_t* rec = a.c.base + vx_kv_page(a.c, page, h, R::BYTES) + (uint64_t)(key >> 4) * R::BYTES;
