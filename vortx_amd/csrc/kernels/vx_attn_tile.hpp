@@ -10,7 +10,9 @@
 // back as a factor, and V's weights: w = exp2(score + e - M), so V of any
 // magnitude fills f16's range, and the weights' sum takes w 2^-e. Four keys that
 // are more than 2^10 apart, some of which a row may not see, have a power each
-// (2 % of the time below; of 78 us for packed documents of dim 64, 7).
+// (2 % of the time below; of 78 us for packed documents of dim 64, 7). Slots that
+// were never written may hold anything: sizes above 31 are no key's, and a scale
+// of V that its size does not allow is taken as 0.
 // (With K as whole numbers, exact in one term, and its scales on the 32-dim
 // products, a tile had 8 matrix instructions fewer and 64 multiply-adds and 32
 // registers a wave more: 430 us where this took 415, 4096 causal tokens of
@@ -118,7 +120,7 @@ struct vx_tile {
         _Float16 fk;
         float sign = 1.f;
         // (seldom: out of the way of the rest, 2 us of 196, eight trees of 61 drafts)
-        if (__builtin_expect(k0 + 32 > last + 1 || __any(far | kfar | (max(size, ksize) == 255u)), 0)) {
+        if (__builtin_expect(k0 + 32 > last + 1 || __any(far | kfar | (max(size, ksize) > 31u)), 0)) {
             // scales of keys that do not exist, which may be anything: 0; those that are not finite: 0, and noted
             const int valid = last + 1 - (k0 + 16 * (int)rec + 4 * (int)g);
             auto fix = [&](uint32_t d, int i) {
@@ -151,14 +153,14 @@ struct vx_tile {
 #pragma unroll
             for (int i = 0; i < 4; ++i) own[i] = far ? e[i] : size;
             f0 = h2{below(own[0]), below(own[1])}, f1 = h2{below(own[2]), below(own[3])};
-            // K's keys that do not exist or are not finite: the others' exponent
+            // K's keys that do not exist, are not finite or were never written: the others' exponent
             const int kvalid = last + 1 - (k0 + 16 * (int)rec + 4 * (int)(m >> 2));
             ksize = 0;
             least = 255u;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const uint32_t v = r.ke >> (8 * i) & 255u;
-                if (i < kvalid && v != 255u) {
+                if (i < kvalid && v < 32u) {
                     ksize = max(ksize, v);
                     least = min(least, v);
                     if (i == (int)(m & 3)) kown = v;
@@ -176,6 +178,24 @@ struct vx_tile {
             const _Float16 f = below(size);
             f0 = f1 = h2{f, f};
             fk = below(ksize);
+            // a scale of V above what the sizes say is of a key that was never
+            // written, which no row sees: 0, so that its weights' zeros stay zeros
+            typedef uint16_t us2 __attribute__((ext_vector_type(2)));
+            us2 most = {};
+#pragma unroll
+            for (int n = 0; n < ITEMS; ++n)
+#pragma unroll
+                for (int i = 0; i < 2 && (NB % (WAVES / 2) == 0 || (int)(wave >> 1) + WAVES / 2 * n < NB); ++i) most = __builtin_elementwise_max(most, __builtin_bit_cast(us2, r.d[n][i] & 0x7FFF7FFFu));
+            const uint32_t limit = max(size, 1u) << 10;
+            if (__builtin_expect(__any(max((uint32_t)most.x, (uint32_t)most.y) >= limit), 0)) {
+#pragma unroll
+                for (int n = 0; n < ITEMS; ++n)
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        if ((r.d[n][i] & 0x7FFFu) >= limit) r.d[n][i] &= 0xFFFF0000u;
+                        if ((r.d[n][i] >> 16 & 0x7FFFu) >= limit) r.d[n][i] &= 0x0000FFFFu;
+                    }
+            }
         }
         if (wave < 2 && m == 4 * g) s.e[rec * 4 + g] = f2{__builtin_ldexpf(sign, power(ksize)), (float)power(size)};
         if (wave < 2 && m == 0) s.bad[rec * 4 + g] = bad;
