@@ -490,9 +490,11 @@ typedef struct vx_attn_opts {
 /* out = softmax(score) V for each query token and head: q and out are
  * [tokens, query heads, dim] f32 views of any strides, query heads a multiple
  * of the cache's heads (query head h reads head h / (query heads / heads)).
- * q is taken as two f16 terms per value (22 bits, scaled by a power of two per
- * row), scores, softmax and sums are f32, products of the exactly decoded
- * cache on the f16 matrix cores. A query that sees no key gives zeros. Keys
+ * q is taken as two f16 terms per value, scaled by a power of two per row (22
+ * bits; fewer of values more than 2^17 below the row's largest), scores, softmax
+ * and sums are f32, products of the exactly decoded cache on the f16 matrix
+ * cores, whatever the sizes of its blocks: a result is as precise as the values
+ * of its own block of 32 dims allow. A query that sees no key gives zeros. Keys
  * that a query does not see never reach its result, whatever they hold; a NaN
  * that it sees in K makes its whole row NaN, one in V the 32 values of that
  * block. opts NULL: scale 1 / sqrt(dim) and no mask.

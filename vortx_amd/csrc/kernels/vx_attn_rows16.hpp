@@ -12,6 +12,9 @@
 // range whatever the magnitude of V.
 // Each of four waves takes every fourth 32 keys, straight from memory to the
 // registers that the matrix instructions read; their sums meet in LDS.
+// Where a row sees a key whose blocks of V are more than 2^10 apart (its size byte
+// says so), P times scale has a power of two for each row and block: under the
+// one of its largest block a block 2^23 smaller would keep 14 bits.
 // Bound: memory and vector instructions together. 32 sequences of 2400 to 8000
 // keys, 32 heads over 8 of 128 in 8 bits: 78 us, 4.5 TB/s of the cache (vector
 // issue 38 %, matrix cores 10 %); one of 131000, 64 heads over 8, values in 4
@@ -244,8 +247,10 @@ struct vx_rows16 {
             }
             // running maximum of score + exponent of V's scales
             float top = -__builtin_inff();
+            // keys that a row sees whose blocks are far apart or not finite
+            const bool rough = __any((rv.e[0] | rv.e[1]) & 0x80808080u);
             {
-                if (__any((rv.e[0] | rv.e[1]) & 0x80808080u)) {  // a scale that is not finite (255): the largest of the others
+                if (__builtin_expect(rough, 0)) {  // the largest of the finite scales
 #pragma unroll
                     for (int t = 0; t < 2; ++t)
 #pragma unroll
@@ -283,6 +288,48 @@ struct vx_rows16 {
                     x[t][i] = __builtin_amdgcn_exp2f(x[t][i] - Mr);
                     l += x[t][i];
                 }
+            auto vfrag = [&](int b, int v) {
+                h2 v0, v1, v2, v3;
+                vx_kv_vfrag<NB, VB>(rv.w[0], b, v, v0, v1);
+                vx_kv_vfrag<NB, VB>(rv.w[1], b, v, v2, v3);
+                return h8{v0.x, v0.y, v1.x, v1.y, v2.x, v2.y, v3.x, v3.y};
+            };
+            if (__builtin_expect(rough, 0)) {
+#pragma unroll
+                for (int b = 0; b < NB; ++b) {
+                    __builtin_amdgcn_sched_barrier(0);  // (one block at a time: registers)
+                    float most = 0.f;
+#pragma unroll
+                    for (int t = 0; t < 2; ++t)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const h2 d = __builtin_bit_cast(h2, rv.s[t][b][i >> 1]);
+                            most = fmaxf(most, fabsf(x[t][i] * (float)(i & 1 ? d.y : d.x)));  // (not a NaN)
+                        }
+                    most = vx_max_rows4(most);
+                    const int e = most > 0x1p-100f ? __builtin_amdgcn_frexp_expf(most) : -100;
+                    h8 ph, pl;
+#pragma unroll
+                    for (int t = 0; t < 2; ++t)
+#pragma unroll
+                        for (int i = 0; i < 4; i += 2) {
+                            const h2 d = __builtin_bit_cast(h2, rv.s[t][b][i >> 1]);
+                            h2 hi, lo;  // (below 2^15)
+                            vx_two_terms(__builtin_ldexpf(x[t][i] * (float)d.x, 15 - e), __builtin_ldexpf(x[t][i + 1] * (float)d.y, 15 - e), hi, lo);
+                            const int n = 4 * t + i;
+                            ph[n] = hi.x, ph[n + 1] = hi.y, pl[n] = lo.x, pl[n + 1] = lo.y;
+                        }
+#pragma unroll
+                    for (int v = 0; v < 2; ++v) {
+                        const h8 vf = vfrag(b, v);
+                        f4 acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, ph, f4{}, 0, 0, 0);
+                        acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, pl, acc, 0, 0, 0);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) o[b][v][i] += __builtin_ldexpf(acc[i], e - 15);
+                    }
+                }
+                continue;
+            }
 #pragma unroll
             for (int b = 0; b < NB; ++b) {
                 h8 ph, pl;
@@ -297,10 +344,7 @@ struct vx_rows16 {
                     }
 #pragma unroll
                 for (int v = 0; v < 2; ++v) {
-                    h2 v0, v1, v2, v3;
-                    vx_kv_vfrag<NB, VB>(rv.w[0], b, v, v0, v1);
-                    vx_kv_vfrag<NB, VB>(rv.w[1], b, v, v2, v3);
-                    const h8 vf = {v0.x, v0.y, v1.x, v1.y, v2.x, v2.y, v3.x, v3.y};
+                    const h8 vf = vfrag(b, v);
                     o[b][v] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, ph, o[b][v], 0, 0, 0);
                     o[b][v] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, pl, o[b][v], 0, 0, 0);
                 }

@@ -8,19 +8,28 @@
 // exact: hi rounds the product, lo = fma(number, scale, -hi). The scales of each
 // four keys are first brought below 2 by a power of two, which K's scores take
 // back as a factor, and V's weights: w = exp2(score + e - M), so V of any
-// magnitude fills f16's range, and the weights' sum takes w 2^-e. Four keys that
-// are more than 2^10 apart, some of which a row may not see, have a power each
-// (2 % of the time below; of 78 us for packed documents of dim 64, 7). Slots that
-// were never written may hold anything: sizes above 31 are no key's, and a scale
-// of V that its size does not allow is taken as 0.
+// magnitude fills f16's range, and the weights' sum takes w 2^-e.
+// That is exact while no scale but 0 is 2^15 below the largest of its four keys.
+// K or V of a record (16 keys) in which some may be further apart (sizes of four
+// keys by more than FAR, or the blocks of a key, which its size byte says), with a
+// scale that is not finite, or never written is rough: the tile has its numbers
+// as they are, and the scales beside them. The scores then take K's scales on
+// each block's product; weight times V's scale goes block by block, by a power of
+// two that each row has there (every tile rough: 4096 causal tokens take 1.35
+// times as long where K is, 1.9 V, eight trees of 61 drafts 1.4 and 2.7).
+// In records that are not rough a scale of V that its size does not allow is of a
+// slot that was never written, which no row sees: 0, so that a weight of 0 times
+// it is 0.
 // (With K as whole numbers, exact in one term, and its scales on the 32-dim
 // products, a tile had 8 matrix instructions fewer and 64 multiply-adds and 32
 // registers a wave more: 430 us where this took 415, 4096 causal tokens of
 // 32 heads of 128.)
 // q is two f16 terms (22 bits, a power of two per row), and so are the weights;
 // of the product's terms the one of two lows is left out (2^-22). M follows the
-// maximum of score + e by steps of more than 2^8 only: the weights have f16's
-// range for that, and most tiles leave the sums O^T = V^T P^T unscaled. P^T is
+// maximum of score + e by steps of more than 2^5 only: most tiles leave the sums
+// O^T = V^T P^T unscaled. The largest weight is 2^10 to 2^15, so two terms, which
+// end at 2^-24, leave out 2^-21 of a value beside others that its e, of another
+// block or a key out of sight, says to be 2^14 larger than they are. P^T is
 // used in the registers S^T was left in: the order of keys within a
 // contraction is free, and V is laid out to it.
 // Bound: matrix and vector issue, which take turns more than they overlap (48
@@ -49,9 +58,9 @@ struct vx_tile {
     struct tile {
         h8 k[NB * 2 * 2 * 64];  // [block][16 dims][hi, lo][half, key]
         h8 v[NB * 2 * 2 * 64];  // [block][16 keys][hi, lo][half, dim]
-        f2 e[8];                // of four keys: 2^exponent of K's scales (negative: see key), exponent of V's
-        f2 key[32];             // of keys far apart: what their own powers are to those, factor and difference
-        uint32_t bad[8];        // their V scales that are not finite, bit 4 block + key
+        _Float16 ks[NB][32], vs[NB][32];  // scales of rough records
+        f2 e[8];                // of four keys: 2^exponent of K's scales, exponent of V's
+        uint32_t rough[2];      // of a record: 1, K's numbers without their scales; 4, V's
     };
 
     struct raw {  // a thread's pieces as loaded
@@ -71,7 +80,8 @@ struct vx_tile {
         }
     }
 
-    static constexpr uint32_t FAR = 10;  // f16 holds both terms of a key that is 2^10 below to 22 bits
+    static constexpr uint32_t FAR = 4;
+    static_assert(FAR + VX_KV_APART <= 14, "a scale 2^15 below the largest is no normal f16 beside it");
     static __device__ __forceinline__ int power(uint32_t size) { return max((int)size - 16, -15); }  // (of no key: size 0)
 
     // the record of the 16 keys from key on; past the end the last one
@@ -100,105 +110,65 @@ struct vx_tile {
         r.e = ((const uint32_t*)(p + R::V_SIZES))[g];
     }
 
-    // decodes a thread's pieces into the tile of the keys from k0 on
-    static __device__ __forceinline__ void store(const vx_attn_args& a, vx_scalar_i32 table, const uint8_t* base, raw& r, tile& s, int k0, int last) {
+    // decodes a thread's pieces into a tile
+    static __device__ __forceinline__ void store(raw& r, tile& s) {
+        typedef uint16_t us2 __attribute__((ext_vector_type(2)));
         const uint32_t t = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(t >> 6), rec = wave & 1, lane = t & 63, m = lane & 15, g = lane >> 4;
-        uint32_t bad = 0;
-        // largest of four sizes, and whether another is far below it
+        // the largest of four sizes, and whether another one (but for zeros) is far below it
         auto largest = [](uint32_t e, bool& far) {
-            typedef uint16_t us2 __attribute__((ext_vector_type(2)));
-            const us2 lo = __builtin_bit_cast(us2, e & 0x00FF00FFu), hi = __builtin_bit_cast(us2, e >> 8 & 0x00FF00FFu);
-            const us2 most = __builtin_elementwise_max(lo, hi), least = __builtin_elementwise_min(lo, hi);
+            const us2 lo = __builtin_bit_cast(us2, e & 0x00FF00FFu), hi = __builtin_bit_cast(us2, e >> 8 & 0x00FF00FFu), one = {1, 1};
+            const us2 most = __builtin_elementwise_max(lo, hi), least = __builtin_elementwise_min(lo - one, hi - one);
             const uint32_t top = max((uint32_t)most.x, (uint32_t)most.y);
-            far = top > min((uint32_t)least.x, (uint32_t)least.y) + FAR;
+            far = top > min((uint32_t)least.x, (uint32_t)least.y) + 1u + FAR;
             return top;
         };
         bool far, kfar;
         uint32_t size = largest(r.e, far), ksize = largest(r.ke, kfar);
-        auto below = [](uint32_t v) { return (_Float16)__builtin_ldexpf(1.f, -power(v)); };
-        h2 f0, f1;  // what V's four keys and K's key are brought down by
-        _Float16 fk;
-        float sign = 1.f;
-        // (seldom: out of the way of the rest, 2 us of 196, eight trees of 61 drafts)
-        if (__builtin_expect(k0 + 32 > last + 1 || __any(far | kfar | (max(size, ksize) > 31u)), 0)) {
-            // scales of keys that do not exist, which may be anything: 0; those that are not finite: 0, and noted
-            const int valid = last + 1 - (k0 + 16 * (int)rec + 4 * (int)g);
-            auto fix = [&](uint32_t d, int i) {
-                if (valid <= 2 * i || (d & 0x7FFFu) >= 0x7C00u) d &= 0xFFFF0000u;
-                if (valid <= 2 * i + 1 || (d >> 16 & 0x7FFFu) >= 0x7C00u) d &= 0x0000FFFFu;
-                return d;
-            };
+        // (a wave has the sizes of all of its record: waves of one record agree)
+        const bool kr = __any(kfar | (ksize > 31u)), vr = __any(far | (size > 31u));
+        if (__builtin_expect(kr, 0)) {
 #pragma unroll
-            for (int n = 0; n < ITEMS; ++n)
-#pragma unroll
-                for (int i = 0; i < 2; ++i) r.d[n][i] = fix(r.d[n][i], i);
-            const uint32_t* sc = (const uint32_t*)(record(a, table, base, k0 + 16 * (int)rec, last) + PK::BYTES + PV::VALS + g * (8 * NB));
-            uint32_t e[4] = {};
-#pragma unroll 1
-            for (int b = 0; b < NB; ++b)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const uint32_t v = vx_kv_size(sc[2 * b + (i >> 1)] >> (16 * (i & 1)));
-                    if (valid <= i) continue;
-                    if (v == 255u) bad |= 1u << (4 * b + i);
-                    else e[i] = max(e[i], v);
-                }
-            size = max(max(e[0], e[1]), max(e[2], e[3]));
-            uint32_t least = size;
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                if (valid > i) least = min(least, e[i]);
-            far = size > least + FAR;
-            uint32_t own[4], kown = 0;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) own[i] = far ? e[i] : size;
-            f0 = h2{below(own[0]), below(own[1])}, f1 = h2{below(own[2]), below(own[3])};
-            // K's keys that do not exist, are not finite or were never written: the others' exponent
-            const int kvalid = last + 1 - (k0 + 16 * (int)rec + 4 * (int)(m >> 2));
-            ksize = 0;
-            least = 255u;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const uint32_t v = r.ke >> (8 * i) & 255u;
-                if (i < kvalid && v < 32u) {
-                    ksize = max(ksize, v);
-                    least = min(least, v);
-                    if (i == (int)(m & 3)) kown = v;
-                }
+            for (int i = 0; i < ITEMS; ++i) {
+                const int b = (int)(wave >> 1) + WAVES / 2 * i;
+                if (NB % (WAVES / 2) != 0 && b >= NB) break;
+                if (g == 0) s.ks[b][16 * rec + m] = __builtin_bit_cast(_Float16, r.kd[i]);
+                r.kd[i] = 0x3C00;  // 1
             }
-            kfar = ksize > least + FAR;
-            if (!kfar) kown = ksize;
-            fk = below(kown);
-            if (far | kfar) sign = -1.f;
-            if (wave < 2 && (m >> 2) == g) {
-                const uint32_t v = m & 2 ? (m & 1 ? own[3] : own[2]) : (m & 1 ? own[1] : own[0]);
-                s.key[rec * 16 + m] = f2{__builtin_ldexpf(1.f, power(kown) - power(ksize)), (float)(power(v) - power(size))};
+            ksize = 16;  // 2^0
+        }
+        if (__builtin_expect(vr, 0)) {
+#pragma unroll
+            for (int i = 0; i < ITEMS; ++i) {
+                const int b = (int)(wave >> 1) + WAVES / 2 * i;
+                if (NB % (WAVES / 2) != 0 && b >= NB) break;
+                if (m == 0) *(u2*)&s.vs[b][16 * rec + 4 * g] = u2{r.d[i][0], r.d[i][1]};
+                r.d[i][0] = r.d[i][1] = 0x3C003C00u;
             }
+            size = 16;
         } else {
-            const _Float16 f = below(size);
-            f0 = f1 = h2{f, f};
-            fk = below(ksize);
-            // a scale of V above what the sizes say is of a key that was never
-            // written, which no row sees: 0, so that its weights' zeros stay zeros
-            typedef uint16_t us2 __attribute__((ext_vector_type(2)));
             us2 most = {};
 #pragma unroll
-            for (int n = 0; n < ITEMS; ++n)
+            for (int i = 0; i < ITEMS; ++i)
 #pragma unroll
-                for (int i = 0; i < 2 && (NB % (WAVES / 2) == 0 || (int)(wave >> 1) + WAVES / 2 * n < NB); ++i) most = __builtin_elementwise_max(most, __builtin_bit_cast(us2, r.d[n][i] & 0x7FFF7FFFu));
+                for (int j = 0; j < 2 && (NB % (WAVES / 2) == 0 || (int)(wave >> 1) + WAVES / 2 * i < NB); ++j)
+                    most = __builtin_elementwise_max(most, __builtin_bit_cast(us2, r.d[i][j] & 0x7FFF7FFFu));
             const uint32_t limit = max(size, 1u) << 10;
             if (__builtin_expect(__any(max((uint32_t)most.x, (uint32_t)most.y) >= limit), 0)) {
 #pragma unroll
-                for (int n = 0; n < ITEMS; ++n)
+                for (int i = 0; i < ITEMS; ++i)
 #pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        if ((r.d[n][i] & 0x7FFFu) >= limit) r.d[n][i] &= 0xFFFF0000u;
-                        if ((r.d[n][i] >> 16 & 0x7FFFu) >= limit) r.d[n][i] &= 0x0000FFFFu;
+                    for (int j = 0; j < 2; ++j) {
+                        if ((r.d[i][j] & 0x7FFFu) >= limit) r.d[i][j] &= 0xFFFF0000u;
+                        if ((r.d[i][j] >> 16 & 0x7FFFu) >= limit) r.d[i][j] &= 0x0000FFFFu;
                     }
             }
         }
-        if (wave < 2 && m == 4 * g) s.e[rec * 4 + g] = f2{__builtin_ldexpf(sign, power(ksize)), (float)power(size)};
-        if (wave < 2 && m == 0) s.bad[rec * 4 + g] = bad;
+        // what V's four keys and K's key are brought down by
+        auto below = [](uint32_t v) { return (_Float16)__builtin_ldexpf(1.f, -power(v)); };
+        const _Float16 f = below(size), fk = below(ksize);
+        const h2 fv = {f, f};
+        if (wave < 2 && m == 4 * g) s.e[rec * 4 + g] = f2{__builtin_ldexpf(1.f, power(ksize)), (float)power(size)};
+        if (wave < 2 && lane == 0) s.rough[rec] = (kr ? 1u : 0u) | (vr ? 4u : 0u);
 #pragma unroll
         for (int i = 0; i < ITEMS; ++i) {
             const int b = (int)(wave >> 1) + WAVES / 2 * i;
@@ -224,7 +194,7 @@ struct vx_tile {
             kat[0] = h8{kh[0].x, kh[0].y, kh[1].x, kh[1].y, kh[2].x, kh[2].y, kh[3].x, kh[3].y};
             kat[64] = h8{kl[0].x, kl[0].y, kl[1].x, kl[1].y, kl[2].x, kl[2].y, kl[3].x, kl[3].y};
             const uint32_t d0 = r.d[i][0], d1 = r.d[i][1];
-            const h2 r0 = __builtin_bit_cast(h2, d0) * f0, r1 = __builtin_bit_cast(h2, d1) * f1;
+            const h2 r0 = __builtin_bit_cast(h2, d0) * fv, r1 = __builtin_bit_cast(h2, d1) * fv;
 #pragma unroll
             for (int v = 0; v < 2; ++v) {
                 h2 x0, x1;
@@ -363,7 +333,7 @@ struct vx_tile {
             if (kbeg + 32 * i < kend) {
                 raw r;
                 load(a, table, base, kbeg + 32 * i, last, r);
-                store(a, table, base, r, sh[i], kbeg + 32 * i, last);
+                store(r, sh[i]);
             }
         __syncthreads();
         uint32_t buf = 0;
@@ -400,27 +370,37 @@ struct vx_tile {
                     __builtin_amdgcn_sched_barrier(6);
                 }
                 __builtin_amdgcn_s_setprio(0);
-                float e[4], apart = 0.f;
+                const uint32_t rough = __builtin_amdgcn_readfirstlane(t.rough[0] | t.rough[1] << 1);  // K: bits 0, 1; V: 2, 3
+                if (__builtin_expect(rough & 3u, 0)) {  // once more, block by block
+                    x = f16v{};
+#pragma unroll
+                    for (int b = 0; b < NB; ++b) {
+                        __builtin_amdgcn_sched_barrier(0);  // (one block's products at a time: registers)
+                        f16v y = {};
+#pragma unroll
+                        for (int j = 0; j < 2; ++j) {
+                            const h8 kh = t.k[(b * 4 + 2 * j) * 64 + lane], kl = t.k[(b * 4 + 2 * j + 1) * 64 + lane];
+                            y = __builtin_amdgcn_mfma_f32_32x32x16_f16(kh, qh[b][j], y, 0, 0, 0);
+                            y = __builtin_amdgcn_mfma_f32_32x32x16_f16(kh, ql[b][j], y, 0, 0, 0);
+                            y = __builtin_amdgcn_mfma_f32_32x32x16_f16(kl, qh[b][j], y, 0, 0, 0);
+                        }
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            const h4 d = *(const h4*)&t.ks[b][8 * j + 4 * h];
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) x[4 * j + i] = __builtin_fmaf(y[4 * j + i], rough >> (j / 2) & 1 ? (float)d[i] : 1.f, x[4 * j + i]);
+                        }
+                    }
+                }
+                float e[4];
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                     const f2 ke = t.e[4 * (j / 2) + 2 * (j % 2) + (int)h];
-                    const float f = fq * fabsf(ke.x);
+                    const float f = fq * ke.x;
                     e[j] = ke.y;
-                    apart = fminf(apart, ke.x);
 #pragma unroll
                     for (int i = 0; i < 4; ++i) x[4 * j + i] *= f;
                 }
-                // keys far apart: own(register, factor and difference)
-                const bool far = __builtin_expect(__any(apart < 0.f), 0);
-                auto each_own = [&](auto own) {
-#pragma unroll
-                    for (int j = 0; j < 4; ++j)
-                        if (t.e[2 * j + (int)h].x < 0.f) {
-#pragma unroll
-                            for (int i = 0; i < 4; ++i) own(4 * j + i, t.key[8 * j + 4 * (int)h + i]);
-                        }
-                };
-                if (__builtin_expect(far, 0)) each_own([&](int i, f2 k) { x[i] *= k.x; });
                 if (a.cap > 0.f) {
                     float big = 0.f;
 #pragma unroll
@@ -461,23 +441,18 @@ struct vx_tile {
                         x[i] = __uint_as_float((v & __float_as_uint(x[i])) | (~v & 0xFF800000u));
                     }
                 }
-                if (__builtin_expect(far, 0)) each_own([&](int i, f2 k) { x[i] += k.y; });
                 // running maximum of score + e: four keys at a time
                 float top = -__builtin_inff();
-                uint32_t bad = 0;
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const int at = 4 * (j / 2) + 2 * (j % 2) + (int)h;
-                    bad |= t.bad[at];
+                for (int j = 0; j < 4; ++j)
                     top = fmaxf(top, fmaxf(fmaxf(x[4 * j], x[4 * j + 1]), fmaxf(x[4 * j + 2], x[4 * j + 3])) + e[j]);
-                }
                 {
                     uint32_t u = __builtin_bit_cast(uint32_t, top), v = u;
                     vx_swap32(u, v);
-                    top = fmaxf(__builtin_bit_cast(float, u), __builtin_bit_cast(float, v)) - 6.f;
+                    top = fmaxf(__builtin_bit_cast(float, u), __builtin_bit_cast(float, v)) - 10.f;
                 }
-                if (__any(top > M + 8.f)) {
-                    const float Mn = top > M + 8.f ? top : M;
+                if (__any(top > M + 5.f)) {
+                    const float Mn = top > M + 5.f ? top : M;
                     const float al = __builtin_amdgcn_exp2f(Mn == -__builtin_inff() ? 0.f : M - Mn);
                     l *= al;
 #pragma unroll
@@ -485,7 +460,6 @@ struct vx_tile {
                     M = Mn;
                 }
                 const float Mr = M == -__builtin_inff() ? 0.f : M;
-                h8 ph[2], pl[2];
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                     const float c = Mr - e[j];
@@ -496,16 +470,65 @@ struct vx_tile {
                         part += x[4 * j + i];
                     }
                     l = __builtin_fmaf(part, __builtin_ldexpf(1.f, -(int)e[j]), l);
-#pragma unroll
-                    for (int i = 0; i < 4; i += 2) {
-                        h2 u, v;
-                        vx_two_terms(x[4 * j + i], x[4 * j + i + 1], minus, u, v);
-                        const int k = 4 * (j % 2) + i;
-                        ph[j / 2][k] = u.x, ph[j / 2][k + 1] = u.y, pl[j / 2][k] = v.x, pl[j / 2][k + 1] = v.y;
-                    }
                 }
-                if (__builtin_expect(far, 0))  // the weights' sum takes w 2^-e of the key's own e
-                    each_own([&](int i, f2 k) { l += x[i] * __builtin_ldexpf(__builtin_ldexpf(1.f, -(int)k.y) - 1.f, -(int)e[i / 4]); });
+                // a weight times its scale, as two f16 terms of eight keys
+                auto terms = [&](int j, h8& hi, h8& lo, auto value) {
+#pragma unroll
+                    for (int i = 0; i < 8; i += 2) {
+                        h2 u, v;
+                        vx_two_terms(value(8 * j + i), value(8 * j + i + 1), minus, u, v);
+                        hi[i] = u.x, hi[i + 1] = u.y, lo[i] = v.x, lo[i + 1] = v.y;
+                    }
+                };
+                if (__builtin_expect(rough >> 2, 0)) {
+                    // 0 for what the row does not see, whose scale may be anything; never 0 for what it sees, whose NaN shows
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) x[i] = see >> (8 * (i / 4) + i % 4) & 1 ? fmaxf(x[i], 0x1p-126f) : 0.f;
+#pragma unroll
+                    for (int b = 0; b < NB; ++b) {
+                        asm volatile("" ::: "memory");  // (one block at a time: registers)
+                        __builtin_amdgcn_sched_barrier(0);
+                        h4 scales[4];
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) scales[j] = *(const h4*)&t.vs[b][8 * j + 4 * h];
+                        auto value = [&](int i) {
+                            const float d = (float)scales[i / 4][i % 4];
+                            return x[i] == 0.f ? 0.f : x[i] * (rough >> (2 + i / 8) & 1 ? d : 1.f);
+                        };
+                        float most = 0.f;
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) most = fmaxf(most, fabsf(value(i)));  // (not a NaN)
+                        {
+                            uint32_t u = __builtin_bit_cast(uint32_t, most), v = u;
+                            vx_swap32(u, v);
+                            most = fmaxf(__builtin_bit_cast(float, u), __builtin_bit_cast(float, v));
+                        }
+                        // (sums below 2^23 2^15 keys: no overflow with 2^55)
+                        const int p = most > 0x1p-40f ? __builtin_amdgcn_frexp_expf(most) : -40;
+                        o[b] *= __builtin_ldexpf(1.f, 15 - p);
+#pragma unroll
+                        for (int j = 0; j < 2; ++j) {
+                            asm volatile("" ::: "memory");
+                            h8 ph, pl;
+                            terms(j, ph, pl, [&](int i) { return __builtin_ldexpf(value(i), 15 - p); });  // (below 2^15)
+                            __builtin_amdgcn_sched_barrier(0);
+                            const h8 vh = t.v[(b * 4 + 2 * j) * 64 + lane];
+                            o[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vh, ph, o[b], 0, 0, 0);
+                            o[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vh, pl, o[b], 0, 0, 0);
+                            const h8 vl = t.v[(b * 4 + 2 * j + 1) * 64 + lane];
+                            o[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vl, ph, o[b], 0, 0, 0);
+                            __builtin_amdgcn_sched_barrier(0);
+                        }
+                        o[b] *= __builtin_ldexpf(1.f, p - 15);
+                    }
+                    // the usual products below then add nothing: in two branches the sums
+                    // were copied, and 60 registers spilled
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) x[i] = 0.f;
+                }
+                h8 ph[2], pl[2];
+#pragma unroll
+                for (int j = 0; j < 2; ++j) terms(j, ph[j], pl[j], [&](int i) { return x[i]; });
                 __builtin_amdgcn_s_setprio(1);
                 h8 vf[3][2];
                 auto vread = [&](int u) {
@@ -525,19 +548,8 @@ struct vx_tile {
                     __builtin_amdgcn_sched_barrier(6);
                 }
                 __builtin_amdgcn_s_setprio(0);
-                if (__any(bad)) {
-                    // values that are not finite, taken as zeros above: NaN for the rows that see their key
-#pragma unroll
-                    for (int b = 0; b < NB; ++b) {
-                        uint32_t keys = 0;
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) keys |= (t.bad[4 * (j / 2) + 2 * (j % 2) + h] >> (4 * b) & 15u) << (8 * j);
-                        const int hit = (keys & see) != 0u;
-                        if (hit | __shfl_xor(hit, 32)) o[b] += __builtin_nanf("");  // (a lane has half of the keys, and half of the dims)
-                    }
-                }
             }
-            if (more) store(a, table, base, r, sh[(buf + PERIOD) % (2 * PERIOD)], kn, last);
+            if (more) store(r, sh[(buf + PERIOD) % (2 * PERIOD)]);
             if (PERIOD == 1 || buf % PERIOD == PERIOD - 1) __syncthreads();
         }
 

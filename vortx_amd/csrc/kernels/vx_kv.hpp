@@ -20,8 +20,10 @@
 // Values are stored with 128 (8 bits) or 8 (4 bits) added. The orders inside
 // a dword are those that masks and byte permutes unpack to pairs of f16.
 // Scales: f16, [g][b][4]: of K for keys 4 g + j, of V the same. Sizes: a byte a
-// key, 16 above the exponent of the largest of its scales (1 to 32; an f16
-// below its normal numbers counts as 2^-15), 255 where one is not finite.
+// key, 16 above the exponent of the largest of its scales (1 to 31; an f16
+// below its normal numbers counts as 2^-15; 0: all are zero), with 128 added
+// where another one that is not zero has an exponent more than VX_KV_APART
+// lower, and 255 where one is not finite.
 #pragma once
 #include <hip/hip_runtime.h>
 #include <stdint.h>
@@ -84,9 +86,10 @@ struct vx_kv_rec {
     static constexpr uint32_t V = vx_kv_part<NB, KB>::BYTES, K_SIZES = V + vx_kv_part<NB, VB>::BYTES, V_SIZES = K_SIZES + 16,
                               BYTES = V_SIZES + 16;
 };
+constexpr uint32_t VX_KV_APART = 10;
 __device__ __forceinline__ uint32_t vx_kv_size(uint32_t d) {  // of a scale's bits
     d &= 0x7FFFu;
-    return d >= 0x7C00u ? 255u : (d >> 10) + 1u;
+    return d >= 0x7C00u ? 255u : d ? (d >> 10) + 1u : 0u;
 }
 
 __device__ __forceinline__ uint64_t vx_kv_page(const vx_kv_geom& c, uint32_t page, uint32_t head, uint32_t rec_bytes) {

@@ -168,6 +168,19 @@ __device__ __forceinline__ uint32_t vx_kv_max_halves(uint32_t v) {
     }
     return v;
 }
+
+// Two size bytes (a half each) of a row whose block has sizes `own`.
+template <int NP>
+__device__ __forceinline__ uint32_t vx_kv_row_sizes(uint32_t own) {
+    uint32_t top = vx_kv_max_halves<NP>(own);
+    // how far the block is below the largest one; not at all if it is all zeros
+    const uint32_t lo = own & 0xFFFFu ? (top & 0xFFFFu) - (own & 0xFFFFu) : 0u, hi = own >> 16 ? (top >> 16) - (own >> 16) : 0u;
+    if (__any((lo > VX_KV_APART) | (hi > VX_KV_APART))) {
+        const uint32_t apart = vx_kv_max_halves<NP>(lo | hi << 16);
+        top |= ((apart & 0xFFFFu) > VX_KV_APART ? 0x80u : 0u) | (apart >> 16 > VX_KV_APART ? 0x800000u : 0u);
+    }
+    return top;
+}
 __device__ __forceinline__ uint32_t vx_kv_bytes(uint32_t lo, uint32_t hi) { return (lo & 255u) | (lo >> 8 & 0xFF00u) | (hi & 255u) << 16 | (hi >> 16) << 24; }
 
 // The dims 4 u + 2 p, + 1 of four keys (codes w, a byte a dim) as the record has them: V
@@ -241,8 +254,8 @@ __device__ __forceinline__ void vx_kv_write_rows(const vx_kv_rows_args& a) {
                 }
                 if (u == 0) *(u2*)(rec + R::V + PV::VALS + ((m >> 2) * NB + b) * 8) = sc;
             }
-            klo = vx_kv_max_halves<NP>(klo), khi = vx_kv_max_halves<NP>(khi);
-            vlo = vx_kv_max_halves<NP>(vlo), vhi = vx_kv_max_halves<NP>(vhi);
+            klo = vx_kv_row_sizes<NP>(klo), khi = vx_kv_row_sizes<NP>(khi);
+            vlo = vx_kv_row_sizes<NP>(vlo), vhi = vx_kv_row_sizes<NP>(vhi);
             if (u == 0 && b == 0) {
                 *(uint32_t*)(rec + R::K_SIZES + m) = vx_kv_bytes(klo, khi);
                 *(uint32_t*)(rec + R::V_SIZES + m) = vx_kv_bytes(vlo, vhi);
@@ -255,7 +268,7 @@ __device__ __forceinline__ void vx_kv_write_rows(const vx_kv_rows_args& a) {
             size = vx_kv_put_k<NB, KB>(rec, m, b, u, k) << 16;
             size |= vx_kv_put_v<NB, VB>(rec + R::V, m, b, u, v);
         }
-        size = vx_kv_max_halves<NP>(size);
+        size = vx_kv_row_sizes<NP>(size);
         if (u == 0 && b == 0) {
             rec[R::K_SIZES + m] = (uint8_t)(size >> 16);
             rec[R::V_SIZES + m] = (uint8_t)size;
