@@ -461,7 +461,8 @@ int vx_kv_read(vx_ctx ctx, vx_stream stream, const vx_mview* k, const vx_mview* 
  *                               starts[s] + j of q and out, at position
  *                               lens[s] - n + j (n its queries)
  * max_queries and max_len are upper bounds that the launch is laid out by;
- * keys past max_len are not seen, queries past max_queries not computed. */
+ * keys past max_len or past the table's pages are not seen (positions stay as
+ * lens says), queries past max_queries not computed. */
 typedef struct vx_attn_batch {
     const int32_t* table;
     const int32_t* lens;
@@ -507,7 +508,8 @@ int vx_attention(vx_ctx ctx, vx_stream stream, const vx_mview* out, const vx_cvi
                  const vx_attn_batch* batch, const vx_attn_opts* opts, void* workspace, uint64_t workspace_bytes);
 
 /* The same for a tree of drafted tokens: the queries of a sequence are its n
- * drafts, whose keys are its last n. Draft j sees the cached keys before them
+ * drafts, whose keys are its last n (of more drafts than keys the first have
+ * none, and are never seen). Draft j sees the cached keys before them
  * (opts' first and window applied; causal and prefix have nothing to do) and
  * draft i where bit i % 32 of tree[token j][i / 32] is set: its ancestors and
  * itself. tree: device array [tokens][tree_stride] of 32-bit words, of which

@@ -38,7 +38,8 @@ __device__ __forceinline__ float vx_max_rows4(float v) {
 
 // A sequence of the batch: queries, keys and where they lie.
 struct vx_attn_seq {
-    int start, n, len;  // first query token, query tokens, keys
+    int start, n, len;  // first query token, query tokens, keys in reach
+    int tail;           // position of the first query (negative where there are more queries than keys)
     uint32_t rows;      // query rows that are computed
 };
 __device__ __forceinline__ vx_attn_seq vx_attn_sequence(const vx_attn_args& a, uint32_t s) {
@@ -46,7 +47,9 @@ __device__ __forceinline__ vx_attn_seq vx_attn_sequence(const vx_attn_args& a, u
     const int T = (int)a.tokens;
     q.start = min(max(a.starts[s], 0), T);
     q.n = min(max(a.starts[s + 1], q.start), T) - q.start;
-    q.len = min(max(a.lens[s], 0), (int)min(a.max_len, a.table_cols << a.c.page_shift));
+    const int all = max(a.lens[s], 0);  // (positions go by it, whatever is in reach)
+    q.len = min(all, (int)min(a.max_len, a.table_cols << a.c.page_shift));
+    q.tail = all - q.n;
     q.rows = min((uint32_t)q.n, a.max_queries) * a.group;
     return q;
 }
@@ -77,7 +80,6 @@ __device__ __forceinline__ int vx_tree_count(const vx_attn_args& a, int token) {
 
 __device__ __forceinline__ vx_attn_row vx_attn_row_of(const vx_attn_args& a, const vx_attn_seq& q, uint32_t s, uint32_t kvh, uint32_t r) {
     vx_attn_row w;
-    const int tail = q.len - q.n;
     if (r >= q.rows) {
         w.pos = w.lo = w.hi = 0;
         w.slope = 0.f;
@@ -87,10 +89,10 @@ __device__ __forceinline__ vx_attn_row vx_attn_row_of(const vx_attn_args& a, con
     vx_attn_token(a, q, kvh, r, token, head);
     w.lo = 0;
     if (a.tree) {
-        w.pos = tail + vx_tree_count(a, (int)token) - 1;
-        w.hi = max(tail, 0);
+        w.pos = q.tail + vx_tree_count(a, (int)token) - 1;
+        w.hi = min(max(q.tail, 0), q.len);
     } else {
-        w.pos = tail + (int)token - q.start;
+        w.pos = q.tail + (int)token - q.start;
         w.hi = q.len;
         if (a.causal) w.hi = min(w.hi, max(w.pos + 1, a.prefix ? a.prefix[s] : 0));
     }
@@ -112,7 +114,7 @@ __device__ __forceinline__ uint32_t vx_attn_sees(const vx_attn_args& a, const vx
     auto from = [&](int key) { return key <= k0 ? 0xFFFFFFFFu : key - k0 > 31 ? 0u : 0xFFFFFFFFu << (key - k0); };  // keys >= key
     uint32_t see = from(w.lo) & ~from(min(w.hi, tail));
     if (a.tree && k0 + 32 > tail) {
-        const int j0 = k0 - tail;  // first draft of the tile (above -32)
+        const int j0 = k0 - tail;  // first draft of the tile (above -32; drafts before key 0 have no key)
         uint32_t bits = 0;
         if (r < q.rows) {
             uint32_t token, head;
@@ -127,7 +129,7 @@ __device__ __forceinline__ uint32_t vx_attn_sees(const vx_attn_args& a, const vx
         if (a.slopes || a.window) {
             const int lane = threadIdx.x & 31, key = k0 + lane;
             int p = key;
-            if (key >= tail && key < q.len) p = q.len - q.n + vx_tree_count(a, q.start + key - (q.len - q.n)) - 1;
+            if (key >= tail && key < q.len) p = q.tail + vx_tree_count(a, q.start + key - q.tail) - 1;
             at[lane] = p;  // (both halves of the wave the same)
             __builtin_amdgcn_wave_barrier();
             if (a.window) {
@@ -165,7 +167,7 @@ __device__ __forceinline__ uint32_t vx_attn_steps(const vx_attn_args& a, const v
     lo = 0;
     if (r0 >= q.rows) return 0u;
     // (32 bits: lengths and windows are below 2^31 - 2^16, query tokens 2^30 at most)
-    const int tail = q.len - q.n;  // position of the first query
+    const int tail = q.tail;
     int p0 = tail - 1, p1 = q.len, from = 0, to = q.len;  // a tree's drafts are anywhere from there on
     if (!a.tree) {
         p0 = tail + (int)(r0 / a.group);

@@ -92,7 +92,7 @@ struct vx_rows16 {
         const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
         const uint32_t row = r0 + m;
         const vx_attn_row w = vx_attn_row_of(a, q, s, kvh, row);
-        const int tail = a.tree ? max(q.len - q.n, 0) : q.len;  // keys from here on: by the tree's bits
+        const int tail = a.tree ? q.tail : q.len;  // keys from here on: by the tree's bits
         int lo = w.hi > w.lo ? w.lo : 0x7FFFFFFF, hi = w.hi > w.lo ? w.hi : 0;
         int lo_all = row < q.rows ? w.lo : 0, hi_all = row < q.rows ? w.hi : 0x7FFFFFFF;
 #pragma unroll
@@ -103,7 +103,7 @@ struct vx_rows16 {
             hi_all = min(hi_all, __shfl_xor(hi_all, o));
         }
         if (a.tree) {
-            lo = min(lo, tail);
+            lo = min(lo, max(tail, 0));
             hi = q.len;
         }
         lo = __builtin_amdgcn_readfirstlane(lo);

@@ -231,7 +231,7 @@ struct vx_tile {
         const uint32_t r0 = rb * ROWS;
         const uint32_t row = r0 + wave * 32 + n;
         const vx_attn_row w = vx_attn_row_of(a, q, s, kvh, row);
-        const int tail = a.tree ? max(q.len - q.n, 0) : q.len;  // keys from here on: by the tree's bits
+        const int tail = a.tree ? q.tail : q.len;  // keys from here on: by the tree's bits
         const int last = q.len - 1;
         __syncthreads();  // (LDS may be another unit's still)
         // what the wave's rows see, and all of them; and the workgroup's
@@ -246,7 +246,7 @@ struct vx_tile {
         }
         const bool rows_here = r0 + wave * 32 < q.rows;  // (the first row's wave: uniform)
         if (a.tree && rows_here) {
-            lo = min(lo, tail);
+            lo = min(lo, max(tail, 0));
             hi = q.len;
         }
         lo = __builtin_amdgcn_readfirstlane(lo);
