@@ -512,8 +512,9 @@ int vx_attention(vx_ctx ctx, vx_stream stream, const vx_mview* out, const vx_cvi
  * none, and are never seen). Draft j sees the cached keys before them
  * (opts' first and window applied; causal and prefix have nothing to do) and
  * draft i where bit i % 32 of tree[token j][i / 32] is set: its ancestors and
- * itself. tree: device array [tokens][tree_stride] of 32-bit words, of which
- * tree_words are read (32 tree_words >= max_queries, else VX_ERR_SHAPE). A
+ * itself; bits past the n drafts stand for nothing. tree: device array
+ * [tokens][tree_stride] of 32-bit words, of which tree_words are read (32
+ * tree_words >= max_queries, else VX_ERR_SHAPE). A
  * draft that sees c drafts is at position lens[s] - n + c - 1, its depth in
  * the tree, for slopes and window. */
 int vx_attention_tree(vx_ctx ctx, vx_stream stream, const vx_mview* out, const vx_cview* q, const vx_kv_cache* cache,

@@ -70,11 +70,12 @@ __device__ __forceinline__ void vx_attn_token(const vx_attn_args& a, const vx_at
     head = kvh * a.group + (r - j * a.group);
 }
 
-// Number of drafts that a token's row of the tree sees.
-__device__ __forceinline__ int vx_tree_count(const vx_attn_args& a, int token) {
+// Number of a sequence's `drafts` that a token's row of the tree sees.
+__device__ __forceinline__ int vx_tree_count(const vx_attn_args& a, int token, int drafts) {
     const uint32_t* w = a.tree + (uint64_t)token * a.tree_stride;
     int n = 0;
-    for (uint32_t i = 0; i < a.tree_words; ++i) n += __builtin_popcount(w[i]);
+    for (uint32_t i = 0; i < a.tree_words && drafts > 0; ++i, drafts -= 32)
+        n += __builtin_popcount(drafts < 32 ? w[i] & ((1u << drafts) - 1u) : w[i]);
     return n;
 }
 
@@ -89,7 +90,7 @@ __device__ __forceinline__ vx_attn_row vx_attn_row_of(const vx_attn_args& a, con
     vx_attn_token(a, q, kvh, r, token, head);
     w.lo = 0;
     if (a.tree) {
-        w.pos = q.tail + vx_tree_count(a, (int)token) - 1;
+        w.pos = q.tail + vx_tree_count(a, (int)token, q.n) - 1;
         w.hi = min(max(q.tail, 0), q.len);
     } else {
         w.pos = q.tail + (int)token - q.start;
@@ -129,7 +130,7 @@ __device__ __forceinline__ uint32_t vx_attn_sees(const vx_attn_args& a, const vx
         if (a.slopes || a.window) {
             const int lane = threadIdx.x & 31, key = k0 + lane;
             int p = key;
-            if (key >= tail && key < q.len) p = q.tail + vx_tree_count(a, q.start + key - q.tail) - 1;
+            if (key >= tail && key < q.len) p = q.tail + vx_tree_count(a, q.start + key - q.tail, q.n) - 1;
             at[lane] = p;  // (both halves of the wave the same)
             __builtin_amdgcn_wave_barrier();
             if (a.window) {
