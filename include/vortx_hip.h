@@ -480,7 +480,7 @@ typedef enum vx_attn_flags {
 /* Options of vx_attention. Zeros: no option; the arrays are device memory. */
 typedef struct vx_attn_opts {
     float scale;           /* of q k^T; 0: 1 / sqrt(dim) */
-    float softcap;         /* c > 0: c tanh(score / c) */
+    float softcap;         /* c > 0: c tanh(score / c) (from 2^64 on as 0, below 2^-64 as 2^-64) */
     const float* slopes;   /* [query heads]: score -= slope |position - key position| */
     const int32_t* prefix; /* [seqs]: keys before it are seen by every query of the sequence, causal or not */
     const int32_t* first;  /* [tokens]: first key that a query sees (where its document begins) */

@@ -241,7 +241,9 @@ static int run_attention(vx_ctx ctx, vx_stream stream, const vx_mview* out, cons
     a.max_len = batch->max_len;
     a.scale = opts && opts->scale != 0.f ? opts->scale : 1.f / std::sqrt((float)cache->dim);
     if (opts) {
-        a.cap = opts->softcap;
+        // score / cap and cap log2(e) must stay among f32's normal numbers: a cap that scores do not come
+        // near changes none, and below 2^-64 no cap leaves a difference between keys
+        a.cap = opts->softcap >= 0x1p64f ? 0.f : opts->softcap > 0.f ? std::max(opts->softcap, 0x1p-64f) : 0.f;
         a.slopes = opts->slopes;
         a.first = opts->first;
         a.window = opts->window >= VX_MOST_KEYS ? 0u : opts->window;  // (none that any key is outside of)
