@@ -49,10 +49,15 @@ struct vx_rows16 {
     }
 
     static __device__ __forceinline__ void load_scales(const uint8_t* p, uint32_t g, uint32_t (&s)[NB][2]) {
+        // (rows of 8 NB bytes: of three blocks every other one begins between two multiples of 16)
+        typedef uint32_t row_u4 __attribute__((ext_vector_type(4), aligned(8)));
+        static_assert(8 * NB % alignof(row_u4) == 0 && PK::VALS % alignof(row_u4) == 0 && PK::BYTES % alignof(row_u4) == 0 &&
+                          PV::VALS % alignof(row_u4) == 0 && REC % alignof(row_u4) == 0,
+                      "a row of scales is not aligned for its loads");
         p += g * (8 * NB);
 #pragma unroll
         for (int b = 0; b + 1 < NB; b += 2) {
-            const u4 v = *(const u4*)(p + 8 * b);
+            const row_u4 v = *(const row_u4*)(p + 8 * b);
             s[b][0] = v.x, s[b][1] = v.y, s[b + 1][0] = v.z, s[b + 1][1] = v.w;
         }
         if constexpr (NB % 2 != 0) {
