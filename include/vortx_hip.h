@@ -21,7 +21,10 @@
  *    except vx_gemv_q_noalloc's shared scratch array (see there): memory a
  *    call needs beyond its operands is passed in by the caller
  *    (vx_gemv_q_ws), like the reference's caller-owned
- *    `shapes: &mut TensorLayoutBuffers` (src/linalg/gemm.rs:47-56).
+ *    `shapes: &mut TensorLayoutBuffers` (src/linalg/gemm.rs:47-56). The
+ *    kernels of the key/value cache and its attention are loaded, a head size
+ *    at a time and once for all threads, by the first call that uses them
+ *    (a few milliseconds; vx_attention_ws_size is such a call).
  */
 #ifndef VORTX_HIP_H
 #define VORTX_HIP_H
@@ -522,7 +525,7 @@ int vx_attention_tree(vx_ctx ctx, vx_stream stream, const vx_mview* out, const v
                       uint32_t tree_stride, void* workspace, uint64_t workspace_bytes);
 
 /* Bytes of workspace that either of them may use for `tokens` query tokens of
- * `q_heads` heads (0: none). */
+ * `q_heads` heads (0: none). Loads their kernels where no call has yet. */
 int vx_attention_ws_size(vx_ctx ctx, const vx_kv_cache* cache, const vx_attn_batch* batch, const vx_attn_opts* opts,
                          uint32_t tokens, uint32_t q_heads, uint64_t* bytes);
 

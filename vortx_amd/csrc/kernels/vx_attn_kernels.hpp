@@ -42,6 +42,4 @@ VX_WIDE(k8v4, 8, 4)
 VX_WIDE(k4v8, 4, 8)
 VX_WIDE(k4v4, 4, 4)
 
-#if VX_NB == 4
-extern "C" __global__ __launch_bounds__(256) void vx_attn_join(vx_attn_args a) { vx_attn_join_rows(a); }
-#endif
+extern "C" __global__ __launch_bounds__(256) void VX_JOIN(vx_attn_args a) { vx_attn_join_rows(a); }

@@ -53,6 +53,7 @@ static const int kWrite[4] = VX_DIMS(kv_write), kRead[4] = VX_DIMS(kv_read), kEv
                  kEach128[4] = VX_DIMS(attn_each128), kEven128[4] = VX_DIMS(attn_even128);
 #undef VX_DIMS
 #define VX_DIMS(f) {K_vx_##f##_d64_k8v8, K_vx_##f##_d96_k8v8, K_vx_##f##_d128_k8v8}
+static const int kJoin[4] = {K_vx_attn_join_d64, K_vx_attn_join_d96, K_vx_attn_join_d128, K_vx_attn_join_d256};
 static const int kEach256[3] = VX_DIMS(attn_each256), kEven256[3] = VX_DIMS(attn_even256);
 #undef VX_DIMS
 
@@ -264,7 +265,7 @@ static int run_attention(vx_ctx ctx, vx_stream stream, const vx_mview* out, cons
     if ((s = launch_struct(ctx, kernel_of(cache, p.kernel), p.grid, p.block, stream, &a))) return s;
     if (p.even) {
         const uint64_t jobs = (uint64_t)batch->max_queries * a.group * batch->seqs * cache->heads;
-        return launch_struct(ctx, K_vx_attn_join, (uint32_t)(p.parts > 8 ? jobs : (jobs + 3) / 4), 256, stream, &a);
+        return launch_struct(ctx, kJoin[dim_index(cache->dim)], (uint32_t)(p.parts > 8 ? jobs : (jobs + 3) / 4), 256, stream, &a);
     }
     return VX_OK;
 }
@@ -324,7 +325,7 @@ int vx_attention_ws_size(vx_ctx ctx, const vx_kv_cache* cache, const vx_attn_bat
     vx::AttnPlan p;
     if ((s = vx::plan_attention(vx::ctx_cus(ctx), cache, batch, opts, q_heads, true, &p))) return s;
     *bytes = p.bytes(cache->dim);
-    return VX_OK;
+    return vx::need_kernel(ctx, vx::kernel_of(cache, p.kernel));
 }
 
 }  // extern "C"

@@ -3,8 +3,9 @@
 //
 // Runtime: the gfx950 code objects built by hipcc --genco are embedded in
 // this library (vx_embed.S); vx_init loads them with hipModuleLoadData and
-// resolves every kernel once; launches go through hipModuleLaunchKernel with
-// the kernel's argument struct (vx_kargs.h) passed by value (kernelParams).
+// resolves every kernel once (the attention's of a head size at their first
+// use); launches go through hipModuleLaunchKernel with the kernel's argument
+// struct (vx_kargs.h) passed by value (kernelParams).
 //
 // Ops: Gemm::dispatch / dispatch_naive / dispatch_tiled of
 // src/linalg/gemm.rs:47-305 (canonicalize, validate, pick a kernel, grid)
@@ -15,7 +16,9 @@
 #include <cstdlib>
 #include <cstring>
 #include <algorithm>
+#include <atomic>
 #include <cmath>
+#include <mutex>
 #include <string>
 #include <vector>
 
@@ -74,10 +77,17 @@ static const char* const kKernelNames[K_COUNT] = {
 #undef K
 };
 // The embedded code objects; every kernel name is unique across them.
-static const unsigned char* const kModules[] = {vx_co_gemm, vx_co_gemv_q, vx_co_copy, vx_co_quantize, vx_co_gemm_q, vx_co_gemm_bf,
-                                               vx_co_attn_d64, vx_co_attn_d96, vx_co_attn_d128, vx_co_attn_d256};
-constexpr int kNumModules = 10;
+static const unsigned char* const kModules[] = {vx_co_gemm, vx_co_gemv_q, vx_co_copy, vx_co_quantize, vx_co_gemm_q, vx_co_gemm_bf};
+constexpr int kNumModules = 6;
 constexpr int kModGemv = 1;  // the module holding vx_scratch
+// The attention's, one a head size, with its kernels: loaded at their first use.
+// A context takes 16 ms with them and 8 without, and most have no use for them.
+static const struct { const unsigned char* image; int first, end; } kLate[] = {
+    {vx_co_attn_d64, K_vx_kv_write_d64_k8v8, K_vx_kv_write_d96_k8v8},
+    {vx_co_attn_d96, K_vx_kv_write_d96_k8v8, K_vx_kv_write_d128_k8v8},
+    {vx_co_attn_d128, K_vx_kv_write_d128_k8v8, K_vx_kv_write_d256_k8v8},
+    {vx_co_attn_d256, K_vx_kv_write_d256_k8v8, K_COUNT}};
+constexpr int kNumLate = 4, kLateFirst = K_vx_kv_write_d64_k8v8;
 
 }  // namespace vx
 
@@ -87,10 +97,13 @@ struct vx_context {
     size_t lds_per_block = 65536;
     hipModule_t mods[vx::kNumModules] = {};
     hipFunction_t fn[vx::K_COUNT] = {};
+    hipModule_t late[vx::kNumLate] = {};         // and its functions: written under late_lock, read once late_ready says so
+    std::atomic<bool> late_ready[vx::kNumLate] = {};
+    std::mutex late_lock;
     // device address of vx_scratch in this context's GEMV module (vx_gemv_q_noalloc)
     void* scratch = nullptr;
     size_t scratch_bytes = 0;
-    // Nothing here changes after vx_init: buffers a call needs beyond its
+    // Nothing else here changes after vx_init: buffers a call needs beyond its
     // operands are the caller's (vx_gemv_q_ws) or the module's scratch.
 };
 
@@ -144,8 +157,44 @@ static int launch_b1(vx_ctx ctx, int k, uint32_t grid, size_t lds, vx_stream str
 
 int ctx_cus(vx_ctx ctx) { return ctx->num_cus; }
 
+// Loading a code object is no stream's work: allowed while this thread captures one.
+struct OutsideCapture {
+    hipStreamCaptureMode mode = hipStreamCaptureModeRelaxed;
+    bool changed = hipThreadExchangeStreamCaptureMode(&mode) == hipSuccess;
+    ~OutsideCapture() {
+        if (changed) (void)hipThreadExchangeStreamCaptureMode(&mode);
+    }
+};
+
+int need_kernel(vx_ctx ctx, int k) {
+    int i = 0;
+    while (k >= kLate[i].end) ++i;
+    if (ctx->late_ready[i].load(std::memory_order_acquire)) return VX_OK;
+    std::lock_guard<std::mutex> lock(ctx->late_lock);
+    if (ctx->late_ready[i].load(std::memory_order_relaxed)) return VX_OK;
+    DeviceGuard guard(ctx->device);
+    OutsideCapture outside;
+    const char* what = "hipModuleLoadData(attention)";
+    hipModule_t mod = nullptr;
+    hipError_t e = hipModuleLoadData(&mod, kLate[i].image);
+    for (int f = kLate[i].first; f < kLate[i].end && e == hipSuccess; ++f) {
+        what = kKernelNames[f];
+        e = hipModuleGetFunction(&ctx->fn[f], mod, what);
+    }
+    if (e != hipSuccess) {
+        (void)hipGetLastError();
+        if (mod) (void)hipModuleUnload(mod);
+        fail_hip(e, what);
+        return VX_ERR_NO_CODE_OBJECT;
+    }
+    ctx->late[i] = mod;
+    ctx->late_ready[i].store(true, std::memory_order_release);
+    return VX_OK;
+}
+
 int launch_struct(vx_ctx ctx, int k, uint32_t grid, uint32_t block, vx_stream stream, const void* args) {
     if (grid == 0) return VX_OK;
+    if (const int s = need_kernel(ctx, k)) return s;
     DeviceGuard guard(ctx->device);
     void* params[] = {const_cast<void*>(args)};
     const hipError_t e = hipModuleLaunchKernel(ctx->fn[k], grid, 1, 1, block, 1, 1, 0, (hipStream_t)stream, params, nullptr);
@@ -197,7 +246,7 @@ static int init(int device, vx_ctx* out) {
             return VX_ERR_NO_CODE_OBJECT;
         }
     }
-    for (int k = 0, at = 0; k < K_COUNT; ++k) {
+    for (int k = 0, at = 0; k < kLateFirst; ++k) {
         e = hipErrorNotFound;
         for (int i = 0; i < kNumModules && e != hipSuccess; ++i) {  // from the module of the kernel before: the list goes by modules
             const int mod = (at + i) % kNumModules;
@@ -1369,6 +1418,8 @@ int vx_destroy(vx_ctx ctx) {
     if (!ctx) return VX_OK;
     vx::DeviceGuard guard(ctx->device);
     for (hipModule_t m : ctx->mods)
+        if (m) (void)hipModuleUnload(m);
+    for (hipModule_t m : ctx->late)
         if (m) (void)hipModuleUnload(m);
     delete ctx;
     return VX_OK;

@@ -9,7 +9,7 @@
 
 namespace vx {
 
-// Every kernel the library launches; resolved by name at vx_init.
+// Every kernel the library launches; resolved by name at vx_init, the attention's at their first use.
 enum Kernel : int {
 #define K(name) K_##name,
 #include "vx_kernel_list.inc"
@@ -25,7 +25,9 @@ struct Canon {
 int canon_view(const void* base, const vx_layout* in, Canon* c, const char* name);
 
 int ctx_cus(vx_ctx ctx);
-// Launches kernel k on the context's device; `args` is its one struct argument.
+// Kernel k of the attention is there: loads the code object of its head size if it is not yet.
+int need_kernel(vx_ctx ctx, int k);
+// Launches such a kernel on the context's device; `args` is its one struct argument.
 int launch_struct(vx_ctx ctx, int k, uint32_t grid, uint32_t block, vx_stream stream, const void* args);
 
 // Records `msg` as this thread's last error and returns `status`.
