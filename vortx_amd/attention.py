@@ -81,7 +81,10 @@ class AttentionPlan:
     """What attention calls of one batch share (:meth:`KvAttention.plan`): the
     cache, the batch's device arrays, options and a workspace. It keeps the
     tensors it was made of alive; their contents may change between calls.
-    Calls that use one plan share its workspace, so they must be ordered."""
+    Calls that use one plan share its workspace, so they must be ordered.
+    ``ws`` and ``ws_bytes`` are the workspace's address (None: none, the keys
+    are not split) and size; ``max_queries``, ``seqs`` and ``tokens`` say what
+    the plan was made for."""
     cache: KvCache
     q_heads: int
     max_queries: int
@@ -94,10 +97,20 @@ class AttentionPlan:
     opts: object         # _ffi.VxAttnOpts
 
     def __post_init__(self):
-        self.ws, self.ws_bytes = self.workspace.data_ptr(), self.workspace.numel()
-        # what _pycall.attend takes: the structs' addresses, the workspace, and what q may be
-        self.call = (self.cache._addr, C.addressof(self.batch), C.addressof(self.opts), self.ws, self.ws_bytes, self.q_heads,
-                     2 ** 32 - 1 if self.first_tokens is None else self.first_tokens)
+        self.workspace = self.workspace
+
+    def __setattr__(self, name, value):
+        set_ = object.__setattr__
+        set_(self, name, value)
+        if "opts" not in self.__dict__:
+            return  # (not all there yet)
+        if name == "workspace":
+            set_(self, "ws", value.data_ptr())
+            set_(self, "ws_bytes", value.numel() * value.element_size())
+        if "ws_bytes" in self.__dict__:
+            # what _pycall.attend takes: the structs' addresses, the workspace, and what q may be
+            set_(self, "call", (self.cache._addr, C.addressof(self.batch), C.addressof(self.opts), self.ws or 0, self.ws_bytes, self.q_heads,
+                                2 ** 32 - 1 if self.first_tokens is None else self.first_tokens))
 
 
 def tree_mask(parents, device="cuda:0"):
