@@ -27,8 +27,16 @@ from ._ffi import VX_Q8_0, VortxError, check, lib
 _WRITE, _READ, _ATTEND, _TREE = (_ADDR[n] for n in ("vx_kv_write", "vx_kv_read", "vx_attention", "vx_attention_tree"))
 
 
+def _u32(**values) -> None:
+    """Refuses what a 32-bit field would hold as another number."""
+    for name, v in values.items():
+        if not 0 <= v < 2 ** 32:
+            raise VortxError(_ffi.VX_ERR_INVALID, f"{name} is {v}: a number from 0 to 2^32 - 1 is expected")
+
+
 def kv_cache_size(pages: int, page_tokens: int, heads: int, dim: int, k_type: int = VX_Q8_0, v_type: int = VX_Q8_0) -> int:
     """Bytes of such a cache (vx_kv_cache_size)."""
+    _u32(pages=pages, page_tokens=page_tokens, heads=heads, dim=dim, k_type=k_type, v_type=v_type)
     n = C.c_uint64()
     check(lib().vx_kv_cache_size(C.byref(_ffi.VxKvCache(None, 0, pages, page_tokens, heads, dim, k_type, v_type)), C.byref(n)))
     return n.value
@@ -180,6 +188,7 @@ class KvAttention(_Context):
         [sequences], keys that every query sees; ``first`` int32 [tokens], the
         first key that a query sees."""
         import torch
+        _u32(q_heads=q_heads, max_queries=max_queries, max_len=max_len, tokens=tokens, window=window)
         o = _ffi.VxAttnOpts(scale, softcap, None, None, None, _ffi.VX_ATTN_CAUSAL if causal else 0, window)
         seqs = lens.shape[0] if isinstance(lens, torch.Tensor) and lens.dim() == 1 else 0
         b = _ffi.VxAttnBatch(_array(table, "table", (seqs, None)), _array(lens, "lens", (None,)),
@@ -190,7 +199,7 @@ class KvAttention(_Context):
             o.prefix = _array(prefix, "prefix", (seqs,))
         if first is not None:
             o.first = _array(first, "first", (None,))
-        tokens = tokens or seqs * max_queries
+        tokens = tokens or min(seqs * max_queries, 2 ** 32 - 1)
         n = C.c_uint64()
         check(lib().vx_attention_ws_size(self._h, C.byref(cache._c), C.byref(b), C.byref(o), tokens, q_heads, C.byref(n)))
         ws = torch.empty(max(16, n.value), dtype=torch.uint8, device=cache.data.device)
