@@ -117,7 +117,7 @@ static int run_rows(vx_ctx ctx, vx_stream stream, const vx_kv_cache* cache, cons
         a.vs[i] = r[1].stride[i];
     }
     a.quads = a.tokens >= VX_QUAD_TOKENS;
-    a.groups = a.quads ? (a.tokens + 3) / 4 : a.tokens;
+    a.groups = a.quads ? (a.tokens - 1) / 4 + 1 : a.tokens;
     const uint64_t units = (uint64_t)a.groups * cache->heads * (cache->dim == 96 ? 4 : cache->dim / 32);
     const uint32_t grid = (uint32_t)std::min<uint64_t>((units + 31) / 32, 1u << 20);
     return launch_struct(ctx, kernel_of(cache, write ? kWrite : kRead), grid, 256, stream, &a);
