@@ -465,7 +465,9 @@ int vx_kv_read(vx_ctx ctx, vx_stream stream, const vx_mview* k, const vx_mview* 
  *                               lens[s] - n + j (n its queries)
  * max_queries and max_len are upper bounds that the launch is laid out by;
  * keys past max_len or past the table's pages are not seen (positions stay as
- * lens says), queries past max_queries not computed. */
+ * lens says), queries past max_queries not computed. seqs * max_queries * query
+ * heads are below 2^24 and seqs * the cache's heads below 2^23, else
+ * VX_ERR_UNSUPPORTED. */
 typedef struct vx_attn_batch {
     const int32_t* table;
     const int32_t* lens;

@@ -163,6 +163,10 @@ static int plan_attention(int num_cus, const vx_kv_cache* c, const vx_attn_batch
     // trees of 244 rows 202 / 203, of 200 rows, 16 sequences, 131 / 113. (256 dims: see the kernels.)
     const bool wide = rows > 128 && c->dim <= 128;
     *p = AttnPlan{};
+    // (a grid has below 2^32 threads, and the join 256 a row; one factor after the other: the products stay in 64 bits)
+    constexpr uint64_t most_rows = 1ull << 24;
+    if (rows >= most_rows || rows * b->seqs >= most_rows || rows * b->seqs * c->heads >= most_rows)
+        return fail(VX_ERR_UNSUPPORTED, "attention: too many query rows (split the batch)");
     // (the keys are dealt out by their number of steps, which is counted in 32 bits)
     const uint64_t most = std::min<uint64_t>(b->max_len, (uint64_t)b->table_cols * c->page_tokens);
     const bool deal = ws && ((rows + 15) / 16) * b->seqs * (most / 64 + 8) < (1ull << 32);
@@ -171,8 +175,7 @@ static int plan_attention(int num_cus, const vx_kv_cache* c, const vx_attn_batch
     const uint64_t places = (uint64_t)num_cus * (p->rows == 256 || c->dim > 128 ? 1 : 2);  // workgroups that the card holds
     const uint64_t rb = (rows + p->rows - 1) / p->rows;
     p->units = rb * b->seqs * c->heads;
-    if (p->units >= (1ull << 23) || rows * b->seqs * c->heads >= (1ull << 24))
-        return fail(VX_ERR_UNSUPPORTED, "attention: too many query rows (split the batch)");
+    if (p->units >= (1ull << 23)) return fail(VX_ERR_UNSUPPORTED, "attention: too many query rows (split the batch)");
     p->row_blocks = (uint32_t)rb;
     p->even = deal && (p->rows == 16 || p->units <= VX_EVEN_UNITS * places);
     p->kernel = p->rows == 16 ? kEven16 : p->rows == 128 ? (p->even ? kEven128 : kEach128) : (p->even ? kEven256 : kEach256);
