@@ -8,6 +8,7 @@
 #include <cstring>
 #include <map>
 #include <mutex>
+#include <set>
 #include <string>
 #include <thread>
 #include <vector>
@@ -28,6 +29,7 @@ static std::mutex lock;
 static std::map<const void*, int> loads;  // by image
 static int live, launches, strict;        // modules; launches; captures that allow stream work only
 static unsigned last_grid;
+static std::set<hipFunction_t> launched;
 static std::atomic<int> fail_after{-1};   // names that resolve before one does not
 static std::map<std::string, hipFunction_t> names;
 static thread_local hipStreamCaptureMode capture = hipStreamCaptureModeGlobal;
@@ -79,6 +81,7 @@ hipError_t hipModuleLaunchKernel(hipFunction_t f, unsigned grid, unsigned, unsig
     std::lock_guard<std::mutex> l(lock);
     ++launches;
     last_grid = grid;
+    launched.insert(f);
     return f ? hipSuccess : hipErrorInvalidHandle;
 }
 hipError_t hipThreadExchangeStreamCaptureMode(hipStreamCaptureMode* m) {

@@ -17,11 +17,9 @@
     }                                                                                                          \
     extern "C" __global__ __launch_bounds__(256, VX_NB <= 4 ? 2 : 1) void VX_CAT(attn_each128, types)(vx_attn_args a) { \
         vx_tile<VX_NB, KB, VB, 4>::each(a);                                                                    \
-    }                                                                                                          \
-    extern "C" __global__ __launch_bounds__(256, VX_NB <= 4 ? 2 : 1) void VX_CAT(attn_even128, types)(vx_attn_args a) { \
-        vx_tile<VX_NB, KB, VB, 4>::even(a);                                                                    \
     }
-// (heads of 256: eight waves' registers do not hold the sums)
+// (heads of 256: eight waves' registers do not hold the sums, and four hold them
+// only with up to 100 registers in memory)
 #if VX_NB <= 4
 #define VX_WIDE(types, KB, VB)                                                                                 \
     extern "C" __global__ __launch_bounds__(512, 2) void VX_CAT(attn_each256, types)(vx_attn_args a) {         \
@@ -31,7 +29,10 @@
         vx_tile<VX_NB, KB, VB, 8>::even(a);                                                                    \
     }
 #else
-#define VX_WIDE(types, KB, VB)
+#define VX_WIDE(types, KB, VB)                                                                                 \
+    extern "C" __global__ __launch_bounds__(256) void VX_CAT(attn_even128, types)(vx_attn_args a) {            \
+        vx_tile<VX_NB, KB, VB, 4>::even(a);                                                                    \
+    }
 #endif
 VX_KERNELS(k8v8, 8, 8)
 VX_KERNELS(k8v4, 8, 4)

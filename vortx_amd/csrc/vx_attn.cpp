@@ -50,12 +50,14 @@ static int kernel_of(const vx_kv_cache* c, const int* d) {
 }
 #define VX_DIMS(f) {K_vx_##f##_d64_k8v8, K_vx_##f##_d96_k8v8, K_vx_##f##_d128_k8v8, K_vx_##f##_d256_k8v8}
 static const int kWrite[4] = VX_DIMS(kv_write), kRead[4] = VX_DIMS(kv_read), kEven16[4] = VX_DIMS(attn_even16),
-                 kEach128[4] = VX_DIMS(attn_each128), kEven128[4] = VX_DIMS(attn_even128);
+                 kEach128[4] = VX_DIMS(attn_each128);
 #undef VX_DIMS
 #define VX_DIMS(f) {K_vx_##f##_d64_k8v8, K_vx_##f##_d96_k8v8, K_vx_##f##_d128_k8v8}
 static const int kJoin[4] = {K_vx_attn_join_d64, K_vx_attn_join_d96, K_vx_attn_join_d128, K_vx_attn_join_d256};
-static const int kEach256[3] = VX_DIMS(attn_each256), kEven256[3] = VX_DIMS(attn_even256);
+static const int kEach256[3] = VX_DIMS(attn_each256);
 #undef VX_DIMS
+static const int kEvenTiles[4] = {K_vx_attn_even256_d64_k8v8, K_vx_attn_even256_d96_k8v8, K_vx_attn_even256_d128_k8v8,
+                                  K_vx_attn_even128_d256_k8v8};
 
 // A [tokens, heads, dim] view.
 struct Rows {
@@ -131,19 +133,26 @@ constexpr uint32_t VX_MOST_KEYS = (1u << 31) - 65536u;  // of a sequence
 // Up to so many rows the 16-row kernel, whose row blocks read the keys again, is
 // faster than the tiles of 128 and 256 rows, which decode them once. Trees of
 // drafts, us, 16 rows / tiles:
-//   dim 128, 1 sequence of 1500 keys   96 rows 18.6 / 25.9   128 rows 19.7 / 27.4
-//            1 of 20000                96      56.0 / 63.5   128      67.9 / 71.4   192 rows 93.7 / 86.4
-//            8 of up to 12000          96       114 / 124    128       145 / 134
-//            32 of up to 2000          96      97.9 / 106    128       124 / 112
-//   dim 64,  4 of up to 6000          128      43.0 / 48.1   192      44.1 / 50.5
-//   dim 256, 4 of up to 6000          128      92.3 / 117    192       132 / 149
-static uint64_t rows16_most(uint32_t dim) { return dim == 96 || dim == 128 ? 112 : 192; }
+//   dim 128, 1 sequence of 300 keys   120 rows 13.9 / 24.2   128 rows 13.9 / 24.5
+//            1 of 1500                120      19.1 / 30.2   128      19.8 / 30.7   192 rows 22.1 / 37.0
+//            1 of 20000               120      56.1 / 57.7   128      57.9 / 58.6   192      78.3 / 72.5
+//            4 of up to 6000          120      47.0 / 50.1   128      56.1 / 60.2
+//            8 of up to 12000         120       116 / 112    128       140 / 129    192       203 / 186
+//            32 of up to 2000         120       112 / 105    128       105 / 95.9   192       162 / 151
+//   dim 96,  1 of 1500                120      17.9 / 27.0   128      17.9 / 27.1
+//            8 of up to 12000         120      89.8 / 105    128      96.4 / 115
+//            32 of up to 2000         120      88.8 / 90.0   128       106 / 100
+//   dim 64,  4 of up to 6000          128      37.1 / 42.2   192      56.4 / 59.8
+//   dim 256, 4 of up to 6000          128       102 / 115    192       181 / 194
+// So batches of many sequences lose up to a tenth just below the bound, and single ones win up to half.
+static uint64_t rows16_most(uint32_t dim) { return dim == 96 || dim == 128 ? 128 : 192; }
 // More units than places: a workgroup each (units of one length, or many of them,
 // fill the card by themselves, and no partial sums are written). Us, a workgroup
 // each / dealt out evenly: 512 units on 256 places, 4096 causal tokens of 32
-// heads of 128, 415 / 476; 480, packed documents, 78 / 119; but 752 of dim 64,
-// two prompts of 3000, 246 / 217. Up to as many: 256, four chunks behind
-// histories of 900 to 3000, 237 / 206; 256, a prompt of 2000, 152 / 146.
+// heads of 128, 382 / 439; 480, windows of 1000 in prompts of up to 2500, 119 /
+// 132; 752 of dim 64, two prompts of up to 3000, 291 / 315. Up to as many: 256,
+// four chunks behind histories of 900 to 3000, 255 / 249; 256, a prompt of 2000,
+// 151 / 145.
 constexpr uint64_t VX_EVEN_UNITS = 1;
 struct AttnPlan {
     const int* kernel;
@@ -159,8 +168,8 @@ static int plan_attention(int num_cus, const vx_kv_cache* c, const vx_attn_batch
                           bool ws, AttnPlan* p) {
     const uint64_t group = q_heads / c->heads, queries = b->max_queries, rows = queries * group;
     // 256 rows a workgroup decode a tile of keys once where two of 128 do it twice; us, 256 / 128
-    // rows: 4096 causal tokens, dim 128 416 / 468, dim 64 225 / 252; chunks behind histories 215 / 218;
-    // trees of 244 rows 202 / 203, of 200 rows, 16 sequences, 131 / 113. (256 dims: see the kernels.)
+    // rows: 4096 causal tokens, dim 128 383 / 430, dim 64 250 / 268; chunks behind histories 208 / 229;
+    // trees of 244 rows 196 / 183, of 200 rows, 16 sequences, 313 / 312. (256 dims: see the kernels.)
     const bool wide = rows > 128 && c->dim <= 128;
     *p = AttnPlan{};
     // (a grid has below 2^32 threads, and the join 256 a row; one factor after the other: the products stay in 64 bits)
@@ -178,7 +187,7 @@ static int plan_attention(int num_cus, const vx_kv_cache* c, const vx_attn_batch
     if (p->units >= (1ull << 23)) return fail(VX_ERR_UNSUPPORTED, "attention: too many query rows (split the batch)");
     p->row_blocks = (uint32_t)rb;
     p->even = deal && (p->rows == 16 || p->units <= VX_EVEN_UNITS * places);
-    p->kernel = p->rows == 16 ? kEven16 : p->rows == 128 ? (p->even ? kEven128 : kEach128) : (p->even ? kEven256 : kEach256);
+    p->kernel = p->even ? (p->rows == 16 ? kEven16 : kEvenTiles) : p->rows == 128 ? kEach128 : kEach256;
     p->grid = (uint32_t)p->units;
     if (p->even) {
         uint64_t span = most;
