@@ -114,7 +114,8 @@ struct vx_tile {
     static __device__ __forceinline__ void store(raw& r, tile& s) {
         typedef uint16_t us2 __attribute__((ext_vector_type(2)));
         const uint32_t t = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(t >> 6), rec = wave & 1, lane = t & 63, m = lane & 15, g = lane >> 4;
-        // the largest of four sizes, and whether another one (but for zeros) is far below it
+        // the largest of four sizes, and whether another one is far below it. 0 is no size: K's zeros are
+        // exact beside any; a key of V's zeros has weight, which the others' exponent would take bits from
         auto largest = [](uint32_t e, bool& far) {
             const us2 lo = __builtin_bit_cast(us2, e & 0x00FF00FFu), hi = __builtin_bit_cast(us2, e >> 8 & 0x00FF00FFu), one = {1, 1};
             const us2 most = __builtin_elementwise_max(lo, hi), least = __builtin_elementwise_min(lo - one, hi - one);

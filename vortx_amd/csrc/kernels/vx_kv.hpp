@@ -21,9 +21,9 @@
 // a dword are those that masks and byte permutes unpack to pairs of f16.
 // Scales: f16, [g][b][4]: of K for keys 4 g + j, of V the same. Sizes: a byte a
 // key, 16 above the exponent of the largest of its scales (1 to 31; an f16
-// below its normal numbers counts as 2^-15; 0: all are zero), with 128 added
-// where another one that is not zero has an exponent more than VX_KV_APART
-// lower, and 255 where one is not finite.
+// below its normal numbers counts as 2^-15; where all are zero, K has 0 and V
+// 1), with 128 added where another one that is not zero has an exponent more
+// than VX_KV_APART lower, and 255 where one is not finite.
 #pragma once
 #include <hip/hip_runtime.h>
 #include <stdint.h>

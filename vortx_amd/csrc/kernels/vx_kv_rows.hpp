@@ -169,10 +169,11 @@ __device__ __forceinline__ uint32_t vx_kv_max_halves(uint32_t v) {
     return v;
 }
 
-// Two size bytes (a half each) of a row whose block has sizes `own`.
+// Two size bytes (a half each) of a row whose block has sizes `own`, `least` at the least.
 template <int NP>
-__device__ __forceinline__ uint32_t vx_kv_row_sizes(uint32_t own) {
-    uint32_t top = vx_kv_max_halves<NP>(own);
+__device__ __forceinline__ uint32_t vx_kv_row_sizes(uint32_t own, uint32_t least) {
+    typedef uint16_t us2 __attribute__((ext_vector_type(2)));
+    uint32_t top = __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(us2, vx_kv_max_halves<NP>(own)), __builtin_bit_cast(us2, least)));
     // how far the block is below the largest one; not at all if it is all zeros
     const uint32_t lo = own & 0xFFFFu ? (top & 0xFFFFu) - (own & 0xFFFFu) : 0u, hi = own >> 16 ? (top >> 16) - (own >> 16) : 0u;
     if (__any((lo > VX_KV_APART) | (hi > VX_KV_APART))) {
@@ -254,8 +255,8 @@ __device__ __forceinline__ void vx_kv_write_rows(const vx_kv_rows_args& a) {
                 }
                 if (u == 0) *(u2*)(rec + R::V + PV::VALS + ((m >> 2) * NB + b) * 8) = sc;
             }
-            klo = vx_kv_row_sizes<NP>(klo), khi = vx_kv_row_sizes<NP>(khi);
-            vlo = vx_kv_row_sizes<NP>(vlo), vhi = vx_kv_row_sizes<NP>(vhi);
+            klo = vx_kv_row_sizes<NP>(klo, 0u), khi = vx_kv_row_sizes<NP>(khi, 0u);
+            vlo = vx_kv_row_sizes<NP>(vlo, 0x00010001u), vhi = vx_kv_row_sizes<NP>(vhi, 0x00010001u);
             if (u == 0 && b == 0) {
                 *(uint32_t*)(rec + R::K_SIZES + m) = vx_kv_bytes(klo, khi);
                 *(uint32_t*)(rec + R::V_SIZES + m) = vx_kv_bytes(vlo, vhi);
@@ -268,7 +269,7 @@ __device__ __forceinline__ void vx_kv_write_rows(const vx_kv_rows_args& a) {
             size = vx_kv_put_k<NB, KB>(rec, m, b, u, k) << 16;
             size |= vx_kv_put_v<NB, VB>(rec + R::V, m, b, u, v);
         }
-        size = vx_kv_row_sizes<NP>(size);
+        size = vx_kv_row_sizes<NP>(size, 1u);
         if (u == 0 && b == 0) {
             rec[R::K_SIZES + m] = (uint8_t)(size >> 16);
             rec[R::V_SIZES + m] = (uint8_t)size;
