@@ -23,8 +23,9 @@
  *    (vx_gemv_q_ws), like the reference's caller-owned
  *    `shapes: &mut TensorLayoutBuffers` (src/linalg/gemm.rs:47-56). The
  *    kernels of the key/value cache and its attention are loaded, a head size
- *    at a time and once for all threads, by the first call that uses them
- *    (a few milliseconds; vx_attention_ws_size is such a call).
+ *    at a time and once for all contexts of a device, by the first call that
+ *    uses them (a few milliseconds; vx_attention_ws_size is such a call), and
+ *    stay loaded.
  */
 #ifndef VORTX_HIP_H
 #define VORTX_HIP_H

@@ -32,12 +32,13 @@ static unsigned last_grid;
 static std::set<hipFunction_t> launched;
 static std::atomic<int> fail_after{-1};   // names that resolve before one does not
 static std::map<std::string, hipFunction_t> names;
+static thread_local int device;
 static thread_local hipStreamCaptureMode capture = hipStreamCaptureModeGlobal;
 
 extern "C" {
-hipError_t hipGetDeviceCount(int* n) { *n = 1; return hipSuccess; }
-hipError_t hipGetDevice(int* d) { *d = 0; return hipSuccess; }
-hipError_t hipSetDevice(int) { return hipSuccess; }
+hipError_t hipGetDeviceCount(int* n) { *n = 2; return hipSuccess; }
+hipError_t hipGetDevice(int* d) { *d = device; return hipSuccess; }
+hipError_t hipSetDevice(int d) { device = d; return hipSuccess; }
 hipError_t hipGetDevicePropertiesR0600(hipDeviceProp_tR0600* p, int) {
     std::memset((void*)p, 0, sizeof *p);
     std::strcpy(p->gcnArchName, "gfx950");

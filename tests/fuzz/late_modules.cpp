@@ -59,20 +59,30 @@ int main() {
     CHECK(write(ctx, 256) == VX_OK && capture == hipStreamCaptureModeGlobal);
     strict = 0;
     CHECK(live == 10);
-    CHECK(vx_destroy(ctx) == VX_OK && live == 0);
-    // threads whose first use is the same
-    CHECK(vx_init(0, &ctx) == VX_OK);
+    // they are all contexts' of the device, and stay
+    vx_ctx other = nullptr;
+    CHECK(vx_init(0, &other) == VX_OK && live == 16);
+    CHECK(write(other, 64) == VX_OK && write(other, 256) == VX_OK && attend(other, 128, nullptr, 0) == VX_OK && live == 16);
+    CHECK(vx_destroy(other) == VX_OK && vx_destroy(ctx) == VX_OK && live == 4);
+    CHECK(vx_init(0, &ctx) == VX_OK && live == 10);
+    CHECK(write(ctx, 64) == VX_OK && live == 10);
+    CHECK(vx_destroy(ctx) == VX_OK && live == 4);
+    // threads whose first use is the same, each with a context of its own and all with one: another device
+    live = launches = 0;
     loads.clear();
-    launches = 0;
+    CHECK(vx_init(1, &ctx) == VX_OK && total() == 6);
     std::vector<std::thread> threads;
     std::atomic<int> bad{0};
     for (int i = 0; i < 16; ++i)
         threads.emplace_back([&, i] {
-            for (int j = 0; j < 50; ++j) bad += write(ctx, i % 2 ? 64 : 256) != VX_OK;
+            vx_ctx own = nullptr;
+            bad += vx_init(1, &own) != VX_OK;
+            for (int j = 0; j < 50; ++j) bad += write(j % 2 ? own : ctx, i % 2 ? 64 : 256) != VX_OK;
+            bad += vx_destroy(own) != VX_OK;
         });
     for (auto& t : threads) t.join();
-    CHECK(!bad && total() == 2 && launches == 800);
-    CHECK(vx_destroy(ctx) == VX_OK && live == 0);
+    CHECK(!bad && loads[vx_co_attn_d64] == 1 && loads[vx_co_attn_d256] == 1 && !loads[vx_co_attn_d128] && launches == 800);
+    CHECK(vx_destroy(ctx) == VX_OK && live == 2);
     if (!failures) std::printf("fine\n");
     return failures != 0;
 }

@@ -1,8 +1,8 @@
 """Which code objects a context loads, and when (CPU only): the library's host
 sources with a HIP runtime that counts instead of loading
 (tests/fuzz/late_modules.cpp). A context that never touches the key/value cache
-loads none of the attention's kernels; one that does loads those of its head
-size, once, whatever threads or captures the first call comes from."""
+loads none of the attention's kernels; the first one on a device that does loads
+those of its head size, for all, whatever threads or captures the call comes from."""
 import os
 import shutil
 import subprocess

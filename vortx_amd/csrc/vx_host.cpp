@@ -80,14 +80,31 @@ static const char* const kKernelNames[K_COUNT] = {
 static const unsigned char* const kModules[] = {vx_co_gemm, vx_co_gemv_q, vx_co_copy, vx_co_quantize, vx_co_gemm_q, vx_co_gemm_bf};
 constexpr int kNumModules = 6;
 constexpr int kModGemv = 1;  // the module holding vx_scratch
-// The attention's, one a head size, with its kernels: loaded at their first use.
-// A context takes 16 ms with them and 8 without, and most have no use for them.
+// The attention's, one a head size, with its kernels: loaded at their first use,
+// once for all contexts of a device, and kept. A context takes 16 ms with them
+// and 8 without, and most have no use for them; with code objects of each context's
+// own a call on a new one took 0.9 ms where it now takes 0.04.
 static const struct { const unsigned char* image; int first, end; } kLate[] = {
     {vx_co_attn_d64, K_vx_kv_write_d64_k8v8, K_vx_kv_write_d96_k8v8},
     {vx_co_attn_d96, K_vx_kv_write_d96_k8v8, K_vx_kv_write_d128_k8v8},
     {vx_co_attn_d128, K_vx_kv_write_d128_k8v8, K_vx_kv_write_d256_k8v8},
     {vx_co_attn_d256, K_vx_kv_write_d256_k8v8, K_COUNT}};
 constexpr int kNumLate = 4, kLateFirst = K_vx_kv_write_d64_k8v8;
+struct LateKernels {  // of a device
+    hipFunction_t fn[K_COUNT - kLateFirst] = {};  // written under `lock`, read once `ready` says so
+    std::atomic<bool> ready[kNumLate] = {};
+    std::mutex lock;
+};
+// Those of a device; never freed, like the code objects.
+static LateKernels* late_of(int device) {
+    static std::mutex lock;
+    static auto* all = new std::vector<LateKernels*>;
+    std::lock_guard<std::mutex> guard(lock);
+    if (all->size() <= (size_t)device) all->resize(device + 1);
+    LateKernels*& l = (*all)[device];
+    if (!l) l = new LateKernels;
+    return l;
+}
 
 }  // namespace vx
 
@@ -96,14 +113,12 @@ struct vx_context {
     int num_cus = 0;
     size_t lds_per_block = 65536;
     hipModule_t mods[vx::kNumModules] = {};
-    hipFunction_t fn[vx::K_COUNT] = {};
-    hipModule_t late[vx::kNumLate] = {};         // and its functions: written under late_lock, read once late_ready says so
-    std::atomic<bool> late_ready[vx::kNumLate] = {};
-    std::mutex late_lock;
+    hipFunction_t fn[vx::kLateFirst] = {};
+    vx::LateKernels* late = nullptr;  // the device's
     // device address of vx_scratch in this context's GEMV module (vx_gemv_q_noalloc)
     void* scratch = nullptr;
     size_t scratch_bytes = 0;
-    // Nothing else here changes after vx_init: buffers a call needs beyond its
+    // Nothing here changes after vx_init: buffers a call needs beyond its
     // operands are the caller's (vx_gemv_q_ws) or the module's scratch.
 };
 
@@ -169,9 +184,10 @@ struct OutsideCapture {
 int need_kernel(vx_ctx ctx, int k) {
     int i = 0;
     while (k >= kLate[i].end) ++i;
-    if (ctx->late_ready[i].load(std::memory_order_acquire)) return VX_OK;
-    std::lock_guard<std::mutex> lock(ctx->late_lock);
-    if (ctx->late_ready[i].load(std::memory_order_relaxed)) return VX_OK;
+    LateKernels& late = *ctx->late;
+    if (late.ready[i].load(std::memory_order_acquire)) return VX_OK;
+    std::lock_guard<std::mutex> lock(late.lock);
+    if (late.ready[i].load(std::memory_order_relaxed)) return VX_OK;
     DeviceGuard guard(ctx->device);
     OutsideCapture outside;
     const char* what = "hipModuleLoadData(attention)";
@@ -179,7 +195,7 @@ int need_kernel(vx_ctx ctx, int k) {
     hipError_t e = hipModuleLoadData(&mod, kLate[i].image);
     for (int f = kLate[i].first; f < kLate[i].end && e == hipSuccess; ++f) {
         what = kKernelNames[f];
-        e = hipModuleGetFunction(&ctx->fn[f], mod, what);
+        e = hipModuleGetFunction(&late.fn[f - kLateFirst], mod, what);
     }
     if (e != hipSuccess) {
         (void)hipGetLastError();
@@ -187,8 +203,7 @@ int need_kernel(vx_ctx ctx, int k) {
         fail_hip(e, what);
         return VX_ERR_NO_CODE_OBJECT;
     }
-    ctx->late[i] = mod;
-    ctx->late_ready[i].store(true, std::memory_order_release);
+    late.ready[i].store(true, std::memory_order_release);
     return VX_OK;
 }
 
@@ -197,7 +212,7 @@ int launch_struct(vx_ctx ctx, int k, uint32_t grid, uint32_t block, vx_stream st
     if (const int s = need_kernel(ctx, k)) return s;
     DeviceGuard guard(ctx->device);
     void* params[] = {const_cast<void*>(args)};
-    const hipError_t e = hipModuleLaunchKernel(ctx->fn[k], grid, 1, 1, block, 1, 1, 0, (hipStream_t)stream, params, nullptr);
+    const hipError_t e = hipModuleLaunchKernel(ctx->late->fn[k - kLateFirst], grid, 1, 1, block, 1, 1, 0, (hipStream_t)stream, params, nullptr);
     if (e != hipSuccess) return fail_hip(e, kKernelNames[k]);
     return VX_OK;
 }
@@ -230,6 +245,7 @@ static int init(int device, vx_ctx* out) {
         delete ctx;
         return fail(VX_ERR_UNSUPPORTED, "device is not gfx950 (MI355X); this library ships gfx950 code only");
     }
+    ctx->late = late_of(device);
     ctx->num_cus = prop.multiProcessorCount;
     ctx->lds_per_block = prop.sharedMemPerBlock;
     auto unload = [&]() {
@@ -1418,8 +1434,6 @@ int vx_destroy(vx_ctx ctx) {
     if (!ctx) return VX_OK;
     vx::DeviceGuard guard(ctx->device);
     for (hipModule_t m : ctx->mods)
-        if (m) (void)hipModuleUnload(m);
-    for (hipModule_t m : ctx->late)
         if (m) (void)hipModuleUnload(m);
     delete ctx;
     return VX_OK;
