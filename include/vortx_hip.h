@@ -528,7 +528,9 @@ int vx_attention_tree(vx_ctx ctx, vx_stream stream, const vx_mview* out, const v
                       uint32_t tree_stride, void* workspace, uint64_t workspace_bytes);
 
 /* Bytes of workspace that either of them may use for `tokens` query tokens of
- * `q_heads` heads (0: none). Loads their kernels where no call has yet. */
+ * `q_heads` heads (0: none; any other number of tokens, like the batch's arrays,
+ * changes nothing: it goes by the bounds). Loads their kernels where no call has
+ * yet. */
 int vx_attention_ws_size(vx_ctx ctx, const vx_kv_cache* cache, const vx_attn_batch* batch, const vx_attn_opts* opts,
                          uint32_t tokens, uint32_t q_heads, uint64_t* bytes);
 

@@ -192,7 +192,7 @@ __device__ __forceinline__ uint64_t vx_div(uint64_t a, uint64_t b) {
 // front, for what it takes to begin and to end: without that the first row
 // blocks of a causal prompt, many short units to a workgroup, took three times
 // the others' time (8192 tokens, 8 heads over 2 of 128, 64-key steps: COST 0
-// 577 us, 2 438, 4 417, 8 443). do_unit takes a unit's keys from..to (end: to its end). A
+// 548 us, 2 417, 4 413, 8 428). do_unit takes a unit's keys from..to (end: to its end). A
 // unit that several workgroups share goes to partial sums:
 // a workgroup's first unit is partial 2 w, its last, if another, 2 w + 1; info
 // has a unit's first partial and their number, for the join.

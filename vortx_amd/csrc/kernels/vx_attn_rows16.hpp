@@ -16,10 +16,10 @@
 // says so), P times scale has a power of two for each row and block: under the
 // one of its largest block a block 2^23 smaller would keep 14 bits.
 // Bound: memory and vector instructions together. 32 sequences of 2400 to 8000
-// keys, 32 heads over 8 of 128 in 8 bits: 78 us, 4.5 TB/s of the cache (vector
-// issue 38 %, matrix cores 10 %); one of 131000, 64 heads over 8, values in 4
-// bits, scores capped: 60 us, 3.6 TB/s (55 %, 12 %). Two waves a SIMD: a third
-// one spills in the loop (120 us for the 78).
+// keys, 32 heads over 8 of 128 in 8 bits: 80 us with the join, 4.4 TB/s of the
+// cache (vector issue 42 %, matrix cores 11 %); one of 131000, 64 heads over 8,
+// values in 4 bits, scores capped: 66 us, 3.3 TB/s (56 %, 12 %). Two waves a SIMD:
+// a third one spills in the loop (120 us where this then took 78).
 #pragma once
 #include "vx_attn.hpp"
 
@@ -388,7 +388,7 @@ struct vx_rows16 {
     }
 
     // Single tokens, small trees: the keys of the batch dealt out evenly. Against
-    // equal splits of every sequence: 32 sequences of 2400 to 8000 keys 91 us, now 78.
+    // equal splits of every sequence: 32 sequences of 2400 to 8000 keys 91 us, then 78 like this.
     static __device__ __forceinline__ void even(const vx_attn_args& a) {
         __shared__ shared sh;
         constexpr uint32_t D = 32 * NB;
@@ -421,7 +421,7 @@ struct vx_rows16 {
 // Joins the partial sums of a query row (vx_attn_deal): 16 to 64 lanes take its
 // dims, four at a time, and the partials go over the groups of lanes, of a wave
 // where a row has up to 8 of them (four rows a workgroup) and of the workgroup
-// above (one row). One group a row took 90 us for 64 rows of 128 partials, this 9.
+// above (one row). One group a row took 90 us for 64 rows of 128 partials, this 11.
 __device__ __forceinline__ void vx_attn_join_rows(const vx_attn_args& a) {
     __shared__ f4 sh_t[256];
     __shared__ f2 sh_ml[64];

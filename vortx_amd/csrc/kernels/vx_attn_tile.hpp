@@ -20,10 +20,10 @@
 // In records that are not rough a scale of V that its size does not allow is of a
 // slot that was never written, which no row sees: 0, so that a weight of 0 times
 // it is 0.
-// (With K as whole numbers, exact in one term, and its scales on the 32-dim
-// products, a tile had 8 matrix instructions fewer and 64 multiply-adds and 32
-// registers a wave more: 430 us where this took 415, 4096 causal tokens of
-// 32 heads of 128.)
+// (With K always as whole numbers, exact in one term, and its scales on the
+// 32-dim products, a tile had 8 matrix instructions fewer and 64 multiply-adds
+// and 32 registers a wave more: 430 us where this then took 415, 4096 causal
+// tokens of 32 heads of 128.)
 // q is two f16 terms (22 bits, a power of two per row), and so are the weights;
 // of the product's terms the one of two lows is left out (2^-22). M follows the
 // maximum of score + e by steps of more than 2^5 only: most tiles leave the sums
@@ -33,10 +33,10 @@
 // used in the registers S^T was left in: the order of keys within a
 // contraction is free, and V is laid out to it.
 // Bound: matrix and vector issue, which take turns more than they overlap (48
-// 32-cycle matrix instructions and 330 vector ones a wave and tile at 128, 450
-// with a cap): 4096 causal tokens of 32 heads of 128, capped, 428 us, 321
-// TFLOP/s of attention, 960 of f16 products (matrix cores busy 44 %, vector
-// issue 53 %).
+// 32-cycle matrix instructions and 420 vector ones a wave and tile at 128, 480
+// with a cap, units' beginnings and ends among them): 4096 causal tokens of 32
+// heads of 128, capped, 424 to 465 us by the card, at 436 us 315 TFLOP/s of
+// attention, 945 of f16 products (matrix cores busy 43 %, vector issue 54 %).
 #pragma once
 #include "vx_attn.hpp"
 

@@ -85,8 +85,8 @@ static int rows_view(const void* base, const vx_layout* l, uint32_t dim, Rows* r
     return VX_OK;
 }
 
-// Tokens by fours from so many on: 333 of 3 heads of 64 read back 3.9 us (one by one 4.3), 8000 of
-// 8 heads of 128 written and read 42 (49). Fewer leave most of the card without work.
+// Tokens by fours from so many on: 333 of 3 heads of 64 read back 4.25 us (one by one 4.15), 8000 of
+// 8 heads of 128 written and read 42.8 (53.7). Fewer leave most of the card without work.
 constexpr uint32_t VX_QUAD_TOKENS = 256;
 static int run_rows(vx_ctx ctx, vx_stream stream, const vx_kv_cache* cache, const vx_cview* k, const vx_cview* v,
                     const int32_t* slots, bool write) {

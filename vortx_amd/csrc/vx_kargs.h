@@ -121,7 +121,7 @@ typedef struct vx_gemv_xq_args {
     int64_t xs_b;
 } vx_gemv_xq_args;
 
-/* Paged key/value cache (the layout of vx_attn.hpp). */
+/* Paged key/value cache (the layout of vx_kv.hpp). */
 typedef struct vx_kv_geom {
     uint8_t* base;
     uint64_t page_bytes;
