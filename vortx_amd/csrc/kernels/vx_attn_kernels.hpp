@@ -19,8 +19,8 @@
         vx_tile<VX_NB, KB, VB, 4>::each(a);                                                                    \
     }
 // (heads of 256: eight waves' registers do not hold the sums, and four hold them
-// with 14 to 22 registers in memory, dealt out 75 to 91; even256 of 128 has 16 or
-// 17 there, each128 up to 13)
+// with 15 to 23 registers in memory, dealt out 76 to 93; even256 of 128 has 17
+// there, each128 up to 16)
 #if VX_NB <= 4
 #define VX_WIDE(types, KB, VB)                                                                                 \
     extern "C" __global__ __launch_bounds__(512, 2) void VX_CAT(attn_each256, types)(vx_attn_args a) {         \

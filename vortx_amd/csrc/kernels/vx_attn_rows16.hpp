@@ -17,7 +17,7 @@
 // one of its largest block a block 2^23 smaller would keep 14 bits.
 // Bound: memory and vector instructions together. 32 sequences of 2400 to 8000
 // keys, 32 heads over 8 of 128 in 8 bits: 80 us with the join, 4.4 TB/s of the
-// cache (vector issue 42 %, matrix cores 11 %); one of 131000, 64 heads over 8,
+// cache (vector issue 43 %, matrix cores 11 %); one of 131000, 64 heads over 8,
 // values in 4 bits, scores capped: 66 us, 3.3 TB/s (56 %, 12 %). Two waves a SIMD:
 // a third one spills in the loop (120 us where this then took 78).
 #pragma once

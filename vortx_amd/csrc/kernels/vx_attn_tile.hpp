@@ -93,6 +93,7 @@ struct vx_tile {
 
     static __device__ __forceinline__ void load(const vx_attn_args& a, vx_scalar_i32 table, const uint8_t* base, int k0, int last, raw& r) {
         const uint32_t t = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(t >> 6), rec = wave & 1, lane = t & 63, m = lane & 15, g = lane >> 4;
+        if (NB < WAVES / 2 && (int)(wave >> 1) >= NB) return;
         const uint8_t* p = record(a, table, base, k0 + 16 * (int)rec, last);
         const uint8_t* sc = p + PK::BYTES + PV::VALS + g * (8 * NB);
 #pragma unroll
@@ -114,6 +115,7 @@ struct vx_tile {
     static __device__ __forceinline__ void store(raw& r, tile& s, int k0, int last) {
         typedef uint16_t us2 __attribute__((ext_vector_type(2)));
         const uint32_t t = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(t >> 6), rec = wave & 1, lane = t & 63, m = lane & 15, g = lane >> 4;
+        if (NB < WAVES / 2 && (int)(wave >> 1) >= NB) return;  // (no pieces: packed documents of dim 64 82 us, with the rest done for nothing 87)
         // the largest of four sizes, and whether another one is far below it. 0 is no size: K's zeros are
         // exact beside any; a key of V's zeros has weight, which the others' exponent would take bits from
         auto largest = [](uint32_t e, bool& far) {

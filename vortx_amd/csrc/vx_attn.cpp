@@ -142,17 +142,17 @@ constexpr uint32_t VX_MOST_KEYS = (1u << 31) - 65536u;  // of a sequence
 //   dim 96,  1 of 1500                120      17.9 / 27.0   128      17.9 / 27.1
 //            8 of up to 12000         120      89.8 / 105    128      96.4 / 115
 //            32 of up to 2000         120      88.8 / 90.0   128       106 / 100
-//   dim 64,  4 of up to 6000          128      37.1 / 42.2   192      56.4 / 59.8
+//   dim 64,  4 of up to 6000          128      37.1 / 42.2   192      57.0 / 61.0
 //   dim 256, 4 of up to 6000          128       102 / 115    192       181 / 194
 // So batches of many sequences lose up to a tenth just below the bound, and single ones win up to half.
 static uint64_t rows16_most(uint32_t dim) { return dim == 96 || dim == 128 ? 128 : 192; }
 // More units than places: a workgroup each (units of one length, or many of them,
 // fill the card by themselves, and no partial sums are written). Us, a workgroup
 // each / dealt out evenly: 512 units on 256 places, 4096 causal tokens of 32
-// heads of 128, 382 / 439; 480, windows of 1000 in prompts of up to 2500, 119 /
-// 132; 752 of dim 64, two prompts of up to 3000, 291 / 315. Up to as many: 256,
-// four chunks behind histories of 900 to 3000, 255 / 249; 256, a prompt of 2000,
-// 151 / 145.
+// heads of 128, 398 / 462; 480, windows of 1000 in prompts of up to 2500, 116 /
+// 133; 752 of dim 64, two prompts of up to 3000, 271 / 289. Up to as many: 256,
+// four chunks behind histories of 900 to 3000, 259 / 255; 256, a prompt of 2000,
+// 153 / 148.
 constexpr uint64_t VX_EVEN_UNITS = 1;
 struct AttnPlan {
     const int* kernel;
@@ -168,7 +168,7 @@ static int plan_attention(int num_cus, const vx_kv_cache* c, const vx_attn_batch
                           bool ws, AttnPlan* p) {
     const uint64_t group = q_heads / c->heads, queries = b->max_queries, rows = queries * group;
     // 256 rows a workgroup decode a tile of keys once where two of 128 do it twice; us, 256 / 128
-    // rows: 4096 causal tokens, dim 128 383 / 430, dim 64 250 / 268; chunks behind histories 208 / 229;
+    // rows, when both were dealt out: 4096 causal tokens, dim 128 383 / 430, dim 64 250 / 268; chunks behind histories 208 / 229;
     // trees of 244 rows 196 / 183, of 200 rows, 16 sequences, 313 / 312. (256 dims: see the kernels.)
     const bool wide = rows > 128 && c->dim <= 128;
     *p = AttnPlan{};
