@@ -453,6 +453,87 @@ int vx_kv_write(vx_ctx ctx, vx_stream stream, const vx_kv_cache* cache, const vx
 int vx_kv_read(vx_ctx ctx, vx_stream stream, const vx_mview* k, const vx_mview* v, const vx_kv_cache* cache,
                const int32_t* slots);
 
+/* How queries and keys are normed and rotated before they meet. Row x of a head:
+ *   VX_ROTATE_NORM   x = x / sqrt(mean(x^2) + eps) * w, w the norm weight of the
+ *                    head (q_weight / k_weight: dim values at w + head * stride,
+ *                    stride 0: one weight for all heads; NULL: 1)
+ *   then, of its first `rotated` dims (even, at most dim; 0: none), pair i, the
+ *   dims i and i + rotated / 2 or, with VX_ROTATE_PAIRS, 2 i and 2 i + 1:
+ *                    (a, b) = (a cos t - b sin t, b cos t + a sin t)
+ *   with t = position * freqs[i]. The other dims stay.
+ * freqs: device array of rotated / 2 doubles, radians a position (8-byte
+ * aligned; NULL if rotated is 0). All of it is computed in 64 bits and rounded
+ * to f32 once, so that far positions keep their angle and a key's code in the
+ * cache does not hang on the order of a sum. */
+typedef enum vx_rotate_flags { VX_ROTATE_PAIRS = 1, VX_ROTATE_NORM = 2 } vx_rotate_flags;
+typedef struct vx_rotation {
+    const double* freqs;
+    const float* q_weight;
+    const float* k_weight;
+    uint32_t q_weight_stride, k_weight_stride; /* 0, or at least dim */
+    uint32_t rotated;
+    uint32_t flags;    /* bitwise OR of vx_rotate_flags */
+    float eps;         /* >= 0 (at 0 a row of zeros gives NaN) */
+    uint32_t reserved; /* must be 0 */
+} vx_rotation;
+
+/* q_out = q and k_out = k, [tokens, heads, dim] f32 views of any strides with
+ * dims up to 256, normed and rotated (one launch). positions: device array
+ * [tokens] (NULL if nothing is rotated). k_out and k may be NULL: queries
+ * alone. An output is its input's view itself (in place) or lies apart from
+ * all inputs. */
+int vx_rotate(vx_ctx ctx, vx_stream stream, const vx_mview* q_out, const vx_cview* q, const vx_mview* k_out,
+              const vx_cview* k, const int32_t* positions, const vx_rotation* how);
+
+/* vx_rotate of q and k, k then written into the cache beside v as vx_kv_write
+ * does it, in one launch: the same bits in q_out and in the cache as the two
+ * calls one after the other. k is only read. q and k have the cache's dim and
+ * the same tokens; q and q_out may be NULL: keys alone. */
+int vx_kv_write_rotated(vx_ctx ctx, vx_stream stream, const vx_kv_cache* cache, const vx_mview* q_out, const vx_cview* q,
+                        const vx_cview* k, const vx_cview* v, const int32_t* positions, const int32_t* slots,
+                        const vx_rotation* how);
+
+/* Which pages of a cache sequences hold. Device memory, all of it state that
+ * vx_kv_resize brings from step to step:
+ *   table [seqs][table_stride]  pages of each sequence, in order (table_cols
+ *                               entries; those past its length mean nothing)
+ *   lens [seqs]                 tokens it holds
+ *   free_pages [pages]          a stack of the pages that none holds: the first
+ *   free_count [1]              so many
+ * page_tokens as in vx_kv_cache; pages, the entries of free_pages, at most
+ * 2^31 / page_tokens; seqs * table_cols is below 2^31 (else
+ * VX_ERR_UNSUPPORTED). A batch of vx_attention takes table and lens as they are. */
+typedef struct vx_kv_pages {
+    int32_t* table;
+    int32_t* lens;
+    int32_t* free_pages;
+    int32_t* free_count;
+    uint32_t seqs, table_cols, table_stride;
+    uint32_t page_tokens, pages;
+    uint32_t reserved; /* must be 0 */
+} vx_kv_pages;
+
+/* Every sequence s is to hold want[s] tokens (device array; negative: as many
+ * as it does). A shorter one gives the pages that it no longer needs back, then
+ * longer ones take those that they need more, in the order of the sequences: one
+ * is served if no page is missing for it and all before it. One that is not
+ * served, or whose table row is too short (it takes no part then), keeps its
+ * length and pages. Pages are given back last sequence and last page first and
+ * taken in the opposite order, so a step that is taken back (want: the lengths
+ * before it) leaves table and stack as they were.
+ * What the step's tokens need, written for `tokens` entries (at least as many as
+ * come in; those past `tokens` have none):
+ *   starts [seqs + 1]     first new token of each sequence, max(0, want - length)
+ *                         of them, and the end: as vx_attn_batch takes them
+ *   slots [tokens]        slot of each (-1: its sequence was not served; -1 past
+ *                         the last token)
+ *   positions [tokens]    position of each in its sequence (0 past the last)
+ * The arrays lie apart from each other. Lengths and page numbers that no call
+ * left there are kept from being read or written past the arrays, but mean
+ * nothing. One launch, and a second for many tokens; no memory beyond these arrays. */
+int vx_kv_resize(vx_ctx ctx, vx_stream stream, const vx_kv_pages* pages, const int32_t* want, int32_t* starts,
+                 int32_t* slots, int32_t* positions, uint32_t tokens);
+
 /* A batch of sequences. Device arrays, read when the kernels run, so they may
  * change between calls (and between replays of a captured graph):
  *   table [seqs][table_stride]  page of each page_tokens keys of a sequence

@@ -60,7 +60,20 @@ class VxAttnOpts(C.Structure):
                 ("first", C.c_void_p), ("flags", C.c_uint32), ("window", C.c_uint32)]
 
 
+class VxRotation(C.Structure):
+    _fields_ = [("freqs", C.c_void_p), ("q_weight", C.c_void_p), ("k_weight", C.c_void_p), ("q_weight_stride", C.c_uint32),
+                ("k_weight_stride", C.c_uint32), ("rotated", C.c_uint32), ("flags", C.c_uint32), ("eps", C.c_float),
+                ("reserved", C.c_uint32)]
+
+
+class VxKvPages(C.Structure):
+    _fields_ = [("table", C.c_void_p), ("lens", C.c_void_p), ("free_pages", C.c_void_p), ("free_count", C.c_void_p),
+                ("seqs", C.c_uint32), ("table_cols", C.c_uint32), ("table_stride", C.c_uint32), ("page_tokens", C.c_uint32),
+                ("pages", C.c_uint32), ("reserved", C.c_uint32)]
+
+
 VX_ATTN_CAUSAL = 1
+VX_ROTATE_PAIRS, VX_ROTATE_NORM = 1, 2
 VX_GEMM_BROADCAST, VX_GEMM_TILE_NARROW, VX_GEMM_TILE_WIDE, VX_GEMM_TILE_SMALL = 1, 2, 4, 8
 
 
@@ -109,6 +122,12 @@ SIGNATURES = [
     ("vx_kv_cache_size", C.c_int, [_P(VxKvCache), _P(C.c_uint64)]),
     ("vx_kv_write", C.c_int, [C.c_void_p, C.c_void_p, _P(VxKvCache), _P(VxCView), _P(VxCView), C.c_void_p]),
     ("vx_kv_read", C.c_int, [C.c_void_p, C.c_void_p, _P(VxMView), _P(VxMView), _P(VxKvCache), C.c_void_p]),
+    ("vx_rotate", C.c_int, [C.c_void_p, C.c_void_p, _P(VxMView), _P(VxCView), _P(VxMView), _P(VxCView), C.c_void_p,
+                            _P(VxRotation)]),
+    ("vx_kv_write_rotated", C.c_int, [C.c_void_p, C.c_void_p, _P(VxKvCache), _P(VxMView), _P(VxCView), _P(VxCView), _P(VxCView),
+                                      C.c_void_p, C.c_void_p, _P(VxRotation)]),
+    ("vx_kv_resize", C.c_int, [C.c_void_p, C.c_void_p, _P(VxKvPages), C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p,
+                               C.c_uint32]),
     ("vx_attention", C.c_int, [C.c_void_p, C.c_void_p, _P(VxMView), _P(VxCView), _P(VxKvCache), _P(VxAttnBatch),
                                _P(VxAttnOpts), C.c_void_p, C.c_uint64]),
     ("vx_attention_tree", C.c_int, [C.c_void_p, C.c_void_p, _P(VxMView), _P(VxCView), _P(VxKvCache), _P(VxAttnBatch),

@@ -13,6 +13,19 @@ can be replayed on new values::
     plan = kv.plan(cache, table, lens, starts, q_heads=32, max_queries=1, max_len=8192)
     kv.write(cache, k, v, slots)     # this step's keys and values [tokens, 8, 128]
     kv.attend(out, q, plan)          # [tokens, 32, 128]
+
+What goes before it in a step: :class:`KvPages` says which pages the sequences
+hold and :meth:`KvAttention.resize` brings it to the step's lengths, with the
+slots and positions of the new tokens, all on the device;
+:meth:`KvAttention.rotate` norms and rotates queries and keys by position, and
+:meth:`KvAttention.write_rotated` does it on their way into the cache::
+
+    pages, step = vx.KvPages(512, 64, seqs=32, cols=128), vx.KvStep(32, tokens=32)
+    plan = kv.plan(cache, pages.table, pages.lens, step.starts, q_heads=32, max_queries=1, max_len=8192)
+    how = kv.rotation(vx.rotation_freqs(128), norm=True, q_weight=wq, k_weight=wk, eps=1e-6)
+    kv.resize(pages, want, step)     # int32 [32]: tokens that each sequence is to hold
+    kv.write_rotated(cache, q, q, k, v, step.positions, step.slots, how)
+    kv.attend(out, q, plan)
 """
 from __future__ import annotations
 
@@ -25,6 +38,7 @@ from . import _ADDR, _Context, _ffi, _stream, _view_of
 from ._ffi import VX_Q8_0, VortxError, check, lib
 
 _WRITE, _READ, _ATTEND, _TREE = (_ADDR[n] for n in ("vx_kv_write", "vx_kv_read", "vx_attention", "vx_attention_tree"))
+_ROTATE, _WRITE_ROTATED, _RESIZE = (_ADDR[n] for n in ("vx_rotate", "vx_kv_write_rotated", "vx_kv_resize"))
 
 
 def _u32(**values) -> None:
@@ -80,8 +94,67 @@ def _array(t, name: str, shape, dtype="int32"):
     return t.data_ptr()
 
 
+def _ptr(t) -> int:
+    return t.data_ptr() or None
+
+
 def _row_stride(t) -> int:
     return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
+class KvPages:
+    """Which of ``pages`` pages of ``page_tokens`` tokens ``seqs`` sequences
+    hold, at most ``cols`` each (vx_kv_pages): int32 GPU tensors ``table``
+    [seqs, cols], ``lens`` [seqs], and the stack of free pages, the first
+    ``free_count`` [1] of ``free`` [pages]. A new one holds nothing, and page 0
+    is on top of the stack. :meth:`KvAttention.resize` changes it."""
+
+    def __init__(self, pages: int, page_tokens: int, seqs: int, cols: int, device="cuda:0"):
+        import torch
+        _u32(pages=pages, page_tokens=page_tokens, seqs=seqs, cols=cols)
+        i32 = dict(dtype=torch.int32, device=device)
+        self.pages, self.page_tokens, self.seqs, self.cols = pages, page_tokens, seqs, cols
+        self.table, self.lens = torch.zeros(seqs, cols, **i32), torch.zeros(seqs, **i32)
+        self.free, self.free_count = torch.arange(pages - 1, -1, -1, **i32), torch.full((1,), pages, **i32)
+        self._c = _ffi.VxKvPages(_ptr(self.table), _ptr(self.lens), _ptr(self.free), _ptr(self.free_count), seqs, cols, cols,
+                                 page_tokens, pages, 0)
+        self._addr = C.addressof(self._c)
+
+
+class KvStep:
+    """What :meth:`KvAttention.resize` says of a step's new tokens, up to
+    ``tokens`` of them: int32 GPU tensors ``starts`` [seqs + 1] (of a batch),
+    ``slots`` and ``positions`` [tokens]."""
+
+    def __init__(self, seqs: int, tokens: int, device="cuda:0"):
+        import torch
+        _u32(seqs=seqs, tokens=tokens)
+        i32 = dict(dtype=torch.int32, device=device)
+        self.seqs, self.tokens = seqs, tokens
+        self.starts = torch.zeros(seqs + 1, **i32)
+        self.slots, self.positions = torch.full((tokens,), -1, **i32), torch.zeros(tokens, **i32)
+        self._call = (_ptr(self.starts), _ptr(self.slots), _ptr(self.positions), tokens)
+
+
+def rotation_freqs(rotated: int, base: float = 10000.0, scale: float = 1.0, device="cuda:0"):
+    """Radians a position of each of ``rotated`` / 2 pairs of dims, float64:
+    scale * base^(-2 i / rotated)."""
+    import torch
+    return (scale * base ** (-2.0 * torch.arange(rotated // 2, dtype=torch.float64) / max(rotated, 1))).to(device)
+
+
+@dataclass
+class Rotation:
+    """How queries and keys are normed and rotated (:meth:`KvAttention.rotation`).
+    It keeps the tensors it was made of alive; their contents may change."""
+    dim: int       # of the heads that it is for (0: any that its rotated dims fit into)
+    q_heads: int   # of weights of their own for each head (0: any)
+    k_heads: int
+    keep: tuple
+    _c: object     # _ffi.VxRotation
+
+    def __post_init__(self):
+        self._call = (C.addressof(self._c), self.dim, self.q_heads, self.k_heads, self._c.rotated)
 
 
 @dataclass
@@ -165,6 +238,105 @@ class KvAttention(_Context):
             return
         kv, vv = (None if t is None else C.byref(_view_of(t, True)) for t in (k, v))
         check(lib().vx_kv_read(self._h, _stream(stream), kv, vv, C.byref(cache._c), self._slots(slots, k, v)))
+
+    def resize(self, pages: KvPages, want, step: KvStep, stream=None) -> None:
+        """Sequence s is to hold ``want[s]`` tokens (int32 [seqs]; negative: as
+        many as it does): shorter ones give pages back, then longer ones take
+        the pages that they need, in order, while there are any
+        (vx_kv_resize). ``step`` gets the starts, slots and positions of the
+        new tokens; a sequence that found too few pages keeps its length, and
+        its tokens have slot -1. ``step.tokens`` has to be at least the new
+        tokens of all sequences."""
+        if step.seqs != pages.seqs:
+            raise VortxError(_ffi.VX_ERR_SHAPE, f"the step is for {step.seqs} sequences, the pages for {pages.seqs}")
+        st = _vx._pycall.kv_resize(_RESIZE, self._ctx, stream, pages._addr, pages.seqs, want, *step._call)
+        if st is not None:
+            if st:
+                check(st)
+            return
+        at = _array(want, "want", (pages.seqs,)) or None
+        check(lib().vx_kv_resize(self._h, _stream(stream), C.byref(pages._c), at, *step._call))
+
+    def rotation(self, freqs, *, pairs: bool = False, norm: bool = False, q_weight=None, k_weight=None, eps: float = 1e-6) -> Rotation:
+        """How :meth:`rotate` and :meth:`write_rotated` treat a head (vx_rotation).
+        ``freqs``: float64 [rotated / 2], radians a position
+        (:func:`rotation_freqs`; None: no rotation) of the dims i and i +
+        rotated / 2 or, with ``pairs``, 2 i and 2 i + 1. ``norm``: each head
+        is divided by sqrt(mean(x^2) + ``eps``) first, and multiplied by
+        ``q_weight`` / ``k_weight``, f32 [dim] or [heads, dim] (None: by nothing)."""
+        import torch
+        r = _ffi.VxRotation()
+        if freqs is not None:
+            if not (isinstance(freqs, torch.Tensor) and freqs.is_cuda and freqs.dtype == torch.float64):
+                raise TypeError("freqs must be a float64 tensor on the GPU")
+            if freqs.dim() != 1 or not freqs.is_contiguous():
+                raise VortxError(_ffi.VX_ERR_SHAPE, "freqs is one row of numbers")
+            r.freqs, r.rotated = _ptr(freqs), 2 * freqs.numel()
+        r.flags = (_ffi.VX_ROTATE_PAIRS if pairs else 0) | (_ffi.VX_ROTATE_NORM if norm else 0)
+        r.eps = eps
+        dims, heads = set(), [0, 0]
+        for i, (n, w) in enumerate((("q", q_weight), ("k", k_weight))):
+            if w is None:
+                continue
+            each = isinstance(w, torch.Tensor) and w.dim() == 2
+            setattr(r, n + "_weight", _array(w, n + "_weight", (None, None) if each else (None,), "float32"))
+            dims.add(w.shape[-1])
+            if each:
+                heads[i] = w.shape[0]
+                setattr(r, n + "_weight_stride", _row_stride(w))
+        if len(dims) > 1:
+            raise VortxError(_ffi.VX_ERR_SHAPE, "q_weight and k_weight have different dims")
+        return Rotation(dims.pop() if dims else 0, *heads, (freqs, q_weight, k_weight), r)
+
+    @staticmethod
+    def _rotation(how, positions, q, k):
+        """Address of the positions; what the rotation's tensors do not hold is refused."""
+        tokens = None
+        for n, v, heads in (("q", q, how.q_heads), ("k", k, how.k_heads)):
+            if v is None:
+                continue
+            l = v.layout
+            if l.rank != 3:
+                raise VortxError(_ffi.VX_ERR_SHAPE, f"{n} is a [tokens, heads, dim] view")
+            tokens = l.size[0]
+            if how.dim and l.size[2] != how.dim:
+                raise VortxError(_ffi.VX_ERR_SHAPE, f"{n} has {l.size[2]} dims, the norm weights {how.dim}")
+            if heads and l.size[1] != heads:
+                raise VortxError(_ffi.VX_ERR_SHAPE, f"{n} has {l.size[1]} heads, its norm weights {heads}")
+        if positions is None:
+            return None
+        return _array(positions, "positions", (tokens,))
+
+    def rotate(self, q_out, q, k_out, k, positions, how: Rotation, stream=None) -> None:
+        """``q_out`` = ``q`` and ``k_out`` = ``k`` ([tokens, heads, dim] f32
+        views; both of the keys' None: queries alone) normed and rotated by
+        ``positions`` (int32 [tokens]). An output may be its input itself."""
+        st = _vx._pycall.rotate(_ROTATE, self._ctx, stream, q_out, q, k_out, k, positions, *how._call)
+        if st is not None:
+            if st:
+                check(st)
+            return
+        ov, qv = _view_of(q_out, True), _view_of(q, False)
+        kov, kv = (None if t is None else _view_of(t, m) for t, m in ((k_out, True), (k, False)))
+        ref = lambda v: None if v is None else C.byref(v)  # noqa: E731
+        check(lib().vx_rotate(self._h, _stream(stream), C.byref(ov), C.byref(qv), ref(kov), ref(kv),
+                              self._rotation(how, positions, qv, kv), C.byref(how._c)))
+
+    def write_rotated(self, cache: KvCache, q_out, q, k, v, positions, slots, how: Rotation, stream=None) -> None:
+        """:meth:`rotate` of ``q`` into ``q_out`` and of ``k``, which goes into
+        the cache's ``slots`` with ``v`` as :meth:`write` puts it there, in one
+        launch (the same bits as the two calls). ``q`` and ``q_out`` None: keys
+        alone."""
+        st = _vx._pycall.kv_write_rotated(_WRITE_ROTATED, self._ctx, stream, cache._addr, q_out, q, k, v, positions, slots, *how._call)
+        if st is not None:
+            if st:
+                check(st)
+            return
+        kv, vv = _view_of(k, False), _view_of(v, False)
+        ov, qv = (None if t is None else _view_of(t, m) for t, m in ((q_out, True), (q, False)))
+        ref = lambda v: None if v is None else C.byref(v)  # noqa: E731
+        check(lib().vx_kv_write_rotated(self._h, _stream(stream), C.byref(cache._c), ref(ov), ref(qv), C.byref(kv), C.byref(vv),
+                                        self._rotation(how, positions, qv, kv), self._slots(slots, k, v), C.byref(how._c)))
 
     @staticmethod
     def _slots(slots, *views):

@@ -14,6 +14,7 @@
 #pragma once
 #include "vx_dpp.hpp"
 #include "vx_kv.hpp"
+#include "vx_rotate.hpp"
 
 #pragma clang fp contract(off)
 
@@ -199,15 +200,33 @@ __device__ __forceinline__ u2 vx_kv_v4(const uint32_t (&w)[4], int p) {
     return u2{c[0] | c[2] << 8 | c[1] << 16 | c[3] << 24, 0u};
 }
 
-template <int NB, int KB, int VB>
-__device__ __forceinline__ void vx_kv_write_rows(const vx_kv_rows_args& a) {
+// Where the keys of a row's lanes come from: as they are, or normed and rotated
+// (by all lanes of the row together).
+struct vx_kv_keys {
+    static constexpr bool TURNED = false;
+};
+template <int LANES>
+struct vx_kv_turned_keys {
+    static constexpr bool TURNED = true;
+    const vx_rotate_args& a;
+    __device__ __forceinline__ f4 row(int64_t t, uint32_t h, uint32_t d) const {
+        vx_r4 x, y;
+        vx_rotate_load(a, a.x[1] + t * a.xs[1][0] + (int64_t)h * a.xs[1][1], a.xs[1][2], d, x, y);
+        const vx_turn turn(a, (uint32_t)t, d);
+        return vx_rotate_row<LANES>(a, turn, a.w[1] ? a.w[1] + (uint64_t)h * a.ws[1] : nullptr, d, x, y);
+    }
+};
+
+// Part `block` of `blocks`.
+template <int NB, int KB, int VB, class KEYS>
+__device__ __forceinline__ void vx_kv_write_rows(const vx_kv_rows_args& a, const KEYS& keys, uint32_t block, uint32_t blocks) {
     using R = vx_kv_rec<NB, KB, VB>;
     using PK = vx_kv_part<NB, KB>;
     using PV = vx_kv_part<NB, VB>;
     constexpr uint32_t NP = NB == 3 ? 4 : NB;  // lanes of a row: 8 NP, a power of two
     const uint64_t units = (uint64_t)a.groups * a.c.heads * NP;
     const uint32_t u = threadIdx.x & 7, b = (threadIdx.x >> 3) % NP;
-    for (uint64_t n = (uint64_t)blockIdx.x * 32 + (threadIdx.x >> 3); n < units; n += (uint64_t)gridDim.x * 32) {
+    for (uint64_t n = (uint64_t)block * 32 + (threadIdx.x >> 3); n < units; n += (uint64_t)blocks * 32) {
         const uint64_t th = n / NP;
         const uint32_t group = (uint32_t)(th / a.c.heads), h = (uint32_t)(th - (uint64_t)group * a.c.heads);
         const vx_kv_tokens run(a, group);
@@ -225,11 +244,15 @@ __device__ __forceinline__ void vx_kv_write_rows(const vx_kv_rows_args& a) {
         const float* vp = a.v + t * a.vs[0] + (int64_t)h * a.vs[1];
         if (four) {
             uint32_t klo = 0, khi = 0, vlo = 0, vhi = 0;
+            f4 x[4], y[4];
+            if constexpr (KEYS::TURNED) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) x[i] = keys.row(t + i, h, d);
+            }
             if (b < NB) {
-                f4 x[4], y[4];
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    x[i] = vx_kv_get4(kp + i * a.ks[0], a.ks[2], d, a.vec);
+                    if constexpr (!KEYS::TURNED) x[i] = vx_kv_get4(kp + i * a.ks[0], a.ks[2], d, a.vec);
                     y[i] = vx_kv_get4(vp + i * a.vs[0], a.vs[2], d, a.vec);
                 }
                 uint32_t w[4];
@@ -265,8 +288,11 @@ __device__ __forceinline__ void vx_kv_write_rows(const vx_kv_rows_args& a) {
             continue;
         }
         uint32_t size = 0;  // of K above, of V below
+        f4 k;
+        if constexpr (KEYS::TURNED) k = keys.row(t, h, d);
         if (b < NB) {
-            const f4 k = vx_kv_get4(kp, a.ks[2], d, a.vec), v = vx_kv_get4(vp, a.vs[2], d, a.vec);
+            if constexpr (!KEYS::TURNED) k = vx_kv_get4(kp, a.ks[2], d, a.vec);
+            const f4 v = vx_kv_get4(vp, a.vs[2], d, a.vec);
             size = vx_kv_put_k<NB, KB>(rec, m, b, u, k) << 16;
             size |= vx_kv_put_v<NB, VB>(rec + R::V, m, b, u, v);
         }

@@ -1,5 +1,6 @@
-// vx_attn.cpp — host side of the quantized key/value cache and the attention
-// over it: checks, kernel choice, and how the keys are split over workgroups.
+// vx_attn.cpp — host side of the quantized key/value cache, what goes into it
+// (pages, rotated rows) and the attention over it: checks, kernel choice, and how
+// the work is split over workgroups.
 #include <algorithm>
 #include <cmath>
 
@@ -49,7 +50,7 @@ static int kernel_of(const vx_kv_cache* c, const int* d) {
     return d[dim_index(c->dim)] + (c->k_type == VX_Q4_0 ? 2 : 0) + (c->v_type == VX_Q4_0 ? 1 : 0);
 }
 #define VX_DIMS(f) {K_vx_##f##_d64_k8v8, K_vx_##f##_d96_k8v8, K_vx_##f##_d128_k8v8, K_vx_##f##_d256_k8v8}
-static const int kWrite[4] = VX_DIMS(kv_write), kRead[4] = VX_DIMS(kv_read), kEven16[4] = VX_DIMS(attn_even16),
+static const int kWrite[4] = VX_DIMS(kv_write), kRead[4] = VX_DIMS(kv_read), kWriteRotated[4] = VX_DIMS(rotate_kv), kEven16[4] = VX_DIMS(attn_even16),
                  kEach128[4] = VX_DIMS(attn_each128);
 #undef VX_DIMS
 #define VX_DIMS(f) {K_vx_##f##_d64_k8v8, K_vx_##f##_d96_k8v8, K_vx_##f##_d128_k8v8}
@@ -88,11 +89,11 @@ static int rows_view(const void* base, const vx_layout* l, uint32_t dim, Rows* r
 // Tokens by fours from so many on: 333 of 3 heads of 64 read back 4.25 us (one by one 4.15), 8000 of
 // 8 heads of 128 written and read 42.8 (53.7). Fewer leave most of the card without work.
 constexpr uint32_t VX_QUAD_TOKENS = 256;
-static int run_rows(vx_ctx ctx, vx_stream stream, const vx_kv_cache* cache, const vx_cview* k, const vx_cview* v,
-                    const int32_t* slots, bool write) {
-    clear_error();
-    if (!ctx) return fail(VX_ERR_INVALID, "null ctx");
-    vx_kv_rows_args a{};
+// The arguments of a call on rows, and its workgroups (0: nothing to do).
+static int plan_rows(const vx_kv_cache* cache, const vx_cview* k, const vx_cview* v, const int32_t* slots, bool write,
+                     vx_kv_rows_args* out, uint32_t* grid) {
+    vx_kv_rows_args& a = *out;
+    *grid = 0;
     int s = check_cache(cache, &a.c);
     if (s) return s;
     if (write ? !k || !v : !k && !v) return fail(VX_ERR_INVALID, "null view");
@@ -121,8 +122,164 @@ static int run_rows(vx_ctx ctx, vx_stream stream, const vx_kv_cache* cache, cons
     a.quads = a.tokens >= VX_QUAD_TOKENS;
     a.groups = a.quads ? (a.tokens - 1) / 4 + 1 : a.tokens;
     const uint64_t units = (uint64_t)a.groups * cache->heads * (cache->dim == 96 ? 4 : cache->dim / 32);
-    const uint32_t grid = (uint32_t)std::min<uint64_t>((units + 31) / 32, 1u << 20);
+    *grid = (uint32_t)std::min<uint64_t>((units + 31) / 32, 1u << 20);
+    return VX_OK;
+}
+
+static int run_rows(vx_ctx ctx, vx_stream stream, const vx_kv_cache* cache, const vx_cview* k, const vx_cview* v,
+                    const int32_t* slots, bool write) {
+    clear_error();
+    if (!ctx) return fail(VX_ERR_INVALID, "null ctx");
+    vx_kv_rows_args a{};
+    uint32_t grid = 0;
+    if (const int s = plan_rows(cache, k, v, slots, write, &a, &grid)) return s;
     return launch_struct(ctx, kernel_of(cache, write ? kWrite : kRead), grid, 256, stream, &a);
+}
+
+static int check_rotation(const vx_rotation* r, uint32_t dim) {
+    if (!r) return fail(VX_ERR_INVALID, "null rotation");
+    if (r->reserved) return fail(VX_ERR_INVALID, "vx_rotation.reserved must be 0");
+    if (r->flags & ~(uint32_t)(VX_ROTATE_PAIRS | VX_ROTATE_NORM)) return fail(VX_ERR_INVALID, "unknown rotation flags");
+    if (r->rotated % 2) return fail(VX_ERR_SHAPE, "an even number of dims is rotated");
+    if (r->rotated > dim) return fail(VX_ERR_SHAPE, "more dims are rotated than a head has");
+    if (r->rotated && !r->freqs) return fail(VX_ERR_INVALID, "null freqs");
+    if ((uintptr_t)r->freqs & 7u) return fail(VX_ERR_INVALID, "freqs is not 8-byte aligned");
+    if (((uintptr_t)r->q_weight | (uintptr_t)r->k_weight) & 3u) return fail(VX_ERR_INVALID, "a norm weight is not 4-byte aligned");
+    if (!(r->flags & VX_ROTATE_NORM)) {
+        if (r->q_weight || r->k_weight) return fail(VX_ERR_INVALID, "norm weights without VX_ROTATE_NORM");
+        return VX_OK;
+    }
+    if (!(r->eps >= 0.f) || !std::isfinite(r->eps)) return fail(VX_ERR_INVALID, "eps is negative or not finite");
+    if ((r->q_weight && r->q_weight_stride && r->q_weight_stride < dim) || (r->k_weight && r->k_weight_stride && r->k_weight_stride < dim))
+        return fail(VX_ERR_INVALID, "norm weights of heads overlap");
+    return VX_OK;
+}
+
+// The arguments for rows q (0) and k (1); either view may be null, outputs too.
+static int plan_rotation(const vx_mview* const (&outs)[2], const vx_cview* const (&ins)[2], uint32_t dim, const int32_t* positions,
+                         const vx_rotation* how, vx_rotate_args* a) {
+    static const char* const names[2][2] = {{"q", "q_out"}, {"k", "k_out"}};
+    int s = check_rotation(how, dim);
+    if (s) return s;
+    const bool norm = how->flags & VX_ROTATE_NORM;
+    const float* const weights[2] = {how->q_weight, how->k_weight};
+    const uint32_t strides[2] = {how->q_weight_stride, how->k_weight_stride};
+    a->pairs = how->flags & VX_ROTATE_PAIRS ? 1 : 0;
+    a->norm = norm;
+    a->dim = dim;
+    a->rotated = how->rotated;
+    a->eps = how->eps;
+    a->freqs = how->freqs;
+    a->positions = positions;
+    a->vec = dim % 4 == 0 && (a->pairs || how->rotated % 8 == 0);
+    bool first = true;
+    for (int i = 0; i < 2; ++i) {
+        if (!ins[i]) continue;
+        Rows r, o;
+        if ((s = rows_view(ins[i]->base, &ins[i]->layout, dim, &r, names[i][0], false))) return s;
+        if (!first && r.tokens != a->tokens) return fail(VX_ERR_SHAPE, "q and k have different tokens");
+        first = false;
+        a->tokens = r.tokens;
+        a->heads[i] = r.heads;
+        a->x[i] = (const float*)r.ptr;
+        a->w[i] = norm ? weights[i] : nullptr;
+        a->ws[i] = strides[i];
+        for (int j = 0; j < 3; ++j) a->xs[i][j] = r.stride[j];
+        if (!r.vec || (a->w[i] && (((uintptr_t)weights[i] & 15u) || strides[i] % 4))) a->vec = 0;
+        if (!outs[i]) continue;
+        if ((s = rows_view(outs[i]->base, &outs[i]->layout, dim, &o, names[i][1], true))) return s;
+        if (o.tokens != r.tokens || o.heads != r.heads) return fail(VX_ERR_SHAPE, i ? "k and k_out have different shapes" : "q and q_out have different shapes");
+        a->y[i] = (float*)o.ptr;
+        for (int j = 0; j < 3; ++j) a->ys[i][j] = o.stride[j];
+        if (!o.vec) a->vec = 0;
+    }
+    if (how->rotated && a->tokens && (!positions || ((uintptr_t)positions & 3u)))
+        return fail(VX_ERR_INVALID, "positions is null or not 4-byte aligned");
+    return VX_OK;
+}
+
+static int lanes_index(uint32_t dim) { return dim <= 64 ? 0 : dim <= 128 ? 1 : 2; }
+
+// How many heads a group of lanes takes for one token's angles, and the workgroups.
+static void split_rotation(int num_cus, vx_rotate_args* a) {
+    const uint32_t heads = a->heads[0] + a->heads[1], groups = 16u >> lanes_index(a->dim);
+    const uint64_t rows = (uint64_t)a->tokens * heads;
+    if (!rows) {
+        a->run = a->chunks = a->blocks = 0;
+        return;
+    }
+    const uint64_t places = (uint64_t)num_cus * 8 * groups;  // rows under way with eight workgroups a CU
+    a->run = (uint32_t)std::min<uint64_t>(heads, std::max<uint64_t>(1, rows / places));
+    a->chunks = (heads + a->run - 1) / a->run;
+    a->blocks = (uint32_t)std::min<uint64_t>(((uint64_t)a->tokens * a->chunks + groups - 1) / groups, 1u << 20);
+}
+
+static int run_rotate(vx_ctx ctx, vx_stream stream, const vx_mview* q_out, const vx_cview* q, const vx_mview* k_out, const vx_cview* k,
+                      const int32_t* positions, const vx_rotation* how) {
+    if (!q || !q_out) return fail(VX_ERR_INVALID, "null view");
+    if (!k != !k_out) return fail(VX_ERR_INVALID, "k without k_out, or k_out without k");
+    Canon c;
+    int s = canon_view(q->base, &q->layout, &c, "q");
+    if (s) return s;
+    const uint32_t dim = c.l.size[3];
+    if (dim == 0 || dim > 256) return fail(VX_ERR_UNSUPPORTED, "heads have 1 to 256 dims");
+    vx_rotate_args a{};
+    if ((s = plan_rotation({q_out, k_out}, {q, k}, dim, positions, how, &a))) return s;
+    split_rotation(ctx_cus(ctx), &a);
+    return launch_struct(ctx, K_vx_rotate_l16 + lanes_index(dim), a.blocks, 256, stream, &a);
+}
+
+static int run_write_rotated(vx_ctx ctx, vx_stream stream, const vx_kv_cache* cache, const vx_mview* q_out, const vx_cview* q,
+                             const vx_cview* k, const vx_cview* v, const int32_t* positions, const int32_t* slots,
+                             const vx_rotation* how) {
+    if (!q != !q_out) return fail(VX_ERR_INVALID, "q without q_out, or q_out without q");
+    vx_kv_rotated_args a{};
+    uint32_t grid = 0;
+    int s = plan_rows(cache, k, v, slots, true, &a.r, &grid);
+    if (s) return s;
+    if ((s = plan_rotation({q_out, nullptr}, {q, k}, cache->dim, positions, how, &a.t))) return s;
+    a.t.heads[1] = 0;  // (they are the writer's)
+    split_rotation(ctx_cus(ctx), &a.t);
+    return launch_struct(ctx, kernel_of(cache, kWriteRotated), a.t.blocks + grid, 256, stream, &a);
+}
+
+// Slots in the workgroup that deals out the pages, up to so many tokens.
+constexpr uint32_t VX_SLOTS_HERE = 4096;
+static int run_resize(vx_ctx ctx, vx_stream stream, const vx_kv_pages* p, const int32_t* want, int32_t* starts, int32_t* slots,
+                      int32_t* positions, uint32_t tokens) {
+    if (!p) return fail(VX_ERR_INVALID, "null pages");
+    if (p->reserved) return fail(VX_ERR_INVALID, "vx_kv_pages.reserved must be 0");
+    if (p->page_tokens < 16 || p->page_tokens > 65536 || (p->page_tokens & (p->page_tokens - 1)))
+        return fail(VX_ERR_UNSUPPORTED, "page_tokens is not a power of two from 16 to 65536");
+    if ((uint64_t)p->pages * p->page_tokens > (1ull << 31)) return fail(VX_ERR_UNSUPPORTED, "a cache has at most 2^31 slots");
+    if (p->table_stride < p->table_cols) return fail(VX_ERR_INVALID, "table_stride smaller than table_cols");
+    if ((uint64_t)p->seqs * p->table_cols >= (1ull << 31) || p->seqs >= (1u << 31))
+        return fail(VX_ERR_UNSUPPORTED, "a table has fewer than 2^31 entries");
+    if (tokens > (1u << 30)) return fail(VX_ERR_UNSUPPORTED, "more than 2^30 tokens");
+    if (!p->free_count || (p->pages && !p->free_pages) || (p->seqs && (!p->lens || !want || (p->table_cols && !p->table))))
+        return fail(VX_ERR_INVALID, "null pages array");
+    if (!starts || (tokens && (!slots || !positions))) return fail(VX_ERR_INVALID, "null output array");
+    if (((uintptr_t)p->table | (uintptr_t)p->lens | (uintptr_t)p->free_pages | (uintptr_t)p->free_count | (uintptr_t)want |
+         (uintptr_t)starts | (uintptr_t)slots | (uintptr_t)positions) & 3u)
+        return fail(VX_ERR_INVALID, "an array is not 4-byte aligned");
+    vx_pages_args a{};
+    a.table = p->table;
+    a.lens = p->lens;
+    a.free_pages = p->free_pages;
+    a.free_count = p->free_count;
+    a.want = want;
+    a.starts = starts;
+    a.slots = slots;
+    a.positions = positions;
+    a.seqs = p->seqs;
+    a.table_cols = p->table_cols;
+    a.table_stride = p->table_stride;
+    while ((1u << a.page_shift) < p->page_tokens) ++a.page_shift;
+    a.pages = p->pages;
+    a.tokens = tokens;
+    a.here = tokens <= VX_SLOTS_HERE;
+    if (const int s = launch_struct(ctx, K_vx_pages_resize, 1, 1024, stream, &a)) return s;
+    return a.here ? VX_OK : launch_struct(ctx, K_vx_pages_slots, (tokens + 1023) / 1024, 256, stream, &a);
 }
 
 // How a call is laid out: the kernel by the query rows of a sequence and head
@@ -304,6 +461,28 @@ int vx_kv_read(vx_ctx ctx, vx_stream stream, const vx_mview* k, const vx_mview* 
     for (int i = 0; i < 2; ++i)
         if (views[i]) c[i] = vx_cview{views[i]->base, views[i]->layout};
     return vx::run_rows(ctx, stream, cache, k ? &c[0] : nullptr, v ? &c[1] : nullptr, slots, false);
+}
+
+int vx_rotate(vx_ctx ctx, vx_stream stream, const vx_mview* q_out, const vx_cview* q, const vx_mview* k_out,
+              const vx_cview* k, const int32_t* positions, const vx_rotation* how) {
+    vx::clear_error();
+    if (!ctx) return vx::fail(VX_ERR_INVALID, "null ctx");
+    return vx::run_rotate(ctx, stream, q_out, q, k_out, k, positions, how);
+}
+
+int vx_kv_write_rotated(vx_ctx ctx, vx_stream stream, const vx_kv_cache* cache, const vx_mview* q_out, const vx_cview* q,
+                        const vx_cview* k, const vx_cview* v, const int32_t* positions, const int32_t* slots,
+                        const vx_rotation* how) {
+    vx::clear_error();
+    if (!ctx) return vx::fail(VX_ERR_INVALID, "null ctx");
+    return vx::run_write_rotated(ctx, stream, cache, q_out, q, k, v, positions, slots, how);
+}
+
+int vx_kv_resize(vx_ctx ctx, vx_stream stream, const vx_kv_pages* pages, const int32_t* want, int32_t* starts,
+                 int32_t* slots, int32_t* positions, uint32_t tokens) {
+    vx::clear_error();
+    if (!ctx) return vx::fail(VX_ERR_INVALID, "null ctx");
+    return vx::run_resize(ctx, stream, pages, want, starts, slots, positions, tokens);
 }
 
 int vx_attention(vx_ctx ctx, vx_stream stream, const vx_mview* out, const vx_cview* q, const vx_kv_cache* cache,

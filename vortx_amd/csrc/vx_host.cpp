@@ -46,6 +46,8 @@ extern const unsigned char vx_co_attn_d128[];
 extern const unsigned char vx_co_attn_d128_end[];
 extern const unsigned char vx_co_attn_d256[];
 extern const unsigned char vx_co_attn_d256_end[];
+// (weak: host sources built without these code objects have none to load)
+extern const unsigned char vx_co_step[] __attribute__((weak));
 }
 
 namespace vx {
@@ -80,7 +82,7 @@ static const char* const kKernelNames[K_COUNT] = {
 static const unsigned char* const kModules[] = {vx_co_gemm, vx_co_gemv_q, vx_co_copy, vx_co_quantize, vx_co_gemm_q, vx_co_gemm_bf};
 constexpr int kNumModules = 6;
 constexpr int kModGemv = 1;  // the module holding vx_scratch
-// The attention's, one a head size, with its kernels: loaded at their first use,
+// The attention's, one a head size, and what stands around it, with their kernels: loaded at their first use,
 // once for all contexts of a device, and kept. A context takes 16 ms with them
 // and 8 without, and most have no use for them; with code objects of each context's
 // own a call on a new one took 0.9 ms where it now takes 0.04.
@@ -88,8 +90,9 @@ static const struct { const unsigned char* image; int first, end; } kLate[] = {
     {vx_co_attn_d64, K_vx_kv_write_d64_k8v8, K_vx_kv_write_d96_k8v8},
     {vx_co_attn_d96, K_vx_kv_write_d96_k8v8, K_vx_kv_write_d128_k8v8},
     {vx_co_attn_d128, K_vx_kv_write_d128_k8v8, K_vx_kv_write_d256_k8v8},
-    {vx_co_attn_d256, K_vx_kv_write_d256_k8v8, K_COUNT}};
-constexpr int kNumLate = 4, kLateFirst = K_vx_kv_write_d64_k8v8;
+    {vx_co_attn_d256, K_vx_kv_write_d256_k8v8, K_vx_pages_resize},
+    {vx_co_step, K_vx_pages_resize, K_COUNT}};
+constexpr int kNumLate = 5, kLateFirst = K_vx_kv_write_d64_k8v8;
 struct LateKernels {  // of a device
     hipFunction_t fn[K_COUNT - kLateFirst] = {};  // written under `lock`, read once `ready` says so
     std::atomic<bool> ready[kNumLate] = {};
@@ -190,9 +193,9 @@ int need_kernel(vx_ctx ctx, int k) {
     if (late.ready[i].load(std::memory_order_relaxed)) return VX_OK;
     DeviceGuard guard(ctx->device);
     OutsideCapture outside;
-    const char* what = "hipModuleLoadData(attention)";
+    const char* what = "hipModuleLoadData(late)";
     hipModule_t mod = nullptr;
-    hipError_t e = hipModuleLoadData(&mod, kLate[i].image);
+    hipError_t e = kLate[i].image ? hipModuleLoadData(&mod, kLate[i].image) : hipErrorNotFound;
     for (int f = kLate[i].first; f < kLate[i].end && e == hipSuccess; ++f) {
         what = kKernelNames[f];
         e = hipModuleGetFunction(&late.fn[f - kLateFirst], mod, what);

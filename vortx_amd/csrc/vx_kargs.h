@@ -144,6 +144,48 @@ typedef struct vx_kv_rows_args {
     uint32_t groups;       /* of tokens: one each, or four */
 } vx_kv_rows_args;
 
+/* Queries and keys, normed and rotated. [0] is of q, [1] of k. */
+typedef struct vx_rotate_args {
+    const float* x[2];     /* element (t, h, d) at x[t*xs[0] + h*xs[1] + d*xs[2]] */
+    float* y[2];           /* (y[1] null: k goes into the cache) */
+    int64_t xs[2][3], ys[2][3];
+    const float* w[2];     /* norm weight of head h, dim d at w[h*ws + d]; null: 1 */
+    const double* freqs;   /* [rotated / 2] */
+    const int32_t* positions;
+    uint32_t ws[2];
+    uint32_t heads[2];
+    uint32_t tokens, dim, rotated;
+    uint32_t pairs, norm;
+    float eps;
+    uint32_t vec;          /* 1: fours of dims, and their partners, are 16-byte aligned everywhere */
+    uint32_t run;          /* heads a group of lanes takes one after the other */
+    uint32_t chunks;       /* such runs a token */
+    uint32_t blocks;       /* workgroups of this part (of vx_kv_write_rotated: the queries') */
+} vx_rotate_args;
+
+/* Rows into the cache whose keys are normed and rotated on the way, and the queries beside them. */
+typedef struct vx_kv_rotated_args {
+    vx_kv_rows_args r;
+    vx_rotate_args t;
+} vx_kv_rotated_args;
+
+/* Pages of sequences that grow and shrink, and the slots of their new tokens. */
+typedef struct vx_pages_args {
+    int32_t* table;
+    int32_t* lens;
+    int32_t* free_pages;
+    int32_t* free_count;
+    const int32_t* want;
+    int32_t* starts;
+    int32_t* slots;
+    int32_t* positions;
+    uint32_t seqs, table_cols, table_stride;
+    uint32_t page_shift, pages;
+    uint32_t tokens;       /* entries of slots and positions */
+    uint32_t here;         /* 1: vx_pages_resize writes them, 0: vx_pages_slots after it */
+    uint32_t pad0;
+} vx_pages_args;
+
 /* Attention over the cache. Query row r = j * group + i of a sequence is its
  * j-th query token, i-th query head of the key/value head. */
 typedef struct vx_attn_args {

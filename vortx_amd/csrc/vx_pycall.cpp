@@ -278,6 +278,80 @@ PyObject* py_kv_read(PyObject*, PyObject* const* a, Py_ssize_t n) {
                                       const int32_t* slots) { return ((decltype(&vx_kv_read))fn)(ctx, st, k, v, c, slots); });
 }
 
+// What a vortx_amd.attention.Rotation says of itself: the address of its
+// vx_rotation, the dim and heads that its weights are for (0: any) and the
+// rotated dims, from a[0]; positions an int32 tensor or None.
+struct Turn {
+    const vx_rotation* how = nullptr;
+    const int32_t* positions = nullptr;
+    uint64_t dim = 0, q_heads = 0, k_heads = 0, rotated = 0;
+    bool read(PyObject* const* a, PyObject* pos, uint32_t tokens) {
+        how = (const vx_rotation*)addr(a[0]);
+        if (!how || !as_u64(a[1], UINT32_MAX, &dim) || !as_u64(a[2], UINT32_MAX, &q_heads) || !as_u64(a[3], UINT32_MAX, &k_heads) ||
+            !as_u64(a[4], UINT32_MAX, &rotated))
+            return false;
+        return pos == Py_None ? !rotated : ints_of(pos, tokens, false, &positions, nullptr, nullptr);
+    }
+    bool fits(const vx_layout& l, uint64_t heads) const {
+        return (!dim || l.size[2] == dim) && (!heads || l.size[1] == heads);
+    }
+};
+
+// rotate(fn, ctx, stream, q_out, q, k_out | None, k | None, positions | None, *Rotation's)
+PyObject* py_rotate(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    if (n != 13) return other_path();
+    auto f = (decltype(&vx_rotate))addr(a[0]);
+    vx_ctx ctx = (vx_ctx)addr(a[1]);
+    vx_stream st;
+    vx_mview qo, ko;
+    vx_cview q, k;
+    Turn t;
+    const bool keys = a[5] != Py_None || a[6] != Py_None;
+    if (!f || PyErr_Occurred() || !rows_of(a[3], &qo) || !rows_of(a[4], &q) || (keys && (!rows_of(a[5], &ko) || !rows_of(a[6], &k))) ||
+        !t.read(a + 8, a[7], q.layout.size[0]) || !t.fits(q.layout, t.q_heads) || (keys && !t.fits(k.layout, t.k_heads)) ||
+        !stream_of(a[2], &st))
+        return other_path();
+    return run([&] { return f(ctx, st, &qo, &q, keys ? &ko : nullptr, keys ? &k : nullptr, t.positions, t.how); });
+}
+
+// kv_write_rotated(fn, ctx, stream, cache, q_out | None, q | None, k, v, positions | None, slots, *Rotation's)
+PyObject* py_kv_write_rotated(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    if (n != 15) return other_path();
+    auto f = (decltype(&vx_kv_write_rotated))addr(a[0]);
+    vx_ctx ctx = (vx_ctx)addr(a[1]);
+    const vx_kv_cache* cache = (const vx_kv_cache*)addr(a[3]);
+    vx_stream st;
+    vx_mview qo;
+    vx_cview q, k, v;
+    Turn t;
+    const int32_t* slots = nullptr;
+    const bool queries = a[4] != Py_None || a[5] != Py_None;
+    if (!f || !cache || PyErr_Occurred() || (queries && (!rows_of(a[4], &qo) || !rows_of(a[5], &q))) || !rows_of(a[6], &k) ||
+        !rows_of(a[7], &v) || !ints_of(a[9], k.layout.size[0], false, &slots, nullptr, nullptr) ||
+        !t.read(a + 10, a[8], k.layout.size[0]) || (queries && !t.fits(q.layout, t.q_heads)) || !t.fits(k.layout, t.k_heads) ||
+        !stream_of(a[2], &st))
+        return other_path();
+    return run([&] { return f(ctx, st, cache, queries ? &qo : nullptr, queries ? &q : nullptr, &k, &v, t.positions, slots, t.how); });
+}
+
+// kv_resize(fn, ctx, stream, pages, seqs, want, starts, slots, positions, tokens): a vx_kv_pages and the outputs by their addresses
+PyObject* py_kv_resize(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    if (n != 10) return other_path();
+    auto f = (decltype(&vx_kv_resize))addr(a[0]);
+    vx_ctx ctx = (vx_ctx)addr(a[1]);
+    const vx_kv_pages* pages = (const vx_kv_pages*)addr(a[3]);
+    vx_stream st;
+    uint64_t seqs = 0, starts = 0, slots = 0, positions = 0, tokens = 0;
+    const int32_t* want = nullptr;
+    if (!f || !pages || PyErr_Occurred() || !as_u64(a[4], UINT32_MAX, &seqs) || !ints_of(a[5], (uint32_t)seqs, false, &want, nullptr, nullptr) ||
+        !as_u64(a[6], UINT64_MAX, &starts) || !as_u64(a[7], UINT64_MAX, &slots) || !as_u64(a[8], UINT64_MAX, &positions) ||
+        !as_u64(a[9], UINT32_MAX, &tokens) || !stream_of(a[2], &st))
+        return other_path();
+    return run([&] {
+        return f(ctx, st, pages, want, (int32_t*)(uintptr_t)starts, (int32_t*)(uintptr_t)slots, (int32_t*)(uintptr_t)positions, (uint32_t)tokens);
+    });
+}
+
 // attend(vx_attention, vx_attention_tree, ctx, stream, out, q, tree | None, cache, batch, opts, workspace, its bytes,
 //        query heads, tokens at most), the plan's structs by their addresses
 PyObject* py_attend(PyObject*, PyObject* const* a, Py_ssize_t n) {
@@ -311,7 +385,9 @@ PyMethodDef methods[] = {{"setup", FAST(py_setup)},           {"gemm", FAST(py_g
                          {"gemv", FAST(py_gemv)},             {"dequantize", FAST(py_dequantize)},
                          {"quantize", FAST(py_quantize)},     {"contiguous", FAST(py_contiguous)},
                          {"kv_write", FAST(py_kv_write)},     {"kv_read", FAST(py_kv_read)},
-                         {"attend", FAST(py_attend)},         {nullptr, nullptr, 0, nullptr}};
+                         {"attend", FAST(py_attend)},         {"rotate", FAST(py_rotate)},
+                         {"kv_write_rotated", FAST(py_kv_write_rotated)}, {"kv_resize", FAST(py_kv_resize)},
+                         {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_pycall", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace
