@@ -615,6 +615,60 @@ int vx_attention_tree(vx_ctx ctx, vx_stream stream, const vx_mview* out, const v
 int vx_attention_ws_size(vx_ctx ctx, const vx_kv_cache* cache, const vx_attn_batch* batch, const vx_attn_opts* opts,
                          uint32_t tokens, uint32_t q_heads, uint64_t* bytes);
 
+/* ------------------------------------------------------------------ */
+/* Products of 8-bit integers with a scale for each token and channel  */
+/* (no reference counterpart)                                          */
+/* ------------------------------------------------------------------ */
+
+/* Rows of 8-bit integers with an f32 scale each, [rows, cols], for the values
+ * scales[row] * integer: activations with a scale for each token, weights
+ * [channels, cols] with one for each channel. Device memory; base 16-byte
+ * aligned, row_stride_bytes a multiple of 16 (so a row's last 16 bytes can be
+ * read whole: what they hold past cols does not matter). */
+typedef struct vx_i8_rows {
+    void* base;
+    float* scales;
+    uint64_t row_stride_bytes;
+    uint32_t rows, cols;
+} vx_i8_rows;
+
+/* The rows of x ([rows, cols] f32 view, any strides) as such: with m the
+ * largest magnitude of a row, its scale is m / 127 and its integers are
+ * rint(x * (127 / m)), within -127..127, each operation one f32 rounding (ties
+ * to even). Where m < 2^-100 scale and integers are 0. A row with a NaN or an
+ * infinity has the scale NaN, which every product with it becomes. Bytes past
+ * cols stay as they are. */
+int vx_i8_quantize(vx_ctx ctx, vx_stream stream, const vx_i8_rows* out, const vx_cview* x);
+
+/* out[t, n] = x.scales[t] * w.scales[n] * sum_k x[t, k] w[n, k]: out is a [T, N]
+ * f32 view of any strides, x [T, K] and w [N, K]. The sum is exact (int32; K up
+ * to 131071, else VX_ERR_UNSUPPORTED, as K = 0 is), what is made of it is within
+ * 1.5 of f32's steps, and the same bits whatever T and whatever x's form. out lies apart from the
+ * inputs. */
+int vx_gemm_i8(vx_ctx ctx, vx_stream stream, const vx_mview* out, const vx_i8_rows* x, const vx_i8_rows* w);
+
+/* The same of x as an f32 [T, K] view, whose rows become integers as
+ * vx_i8_quantize makes them: for one or two tokens (rows of up to 32768 bytes in
+ * all) inside the product, one launch, otherwise in `workspace` before it. workspace: device memory,
+ * 16-byte aligned, at least vx_gemm_i8_ws_size bytes (VX_ERR_INVALID if not;
+ * NULL where none is needed); calls that share one must be ordered. */
+int vx_gemm_i8_x(vx_ctx ctx, vx_stream stream, const vx_mview* out, const vx_cview* x, const vx_i8_rows* w,
+                 void* workspace, uint64_t workspace_bytes);
+
+/* Bytes of workspace for `tokens` rows of `cols` f32 values (0: none). */
+int vx_gemm_i8_ws_size(uint32_t tokens, uint32_t cols, uint64_t* bytes);
+
+/* Activations of vx_gemm_i8_gated: g / (1 + e^-g); g / 2 (1 + tanh(sqrt(2 / pi)
+ * (g + 0.044715 g^3))); g / 2 erfc(-g / sqrt(2)); max(g, 0). */
+typedef enum vx_act { VX_ACT_SILU = 0, VX_ACT_GELU_TANH = 1, VX_ACT_GELU = 2, VX_ACT_RELU = 3 } vx_act;
+
+/* The gated half of a feed-forward block, out = act(x gate^T) * (x up^T), both
+ * products as vx_gemm_i8 forms them, in one kernel: gate and up [N, K], out [T, N]. */
+int vx_gemm_i8_gated(vx_ctx ctx, vx_stream stream, const vx_mview* out, const vx_i8_rows* x, const vx_i8_rows* gate,
+                     const vx_i8_rows* up, uint32_t act);
+int vx_gemm_i8_gated_x(vx_ctx ctx, vx_stream stream, const vx_mview* out, const vx_cview* x, const vx_i8_rows* gate,
+                       const vx_i8_rows* up, uint32_t act, void* workspace, uint64_t workspace_bytes);
+
 /* Block geometry of a vx_qtype: weights per block and bytes per block. */
 int vx_qtype_info(uint32_t qtype, uint32_t* block_weights,
                   uint32_t* block_bytes);

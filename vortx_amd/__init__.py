@@ -14,6 +14,8 @@ Python-side mirror of the reference interface for this path:
   attention over it (vortx_amd.attention), with the page tables
   (:class:`KvPages`) and the rotation of queries and keys that go before it,
   which the reference does not have;
+* :class:`Int8Gemm` — products of 8-bit integers with a scale for each token and
+  channel, plain and gated (vortx_amd.int8), which the reference does not have;
 * :class:`GGUFFile` — GGUF model files (vortx_amd.gguf), which feed real
   quantized weights to :class:`QuantGemv`.
 
@@ -33,7 +35,7 @@ from . import _ffi
 from ._ffi import (NONE_STRIDE, ROUTE_EMPTY, ROUTE_GEMV, ROUTE_NAIVE, ROUTE_TILED, VX_Q4_0, VX_Q4_K, VX_Q8_0,
                    VortxError, check, lib)
 
-__all__ = ["TensorLayout", "layout_extent", "XQ", "xq_size", "Gemm", "QuantGemv", "QWeight", "Contiguous", "KvCache", "KvAttention", "AttentionPlan", "KvPages", "KvStep", "Rotation", "rotation_freqs", "kv_cache_size", "tree_mask", "GGUFFile", "VortxError", "VX_Q4_0", "VX_Q8_0", "VX_Q4_K",
+__all__ = ["TensorLayout", "layout_extent", "XQ", "xq_size", "Gemm", "QuantGemv", "QWeight", "Contiguous", "KvCache", "KvAttention", "AttentionPlan", "KvPages", "KvStep", "Rotation", "rotation_freqs", "kv_cache_size", "tree_mask", "Int8Gemm", "Int8Rows", "GGUFFile", "VortxError", "VX_Q4_0", "VX_Q8_0", "VX_Q4_K",
            "ROUTE_NAIVE", "ROUTE_TILED", "ROUTE_GEMV", "ROUTE_EMPTY", "qtype_info", "lib"]
 
 # Load eagerly: a missing library must fail at import, not at first call.
@@ -53,11 +55,13 @@ except ImportError:
     class _pycall:
         gemm = gemv = quantize = dequantize = contiguous = setup = staticmethod(lambda *args: None)
         kv_write = kv_read = attend = rotate = kv_write_rotated = kv_resize = setup
+        gemm_i8 = i8_quantize = setup
 
 _ADDR = {name: C.cast(getattr(lib(), name), C.c_void_p).value
          for name in ("vx_gemm_f32", "vx_gemm_f32_ex", "vx_gemv_q_ex", "vx_gemv_q_ws", "vx_dequantize", "vx_quantize",
                       "vx_contiguous", "vx_kv_write", "vx_kv_read", "vx_attention", "vx_attention_tree", "vx_rotate",
-                      "vx_kv_write_rotated", "vx_kv_resize")}
+                      "vx_kv_write_rotated", "vx_kv_resize", "vx_i8_quantize", "vx_gemm_i8", "vx_gemm_i8_x", "vx_gemm_i8_gated",
+                      "vx_gemm_i8_gated_x")}
 _GEMM, _GEMM_EX = _ADDR["vx_gemm_f32"], _ADDR["vx_gemm_f32_ex"]
 _GEMV_EX, _GEMV_WS = _ADDR["vx_gemv_q_ex"], _ADDR["vx_gemv_q_ws"]
 
@@ -479,6 +483,7 @@ class Contiguous(_Context):
         check(lib().vx_contiguous(self._h, _stream(stream), C.byref(ov), C.byref(tv), off))
 
 
+from .int8 import Int8Gemm, Int8Rows  # noqa: E402
 from .gguf import GGUFFile  # noqa: E402  (needs QWeight and TensorLayout above)
 from .attention import (AttentionPlan, KvAttention, KvCache, KvPages, KvStep, Rotation, kv_cache_size,  # noqa: E402
                         rotation_freqs, tree_mask)  # noqa: E402

@@ -72,6 +72,11 @@ class VxKvPages(C.Structure):
                 ("pages", C.c_uint32), ("reserved", C.c_uint32)]
 
 
+class VxI8Rows(C.Structure):
+    _fields_ = [("base", C.c_void_p), ("scales", C.c_void_p), ("row_stride_bytes", C.c_uint64), ("rows", C.c_uint32),
+                ("cols", C.c_uint32)]
+
+
 VX_ATTN_CAUSAL = 1
 VX_ROTATE_PAIRS, VX_ROTATE_NORM = 1, 2
 VX_GEMM_BROADCAST, VX_GEMM_TILE_NARROW, VX_GEMM_TILE_WIDE, VX_GEMM_TILE_SMALL = 1, 2, 4, 8
@@ -134,6 +139,13 @@ SIGNATURES = [
                                     _P(VxAttnOpts), C.c_void_p, C.c_uint32, C.c_uint32, C.c_void_p, C.c_uint64]),
     ("vx_attention_ws_size", C.c_int, [C.c_void_p, _P(VxKvCache), _P(VxAttnBatch), _P(VxAttnOpts), C.c_uint32,
                                        C.c_uint32, _P(C.c_uint64)]),
+    ("vx_i8_quantize", C.c_int, [C.c_void_p, C.c_void_p, _P(VxI8Rows), _P(VxCView)]),
+    ("vx_gemm_i8", C.c_int, [C.c_void_p, C.c_void_p, _P(VxMView), _P(VxI8Rows), _P(VxI8Rows)]),
+    ("vx_gemm_i8_x", C.c_int, [C.c_void_p, C.c_void_p, _P(VxMView), _P(VxCView), _P(VxI8Rows), C.c_void_p, C.c_uint64]),
+    ("vx_gemm_i8_ws_size", C.c_int, [C.c_uint32, C.c_uint32, _P(C.c_uint64)]),
+    ("vx_gemm_i8_gated", C.c_int, [C.c_void_p, C.c_void_p, _P(VxMView), _P(VxI8Rows), _P(VxI8Rows), _P(VxI8Rows), C.c_uint32]),
+    ("vx_gemm_i8_gated_x", C.c_int, [C.c_void_p, C.c_void_p, _P(VxMView), _P(VxCView), _P(VxI8Rows), _P(VxI8Rows), C.c_uint32,
+                                     C.c_void_p, C.c_uint64]),
     ("vx_qtype_info", C.c_int, [C.c_uint32, _P(C.c_uint32), _P(C.c_uint32)]),
     ("vx_layout_contiguous", C.c_int, [_P(C.c_uint32), C.c_uint32, _P(VxLayout)]),
     ("vx_layout_canonicalize", C.c_int, [_P(VxLayout), _P(VxLayout)]),

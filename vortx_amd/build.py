@@ -34,8 +34,8 @@ ARCH = "gfx950"
 MODULES = {"vx_co_gemm": "gemm.hip", "vx_co_gemv_q": "gemv_q.hip", "vx_co_copy": "copy.hip",
            "vx_co_quantize": "quantize.hip", "vx_co_gemm_q": "gemm_q.hip",
            "vx_co_gemm_bf": "gemm_bf.hip", **{f"vx_co_attn_d{d}": f"attn_d{d}.hip" for d in (64, 96, 128, 256)},
-           "vx_co_step": "step.hip"}
-HOST_SOURCES = ["vx_host.cpp", "vx_attn.cpp", "vx_layout.cpp", "vx_gguf.cpp"]
+           "vx_co_step": "step.hip", "vx_co_i8": "i8.hip"}
+HOST_SOURCES = ["vx_host.cpp", "vx_attn.cpp", "vx_i8.cpp", "vx_layout.cpp", "vx_gguf.cpp"]
 
 HIPCC_FLAGS = [
     "--genco", f"--offload-arch={ARCH}", "-O3", "-std=c++17",

@@ -48,6 +48,7 @@ extern const unsigned char vx_co_attn_d256[];
 extern const unsigned char vx_co_attn_d256_end[];
 // (weak: host sources built without these code objects have none to load)
 extern const unsigned char vx_co_step[] __attribute__((weak));
+extern const unsigned char vx_co_i8[] __attribute__((weak));
 }
 
 namespace vx {
@@ -91,8 +92,9 @@ static const struct { const unsigned char* image; int first, end; } kLate[] = {
     {vx_co_attn_d96, K_vx_kv_write_d96_k8v8, K_vx_kv_write_d128_k8v8},
     {vx_co_attn_d128, K_vx_kv_write_d128_k8v8, K_vx_kv_write_d256_k8v8},
     {vx_co_attn_d256, K_vx_kv_write_d256_k8v8, K_vx_pages_resize},
-    {vx_co_step, K_vx_pages_resize, K_COUNT}};
-constexpr int kNumLate = 5, kLateFirst = K_vx_kv_write_d64_k8v8;
+    {vx_co_step, K_vx_pages_resize, K_vx_i8_quantize_c4},
+    {vx_co_i8, K_vx_i8_quantize_c4, K_COUNT}};
+constexpr int kNumLate = 6, kLateFirst = K_vx_kv_write_d64_k8v8;
 struct LateKernels {  // of a device
     hipFunction_t fn[K_COUNT - kLateFirst] = {};  // written under `lock`, read once `ready` says so
     std::atomic<bool> ready[kNumLate] = {};
@@ -210,12 +212,12 @@ int need_kernel(vx_ctx ctx, int k) {
     return VX_OK;
 }
 
-int launch_struct(vx_ctx ctx, int k, uint32_t grid, uint32_t block, vx_stream stream, const void* args) {
+int launch_struct(vx_ctx ctx, int k, uint32_t grid, uint32_t block, vx_stream stream, const void* args, uint32_t lds) {
     if (grid == 0) return VX_OK;
     if (const int s = need_kernel(ctx, k)) return s;
     DeviceGuard guard(ctx->device);
     void* params[] = {const_cast<void*>(args)};
-    const hipError_t e = hipModuleLaunchKernel(ctx->late->fn[k - kLateFirst], grid, 1, 1, block, 1, 1, 0, (hipStream_t)stream, params, nullptr);
+    const hipError_t e = hipModuleLaunchKernel(ctx->late->fn[k - kLateFirst], grid, 1, 1, block, 1, 1, lds, (hipStream_t)stream, params, nullptr);
     if (e != hipSuccess) return fail_hip(e, kKernelNames[k]);
     return VX_OK;
 }

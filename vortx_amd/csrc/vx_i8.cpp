@@ -1,0 +1,205 @@
+// vx_i8.cpp — host side of the products of 8-bit integers: checks and kernel choice.
+#include <algorithm>
+
+#include "vx_internal.hpp"
+#include "vx_kargs.h"
+
+namespace vx {
+
+// Sums of K products of up to 128^2 stay within 31 bits.
+constexpr uint32_t VX_I8_MOST_COLS = 131071;
+
+static int check_rows(const vx_i8_rows* r) {
+    if (!r) return fail(VX_ERR_INVALID, "null rows");
+    if (r->row_stride_bytes < r->cols) return fail(VX_ERR_INVALID, "row_stride_bytes smaller than a row");
+    if ((uintptr_t)r->base & 15u || r->row_stride_bytes % 16) return fail(VX_ERR_UNSUPPORTED, "rows of 8-bit integers are 16-byte aligned");
+    if ((uintptr_t)r->scales & 3u) return fail(VX_ERR_INVALID, "scales is not 4-byte aligned");
+    if (r->rows && (!r->scales || (r->cols && !r->base))) return fail(VX_ERR_INVALID, "null base or scales");
+    return VX_OK;
+}
+
+// A [rows, cols] view of f32.
+struct Matrix {
+    uintptr_t ptr;
+    uint32_t rows, cols;
+    int64_t stride[2];
+    bool vec;  // stride 1 along a row, 16-byte aligned rows
+};
+static int matrix_view(const void* base, const vx_layout* l, Matrix* m, const char* name, bool written) {
+    Canon c;
+    const int s = canon_view(base, l, &c, name);
+    if (s) return s;
+    if (c.l.size[0] != 1 || c.l.size[1] != 1) return fail(VX_ERR_SHAPE, "a view of rank 2 is expected");
+    m->ptr = c.ptr;
+    m->rows = c.l.size[2];
+    m->cols = c.l.size[3];
+    m->stride[0] = c.l.stride[2];
+    m->stride[1] = c.l.stride[3];
+    if (written)
+        for (int i = 0; i < 2; ++i)
+            if (c.l.size[i + 2] > 1 && m->stride[i] == 0) return fail(VX_ERR_INVALID, "a written view has a zero stride on a dimension of size > 1");
+    m->vec = m->stride[1] == 1 && (c.ptr & 15u) == 0 && (m->rows == 1 || m->stride[0] % 4 == 0);
+    return VX_OK;
+}
+
+static int quantize(vx_ctx ctx, vx_stream stream, const vx_i8_rows* out, const Matrix& x) {
+    if (!out->rows) return VX_OK;
+    vx_i8_quant_args a{};
+    a.x = (const float*)x.ptr;
+    a.xs[0] = x.stride[0];
+    a.xs[1] = x.stride[1];
+    a.out = (int8_t*)out->base;
+    a.row_stride = out->row_stride_bytes;
+    a.scales = out->scales;
+    a.rows = out->rows;
+    a.cols = out->cols;
+    // rows of up to 4096 stay in 16 registers a thread, longer ones in 64
+    const int k = !x.vec ? K_vx_i8_quantize_any : out->cols <= 4096 ? K_vx_i8_quantize_c4 : K_vx_i8_quantize_c16;
+    return launch_struct(ctx, k, std::min(out->rows, 1u << 20), 256, stream, &a);
+}
+
+static uint64_t up(uint64_t n, uint64_t to) { return (n + to - 1) / to * to; }
+
+// x that a product quantizes itself (one launch, each workgroup for itself) up to so many tokens and bytes of codes.
+constexpr uint32_t VX_I8_OWN_TOKENS = 2, VX_I8_OWN_BYTES = 32768;
+static bool own_x(uint32_t T, uint32_t K) { return T <= VX_I8_OWN_TOKENS && up(K, 64) * T <= VX_I8_OWN_BYTES; }
+
+static uint64_t ws_bytes(uint32_t T, uint32_t K) { return own_x(T, K) ? 0 : up(K, 128) * T + up(4ull * T, 16); }
+
+struct I8Plan {
+    int kernel;
+    uint32_t tokens, channels;  // of a workgroup
+    uint32_t block, lds;
+};
+static I8Plan plan_gemm(int num_cus, const vx_i8_args& a, bool gated) {
+    const int g = gated ? 1 : 0;
+    const bool near = a.xs < (1u << 24) && a.ws[0] < (1u << 24) && a.ws[1] < (1u << 24);  // a tile's rows within 32 bits
+    if (a.xf || a.T <= 128 || !near) {
+        // 16 tt tokens by 16 nt channels
+        struct Direct { int kernel; uint32_t tt, nt[2]; };
+        static const Direct kDirect[4] = {{K_vx_i8_direct_x, 1, {1, 1}}, {K_vx_i8_direct_t1, 1, {1, 1}}, {K_vx_i8_direct_t2, 2, {2, 1}},
+                                          {K_vx_i8_direct_t4, 4, {2, 1}}};
+        const Direct& d = kDirect[a.xf ? 0 : a.T <= 16 ? 1 : a.T <= 32 ? 2 : 3];
+        const uint32_t sums = std::min(d.tt * d.nt[g], gated ? 4u : 8u) * (gated ? 2 : 1);
+        return {d.kernel + g, 16 * d.tt, 16 * d.nt[g], 512, a.x_bytes + sums * 8192};
+    }
+    // tiles of 256 where they fill the card
+    const uint32_t cn = gated ? 128 : 256;
+    const uint64_t wide = (uint64_t)((a.T + 255) / 256) * ((a.N + cn - 1) / cn);
+    const uint32_t side = wide * 2 > (uint64_t)num_cus ? 256 : 128;
+    return {(side == 256 ? K_vx_i8_tile256 : K_vx_i8_tile128) + g, side, gated ? side / 2 : side, 2 * side, 0};
+}
+
+static int run_gemm(vx_ctx ctx, vx_stream stream, const vx_mview* out, const vx_i8_rows* xq, const vx_cview* xf, const vx_i8_rows* w,
+                    const vx_i8_rows* up_w, uint32_t act, void* ws, uint64_t ws_size) {
+    clear_error();
+    if (!ctx) return fail(VX_ERR_INVALID, "null ctx");
+    if (!out || (!xq && !xf)) return fail(VX_ERR_INVALID, "null view");
+    Matrix o, x{};
+    int s = matrix_view(out->base, &out->layout, &o, "out", true);
+    if (s) return s;
+    if ((s = check_rows(w)) || (up_w && (s = check_rows(up_w)))) return s;
+    if (xq) {
+        if ((s = check_rows(xq))) return s;
+        x.rows = xq->rows;
+        x.cols = xq->cols;
+    } else if ((s = matrix_view(xf->base, &xf->layout, &x, "x", false))) {
+        return s;
+    }
+    if (act > VX_ACT_RELU) return fail(VX_ERR_INVALID, "unknown activation");
+    if (x.cols != w->cols || o.rows != x.rows || o.cols != w->rows || (up_w && (up_w->rows != w->rows || up_w->cols != w->cols)))
+        return fail(VX_ERR_SHAPE, "incompatible shapes: out [T, N], x [T, K], weights [N, K]");
+    if (w->cols == 0) return fail(VX_ERR_UNSUPPORTED, "rows of no columns");
+    if (w->cols > VX_I8_MOST_COLS) return fail(VX_ERR_UNSUPPORTED, "more than 131071 columns");
+    if ((uintptr_t)ws & 15u) return fail(VX_ERR_INVALID, "workspace is not 16-byte aligned");
+    vx_i8_args a{};
+    a.T = x.rows;
+    a.N = w->rows;
+    a.K = w->cols;
+    if (xf && ws_size < ws_bytes(a.T, a.K)) return fail(VX_ERR_INVALID, "workspace smaller than vx_gemm_i8_ws_size");
+    if (xf && ws_bytes(a.T, a.K) && !ws) return fail(VX_ERR_INVALID, "null workspace");
+    if (a.T == 0 || a.N == 0) return VX_OK;
+    const bool gated = up_w != nullptr;
+    const vx_i8_rows* ws2[2] = {w, gated ? up_w : w};
+    for (int i = 0; i < 2; ++i) {
+        a.w[i] = (const int8_t*)ws2[i]->base;
+        a.ws[i] = ws2[i]->row_stride_bytes;
+        a.wscale[i] = ws2[i]->scales;
+    }
+    a.out = (float*)o.ptr;
+    a.os[0] = o.stride[0];
+    a.os[1] = o.stride[1];
+    a.out_vec = o.vec;
+    a.act = act;
+    const bool own = xf && own_x(a.T, a.K);
+    vx_i8_rows rows;
+    if (xf && !own) {
+        const uint64_t stride = up(a.K, 128);
+        rows = vx_i8_rows{ws, (float*)((char*)ws + stride * a.T), stride, a.T, a.K};
+        xq = &rows;
+    }
+    if (own) {
+        a.xf = (const float*)x.ptr;
+        a.xfs[0] = x.stride[0];
+        a.xfs[1] = x.stride[1];
+        a.xf_vec = x.vec;
+        a.pitch = (uint32_t)up(a.K, 64) + 16;
+        a.x_bytes = (uint32_t)up(a.T * (uint64_t)a.pitch + 8 * 16 * 4 + 64, 16);
+    } else {
+        a.x = (const int8_t*)xq->base;
+        a.xs = xq->row_stride_bytes;
+        a.xscale = xq->scales;
+    }
+    const I8Plan p = plan_gemm(ctx_cus(ctx), a, gated);
+    a.tiles_t = (a.T - 1) / p.tokens + 1;
+    a.tiles_n = (a.N - 1) / p.channels + 1;
+    if ((uint64_t)a.tiles_t * a.tiles_n >= (1u << 22)) return fail(VX_ERR_UNSUPPORTED, "too many outputs (split the call)");
+    if (xf && !own && (s = quantize(ctx, stream, &rows, x))) return s;
+    return launch_struct(ctx, p.kernel, a.tiles_t * a.tiles_n, p.block, stream, &a, p.lds);
+}
+
+}  // namespace vx
+
+extern "C" {
+
+int vx_i8_quantize(vx_ctx ctx, vx_stream stream, const vx_i8_rows* out, const vx_cview* x) {
+    vx::clear_error();
+    if (!ctx) return vx::fail(VX_ERR_INVALID, "null ctx");
+    if (!x) return vx::fail(VX_ERR_INVALID, "null view");
+    vx::Matrix m;
+    int s = vx::check_rows(out);
+    if (s) return s;
+    if ((s = vx::matrix_view(x->base, &x->layout, &m, "x", false))) return s;
+    if (m.rows != out->rows || m.cols != out->cols) return vx::fail(VX_ERR_SHAPE, "x and out have different shapes");
+    return vx::quantize(ctx, stream, out, m);
+}
+
+int vx_gemm_i8_ws_size(uint32_t tokens, uint32_t cols, uint64_t* bytes) {
+    vx::clear_error();
+    if (!bytes) return vx::fail(VX_ERR_INVALID, "null bytes");
+    *bytes = vx::ws_bytes(tokens, cols);
+    return VX_OK;
+}
+
+int vx_gemm_i8(vx_ctx ctx, vx_stream stream, const vx_mview* out, const vx_i8_rows* x, const vx_i8_rows* w) {
+    return vx::run_gemm(ctx, stream, out, x, nullptr, w, nullptr, 0, nullptr, 0);
+}
+
+int vx_gemm_i8_x(vx_ctx ctx, vx_stream stream, const vx_mview* out, const vx_cview* x, const vx_i8_rows* w, void* workspace,
+                 uint64_t workspace_bytes) {
+    return vx::run_gemm(ctx, stream, out, nullptr, x, w, nullptr, 0, workspace, workspace_bytes);
+}
+
+int vx_gemm_i8_gated(vx_ctx ctx, vx_stream stream, const vx_mview* out, const vx_i8_rows* x, const vx_i8_rows* gate,
+                     const vx_i8_rows* up, uint32_t act) {
+    if (!up) return vx::clear_error(), vx::fail(VX_ERR_INVALID, "null rows");
+    return vx::run_gemm(ctx, stream, out, x, nullptr, gate, up, act, nullptr, 0);
+}
+
+int vx_gemm_i8_gated_x(vx_ctx ctx, vx_stream stream, const vx_mview* out, const vx_cview* x, const vx_i8_rows* gate,
+                       const vx_i8_rows* up, uint32_t act, void* workspace, uint64_t workspace_bytes) {
+    if (!up) return vx::clear_error(), vx::fail(VX_ERR_INVALID, "null rows");
+    return vx::run_gemm(ctx, stream, out, nullptr, x, gate, up, act, workspace, workspace_bytes);
+}
+
+}  // extern "C"

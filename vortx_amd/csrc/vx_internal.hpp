@@ -27,8 +27,8 @@ int canon_view(const void* base, const vx_layout* in, Canon* c, const char* name
 int ctx_cus(vx_ctx ctx);
 // Kernel k of the attention is there: loads the code object of its head size if it is not yet.
 int need_kernel(vx_ctx ctx, int k);
-// Launches such a kernel on the context's device; `args` is its one struct argument.
-int launch_struct(vx_ctx ctx, int k, uint32_t grid, uint32_t block, vx_stream stream, const void* args);
+// Launches such a kernel on the context's device; `args` is its one struct argument, `lds` bytes beside its own.
+int launch_struct(vx_ctx ctx, int k, uint32_t grid, uint32_t block, vx_stream stream, const void* args, uint32_t lds = 0);
 
 // Records `msg` as this thread's last error and returns `status`.
 int fail(int status, const char* msg);

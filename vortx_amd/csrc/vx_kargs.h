@@ -186,6 +186,37 @@ typedef struct vx_pages_args {
     uint32_t pad0;
 } vx_pages_args;
 
+/* Rows of f32 to 8-bit integers with a scale each. */
+typedef struct vx_i8_quant_args {
+    const float* x;        /* element (row, k) at x[row*xs[0] + k*xs[1]] */
+    int64_t xs[2];
+    int8_t* out;
+    uint64_t row_stride;   /* bytes */
+    float* scales;
+    uint32_t rows, cols;
+} vx_i8_quant_args;
+
+/* Products of such rows: x [T, K] by w [N, K] (of a gated one, w[0] gate and w[1] up). */
+typedef struct vx_i8_args {
+    const int8_t* w[2];
+    uint64_t ws[2];        /* bytes between rows */
+    const float* wscale[2];
+    const int8_t* x;
+    uint64_t xs;
+    const float* xscale;
+    const float* xf;       /* kernels that quantize x themselves: element (t, k) at xf[t*xfs[0] + k*xfs[1]] */
+    int64_t xfs[2];
+    float* out;            /* element (t, n) at out[t*os[0] + n*os[1]] */
+    int64_t os[2];
+    uint32_t T, N, K;
+    uint32_t act;
+    uint32_t tiles_t, tiles_n;
+    uint32_t out_vec;      /* 1: os[1] == 1 and fours of channels 16-byte aligned */
+    uint32_t xf_vec;       /* 1: xfs[1] == 1 and 16-byte aligned rows */
+    uint32_t pitch;        /* bytes between x's rows in LDS, of such kernels */
+    uint32_t x_bytes;      /* of LDS that x, its maxima and scales take */
+} vx_i8_args;
+
 /* Attention over the cache. Query row r = j * group + i of a sequence is its
  * j-th query token, i-th query head of the key/value head. */
 typedef struct vx_attn_args {

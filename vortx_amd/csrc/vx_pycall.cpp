@@ -352,6 +352,51 @@ PyObject* py_kv_resize(PyObject*, PyObject* const* a, Py_ssize_t n) {
     });
 }
 
+// i8_quantize(fn, ctx, stream, rows, x), rows the address of a vx_i8_rows
+PyObject* py_i8_quantize(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    if (n != 5) return other_path();
+    auto f = (decltype(&vx_i8_quantize))addr(a[0]);
+    vx_ctx ctx = (vx_ctx)addr(a[1]);
+    const vx_i8_rows* rows = (const vx_i8_rows*)addr(a[3]);
+    vx_stream st;
+    vx_cview x;
+    if (!f || !rows || PyErr_Occurred() || !view_of(a[4], false, &x) || !stream_of(a[2], &st)) return other_path();
+    return run([&] { return f(ctx, st, rows, &x); });
+}
+
+// gemm_i8(fn, ctx, stream, out, x, w, up | None, act, workspace | None): fn a vx_gemm_i8 or vx_gemm_i8_gated with x the
+// address of a vx_i8_rows, or their _x forms with x a tensor; w and up addresses
+PyObject* py_gemm_i8(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    if (n != 9) return other_path();
+    void* fn = addr(a[0]);
+    vx_ctx ctx = (vx_ctx)addr(a[1]);
+    const vx_i8_rows *w = (const vx_i8_rows*)addr(a[5]), *u = nullptr;
+    const bool rows = PyLong_CheckExact(a[4]), gated = a[6] != Py_None;
+    if (gated && !(u = (const vx_i8_rows*)addr(a[6]))) return other_path();
+    vx_stream st;
+    vx_mview o;
+    vx_cview x;
+    uint64_t act = 0, wp = 0, wn = 0;
+    const vx_i8_rows* xq = rows ? (const vx_i8_rows*)addr(a[4]) : nullptr;
+    if (!fn || !w || (rows && !xq) || PyErr_Occurred() || !view_of(a[3], false, &o) || (!rows && !view_of(a[4], false, &x)) ||
+        !as_u64(a[7], UINT32_MAX, &act) || !stream_of(a[2], &st))
+        return other_path();
+    if (rows)
+        return run([&] {
+            return gated ? ((decltype(&vx_gemm_i8_gated))fn)(ctx, st, &o, xq, w, u, (uint32_t)act) : ((decltype(&vx_gemm_i8))fn)(ctx, st, &o, xq, w);
+        });
+    if (a[8] != Py_None) {
+        if (!is_gpu_tensor(a[8])) return other_path();
+        Ref c(PyObject_CallMethodNoArgs(a[8], s_is_contiguous));
+        if (c.o != Py_True || !call_u64(a[8], s_data_ptr, UINT64_MAX, &wp) || !attr_u64(a[8], s_nbytes, UINT64_MAX, &wn)) return other_path();
+    }
+    void* ws = (void*)(uintptr_t)wp;
+    return run([&] {
+        return gated ? ((decltype(&vx_gemm_i8_gated_x))fn)(ctx, st, &o, &x, w, u, (uint32_t)act, ws, wn)
+                     : ((decltype(&vx_gemm_i8_x))fn)(ctx, st, &o, &x, w, ws, wn);
+    });
+}
+
 // attend(vx_attention, vx_attention_tree, ctx, stream, out, q, tree | None, cache, batch, opts, workspace, its bytes,
 //        query heads, tokens at most), the plan's structs by their addresses
 PyObject* py_attend(PyObject*, PyObject* const* a, Py_ssize_t n) {
@@ -387,6 +432,7 @@ PyMethodDef methods[] = {{"setup", FAST(py_setup)},           {"gemm", FAST(py_g
                          {"kv_write", FAST(py_kv_write)},     {"kv_read", FAST(py_kv_read)},
                          {"attend", FAST(py_attend)},         {"rotate", FAST(py_rotate)},
                          {"kv_write_rotated", FAST(py_kv_write_rotated)}, {"kv_resize", FAST(py_kv_resize)},
+                         {"i8_quantize", FAST(py_i8_quantize)}, {"gemm_i8", FAST(py_gemm_i8)},
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_pycall", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
