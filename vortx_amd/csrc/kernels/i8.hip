@@ -243,124 +243,197 @@ VX_I8_DIRECT(vx_i8_direct_t4, 4, 2, 2, false, false)
 VX_I8_DIRECT(vx_i8_direct_t4_gated, 4, 1, 2, true, false)
 
 // ---------------------------------------------------------------- many tokens
-// A tile of MT tokens by MN rows of weights (of a gated product half gate, half up,
-// 16 and 16 in turn, so that a lane has both sums of an output), WT x WN waves. A
-// stage is 64 bytes of K of both, brought from memory straight into LDS; four stages
-// go round, three on their way while one is multiplied, with one barrier each. The
-// 16-byte pieces of a row are stored in an order that goes by the row, so that the
-// lanes of a fragment (16 rows, one piece each) meet all banks.
+// Tiles of MT tokens by MN rows of weights (of a gated product half gate, half up,
+// 16 and 16 in turn, so that a lane has both sums of an output), WT x WN waves, a
+// workgroup one after the other. A stage is 128 bytes of K, whole cache lines, in two
+// halves that a matrix instruction takes 64 bytes of; a unit is one operand of a stage,
+// brought from memory straight into LDS, and five units go round: two are multiplied
+// while three are on their way. The 16-byte pieces of a row are stored in an order that
+// goes by the row, so that the lanes of a fragment (16 rows, one piece each) meet all
+// banks.
 template <int MT, int MN, int WT, int WN, bool GATED>
 struct vx_i8_tile {
+    static_assert(MT == MN, "units of one size");
     static constexpr int WAVES = WT * WN, THREADS = 64 * WAVES;
     static constexpr int FT = MT / (16 * WT), FN = MN / (16 * WN);  // fragments of a wave
-    static constexpr uint32_t STAGE = 64 * (MT + MN), STAGES = 4;
-    static constexpr int PIECES = (MT + MN) / 16 / WAVES;  // loads of a wave and stage, 16 rows each
-    static_assert(PIECES * WAVES * 16 == MT + MN && (MN / 16) % PIECES == 0, "a wave's loads are all of one operand");
+    static constexpr uint32_t UNIT = 128 * MT, UNITS = 5;
+    static constexpr int PIECES = MT / 8 / WAVES;  // loads of a wave and unit, 8 rows each
+    static_assert(PIECES * WAVES * 8 == MT && PIECES == 4, "a wave loads 32 rows of a unit");
 
-    // piece `c` (of four) of row r within a stage's operand
-    static __device__ __forceinline__ uint32_t at(uint32_t r, uint32_t c) { return r * 64 + ((c ^ (r >> 1)) & 3) * 16; }
+    // piece `c` (of eight) of row r within a unit
+    static __device__ __forceinline__ uint32_t at(uint32_t r, uint32_t c) { return r * 128 + ((c ^ (r >> 1)) & 7) * 16; }
 
-    static __device__ __forceinline__ void run(const vx_i8_args& a) {
-        __shared__ __align__(1024) uint8_t lds[STAGE * STAGES];
-        const uint32_t tid = threadIdx.x, lane = tid & 63, m = lane & 15, kg = lane >> 4;
-        const uint32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-        const uint32_t tile = vx_xcd_order(blockIdx.x, a.tiles_t * a.tiles_n);
-        constexpr uint32_t CH = GATED ? MN / 2 : MN;  // channels of a tile
-        const uint32_t t0 = tile % a.tiles_t * MT, n0 = tile / a.tiles_t * CH;
-        // this wave's loads: 16 rows of the weights (first in LDS) or of x, four lanes a row
-        uint32_t off[PIECES], cut[PIECES];  // of a stage inside K, and of the last one
-        const uint32_t S = (a.K + 63) / 64, last = 64 * (S - 1);
-        const uint32_t row0 = wave * PIECES * 16;
-        const bool weights = row0 < MN;
-        const int8_t* base[PIECES];
+    const vx_i8_args& a;
+    const uint32_t tid, lane, m, kg, wave, S, last;
+    uint32_t off_w[PIECES], off_x[PIECES];  // within the operands' first stage
+    i4v base_w[2], base_x;
+    uint32_t t0, n0, lds0;
+
+    static __device__ __forceinline__ i4v buffer(const int8_t* p) {  // without an end
+        const uint64_t u = (uint64_t)(uintptr_t)p;
+        return i4v{(int)__builtin_amdgcn_readfirstlane((int)(uint32_t)u), (int)(__builtin_amdgcn_readfirstlane((int)(uint32_t)(u >> 32)) & 0xFFFF), -1, 0x00027000};
+    }
+    __device__ __forceinline__ vx_i8_tile(const vx_i8_args& a_, uint8_t* lds)
+        : a(a_), tid(threadIdx.x), lane(tid & 63), m(lane & 15), kg(lane >> 4), wave(__builtin_amdgcn_readfirstlane(tid >> 6)),
+          S((a_.K + 127) / 128), last(128 * (S - 1)),
+          lds0(__builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)lds)) {}
+
+    // The loads of tile `id` of all in their order.
+    __device__ __forceinline__ void place(uint32_t id) {
+        // in bands of eight tiles of tokens: the 32 tiles that an XCD works on at a time are 8 by 4,
+        // so that its L2 takes 12 operands of a tile from farther away, where 16 by 2 takes 18
+        const uint32_t tile = vx_xcd_order(id, a.tiles_t * a.tiles_n), band = tile / (8 * a.tiles_n), in = tile - band * 8 * a.tiles_n;
+        const uint32_t high = min(8u, a.tiles_t - 8 * band);
+        t0 = (8 * band + in % high) * MT;
+        n0 = in / high * (GATED ? MN / 2 : MN);
+        base_w[0] = buffer(a.w[0] + (uint64_t)n0 * a.ws[0]);
+        base_w[1] = GATED ? buffer(a.w[1] + (uint64_t)n0 * a.ws[1]) : base_w[0];
+        base_x = buffer(a.x + (uint64_t)t0 * a.xs);
 #pragma unroll
         for (int p = 0; p < PIECES; ++p) {
-            const uint32_t r = row0 + 16 * p + lane / 4, c = ((lane & 3) ^ (r >> 1)) & 3;
-            uint64_t row;
-            if (weights) {
-                const uint32_t g = GATED ? (row0 / 16 + p) & 1 : 0;  // (a piece is all gate or all up)
-                const uint32_t n = GATED ? n0 + r / 32 * 16 + r % 16 : n0 + r;
-                base[p] = a.w[g] + (uint64_t)n0 * a.ws[g];
-                row = (uint64_t)(min(n, a.N - 1u) - n0) * a.ws[g];
-            } else {
-                base[p] = a.x + (uint64_t)t0 * a.xs;
-                row = (uint64_t)(min(t0 + r - MN, a.T - 1u) - t0) * a.xs;
-            }
-            off[p] = (uint32_t)row + 16 * c;
-            cut[p] = (uint32_t)row + (last + 16 * c < a.K ? last + 16 * c : 0u);
+            const uint32_t r = wave * 32 + 8 * p + lane / 8, c = piece(p);
+            const uint32_t n = GATED ? n0 + r / 32 * 16 + r % 16 : n0 + r;  // (a piece is all gate or all up)
+            const uint32_t w = (min(n, a.N - 1u) - n0) * (uint32_t)a.ws[GATED ? p / 2 : 0], x = (min(t0 + r, a.T - 1u) - t0) * (uint32_t)a.xs;
+            off_w[p] = w + 16 * c;
+            off_x[p] = x + 16 * c;
         }
-        const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)lds;
-        auto request = [&](uint32_t s) {
+    }
+    // which piece of its row this lane has
+    __device__ __forceinline__ uint32_t piece(int p) const { return ((lane & 7) ^ (4 * p + lane / 16)) & 7; }
+    __device__ __forceinline__ void load(const uint32_t (&from)[PIECES], const i4v& b0, const i4v& b1, uint32_t slot, uint32_t k) {
+        const uint32_t to = lds0 + slot * UNIT + wave * 4096;
 #pragma unroll
-            for (int p = 0; p < PIECES; ++p) {
-                const uint64_t b = (uint64_t)(uintptr_t)base[p];
-                i4v rsrc;
-                rsrc.x = __builtin_amdgcn_readfirstlane((int)(uint32_t)b);
-                rsrc.y = __builtin_amdgcn_readfirstlane((int)(uint32_t)(b >> 32) & 0xFFFF);
-                rsrc.z = -1;
-                rsrc.w = 0x00027000;
-                const uint32_t to = __builtin_amdgcn_readfirstlane(lds0 + (s % STAGES) * STAGE + (row0 + 16 * p) * 64);
-                const uint32_t v = s + 1 == S ? cut[p] : off[p], k = __builtin_amdgcn_readfirstlane(s + 1 == S ? 0u : 64 * s);
-                asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
-                             :: "s"(to), "v"(v), "s"(rsrc), "s"(k) : "memory");
-            }
-        };
-        i4v acc[FN][FT];
+        for (int p = 0; p < PIECES; ++p)
+            asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
+                         :: "s"(to + 1024 * p), "v"(from[p]), "s"(p / 2 ? b1 : b0), "s"(k) : "memory");
+    }
+    // Unit u of the tile: the weights of stage u / 2 or x. In the last stage pieces past K are the row's first (and count for nothing).
+    __device__ __forceinline__ void request(uint32_t u, uint32_t slot) {
+        const uint32_t s = u / 2;
+        if (s >= S) return;
+        const bool end = s + 1 == S && a.K % 128;
+        uint32_t from[PIECES];
 #pragma unroll
-        for (int i = 0; i < FN; ++i)
-#pragma unroll
-            for (int j = 0; j < FT; ++j) acc[i][j] = i4v{};
+        for (int p = 0; p < PIECES; ++p) {
+            const uint32_t k = 16 * piece(p);
+            from[p] = (u & 1 ? off_x[p] : off_w[p]) + (end ? (last + k < a.K ? last : 0u - k) : 128 * s);
+        }
+        load(from, u & 1 ? base_x : base_w[0], u & 1 ? base_x : base_w[1], slot, 0);
+    }
+
+    __device__ __forceinline__ void run(uint8_t* lds) {
         const uint32_t wn = wave % WN * (16 * FN), wt = wave / WN * (16 * FT);
+        const uint32_t tiles = a.tiles_t * a.tiles_n;
+        i4v acc[FN][FT], x[2][FT], w[2][FN];
+        auto fetch = [&](int b, uint32_t slot_w, uint32_t slot_x, uint32_t half) {
+            const uint8_t *pw = lds + slot_w * UNIT, *px = lds + slot_x * UNIT;
 #pragma unroll
-        for (uint32_t s = 0; s < STAGES - 1; ++s)
-            if (s < S) request(s);
-        for (uint32_t s = 0; s < S; ++s) {
-            // stage s is there (later ones may be on their way), and no wave still reads the one before it
-            if (s + 2 < S) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" :: "n"(2 * PIECES) : "memory");
-            else if (s + 1 < S) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" :: "n"(PIECES) : "memory");
-            else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-            if (s + STAGES - 1 < S) request(s + STAGES - 1);
-            uint8_t* stage = lds + (s % STAGES) * STAGE;
-            if (s + 1 == S && a.K % 64) {  // x past K becomes zeros
-                const uint32_t have = a.K % 64;
-                for (uint32_t i = tid; i < MT * 4; i += THREADS) {
-                    const uint32_t r = i / 4, c = i % 4;
-                    uint8_t* p = stage + MN * 64 + at(r, c);
+            for (int j = 0; j < FT; ++j) x[b][j] = *(const i4v*)(px + at(wt + 16 * j + m, 4 * half + kg));
 #pragma unroll
-                    for (uint32_t w = 0; w < 4; ++w) {
-                        const int32_t n = (int32_t)have - (int32_t)(16 * c + 4 * w);
-                        uint32_t* q = (uint32_t*)p + w;
-                        if (n < 4) *q = n <= 0 ? 0u : *q & ((1u << (8 * n)) - 1u);
-                    }
+            for (int i = 0; i < FN; ++i) w[b][i] = *(const i4v*)(pw + at(wn + 16 * i + m, 4 * half + kg));
+        };
+        auto multiply = [&](int b) {
+#pragma unroll
+            for (int i = 0; i < FN; ++i)
+#pragma unroll
+                for (int j = 0; j < FT; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w[b][i], x[b][j], acc[i][j], 0, 0, 0);
+        };
+        // x past K in the last stage becomes zeros
+        auto clear = [&](uint32_t slot) {
+            const uint32_t have = a.K - last;
+            if (have == 128) return;
+            for (uint32_t i = tid; i < MT * 8; i += THREADS) {
+                const uint32_t r = i / 8, c = i % 8;
+#pragma unroll
+                for (uint32_t d = 0; d < 4; ++d) {
+                    const int32_t n = (int32_t)have - (int32_t)(16 * c + 4 * d);
+                    uint32_t* q = (uint32_t*)(lds + slot * UNIT + at(r, c)) + d;
+                    if (n < 4) *q = n <= 0 ? 0u : *q & ((1u << (8 * n)) - 1u);
                 }
-                asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
             }
-            i4v x[FT];
+            asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        };
+        auto next = [](uint32_t slot, uint32_t by) { return slot + by >= UNITS ? slot + by - UNITS : slot + by; };
+
+        uint32_t id = blockIdx.x;
+        place(id);
+        for (uint32_t u = 0; u < UNITS; ++u) request(u, u);
+        while (true) {
 #pragma unroll
-            for (int j = 0; j < FT; ++j) x[j] = *(const i4v*)(stage + MN * 64 + at(wt + 16 * j + m, kg));
+            for (int i = 0; i < FN; ++i)
 #pragma unroll
-            for (int i = 0; i < FN; ++i) {
-                const i4v w = *(const i4v*)(stage + at(wn + 16 * i + m, kg));
-#pragma unroll
-                for (int j = 0; j < FT; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w, x[j], acc[i][j], 0, 0, 0);
+                for (int j = 0; j < FT; ++j) acc[i][j] = i4v{};
+            // stage 0 is there (its units are the oldest requests; stores of the tile before may be among the newer ones)
+            if (S > 2) asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" :: "n"(3 * PIECES) : "memory");
+            else if (S > 1) asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" :: "n"(2 * PIECES) : "memory");
+            else asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
+            if (S == 1) clear(1);
+            uint32_t at_w = 0, at_x = 1;  // slots of stage s
+            fetch(0, at_w, at_x, 0);
+            uint32_t s = 0;
+            // While a half is multiplied, the next one is read. At the barrier every wave has the whole of
+            // stage s in registers, stage s + 1 is there and the weights of s + 2 may be on their way; the two
+            // free slots take x of s + 2 and the weights of s + 3.
+            for (; s + 4 < S; ++s) {
+                fetch(1, at_w, at_x, 1);
+                multiply(0);
+                asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" :: "n"(PIECES) : "memory");
+                load(off_x, base_x, base_x, at_w, 128 * (s + 2));
+                load(off_w, base_w[0], base_w[1], at_x, 128 * (s + 3));
+                at_w = next(at_w, 2);
+                at_x = next(at_x, 2);
+                fetch(0, at_w, at_x, 0);
+                multiply(1);
             }
-        }
-#pragma unroll
-        for (int j = 0; j < FT; ++j) {
-            const uint32_t t = t0 + wt + 16 * j + m;
-            const float sx = a.xscale[min(t, a.T - 1u)];
-#pragma unroll
-            for (int i = 0; i < FN; i += GATED ? 2 : 1) {
-                const uint32_t n = n0 + (GATED ? (wn + 16 * i) / 2 : wn + 16 * i) + 4 * kg;
-                vx_i8_finish4<GATED>(a, t, n, sx, acc[i][j], GATED ? acc[i + 1][j] : i4v{}, vx_i8_scales4(a.wscale[0], n, a.N),
-                                     GATED ? vx_i8_scales4(a.wscale[1], n, a.N) : f4v{});
+            for (; s < S; ++s) {
+                fetch(1, at_w, at_x, 1);
+                multiply(0);
+                if (s + 1 < S) {
+                    if (s + 2 < S) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" :: "n"(PIECES) : "memory");
+                    else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+                    request(2 * s + 5, at_w);
+                    request(2 * s + 6, at_x);
+                    at_w = next(at_w, 2);
+                    at_x = next(at_x, 2);
+                    if (s + 2 == S) clear(at_x);
+                    fetch(0, at_w, at_x, 0);
+                }
+                multiply(1);
             }
+            // the results, under the first loads of the next tile (after the scales: loads end in order)
+            const uint32_t tt = t0 + wt + m, nn = n0 + (GATED ? wn / 2 : wn) + 4 * kg;
+            float sx[FT];
+            f4v sw[FN];
+#pragma unroll
+            for (int j = 0; j < FT; ++j) sx[j] = a.xscale[min(tt + 16 * j, a.T - 1u)];
+#pragma unroll
+            for (int i = 0; i < FN; ++i) sw[i] = vx_i8_scales4(a.wscale[GATED ? i & 1 : 0], nn + 16 * (GATED ? i / 2 : i), a.N);
+#pragma unroll
+            for (int j = 0; j < FT; ++j) asm volatile("" : "+v"(sx[j]));
+#pragma unroll
+            for (int i = 0; i < FN; ++i) asm volatile("" : "+v"(sw[i]));
+            id += gridDim.x;
+            const bool more = id < tiles;
+            asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+            if (more) {
+                place(id);
+                for (uint32_t u = 0; u < UNITS; ++u) request(u, u);
+            }
+#pragma unroll
+            for (int j = 0; j < FT; ++j)
+#pragma unroll
+                for (int i = 0; i < FN; i += GATED ? 2 : 1)
+                    vx_i8_finish4<GATED>(a, tt + 16 * j, nn + 16 * (GATED ? i / 2 : i), sx[j], acc[i][j], GATED ? acc[i + 1][j] : i4v{}, sw[i],
+                                         GATED ? sw[i + 1] : f4v{});
+            if (!more) break;
         }
     }
 };
 #define VX_I8_TILE(name, MT, MN, WT, WN, GATED)                                                  \
     extern "C" __global__ __launch_bounds__(64 * WT * WN) void name(vx_i8_args a) {              \
-        vx_i8_tile<MT, MN, WT, WN, GATED>::run(a);                                               \
+        using tile = vx_i8_tile<MT, MN, WT, WN, GATED>;                                          \
+        __shared__ __align__(1024) uint8_t lds[tile::UNIT * tile::UNITS];                        \
+        tile(a, lds).run(lds);                                                                   \
     }
 VX_I8_TILE(vx_i8_tile256, 256, 256, 2, 4, false)
 VX_I8_TILE(vx_i8_tile256_gated, 256, 256, 2, 4, true)

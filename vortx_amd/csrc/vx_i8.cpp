@@ -69,7 +69,7 @@ static uint64_t ws_bytes(uint32_t T, uint32_t K) { return own_x(T, K) ? 0 : up(K
 struct I8Plan {
     int kernel;
     uint32_t tokens, channels;  // of a workgroup
-    uint32_t block, lds;
+    uint32_t block, lds, grid;  // grid: most workgroups, each then has several tiles (0: one each)
 };
 static I8Plan plan_gemm(int num_cus, const vx_i8_args& a, bool gated) {
     const int g = gated ? 1 : 0;
@@ -81,13 +81,13 @@ static I8Plan plan_gemm(int num_cus, const vx_i8_args& a, bool gated) {
                                           {K_vx_i8_direct_t4, 4, {2, 1}}};
         const Direct& d = kDirect[a.xf ? 0 : a.T <= 16 ? 1 : a.T <= 32 ? 2 : 3];
         const uint32_t sums = std::min(d.tt * d.nt[g], gated ? 4u : 8u) * (gated ? 2 : 1);
-        return {d.kernel + g, 16 * d.tt, 16 * d.nt[g], 512, a.x_bytes + sums * 8192};
+        return {d.kernel + g, 16 * d.tt, 16 * d.nt[g], 512, a.x_bytes + sums * 8192, 0};
     }
     // tiles of 256 where they fill the card
     const uint32_t cn = gated ? 128 : 256;
     const uint64_t wide = (uint64_t)((a.T + 255) / 256) * ((a.N + cn - 1) / cn);
     const uint32_t side = wide * 2 > (uint64_t)num_cus ? 256 : 128;
-    return {(side == 256 ? K_vx_i8_tile256 : K_vx_i8_tile128) + g, side, gated ? side / 2 : side, 2 * side, 0};
+    return {(side == 256 ? K_vx_i8_tile256 : K_vx_i8_tile128) + g, side, gated ? side / 2 : side, 2 * side, 0, (uint32_t)num_cus * (side == 256 ? 1 : 2)};
 }
 
 static int run_gemm(vx_ctx ctx, vx_stream stream, const vx_mview* out, const vx_i8_rows* xq, const vx_cview* xf, const vx_i8_rows* w,
@@ -155,7 +155,8 @@ static int run_gemm(vx_ctx ctx, vx_stream stream, const vx_mview* out, const vx_
     a.tiles_n = (a.N - 1) / p.channels + 1;
     if ((uint64_t)a.tiles_t * a.tiles_n >= (1u << 22)) return fail(VX_ERR_UNSUPPORTED, "too many outputs (split the call)");
     if (xf && !own && (s = quantize(ctx, stream, &rows, x))) return s;
-    return launch_struct(ctx, p.kernel, a.tiles_t * a.tiles_n, p.block, stream, &a, p.lds);
+    const uint32_t tiles = a.tiles_t * a.tiles_n;
+    return launch_struct(ctx, p.kernel, p.grid ? std::min(tiles, p.grid) : tiles, p.block, stream, &a, p.lds);
 }
 
 }  // namespace vx
