@@ -478,7 +478,7 @@ typedef struct vx_rotation {
 } vx_rotation;
 
 /* q_out = q and k_out = k, [tokens, heads, dim] f32 views of any strides with
- * dims up to 256, normed and rotated (one launch). positions: device array
+ * dims up to 256, normed and rotated (one launch for up to 2^20 tokens). positions: device array
  * [tokens] (NULL if nothing is rotated). k_out and k may be NULL: queries
  * alone. An output is its input's view itself (in place) or lies apart from
  * all inputs. */

@@ -76,8 +76,14 @@ int main() {
         CHECK(rotate(how) == VX_OK && launches == 1);
         launches = 0;
         CHECK(vx_rotate(ctx, nullptr, &qo, &q, nullptr, nullptr, kPos, &how) == VX_OK && launches == 1);
+        q.layout.stride[0] += 1;
+        CHECK(rotate(how) == VX_OK && launches == 2);
         launches = 0;
     }
+    q = in_of((1u << 21) + 5, 1, 64), qo = out_of((1u << 21) + 5, 1, 64);  // in pieces
+    how.rotated = 64;
+    CHECK(vx_rotate(ctx, nullptr, &qo, &q, nullptr, nullptr, kPos, &how) == VX_OK && launches == 3);
+    launches = 0;
     q = in_of(0, 8, 64), qo = out_of(0, 8, 64), k = in_of(0, 2, 64), ko = out_of(0, 2, 64), how.rotated = 64;
     CHECK(rotate(how) == VX_OK && launches == 0);
     how.rotated = 0, how.freqs = nullptr;  // a norm alone
@@ -105,6 +111,13 @@ int main() {
                 q = in_of(5, 8, dim), qo = out_of(5, 8, dim), k = in_of(5, 2, dim), v = in_of(5, 2, dim);
                 CHECK(write(kPos) == VX_OK && launches == 1);
                 CHECK(vx_kv_write_rotated(ctx, nullptr, &c, nullptr, nullptr, &k, &v, kPos, kPos, &how) == VX_OK && launches == 2);
+                k.layout.stride[0] += 1;  // rows that are not aligned
+                CHECK(write(kPos) == VX_OK && launches == 3);
+                q = in_of(9000, 8, dim), qo = out_of(9000, 8, dim), k = in_of(9000, 2, dim), v = in_of(9000, 2, dim);
+                CHECK(write(kPos) == VX_OK && launches == 5);  // many: keys and values, then queries
+                CHECK(vx_kv_write_rotated(ctx, nullptr, &c, nullptr, nullptr, &k, &v, kPos, kPos, &how) == VX_OK && launches == 6);
+                k.layout.stride[0] += 1;
+                CHECK(write(kPos) == VX_OK && launches == 7);
                 launches = 0;
             }
     // ---- pages

@@ -7,7 +7,7 @@
 #define VX_CAT(f, types) VX_NAME(f, types)
 #define VX_KERNELS(types, KB, VB)                                                                              \
     extern "C" __global__ __launch_bounds__(256) void VX_CAT(kv_write, types)(vx_kv_rows_args a) {             \
-        vx_kv_write_rows<VX_NB, KB, VB>(a, vx_kv_keys{}, blockIdx.x, gridDim.x);                               \
+        vx_kv_write_rows<VX_NB, KB, VB>(a);                                                                    \
     }                                                                                                          \
     extern "C" __global__ __launch_bounds__(256) void VX_CAT(kv_read, types)(vx_kv_rows_args a) {              \
         vx_kv_read_rows<VX_NB, KB, VB>(a);                                                                     \

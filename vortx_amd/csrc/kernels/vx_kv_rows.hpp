@@ -200,40 +200,57 @@ __device__ __forceinline__ u2 vx_kv_v4(const uint32_t (&w)[4], int p) {
     return u2{c[0] | c[2] << 8 | c[1] << 16 | c[3] << 24, 0u};
 }
 
-// Where the keys of a row's lanes come from: as they are, or normed and rotated
-// (by all lanes of the row together).
+// Where the keys of a row's lanes come from: as they are, normed and rotated on the
+// way (by all lanes of the row together), or normed and rotated before, in LDS.
 struct vx_kv_keys {
     static constexpr bool TURNED = false;
 };
-template <int LANES>
+template <int LANES, bool VEC>
 struct vx_kv_turned_keys {
     static constexpr bool TURNED = true;
     const vx_rotate_args& a;
-    __device__ __forceinline__ f4 row(int64_t t, uint32_t h, uint32_t d) const {
+    const vx_angles& angles;
+    __device__ __forceinline__ f4 row(int64_t t, uint32_t h, uint32_t d) const { return row(vx_turn(a, angles, (uint32_t)t, d), t, h, d); }
+    __device__ __forceinline__ f4 row(vx_turn turn, int64_t t, uint32_t h, uint32_t d) const {
+        const vx_rotate_rows_args& k = a.part[1];
         vx_r4 x, y;
-        vx_rotate_load(a, a.x[1] + t * a.xs[1][0] + (int64_t)h * a.xs[1][1], a.xs[1][2], d, x, y);
-        const vx_turn turn(a, (uint32_t)t, d);
-        return vx_rotate_row<LANES>(a, turn, a.w[1] ? a.w[1] + (uint64_t)h * a.ws[1] : nullptr, d, x, y);
+        vx_rotate_load<VEC>(a, k.x + t * k.xs[0] + (int64_t)h * k.xs[1], k.xs[2], d, x, y);
+        if (k.w) {
+            vx_r4 wx, wy;
+            vx_rotate_load<VEC>(a, k.w + (uint64_t)h * k.ws, 1, d, wx, wy);
+            turn.weigh(a, wx, wy);
+        }
+        return vx_rotate_row<LANES, VEC>(a, turn, x, y);
     }
 };
+struct vx_kv_staged_keys {
+    static constexpr bool TURNED = true;
+    const float* rows;
+    uint32_t t0, h0, heads, dim;
+    __device__ __forceinline__ f4 row(int64_t t, uint32_t h, uint32_t d) const {
+        return d < dim ? *(const f4*)(rows + (((uint32_t)t - t0) * heads + (h - h0)) * dim + d) : f4{};
+    }
+};
+// Heads whose rows of eight tokens and three have room there.
+template <int NB>
+struct vx_kv_staged {
+    static constexpr uint32_t HEADS = VX_ROTATE_STAGE / (32 * NB * VX_ANGLE_TOKENS), FLOATS = HEADS * 32 * NB * VX_ANGLE_TOKENS,
+                              PLACES = VX_ANGLE_TOKENS * 16 * NB;
+};
 
-// Part `block` of `blocks`.
-template <int NB, int KB, int VB, class KEYS>
-__device__ __forceinline__ void vx_kv_write_rows(const vx_kv_rows_args& a, const KEYS& keys, uint32_t block, uint32_t blocks) {
+// A group of tokens' rows of head h, by the lanes (b, u) of a row. FOURS: groups may
+// be of four tokens.
+template <int NB, int KB, int VB, bool FOURS, class KEYS>
+__device__ __forceinline__ void vx_kv_write_unit(const vx_kv_rows_args& a, const KEYS& keys, uint32_t group, uint32_t h, uint32_t b, uint32_t u) {
     using R = vx_kv_rec<NB, KB, VB>;
     using PK = vx_kv_part<NB, KB>;
     using PV = vx_kv_part<NB, VB>;
     constexpr uint32_t NP = NB == 3 ? 4 : NB;  // lanes of a row: 8 NP, a power of two
-    const uint64_t units = (uint64_t)a.groups * a.c.heads * NP;
-    const uint32_t u = threadIdx.x & 7, b = (threadIdx.x >> 3) % NP;
-    for (uint64_t n = (uint64_t)block * 32 + (threadIdx.x >> 3); n < units; n += (uint64_t)blocks * 32) {
-        const uint64_t th = n / NP;
-        const uint32_t group = (uint32_t)(th / a.c.heads), h = (uint32_t)(th - (uint64_t)group * a.c.heads);
         const vx_kv_tokens run(a, group);
         const uint32_t d = 32 * b + 4 * u;
 #pragma unroll 1
         for (uint32_t i = 0; i < run.count; ++i) {  // (the same for the row's lanes)
-        const bool four = run.fours >> i & 1u;
+        const bool four = FOURS && run.fours >> i & 1u;
         if (!four && !(run.ones >> i & 1u)) continue;
         const int64_t t = run.first + i;
         const uint32_t slot = (uint32_t)a.slots[t];
@@ -302,7 +319,68 @@ __device__ __forceinline__ void vx_kv_write_rows(const vx_kv_rows_args& a, const
             rec[R::V_SIZES + m] = (uint8_t)size;
         }
         }
+}
+
+template <int NB, int KB, int VB>
+__device__ __forceinline__ void vx_kv_write_rows(const vx_kv_rows_args& a) {
+    constexpr uint32_t NP = NB == 3 ? 4 : NB;
+    const uint64_t units = (uint64_t)a.groups * a.c.heads * NP;
+    const uint32_t u = threadIdx.x & 7, b = (threadIdx.x >> 3) % NP;
+    for (uint64_t n = (uint64_t)blockIdx.x * 32 + (threadIdx.x >> 3); n < units; n += (uint64_t)gridDim.x * 32) {
+        const uint64_t th = n / NP;
+        const uint32_t group = (uint32_t)(th / a.c.heads), h = (uint32_t)(th - (uint64_t)group * a.c.heads);
+        vx_kv_write_unit<NB, KB, VB, true>(a, vx_kv_keys{}, group, h, b, u);
     }
+}
+
+// The same with keys that are normed and rotated on the way: workgroup `job` has
+// some tokens of some heads.
+template <int NB, int KB, int VB, int LANES, bool VEC>
+__device__ __forceinline__ void vx_kv_write_turned(const vx_kv_rows_args& a, const vx_rotate_args& r, uint32_t job, double2* lds) {
+    constexpr uint32_t ROWS = 256 / LANES;
+    const vx_rotate_rows_args& k = r.part[1];
+    const uint32_t u = threadIdx.x & 7, b = (threadIdx.x % LANES) >> 3, n = k.block_tokens;
+    const uint32_t t0 = job / k.chunks * n, h0 = job % k.chunks * k.run;
+    const vx_angles angles(r, lds, t0, n);
+    const vx_kv_turned_keys<LANES, VEC> keys{r, angles};
+    const uint32_t tokens = min(n, a.tokens - t0), heads = min(k.run, a.c.heads - h0);
+#pragma unroll 1
+    for (uint32_t i = threadIdx.x / LANES; i < tokens * heads; i += ROWS)
+        vx_kv_write_unit<NB, KB, VB, false>(a, keys, t0 + i % tokens, h0 + i / tokens, b, u);
+}
+
+// Many tokens: eight, and up to three that a group of four slots may reach past them,
+// turned into LDS first (the registers of a four and of a rotation together would
+// leave two waves a SIMD), then written by fours.
+template <int NB, int KB, int VB, int LANES>
+__device__ __forceinline__ void vx_kv_write_staged(const vx_kv_rows_args& a, const vx_rotate_args& r, uint32_t job, double2* lds, float* rows) {
+    constexpr uint32_t ROWS = 256 / LANES;
+    const vx_rotate_rows_args& k = r.part[1];
+    const uint32_t t0 = job / k.chunks * 8, h0 = job % k.chunks * k.run, heads = min(k.run, a.c.heads - h0);
+    const vx_angles angles(r, lds, t0, VX_ANGLE_TOKENS);
+    const vx_kv_turned_keys<LANES, true> keys{r, angles};
+    const uint32_t d = 4 * (threadIdx.x % LANES), g = threadIdx.x / LANES, tokens = min(VX_ANGLE_TOKENS, a.tokens - t0);
+    // a group of lanes has a token (with four groups: two) for all heads, and then some rows of the last three
+#pragma unroll 1
+    for (uint32_t i = g; i < min(8u, tokens); i += ROWS) {
+        const vx_turn turn(r, angles, t0 + i, d);
+#pragma unroll 1
+        for (uint32_t h = 0; h < heads; ++h) {
+            const f4 v = keys.row(turn, t0 + i, h0 + h, d);
+            if (d < 32 * NB) *(f4*)(rows + (i * heads + h) * 32 * NB + d) = v;
+        }
+    }
+#pragma unroll 1
+    for (uint32_t i = 8 * heads + g; i < tokens * heads; i += ROWS) {
+        const f4 v = keys.row(t0 + i / heads, h0 + i % heads, d);
+        if (d < 32 * NB) *(f4*)(rows + i * 32 * NB + d) = v;
+    }
+    __syncthreads();
+    const vx_kv_staged_keys staged{rows, t0, h0, heads, 32 * NB};
+    const uint32_t groups = min(2u, a.groups - t0 / 4);
+#pragma unroll 1
+    for (uint32_t i = threadIdx.x / LANES; i < groups * heads; i += ROWS)
+        vx_kv_write_unit<NB, KB, VB, true>(a, staged, t0 / 4 + i % groups, h0 + i / groups, (threadIdx.x % LANES) >> 3, threadIdx.x & 7);
 }
 
 __device__ __forceinline__ void vx_kv_set4(float* p, int64_t sd, uint32_t d, bool vec, f4 x) {

@@ -1,12 +1,13 @@
 // vx_rotate.hpp — rows of heads normed and rotated, four dims a lane.
 //
-// Everything between the load and the store is f64 and rounded once: a key's
-// codes in the cache follow from the result, and next to a border between two
-// codes f32 sums of another order would give another code. The f64 units carry
-// it: a value takes some 10 operations, 8000 tokens of 48 heads of 128 0.5 G of
-// them, 13 us of the card's f64 rate beside 80 us of HBM traffic. A row's dims lie in one
-// wave, which loads all of them (its partners' too) before it stores any, so a
-// row may be overwritten in place.
+// A workgroup has its tokens' angles in LDS for all its heads. Everything between the
+// load and the store is f64 and rounded once: a key's codes in the cache follow from
+// the result, and next to a border between two codes f32 sums of another order would
+// give another code. f64 multiply-adds run at f32's rate here, two thirds of the time
+// that the rows take from and to memory: 8000 tokens of 32 heads of 128, normed, 65 us,
+// 4.0 TB/s, where a large copy reaches 4.8. A row's dims lie in one wave, which loads
+// all of them (its partners' too) before it stores any, so a row may be overwritten in
+// place.
 #pragma once
 #include <hip/hip_runtime.h>
 #include <stdint.h>
@@ -47,6 +48,15 @@ __device__ __forceinline__ void vx_sin_cos(double a, double& s, double& c) {
     if ((k + 1) & 2) c = -c;
 }
 
+// 1 / sqrt(a), the instruction's estimate made better twice; 0 for infinity, NaN for 0.
+__device__ __forceinline__ double vx_inverse_root(double a) {
+    double y = __builtin_amdgcn_rsq(a);
+    const double h = 0.5 * a;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) y = y * __builtin_fma(-h * y, y, 1.5);
+    return a < __builtin_inf() ? y : a == a ? 0.0 : a;
+}
+
 template <int CTRL>
 __device__ __forceinline__ double vx_dpp64(double v) {
     const uint64_t u = __builtin_bit_cast(uint64_t, v);
@@ -66,117 +76,155 @@ __device__ __forceinline__ double vx_sum_lanes(double v) {
     return v;
 }
 
-// Cosines and signed sines of a lane's dims d .. d + 3: dim e becomes x[e] c[e] + partner s[e].
+// Cosines and sines of some tokens' pairs, in LDS: each is computed by one thread and
+// read by all heads. Pair i of a token lies at (i % 4) quarter + i / 4, so that lanes
+// with four neighbouring pairs each read neighbouring places.
+struct vx_angles {
+    double2* at;
+    uint32_t first, quarter;  // first token; a quarter of a token's places
+    // of n tokens (those past the last one: as the last)
+    __device__ __forceinline__ vx_angles(const vx_rotate_args& a, double2* lds, uint32_t t0, uint32_t n) : at(lds), first(t0), quarter((a.rotated / 2 + 3) / 4) {
+        const uint32_t half = a.rotated / 2;
+#pragma unroll 1
+        for (uint32_t j = threadIdx.x; j < n * half; j += 256) {
+            const uint32_t t = j / half, i = j - t * half;
+            const double pos = a.positions[min(t0 + t, a.tokens - 1u)];
+            double2 v;
+            vx_sin_cos(pos * a.freqs[i], v.y, v.x);
+            at[(t * 4 + i % 4) * quarter + i / 4] = v;
+        }
+        __syncthreads();
+    }
+    __device__ __forceinline__ double2 get(uint32_t t, uint32_t i) const { return at[((t - first) * 4 + i % 4) * quarter + i / 4]; }
+};
+constexpr uint32_t VX_ANGLE_TOKENS = 11;  // of a workgroup at most: eight, and three that a group of four may reach past them
+constexpr uint32_t VX_ANGLE_PLACES = VX_ANGLE_TOKENS * 128;
+#define VX_ROTATE_TOKENS(LANES) ((LANES) > 32 ? 4 : 8)  // of a workgroup, where there are many
+
+// What a lane's dims d .. d + 3 of a token are made of: dim e becomes (x[e] c[e] +
+// partner s[e]) times the row's norm, with the cosine and the signed sine times the norm weights.
 struct vx_turn {
     double c[4], s[4];
-    uint32_t on;  // bit e: dim d + e is rotated
-    __device__ __forceinline__ vx_turn(const vx_rotate_args& a, uint32_t t, uint32_t d) {
-        on = 0;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) c[e] = s[e] = 0;
-        if (d >= a.rotated) return;
-        const double pos = a.positions[t];
+    uint32_t on;  // bit e: dim d + e is rotated (otherwise the partner is left out: it may be infinite)
+    __device__ __forceinline__ vx_turn(const vx_rotate_args& a, const vx_angles& g, uint32_t t, uint32_t d) : on(0) {
         const uint32_t half = a.rotated / 2;
 #pragma unroll
         for (uint32_t e = 0; e < 4; ++e) {
-            if (a.pairs && (e & 1)) {  // (the pair's other half: d is a multiple of 4)
-                c[e] = c[e - 1];
-                s[e] = -s[e - 1];
-                if (d + e < a.rotated) on |= 1u << e;
-                continue;
-            }
+            c[e] = 1.0;
+            s[e] = 0.0;
             const uint32_t i = d + e;
             if (i >= a.rotated) continue;
-            const bool second = !a.pairs && i >= half;
-            vx_sin_cos(pos * a.freqs[a.pairs ? i / 2 : second ? i - half : i], s[e], c[e]);
-            if (!second) s[e] = -s[e];
             on |= 1u << e;
+            const bool second = a.pairs ? e & 1 : i >= half;  // (d is a multiple of 4)
+            const double2 v = g.get(t, a.pairs ? i / 2 : second ? i - half : i);
+            c[e] = v.x;
+            s[e] = second ? v.y : -v.y;
+        }
+    }
+    // times the weights of the dims and of their partners
+    __device__ __forceinline__ void weigh(const vx_rotate_args& a, vx_r4 x, vx_r4 y) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            c[e] *= x[e];
+            s[e] *= a.pairs ? x[e ^ 1] : y[e];
         }
     }
 };
 
-// Dims d .. d + 3 of a row at p (element stride sd) and, if nothing else holds them, their partners.
+// Dims d .. d + 3 of a row at p (element stride sd) and, if nothing else holds them,
+// their partners. VEC: fours of dims, and their partners, are 16-byte aligned everywhere.
+template <bool VEC>
 __device__ __forceinline__ void vx_rotate_load(const vx_rotate_args& a, const float* p, int64_t sd, uint32_t d, vx_r4& x, vx_r4& y) {
     x = y = vx_r4{};
     if (d >= a.dim) return;
     const uint32_t half = a.rotated / 2;
-    if (a.vec) {
+    if constexpr (VEC) {
         x = *(const vx_r4*)(p + d);
         if (!a.pairs && d < a.rotated) y = *(const vx_r4*)(p + (d < half ? d + half : d - half));
-        return;
-    }
+    } else {
 #pragma unroll
-    for (uint32_t e = 0; e < 4; ++e) {
-        const uint32_t i = d + e;
-        if (i >= a.dim) continue;
-        x[e] = p[i * sd];
-        if (!a.pairs && i < a.rotated) y[e] = p[(i < half ? i + half : i - half) * sd];
+        for (uint32_t e = 0; e < 4; ++e) {
+            const uint32_t i = d + e;
+            if (i >= a.dim) continue;
+            x[e] = p[i * sd];
+            if (!a.pairs && i < a.rotated) y[e] = p[(i < half ? i + half : i - half) * sd];
+        }
     }
 }
 
-// The row's dims d .. d + 3, of which x and the partners y are loaded; w: the row's norm weight or null.
-template <int LANES>
-__device__ __forceinline__ vx_r4 vx_rotate_row(const vx_rotate_args& a, const vx_turn& t, const float* w, uint32_t d, vx_r4 x, vx_r4 y) {
-    double v[4], u[4];
+// The row's dims d .. d + 3, of which x and the partners y are loaded. (VEC: all four are rotated or none.)
+template <int LANES, bool VEC>
+__device__ __forceinline__ vx_r4 vx_rotate_row(const vx_rotate_args& a, const vx_turn& t, vx_r4 x, vx_r4 y) {
+    double v[4], r[4];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) v[e] = x[e];
-    vx_r4 wx = {1.f, 1.f, 1.f, 1.f}, wy = wx;
-    if (w) {
-        int64_t one = 1;
-        vx_rotate_load(a, w, one, d, wx, wy);
+    for (int e = 0; e < 4; ++e) {
+        v[e] = x[e];
+        r[e] = v[e] * t.c[e];
+    }
+    if (VEC ? t.on != 0 : true) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (VEC || t.on >> e & 1u) r[e] = __builtin_fma(a.pairs ? v[e ^ 1] : (double)y[e], t.s[e], r[e]);
     }
     if (a.norm) {
         double m = 0;
 #pragma unroll
         for (int e = 0; e < 4; ++e) m = __builtin_fma(v[e], v[e], m);
-        const double inv = 1.0 / __builtin_sqrt(vx_sum_lanes<LANES>(m) / a.dim + (double)a.eps);
+        const double inv = vx_inverse_root(__builtin_fma(vx_sum_lanes<LANES>(m), a.per_dim, (double)a.eps));
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            v[e] = v[e] * inv * wx[e];
-            u[e] = y[e] * inv * wy[e];
-        }
-    } else {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) u[e] = y[e];
+        for (int e = 0; e < 4; ++e) r[e] *= inv;
     }
-    if (a.pairs) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) u[e] = v[e ^ 1];
-    }
-    vx_r4 r;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) r[e] = (float)(t.on >> e & 1u ? __builtin_fma(v[e], t.c[e], u[e] * t.s[e]) : v[e]);
-    return r;
+    return vx_r4{(float)r[0], (float)r[1], (float)r[2], (float)r[3]};
 }
 
+template <bool VEC>
 __device__ __forceinline__ void vx_rotate_store(const vx_rotate_args& a, float* p, int64_t sd, uint32_t d, vx_r4 r) {
     if (d >= a.dim) return;
-    if (a.vec) {
+    if constexpr (VEC) {
         *(vx_r4*)(p + d) = r;
-        return;
-    }
+    } else {
 #pragma unroll
-    for (uint32_t e = 0; e < 4; ++e)
-        if (d + e < a.dim) p[(d + e) * sd] = r[e];
+        for (uint32_t e = 0; e < 4; ++e)
+            if (d + e < a.dim) p[(d + e) * sd] = r[e];
+    }
 }
 
-// The rows of part `block` of a.blocks: a group of LANES lanes has a token's angles for a.run heads.
-template <int LANES>
-__device__ __forceinline__ void vx_rotate_rows(const vx_rotate_args& a, uint32_t block) {
+// Workgroup `job` of one part's rows: q.block_tokens tokens (one, or as many as a
+// workgroup has groups of LANES lanes, eight at most), q.run heads of them. A group has
+// one token, and two heads under way.
+template <int LANES, bool VEC>
+__device__ __forceinline__ void vx_rotate_rows(const vx_rotate_args& a, const vx_rotate_rows_args& q, uint32_t job, double2* lds) {
     constexpr uint32_t GROUPS = 256 / LANES;
-    const uint32_t d = 4 * (threadIdx.x % LANES), H = a.heads[0] + a.heads[1];
-    const uint64_t jobs = (uint64_t)a.tokens * a.chunks;
-    for (uint64_t n = (uint64_t)block * GROUPS + threadIdx.x / LANES; n < jobs; n += (uint64_t)a.blocks * GROUPS) {
-        const uint32_t t = (uint32_t)(n / a.chunks), h0 = (uint32_t)(n - (uint64_t)t * a.chunks) * a.run;
-        const vx_turn turn(a, t, d);
-        for (uint32_t h = h0; h < min(H, h0 + a.run); ++h) {
-            const uint32_t i = h >= a.heads[0], head = i ? h - a.heads[0] : h;
-            const float* p = a.x[i] + (int64_t)t * a.xs[i][0] + (int64_t)head * a.xs[i][1];
-            const float* w = a.w[i] ? a.w[i] + (uint64_t)head * a.ws[i] : nullptr;
-            vx_r4 x, y;
-            vx_rotate_load(a, p, a.xs[i][2], d, x, y);
-            const vx_r4 r = vx_rotate_row<LANES>(a, turn, w, d, x, y);
-            vx_rotate_store(a, a.y[i] + (int64_t)t * a.ys[i][0] + (int64_t)head * a.ys[i][1], a.ys[i][2], d, r);
+    const uint32_t d = 4 * (threadIdx.x % LANES), g = threadIdx.x / LANES, n = q.block_tokens;
+    const uint32_t t0 = job / q.chunks * n, h0 = job % q.chunks * q.run, end = min(h0 + q.run, q.heads);
+    const vx_angles angles(a, lds, t0, n);
+    const uint32_t t = t0 + (n > 1 ? g % VX_ROTATE_TOKENS(LANES) : 0u), step = n > 1 ? GROUPS / VX_ROTATE_TOKENS(LANES) : GROUPS;
+    if (t >= a.tokens) return;
+    vx_turn turn(a, angles, t, d);
+    vx_r4 wx, wy;
+    const bool each = q.w && q.ws;  // a weight for each head
+    if (q.w && !each) {
+        vx_rotate_load<VEC>(a, q.w, 1, d, wx, wy);
+        turn.weigh(a, wx, wy);
+    }
+    const float* p = q.x + t * q.xs[0];
+    float* o = q.y + t * q.ys[0];
+#pragma unroll 1
+    for (uint32_t h = h0 + (n > 1 ? g / VX_ROTATE_TOKENS(LANES) : g); h < end; h += 2 * step) {
+        vx_r4 x[2], y[2];
+#pragma unroll
+        for (uint32_t j = 0; j < 2; ++j)
+            if (h + j * step < end) vx_rotate_load<VEC>(a, p + (h + j * step) * q.xs[1], q.xs[2], d, x[j], y[j]);
+#pragma unroll
+        for (uint32_t j = 0; j < 2; ++j) {
+            const uint32_t k = h + j * step;
+            if (k >= end) continue;
+            vx_turn own = turn;
+            if (each) {
+                vx_rotate_load<VEC>(a, q.w + (uint64_t)k * q.ws, 1, d, wx, wy);
+                own.weigh(a, wx, wy);
+            }
+            vx_rotate_store<VEC>(a, o + k * q.ys[1], q.ys[2], d, vx_rotate_row<LANES, VEC>(a, own, x[j], y[j]));
         }
     }
 }

@@ -50,13 +50,15 @@ static int kernel_of(const vx_kv_cache* c, const int* d) {
     return d[dim_index(c->dim)] + (c->k_type == VX_Q4_0 ? 2 : 0) + (c->v_type == VX_Q4_0 ? 1 : 0);
 }
 #define VX_DIMS(f) {K_vx_##f##_d64_k8v8, K_vx_##f##_d96_k8v8, K_vx_##f##_d128_k8v8, K_vx_##f##_d256_k8v8}
-static const int kWrite[4] = VX_DIMS(kv_write), kRead[4] = VX_DIMS(kv_read), kWriteRotated[4] = VX_DIMS(rotate_kv), kEven16[4] = VX_DIMS(attn_even16),
+static const int kWrite[4] = VX_DIMS(kv_write), kRead[4] = VX_DIMS(kv_read), kRotateKv[4] = VX_DIMS(rotate_kv), kRotateKv4[4] = VX_DIMS(rotate_kv4), kEven16[4] = VX_DIMS(attn_even16),
                  kEach128[4] = VX_DIMS(attn_each128);
 #undef VX_DIMS
 #define VX_DIMS(f) {K_vx_##f##_d64_k8v8, K_vx_##f##_d96_k8v8, K_vx_##f##_d128_k8v8}
 static const int kJoin[4] = {K_vx_attn_join_d64, K_vx_attn_join_d96, K_vx_attn_join_d128, K_vx_attn_join_d256};
 static const int kEach256[3] = VX_DIMS(attn_each256);
 #undef VX_DIMS
+static const int kRotateKvStrided[4] = {K_vx_rotate_kv_d64_s_k8v8, K_vx_rotate_kv_d96_s_k8v8, K_vx_rotate_kv_d128_s_k8v8,
+                                        K_vx_rotate_kv_d256_s_k8v8};
 static const int kEvenTiles[4] = {K_vx_attn_even256_d64_k8v8, K_vx_attn_even256_d96_k8v8, K_vx_attn_even256_d128_k8v8,
                                   K_vx_attn_even128_d256_k8v8};
 
@@ -155,9 +157,10 @@ static int check_rotation(const vx_rotation* r, uint32_t dim) {
     return VX_OK;
 }
 
-// The arguments for rows q (0) and k (1); either view may be null, outputs too.
+// The arguments for rows q (0) and k (1); either view may be null, outputs too. vec:
+// fours of dims, and their partners, are 16-byte aligned everywhere.
 static int plan_rotation(const vx_mview* const (&outs)[2], const vx_cview* const (&ins)[2], uint32_t dim, const int32_t* positions,
-                         const vx_rotation* how, vx_rotate_args* a) {
+                         const vx_rotation* how, vx_rotate_args* a, bool* vec) {
     static const char* const names[2][2] = {{"q", "q_out"}, {"k", "k_out"}};
     int s = check_rotation(how, dim);
     if (s) return s;
@@ -167,31 +170,33 @@ static int plan_rotation(const vx_mview* const (&outs)[2], const vx_cview* const
     a->pairs = how->flags & VX_ROTATE_PAIRS ? 1 : 0;
     a->norm = norm;
     a->dim = dim;
+    a->per_dim = 1.0 / dim;
     a->rotated = how->rotated;
     a->eps = how->eps;
     a->freqs = how->freqs;
     a->positions = positions;
-    a->vec = dim % 4 == 0 && (a->pairs || how->rotated % 8 == 0);
+    *vec = dim % 4 == 0 && how->rotated % (a->pairs ? 4 : 8) == 0;
     bool first = true;
     for (int i = 0; i < 2; ++i) {
         if (!ins[i]) continue;
+        vx_rotate_rows_args& p = a->part[i];
         Rows r, o;
         if ((s = rows_view(ins[i]->base, &ins[i]->layout, dim, &r, names[i][0], false))) return s;
         if (!first && r.tokens != a->tokens) return fail(VX_ERR_SHAPE, "q and k have different tokens");
         first = false;
         a->tokens = r.tokens;
-        a->heads[i] = r.heads;
-        a->x[i] = (const float*)r.ptr;
-        a->w[i] = norm ? weights[i] : nullptr;
-        a->ws[i] = strides[i];
-        for (int j = 0; j < 3; ++j) a->xs[i][j] = r.stride[j];
-        if (!r.vec || (a->w[i] && (((uintptr_t)weights[i] & 15u) || strides[i] % 4))) a->vec = 0;
+        p.heads = r.heads;
+        p.x = (const float*)r.ptr;
+        p.w = norm ? weights[i] : nullptr;
+        p.ws = strides[i];
+        for (int j = 0; j < 3; ++j) p.xs[j] = r.stride[j];
+        if (!r.vec || (p.w && (((uintptr_t)weights[i] & 15u) || strides[i] % 4))) *vec = false;
         if (!outs[i]) continue;
         if ((s = rows_view(outs[i]->base, &outs[i]->layout, dim, &o, names[i][1], true))) return s;
         if (o.tokens != r.tokens || o.heads != r.heads) return fail(VX_ERR_SHAPE, i ? "k and k_out have different shapes" : "q and q_out have different shapes");
-        a->y[i] = (float*)o.ptr;
-        for (int j = 0; j < 3; ++j) a->ys[i][j] = o.stride[j];
-        if (!o.vec) a->vec = 0;
+        p.y = (float*)o.ptr;
+        for (int j = 0; j < 3; ++j) p.ys[j] = o.stride[j];
+        if (!o.vec) *vec = false;
     }
     if (how->rotated && a->tokens && (!positions || ((uintptr_t)positions & 3u)))
         return fail(VX_ERR_INVALID, "positions is null or not 4-byte aligned");
@@ -200,18 +205,34 @@ static int plan_rotation(const vx_mview* const (&outs)[2], const vx_cview* const
 
 static int lanes_index(uint32_t dim) { return dim <= 64 ? 0 : dim <= 128 ? 1 : 2; }
 
-// How many heads a group of lanes takes for one token's angles, and the workgroups.
-static void split_rotation(int num_cus, vx_rotate_args* a) {
-    const uint32_t heads = a->heads[0] + a->heads[1], groups = 16u >> lanes_index(a->dim);
-    const uint64_t rows = (uint64_t)a->tokens * heads;
-    if (!rows) {
-        a->run = a->chunks = a->blocks = 0;
-        return;
+// Tokens and heads of a workgroup: `many` tokens and as many heads as leave the card
+// full, whose angles are computed once for them; where there are few rows, one token
+// and as many heads as its lanes take at once.
+static void split_rows(int num_cus, uint32_t tokens, uint32_t dim, uint32_t many, vx_rotate_rows_args* p) {
+    p->block_tokens = p->run = p->chunks = p->blocks = 0;
+    if (!tokens || !p->heads) return;
+    const uint64_t at_once = 16u >> lanes_index(dim), rows = (uint64_t)tokens * p->heads;
+    p->block_tokens = rows / at_once >= (uint64_t)num_cus * 4 ? many : 1;
+    const uint64_t groups = ((uint64_t)tokens + p->block_tokens - 1) / p->block_tokens;
+    // (six workgroups a CU end about together, and each has its angles for more heads than with twelve: us, six / twelve /
+    // three, 4097 tokens of 32 heads of 80 19.7 / 23.8 / 19.8; 8000 of 32 of 128 65 / 63 / 66, of 8 into the cache 46 / 59 / 44)
+    const uint64_t most = std::max<uint64_t>(std::max<uint64_t>(1, at_once / p->block_tokens), groups * p->heads / ((uint64_t)num_cus * 6));
+    p->chunks = (uint32_t)((p->heads + most - 1) / most);
+    p->run = (p->heads + p->chunks - 1) / p->chunks;
+    p->chunks = (p->heads + p->run - 1) / p->run;
+    p->blocks = (uint32_t)(groups * p->chunks);
+}
+
+// One launch for tokens [t, t + n) of a part or of both: a workgroup is a job, so that
+// calls beyond a grid's size go in pieces.
+constexpr uint32_t VX_ROTATE_PIECE = 1u << 20;
+static void move_rows(vx_rotate_args* a, uint32_t tokens) {  // on by so many tokens
+    for (auto& p : a->part) {
+        if (p.x) p.x += p.xs[0] * tokens;
+        if (p.y) p.y += p.ys[0] * tokens;
     }
-    const uint64_t places = (uint64_t)num_cus * 8 * groups;  // rows under way with eight workgroups a CU
-    a->run = (uint32_t)std::min<uint64_t>(heads, std::max<uint64_t>(1, rows / places));
-    a->chunks = (heads + a->run - 1) / a->run;
-    a->blocks = (uint32_t)std::min<uint64_t>(((uint64_t)a->tokens * a->chunks + groups - 1) / groups, 1u << 20);
+    if (a->positions) a->positions += tokens;
+    a->tokens -= tokens;
 }
 
 static int run_rotate(vx_ctx ctx, vx_stream stream, const vx_mview* q_out, const vx_cview* q, const vx_mview* k_out, const vx_cview* k,
@@ -224,9 +245,16 @@ static int run_rotate(vx_ctx ctx, vx_stream stream, const vx_mview* q_out, const
     const uint32_t dim = c.l.size[3];
     if (dim == 0 || dim > 256) return fail(VX_ERR_UNSUPPORTED, "heads have 1 to 256 dims");
     vx_rotate_args a{};
-    if ((s = plan_rotation({q_out, k_out}, {q, k}, dim, positions, how, &a))) return s;
-    split_rotation(ctx_cus(ctx), &a);
-    return launch_struct(ctx, K_vx_rotate_l16 + lanes_index(dim), a.blocks, 256, stream, &a);
+    bool vec = false;
+    if ((s = plan_rotation({q_out, k_out}, {q, k}, dim, positions, how, &a, &vec))) return s;
+    while (a.tokens && !s) {
+        vx_rotate_args one = a;
+        one.tokens = std::min(a.tokens, VX_ROTATE_PIECE);
+        for (auto& p : one.part) split_rows(ctx_cus(ctx), one.tokens, dim, dim > 128 ? 4 : 8, &p);
+        s = launch_struct(ctx, (vec ? K_vx_rotate_l16 : K_vx_rotate_l16_s) + lanes_index(dim), one.part[0].blocks + one.part[1].blocks, 256, stream, &one);
+        move_rows(&a, one.tokens);
+    }
+    return s;
 }
 
 static int run_write_rotated(vx_ctx ctx, vx_stream stream, const vx_kv_cache* cache, const vx_mview* q_out, const vx_cview* q,
@@ -237,10 +265,33 @@ static int run_write_rotated(vx_ctx ctx, vx_stream stream, const vx_kv_cache* ca
     uint32_t grid = 0;
     int s = plan_rows(cache, k, v, slots, true, &a.r, &grid);
     if (s) return s;
-    if ((s = plan_rotation({q_out, nullptr}, {q, k}, cache->dim, positions, how, &a.t))) return s;
-    a.t.heads[1] = 0;  // (they are the writer's)
-    split_rotation(ctx_cus(ctx), &a.t);
-    return launch_struct(ctx, kernel_of(cache, kWriteRotated), a.t.blocks + grid, 256, stream, &a);
+    bool vec = false;
+    if ((s = plan_rotation({q_out, nullptr}, {q, k}, cache->dim, positions, how, &a.t, &vec))) return s;
+    if (!grid) a.t.part[1].heads = 0;  // (a cache without pages)
+    while (a.t.tokens && !s) {
+        vx_kv_rotated_args one = a;
+        vx_rotate_rows_args *qs = &one.t.part[0], *ks = &one.t.part[1];
+        one.r.tokens = one.t.tokens = std::min(a.t.tokens, VX_ROTATE_PIECE);
+        split_rows(ctx_cus(ctx), one.t.tokens, cache->dim, cache->dim > 128 ? 4 : 8, qs);
+        split_rows(ctx_cus(ctx), one.t.tokens, cache->dim, 8, ks);
+        one.r.quads = vec && ks->block_tokens == 8;
+        one.r.groups = one.r.quads ? (one.r.tokens - 1) / 4 + 1 : one.r.tokens;
+        if (one.r.quads) {
+            ks->run = std::min(ks->run, VX_ROTATE_STAGE / (cache->dim * 11u));
+            ks->chunks = (ks->heads + ks->run - 1) / ks->run;
+            ks->blocks = (one.t.tokens + 7) / 8 * ks->chunks;
+            s = launch_struct(ctx, kernel_of(cache, kRotateKv4), ks->blocks, 256, stream, &one);
+            ks->blocks = 0;
+            if (!s) s = launch_struct(ctx, K_vx_rotate_l16 + lanes_index(cache->dim), qs->blocks, 256, stream, &one.t);
+        } else {
+            s = launch_struct(ctx, kernel_of(cache, vec ? kRotateKv : kRotateKvStrided), qs->blocks + ks->blocks, 256, stream, &one);
+        }
+        move_rows(&a.t, one.t.tokens);
+        a.r.k += a.r.ks[0] * one.t.tokens;
+        a.r.v += a.r.vs[0] * one.t.tokens;
+        a.r.slots += one.t.tokens;
+    }
+    return s;
 }
 
 // Slots in the workgroup that deals out the pages, up to so many tokens.
@@ -278,7 +329,9 @@ static int run_resize(vx_ctx ctx, vx_stream stream, const vx_kv_pages* p, const 
     a.pages = p->pages;
     a.tokens = tokens;
     a.here = tokens <= VX_SLOTS_HERE;
-    if (const int s = launch_struct(ctx, K_vx_pages_resize, 1, 1024, stream, &a)) return s;
+    a.vec = (((uintptr_t)slots | (uintptr_t)positions) & 15u) == 0;
+    a.threads = p->seqs <= 256 && tokens <= 1024 ? 256 : 1024;
+    if (const int s = launch_struct(ctx, K_vx_pages_resize, 1, a.threads, stream, &a)) return s;
     return a.here ? VX_OK : launch_struct(ctx, K_vx_pages_slots, (tokens + 1023) / 1024, 256, stream, &a);
 }
 

@@ -144,24 +144,31 @@ typedef struct vx_kv_rows_args {
     uint32_t groups;       /* of tokens: one each, or four */
 } vx_kv_rows_args;
 
-/* Queries and keys, normed and rotated. [0] is of q, [1] of k. */
+/* Rows of heads, normed and rotated: the queries or the keys of a call. */
+typedef struct vx_rotate_rows_args {
+    const float* x;        /* element (t, h, d) at x[t*xs[0] + h*xs[1] + d*xs[2]] */
+    float* y;              /* (null: keys on their way into the cache) */
+    int64_t xs[3], ys[3];
+    const float* w;        /* norm weight of head h, dim d at w[h*ws + d]; null: 1 */
+    uint32_t ws;
+    uint32_t heads;
+    uint32_t block_tokens; /* tokens of a workgroup */
+    uint32_t run;          /* heads of a workgroup */
+    uint32_t chunks;       /* such runs a token */
+    uint32_t blocks;       /* workgroups */
+} vx_rotate_rows_args;
 typedef struct vx_rotate_args {
-    const float* x[2];     /* element (t, h, d) at x[t*xs[0] + h*xs[1] + d*xs[2]] */
-    float* y[2];           /* (y[1] null: k goes into the cache) */
-    int64_t xs[2][3], ys[2][3];
-    const float* w[2];     /* norm weight of head h, dim d at w[h*ws + d]; null: 1 */
+    vx_rotate_rows_args part[2];  /* queries, keys */
     const double* freqs;   /* [rotated / 2] */
     const int32_t* positions;
-    uint32_t ws[2];
-    uint32_t heads[2];
+    double per_dim;        /* 1 / dim */
     uint32_t tokens, dim, rotated;
     uint32_t pairs, norm;
     float eps;
-    uint32_t vec;          /* 1: fours of dims, and their partners, are 16-byte aligned everywhere */
-    uint32_t run;          /* heads a group of lanes takes one after the other */
-    uint32_t chunks;       /* such runs a token */
-    uint32_t blocks;       /* workgroups of this part (of vx_kv_write_rotated: the queries') */
 } vx_rotate_args;
+
+/* Floats of LDS for keys of eleven tokens that are turned before they are written. */
+#define VX_ROTATE_STAGE 6144
 
 /* Rows into the cache whose keys are normed and rotated on the way, and the queries beside them. */
 typedef struct vx_kv_rotated_args {
@@ -183,6 +190,8 @@ typedef struct vx_pages_args {
     uint32_t page_shift, pages;
     uint32_t tokens;       /* entries of slots and positions */
     uint32_t here;         /* 1: vx_pages_resize writes them, 0: vx_pages_slots after it */
+    uint32_t threads;      /* of vx_pages_resize: a multiple of 64 up to 1024 */
+    uint32_t vec;          /* 1: slots and positions are 16-byte aligned */
     uint32_t pad0;
 } vx_pages_args;
 
