@@ -648,9 +648,9 @@ int vx_i8_quantize(vx_ctx ctx, vx_stream stream, const vx_i8_rows* out, const vx
 int vx_gemm_i8(vx_ctx ctx, vx_stream stream, const vx_mview* out, const vx_i8_rows* x, const vx_i8_rows* w);
 
 /* The same of x as an f32 [T, K] view, whose rows become integers as
- * vx_i8_quantize makes them: for one or two tokens (rows of up to 32768 bytes in
- * all) inside the product, one launch, otherwise in `workspace` before it. workspace: device memory,
- * 16-byte aligned, at least vx_gemm_i8_ws_size bytes (VX_ERR_INVALID if not;
+ * vx_i8_quantize makes them: for one token (of up to 65536 values) and for up to
+ * four of 4096 or two of 8192 values inside the product, one launch, otherwise in
+ * `workspace` before it. workspace: device memory, 16-byte aligned, at least vx_gemm_i8_ws_size bytes (VX_ERR_INVALID if not;
  * NULL where none is needed); calls that share one must be ordered. */
 int vx_gemm_i8_x(vx_ctx ctx, vx_stream stream, const vx_mview* out, const vx_cview* x, const vx_i8_rows* w,
                  void* workspace, uint64_t workspace_bytes);

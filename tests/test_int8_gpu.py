@@ -134,7 +134,7 @@ def test_quantize(i8, rows, cols):
 
 
 @pytest.mark.parametrize("T,N,K", [(1, 100, 1), (1, 33, 63), (1, 512, 4096), (1, 70, 32768), (1, 70, 32769), (2, 40, 1000), (2, 48, 16384),
-                                   (2, 48, 16385), (3, 40, 1000), (16, 128, 4090), (40, 100, 515), (150, 200, 300), (513, 700, 129), (1, 16, 8191)])
+                                   (2, 48, 16385), (3, 40, 1000), (3, 1030, 129), (4, 700, 4096), (4, 50, 4097), (4, 300, 2049), (2, 90, 8192), (2, 5000, 8100), (3, 4300, 3333), (1, 70, 65536), (5, 40, 64), (1, 4200, 127), (16, 128, 4090), (40, 100, 515), (150, 200, 300), (513, 700, 129), (1, 16, 8191)])
 def test_f32_rows_are_quantized_as_by_themselves(i8, T, N, K):
     """Bit for bit the product of vx_i8_quantize's rows, also from rows that are not aligned or not contiguous."""
     note(f"f32 rows {T} x {N} x {K}")
@@ -272,25 +272,26 @@ def test_two_streams_and_a_graph(i8):
 
 
 def test_empty_and_refused(i8):
-    w, x = vx.Int8Rows.empty(32, 64), torch.zeros(4, 64, device=DEV)
+    w, x = vx.Int8Rows.empty(32, 64), torch.zeros(6, 64, device=DEV)  # (more tokens than go without a workspace)
     up = vx.Int8Rows.empty(32, 64)
-    ws = i8.workspace(4, 64)
+    ws = i8.workspace(6, 64)
+    assert [i8.workspace_size(*n) > 0 for n in ((4, 4096), (2, 8192), (1, 65536), (5, 128), (4, 4097), (2, 8193), (1, 65537))] == [False] * 3 + [True] * 4
     i8.dispatch(torch.empty(0, 32, device=DEV), torch.empty(0, 64, device=DEV), w)
-    i8.dispatch(torch.empty(4, 0, device=DEV), x, vx.Int8Rows.empty(0, 64), workspace=ws)
-    out = torch.empty(4, 32, device=DEV)
+    i8.dispatch(torch.empty(6, 0, device=DEV), x, vx.Int8Rows.empty(0, 64), workspace=ws)
+    out = torch.empty(6, 32, device=DEV)
     for call in [lambda: i8.dispatch(out, x, w),                                            # no workspace
                  lambda: i8.dispatch(out, x, w, workspace=ws[:16]),
                  lambda: i8.dispatch(out, x, w, workspace=torch.empty(4096, dtype=torch.uint8, device=DEV)[1:]),
                  lambda: i8.dispatch(out, x[:, :60], w, workspace=ws),
                  lambda: i8.dispatch(out[:, :31], x, w, workspace=ws),
                  lambda: i8.dispatch(out[:3], x, w, workspace=ws),
-                 lambda: i8.dispatch(out[:1].expand(4, 32), x, w, workspace=ws),
-                 lambda: i8.dispatch(out[None].expand(2, 4, 32), x, w, workspace=ws),
+                 lambda: i8.dispatch(out[:1].expand(6, 32), x, w, workspace=ws),
+                 lambda: i8.dispatch(out[None].expand(2, 6, 32), x, w, workspace=ws),
                  lambda: i8.dispatch_gated(out, x, w, up, "tanh", workspace=ws),
                  lambda: i8.dispatch_gated(out, x, w, vx.Int8Rows.empty(33, 64), workspace=ws),
                  lambda: i8.dispatch_gated(out, x, w, vx.Int8Rows.empty(32, 65), workspace=ws),
-                 lambda: i8.dispatch(out, torch.zeros(4, 0, device=DEV), vx.Int8Rows.empty(32, 0), workspace=ws),
-                 lambda: i8.dispatch(out, vx.Int8Rows.empty(4, 131072), vx.Int8Rows.empty(32, 131072)),
+                 lambda: i8.dispatch(out, torch.zeros(6, 0, device=DEV), vx.Int8Rows.empty(32, 0), workspace=ws),
+                 lambda: i8.dispatch(out, vx.Int8Rows.empty(6, 131072), vx.Int8Rows.empty(32, 131072)),
                  lambda: i8.quantize(w, x),
                  lambda: vx.Int8Rows(torch.zeros(4, 24, dtype=torch.int8, device=DEV), torch.zeros(3, device=DEV)),
                  lambda: vx.Int8Rows(torch.zeros(2, 20, dtype=torch.int8, device=DEV), torch.zeros(2, device=DEV)),   # the last row ends too early
@@ -298,7 +299,7 @@ def test_empty_and_refused(i8):
                  lambda: vx.Int8Rows(torch.zeros(4, 32, dtype=torch.int8, device=DEV), torch.zeros(4, device=DEV), 33)]:
         with pytest.raises(vx.VortxError):
             call()
-    odd = vx.Int8Rows(torch.zeros(4, 24, dtype=torch.int8, device=DEV), torch.zeros(4, device=DEV), 8)
+    odd = vx.Int8Rows(torch.zeros(6, 24, dtype=torch.int8, device=DEV), torch.zeros(6, device=DEV), 8)
     with pytest.raises(vx.VortxError):
         i8.quantize(odd, x[:, :8])
     for call in [lambda: i8.dispatch(out, x.double(), w, workspace=ws), lambda: i8.dispatch(out.half(), x, w, workspace=ws),

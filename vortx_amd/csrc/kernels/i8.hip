@@ -7,6 +7,17 @@
 // columns, so that a lane ends with four neighbouring channels of a token.
 #include "vx_i8.hpp"
 
+// The largest of the 64 lanes' numbers, by lane moves (lanes without a source take part with 0).
+__device__ __forceinline__ uint32_t vx_wave_max(uint32_t v) {
+    v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0xB1, 0xF, 0xF, false));
+    v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x4E, 0xF, 0xF, false));
+    v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x141, 0xF, 0xF, false));
+    v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x140, 0xF, 0xF, false));
+    v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x142, 0xA, 0xF, false));
+    v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x143, 0xC, 0xF, false));
+    return (uint32_t)__builtin_amdgcn_readlane((int)v, 63);
+}
+
 // ---------------------------------------------------------------- quantize
 // A workgroup a row. C fours of each thread stay in registers between the two
 // passes over a row (its largest value, its codes); what is longer is read again.
@@ -30,8 +41,7 @@ __device__ __forceinline__ void vx_i8_quantize_row(const vx_i8_quant_args& a, ui
     } else {
         for (uint32_t k = tid; k < K; k += 256) m = max(m, vx_abs_bits(p[(int64_t)k * a.xs[1]]));
     }
-#pragma unroll
-    for (int o = 32; o; o >>= 1) m = max(m, (uint32_t)__shfl_xor((int)m, o));
+    m = vx_wave_max(m);
     if ((tid & 63) == 0) part[tid >> 6] = m;
     __syncthreads();
     m = max(max(part[0], part[1]), max(part[2], part[3]));
@@ -68,13 +78,15 @@ __device__ __forceinline__ uint32_t vx_xcd_order(uint32_t id, uint32_t n) {
     return x * each + min(x, more) + i;
 }
 
+// A barrier for what is in LDS: loads from memory stay on their way.
+__device__ __forceinline__ void vx_lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+
 // ---------------------------------------------------------------- few tokens
 // TT x 16 tokens by NT x 16 channels (of each matrix) a workgroup of eight waves,
 // which have K's pieces of 64 U bytes in turn, straight from memory to the matrix
-// cores; their sums meet in LDS at the end. Bound by W's bytes. F32X: x comes as f32
-// (its tokens at most 16) and every workgroup quantizes it for itself into LDS,
-// under its first loads of W, which saves the launch that would do it.
-template <int TT, int NT, int U, bool GATED, bool F32X>
+// cores; their sums meet in LDS at the end. Bound by what a CU takes from L2 and
+// memory.
+template <int TT, int NT, int U, bool GATED>
 struct vx_i8_direct {
     static constexpr int G = GATED ? 2 : 1, A = NT * G;
     i4v wr[2][U][A], xr[2][U][TT];
@@ -100,11 +112,8 @@ struct vx_i8_direct {
             const uint32_t n = min(n0 + 16u * (i / G) + m, a.N - 1u);
             wp[i] = a.w[i % G] + (uint64_t)n * a.ws[i % G] + 16 * kg;
         }
-        if constexpr (!F32X)
 #pragma unroll
-            for (int j = 0; j < TT; ++j) xp[j] = a.x + (uint64_t)min(t0 + 16u * j + m, a.T - 1u) * a.xs + 16 * kg;
-        const uint32_t pitch = a.pitch;  // of x's rows in LDS
-        const uint8_t* xl = lds + min(m, a.T - 1u) * pitch + 16 * kg;
+        for (int j = 0; j < TT; ++j) xp[j] = a.x + (uint64_t)min(t0 + 16u * j + m, a.T - 1u) * a.xs + 16 * kg;
 #pragma unroll
         for (int i = 0; i < A; ++i)
 #pragma unroll
@@ -116,16 +125,14 @@ struct vx_i8_direct {
             for (int u = 0; u < U; ++u)
 #pragma unroll
                 for (int i = 0; i < A; ++i) wr[b][u][i] = *(const i4v*)(wp[i] + (uint64_t)c * P + 64 * u);
-            if constexpr (!F32X)
 #pragma unroll
-                for (int u = 0; u < U; ++u)
+            for (int u = 0; u < U; ++u)
 #pragma unroll
-                    for (int j = 0; j < TT; ++j) xr[b][u][j] = *(const i4v*)(xp[j] + (uint64_t)c * P + 64 * u);
+                for (int j = 0; j < TT; ++j) xr[b][u][j] = *(const i4v*)(xp[j] + (uint64_t)c * P + 64 * u);
         };
-        auto multiply = [&](int b, uint32_t c) {
+        auto multiply = [&](int b) {
 #pragma unroll
             for (int u = 0; u < U; ++u) {
-                if constexpr (F32X) xr[b][u][0] = *(const i4v*)(xl + c * P + 64 * u);
 #pragma unroll
                 for (int i = 0; i < A; ++i)
 #pragma unroll
@@ -134,13 +141,11 @@ struct vx_i8_direct {
             }
         };
         if (wave < full) load(0, wave);
-        float* sx = nullptr;
-        if constexpr (F32X) sx = quantize(a, lds);
         for (uint32_t c = wave; c < full; c += 16) {
             if (c + 8 < full) load(1, c + 8);
-            multiply(0, c);
+            multiply(0);
             if (c + 16 < full) load(0, c + 16);
-            if (c + 8 < full) multiply(1, c + 8);
+            if (c + 8 < full) multiply(1);
         }
         // the rest of K, 64 bytes a wave; nothing past the 16 bytes that K ends in is read
         const uint32_t left = a.K - full * P;
@@ -151,10 +156,7 @@ struct vx_i8_direct {
 #pragma unroll
             for (int i = 0; i < A; ++i) w[i] = *(const i4v*)(wp[i] + (have > 0 ? (int64_t)k : -16 * (int64_t)kg));
 #pragma unroll
-            for (int j = 0; j < TT; ++j) {
-                if constexpr (F32X) x[j] = *(const i4v*)(xl + k);  // (zeros past K)
-                else x[j] = masked(*(const i4v*)(xp[j] + (have > 0 ? (int64_t)k : -16 * (int64_t)kg)), have);
-            }
+            for (int j = 0; j < TT; ++j) x[j] = masked(*(const i4v*)(xp[j] + (have > 0 ? (int64_t)k : -16 * (int64_t)kg)), have);
 #pragma unroll
             for (int i = 0; i < A; ++i)
 #pragma unroll
@@ -162,7 +164,7 @@ struct vx_i8_direct {
         }
         // the eight waves' sums, eight fragments (of a product, or pairs of two) a round
         constexpr int F = NT * TT, R = GATED ? 4 : 8;
-        i4v* sums = (i4v*)(lds + (F32X ? a.x_bytes : 0));
+        i4v* sums = (i4v*)lds;
 #pragma unroll
         for (int f0 = 0; f0 < F; f0 += R) {
             if (f0) __syncthreads();
@@ -179,68 +181,267 @@ struct vx_i8_direct {
 #pragma unroll
                     for (int v = 0; v < 8; ++v) s[g] += sums[((wave * G + g) * 8 + v) * 64 + lane];
                 const uint32_t t = t0 + 16 * (f % TT) + m, n = n0 + 16 * (f / TT) + 4 * kg;
-                const float scale = F32X ? sx[min(m, a.T - 1u)] : a.xscale[min(t, a.T - 1u)];
-                vx_i8_finish4<GATED>(a, t, n, scale, s[0], s[1], vx_i8_scales4(a.wscale[0], n, a.N),
+                vx_i8_finish4<GATED>(a, t, n, a.xscale[min(t, a.T - 1u)], s[0], s[1], vx_i8_scales4(a.wscale[0], n, a.N),
                                      GATED ? vx_i8_scales4(a.wscale[1], n, a.N) : f4v{});
             }
         }
     }
-
-    // x's rows as codes in LDS, zeros from K to the next multiple of 64; returns their scales.
-    static __device__ __forceinline__ float* quantize(const vx_i8_args& a, uint8_t* lds) {
-        const uint32_t tid = threadIdx.x, K = a.K;
-        uint32_t* part = (uint32_t*)(lds + a.T * a.pitch);
-        float* sx = (float*)(part + 8 * 16);
-        const bool vec = a.xf_vec;
-        auto get = [&](const float* p, uint32_t k) {
-            f4v v = {};
-            if (vec && k + 4 <= K) return *(const f4v*)(p + k);
-#pragma unroll
-            for (uint32_t i = 0; i < 4; ++i)
-                if (k + i < K) v[i] = p[(int64_t)(k + i) * a.xfs[1]];
-            return v;
-        };
-        for (uint32_t t = 0; t < a.T; ++t) {
-            const float* p = a.xf + (int64_t)t * a.xfs[0];
-            uint32_t m = 0;
-#pragma unroll 4
-            for (uint32_t k = 4 * tid; k < K; k += 2048) m = vx_max4(m, get(p, k));
-#pragma unroll
-            for (int o = 32; o; o >>= 1) m = max(m, (uint32_t)__shfl_xor((int)m, o));
-            if ((tid & 63) == 0) part[t * 8 + (tid >> 6)] = m;
-        }
-        __syncthreads();
-        const uint32_t end = (K + 63) / 64 * 64;
-        for (uint32_t t = 0; t < a.T; ++t) {
-            uint32_t m = 0;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) m = max(m, part[t * 8 + i]);
-            float r;
-            const float d = vx_i8_scale(m, r);
-            if (tid == 0) sx[t] = d;
-            const float* p = a.xf + (int64_t)t * a.xfs[0];
-#pragma unroll 4
-            for (uint32_t k = 4 * tid; k < end; k += 2048) *(uint32_t*)(lds + t * a.pitch + k) = k < K ? vx_i8_codes(get(p, k), r) : 0u;
-        }
-        __syncthreads();
-        return sx;
-    }
 };
 
 extern __shared__ __align__(16) uint8_t vx_i8_lds[];
-#define VX_I8_DIRECT(name, TT, NT, U, GATED, F32X)                                   \
+#define VX_I8_DIRECT(name, TT, NT, U, GATED)                                         \
     extern "C" __global__ __launch_bounds__(512) void name(vx_i8_args a) {           \
-        vx_i8_direct<TT, NT, U, GATED, F32X> d;                                      \
+        vx_i8_direct<TT, NT, U, GATED> d;                                            \
         d.run(a, vx_i8_lds);                                                         \
     }
-VX_I8_DIRECT(vx_i8_direct_x, 1, 1, 4, false, true)
-VX_I8_DIRECT(vx_i8_direct_x_gated, 1, 1, 4, true, true)
-VX_I8_DIRECT(vx_i8_direct_t1, 1, 1, 4, false, false)
-VX_I8_DIRECT(vx_i8_direct_t1_gated, 1, 1, 4, true, false)
-VX_I8_DIRECT(vx_i8_direct_t2, 2, 2, 2, false, false)
-VX_I8_DIRECT(vx_i8_direct_t2_gated, 2, 1, 2, true, false)
-VX_I8_DIRECT(vx_i8_direct_t4, 4, 2, 2, false, false)
-VX_I8_DIRECT(vx_i8_direct_t4_gated, 4, 1, 2, true, false)
+VX_I8_DIRECT(vx_i8_direct_t1, 1, 1, 2, false)
+VX_I8_DIRECT(vx_i8_direct_t1_gated, 1, 1, 4, true)
+VX_I8_DIRECT(vx_i8_direct_t2, 2, 2, 2, false)
+VX_I8_DIRECT(vx_i8_direct_t2_gated, 2, 1, 2, true)
+VX_I8_DIRECT(vx_i8_direct_t4, 4, 2, 2, false)
+VX_I8_DIRECT(vx_i8_direct_t4_gated, 4, 1, 2, true)
+VX_I8_DIRECT(vx_i8_direct_t4_wide, 4, 4, 1, false)
+VX_I8_DIRECT(vx_i8_direct_t4_wide_gated, 4, 2, 1, true)
+
+// ---------------------------------------------------------------- one to four tokens of f32
+// A workgroup of 16 waves a CU. A wave reads a row of the weights as it lies in memory,
+// 1 KB a load and four loads a step (of a gated product a row of each), DEPTH steps ahead
+// over the ends of its rows, against x's codes in LDS on the dot-product units; a.split
+// waves share a row where there are fewer rows than waves. x is quantized into LDS by
+// each workgroup for itself, under its first loads, which saves the launch that would
+// do it. Bound by HBM, the weights' bytes, and what a launch takes to begin; a step is
+// kept short, because with 100 instructions more a kilobyte their issue was the bound
+// (STREAM_NUMBERS).
+template <int TT, bool GATED, int DEPTH>
+struct vx_i8_stream {
+    static constexpr int G = GATED ? 2 : 1;
+
+    // What a thread has of x: four values of every 4096 of a row, row after row; of a few they stay in registers.
+    static constexpr uint32_t KEEP = 4;
+    f4v kept[KEEP];
+    static __device__ __forceinline__ f4v get(const vx_i8_args& a, uint32_t t, uint32_t k) {
+        const float* p = a.xf + (int64_t)t * a.xfs[0];
+        f4v v = {};
+        if (a.xf_vec && k + 4 <= a.K) return *(const f4v*)(p + k);
+#pragma unroll
+        for (uint32_t i = 0; i < 4; ++i)
+            if (k + i < a.K) v[i] = p[(int64_t)(k + i) * a.xfs[1]];
+        return v;
+    }
+    __device__ __forceinline__ void keep(const vx_i8_args& a, uint32_t each) {  // each: such fours of a row
+#pragma unroll
+        for (uint32_t j = 0; j < KEEP; ++j)
+            if (j < each * a.T) kept[j] = get(a, j / each, (j % each) * 4096 + 4 * threadIdx.x);
+    }
+    // x's rows as codes in LDS, zeros from K to the next multiple of 4096; returns their scales.
+    __device__ __forceinline__ const float* quantize(const vx_i8_args& a, uint8_t* lds, uint32_t each) {
+        const uint32_t tid = threadIdx.x, end = (a.K + 4095) / 4096 * 4096;
+        uint32_t* part = (uint32_t*)(lds + a.T * a.pitch);
+        float* sx = (float*)(part + VX_I8_OWN_TOKENS * 16);
+        const bool few = each * a.T <= KEEP;
+        for (uint32_t t = 0; t < a.T; ++t) {
+            uint32_t m = 0;
+            if (few) {
+#pragma unroll
+                for (uint32_t j = 0; j < KEEP; ++j)
+                    if (j / each == t) m = vx_max4(m, kept[j]);
+            } else {
+                for (uint32_t k = 4 * tid; k < a.K; k += 4096) m = vx_max4(m, get(a, t, k));
+            }
+            m = vx_wave_max(m);
+            if ((tid & 63) == 0) part[t * 16 + (tid >> 6)] = m;
+        }
+        vx_lds_barrier();
+        for (uint32_t t = 0; t < a.T; ++t) {
+            uint32_t m = 0;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) m = max(m, part[t * 16 + i]);
+            float r;
+            const float d = vx_i8_scale(m, r);
+            if (tid == 0) sx[t] = d;
+            auto put = [&](uint32_t k, f4v v) {
+                if (k < end) *(uint32_t*)(lds + t * a.pitch + k) = k < a.K ? vx_i8_codes(v, r) : 0u;
+            };
+            if (few) {
+#pragma unroll
+                for (uint32_t j = 0; j < KEEP; ++j)
+                    if (j / each == t) put((j % each) * 4096 + 4 * tid, kept[j]);
+            } else {
+                for (uint32_t k = 4 * tid; k < end; k += 4096) put(k, get(a, t, k));
+            }
+        }
+        vx_lds_barrier();
+        return sx;
+    }
+
+    static __device__ __forceinline__ int wave_sum(int v) {
+        v += __builtin_amdgcn_update_dpp(0, v, 0xB1, 0xF, 0xF, false);
+        v += __builtin_amdgcn_update_dpp(0, v, 0x4E, 0xF, 0xF, false);
+        v += __builtin_amdgcn_update_dpp(0, v, 0x141, 0xF, 0xF, false);
+        v += __builtin_amdgcn_update_dpp(0, v, 0x140, 0xF, 0xF, false);
+        v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);
+        v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);
+        return __builtin_amdgcn_readlane(v, 63);
+    }
+
+    i4v w[DEPTH][G][4];
+    int acc[G][TT];
+    float sw[G];       // the row's scales
+    uint32_t part[4];  // where this lane's pieces of a row's last step lie
+
+    __device__ __forceinline__ void load(const vx_i8_args& a, int b, uint32_t row, uint32_t c, bool last) {
+        row = min(row, a.N - 1u);
+#pragma unroll
+        for (int g = 0; g < G; ++g) {
+            const int8_t* p = a.w[g] + (uint64_t)row * a.ws[g] + 4096 * c;
+            if (last) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) w[b][g][i] = *(const i4v*)(p + part[i]);
+            } else {
+                const uint32_t at = 16 * (threadIdx.x & 63);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) w[b][g][i] = *(const i4v*)(p + at + 1024 * i);
+            }
+        }
+    }
+    __device__ __forceinline__ void multiply(const uint8_t* x, uint32_t pitch, int b) {
+#pragma unroll
+        for (int t = 0; t < TT; ++t)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const i4v v = *(const i4v*)(x + t * pitch + 1024 * i);
+#pragma unroll
+                for (int g = 0; g < G; ++g)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) acc[g][t] = __builtin_amdgcn_sdot4(w[b][g][i][j], v[j], acc[g][t], false);
+            }
+    }
+    // by scalar loads: the weights' loads are not waited for with them
+    __device__ __forceinline__ void scales(const vx_i8_args& a, uint32_t row) {
+        typedef const __attribute__((address_space(4))) float* scalars;
+#pragma unroll
+        for (int g = 0; g < G; ++g) sw[g] = ((scalars)(uintptr_t)a.wscale[g])[min(row, a.N - 1u)];
+    }
+    // The row's end: its sums meet, lane t writes token t's value.
+    __device__ __forceinline__ void finish(const vx_i8_args& a, int* sums, uint32_t wave, uint32_t share, uint32_t row, uint32_t round, vx_i8_scaled x) {
+        const uint32_t lane = threadIdx.x & 63;
+        int s[G];
+#pragma unroll
+        for (int g = 0; g < G; ++g) {
+            s[g] = 0;
+#pragma unroll
+            for (int t = 0; t < TT; ++t) {
+                const int v = wave_sum(acc[g][t]);
+                if (lane == (uint32_t)t) s[g] = v;
+                acc[g][t] = 0;
+            }
+        }
+        if (a.split > 1) {  // (two places in turn: a place is written again behind the barrier after its reading)
+            int* at = sums + round % 2 * (16 * G * TT);
+#pragma unroll
+            for (int g = 0; g < G; ++g)
+                if (lane < TT) at[(wave * G + g) * TT + lane] = s[g];
+            vx_lds_barrier();
+#pragma unroll
+            for (int g = 0; g < G; ++g) {
+                s[g] = 0;
+                for (uint32_t v = 0; v < a.split; ++v) s[g] += at[((wave - share + v) * G + g) * TT + min(lane, TT - 1u)];
+            }
+        }
+        if (share == 0 && lane < a.T && row < a.N) {
+            float v = vx_i8_value(s[0], x, vx_i8_scaled(sw[0]));
+            if constexpr (GATED) v = vx_act(a.act, v) * vx_i8_value(s[1], x, vx_i8_scaled(sw[1]));
+            a.out[lane * a.os[0] + row * a.os[1]] = v;
+        }
+    }
+
+    __device__ __forceinline__ void run(const vx_i8_args& a, uint8_t* lds) {
+        const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+        const uint32_t per = 16 / a.split, share = wave % a.split;  // rows of a workgroup at a time; which part of its row
+        const uint32_t hop = a.tiles_n * per, rounds = (a.N + hop - 1) / hop;
+        const uint32_t fours = (a.K + 4095) / 4096, steps = (fours + a.split - 1) / a.split;  // of a row, and of a wave's share
+#pragma unroll
+        for (uint32_t i = 0; i < 4; ++i) {
+            const uint32_t at = 1024 * i + 16 * lane;
+            part[i] = (fours - 1) * 4096 + at < a.K ? at : 0u;  // (past K: something of the row, times zeros)
+        }
+#pragma unroll
+        for (int g = 0; g < G; ++g)
+#pragma unroll
+            for (int t = 0; t < TT; ++t) acc[g][t] = 0;
+        // Loads arrive in the order of their requests: x goes before the weights, so that it is quantized while those
+        // are on their way.
+        if (fours * a.T <= KEEP) keep(a, fours);
+        asm volatile("" ::: "memory");
+        uint32_t row = blockIdx.x * per + wave / a.split, c = share, round = 0;  // the step at hand: 4096 bytes c of a row
+        uint32_t row_l = row, c_l = share;                                      // and the next one to request
+        // (past a row's share: its last ones again, and nothing comes of it; past the last row, the last row)
+        auto request = [&](int b) {
+            const uint32_t k = min(c_l, fours - 1u);
+            load(a, b, row_l, k, k + 1 == fours);
+            if ((c_l += a.split) >= steps * a.split) c_l = share, row_l = min(row_l + hop, a.N);
+        };
+        const uint32_t all = rounds * steps;
+        const bool few = all < DEPTH;
+        const float* sx;
+        if (few) {
+            request(0);
+            asm volatile("" ::: "memory");
+            sx = quantize(a, lds, fours);
+        } else {
+#pragma unroll
+            for (int b = 0; b < DEPTH; ++b) request(b);
+            asm volatile("" ::: "memory");
+            sx = quantize(a, lds, fours);
+        }
+        const vx_i8_scaled scale(sx[min(lane, a.T - 1u)]);
+        int* sums = (int*)(lds + a.x_bytes);  // [2][16 waves][G][TT], of rows that waves share
+        auto take = [&](int b) {
+            if (c < fours) multiply(lds + 16 * lane + 4096 * c, a.pitch, b);
+            if ((c += a.split) < steps * a.split) return;
+            finish(a, sums, wave, share, row, round, scale);
+            c = share;
+            row += hop;
+            ++round;
+            scales(a, row);
+        };
+        scales(a, row);
+        if (few) {
+            for (uint32_t q = 0; q < all; ++q) {
+                take(0);
+                if (q + 1 < all) request(0);
+            }
+            return;
+        }
+        uint32_t q = 0;
+        for (; q + 2 * DEPTH <= all; q += DEPTH)
+#pragma unroll
+            for (int b = 0; b < DEPTH; ++b) {
+                take(b);
+                request(b);
+            }
+        const uint32_t left = all - q;  // DEPTH to 2 DEPTH - 1, the first DEPTH of them requested
+#pragma unroll
+        for (int b = 0; b < DEPTH; ++b) {
+            take(b);
+            if ((uint32_t)b + DEPTH < left) request(b);
+        }
+#pragma unroll
+        for (int b = 0; b < DEPTH; ++b)
+            if ((uint32_t)b + DEPTH < left) take(b);
+    }
+};
+#define VX_I8_STREAM(name, TT, GATED, DEPTH)                                         \
+    extern "C" __global__ __launch_bounds__(1024) void name(vx_i8_args a) {          \
+        vx_i8_stream<TT, GATED, DEPTH> s;                                            \
+        s.run(a, vx_i8_lds);                                                         \
+    }
+VX_I8_STREAM(vx_i8_stream_t1, 1, false, 2)
+VX_I8_STREAM(vx_i8_stream_t1_gated, 1, true, 1)
+VX_I8_STREAM(vx_i8_stream_t2, 2, false, 2)
+VX_I8_STREAM(vx_i8_stream_t2_gated, 2, true, 1)
+VX_I8_STREAM(vx_i8_stream_t4, 4, false, 2)
+VX_I8_STREAM(vx_i8_stream_t4_gated, 4, true, 1)
 
 // ---------------------------------------------------------------- many tokens
 // Tiles of MT tokens by MN rows of weights (of a gated product half gate, half up,
@@ -353,6 +554,15 @@ struct vx_i8_tile {
             }
             asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
         };
+        // all units but the last n requested are there, for all waves
+        auto arrived = [](uint32_t n) {
+            switch (n) {
+                case 3: asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" :: "n"(3 * PIECES) : "memory"); break;
+                case 2: asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" :: "n"(2 * PIECES) : "memory"); break;
+                case 1: asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" :: "n"(PIECES) : "memory"); break;
+                default: asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+            }
+        };
         auto next = [](uint32_t slot, uint32_t by) { return slot + by >= UNITS ? slot + by - UNITS : slot + by; };
 
         uint32_t id = blockIdx.x;
@@ -364,9 +574,7 @@ struct vx_i8_tile {
 #pragma unroll
                 for (int j = 0; j < FT; ++j) acc[i][j] = i4v{};
             // stage 0 is there (its units are the oldest requests; stores of the tile before may be among the newer ones)
-            if (S > 2) asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" :: "n"(3 * PIECES) : "memory");
-            else if (S > 1) asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" :: "n"(2 * PIECES) : "memory");
-            else asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
+            arrived(min(2 * S, UNITS) - 2);
             if (S == 1) clear(1);
             uint32_t at_w = 0, at_x = 1;  // slots of stage s
             fetch(0, at_w, at_x, 0);
@@ -389,10 +597,9 @@ struct vx_i8_tile {
                 fetch(1, at_w, at_x, 1);
                 multiply(0);
                 if (s + 1 < S) {
-                    if (s + 2 < S) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" :: "n"(PIECES) : "memory");
-                    else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-                    request(2 * s + 5, at_w);
-                    request(2 * s + 6, at_x);
+                    arrived(min(2 * S, 2 * s + UNITS) - (2 * s + 4));
+                    request(2 * s + UNITS, at_w);
+                    request(2 * s + UNITS + 1, at_x);
                     at_w = next(at_w, 2);
                     at_x = next(at_x, 2);
                     if (s + 2 == S) clear(at_x);

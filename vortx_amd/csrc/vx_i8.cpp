@@ -60,9 +60,14 @@ static int quantize(vx_ctx ctx, vx_stream stream, const vx_i8_rows* out, const M
 
 static uint64_t up(uint64_t n, uint64_t to) { return (n + to - 1) / to * to; }
 
-// x that a product quantizes itself (one launch, each workgroup for itself) up to so many tokens and bytes of codes.
-constexpr uint32_t VX_I8_OWN_TOKENS = 2, VX_I8_OWN_BYTES = 32768;
-static bool own_x(uint32_t T, uint32_t K) { return T <= VX_I8_OWN_TOKENS && up(K, 64) * T <= VX_I8_OWN_BYTES; }
+// x that a product quantizes itself (one launch, each workgroup for itself): one token of up to 65536 values, or up to
+// four whose values stay in the workgroup's registers, 16 a thread (4096 values and up to four tokens, 8192 and two). By
+// itself / by a launch before it, 11008 x 4096, us: four tokens 16.8 / 17.2, five as four would be 17.3; 4096 x 11008,
+// four tokens 21.2 / 19.
+static bool own_x(uint32_t T, uint32_t K) {
+    const uint64_t fours = (K + 4095ull) / 4096;
+    return T == 1 ? fours <= 16 : T <= VX_I8_OWN_TOKENS && fours * T <= 4;
+}
 
 static uint64_t ws_bytes(uint32_t T, uint32_t K) { return own_x(T, K) ? 0 : up(K, 128) * T + up(4ull * T, 16); }
 
@@ -70,24 +75,43 @@ struct I8Plan {
     int kernel;
     uint32_t tokens, channels;  // of a workgroup
     uint32_t block, lds, grid;  // grid: most workgroups, each then has several tiles (0: one each)
+    uint32_t split;
 };
+// What a kernel takes is close to what a CU has to load, the rows of x and of the weights of all its workgroups, at
+// some 37 GB/s from L2 (the kernels that go over tiles at 47, where the matrix cores are as long). Us, at 4096 columns:
+//   128 x 4096 (N)   direct 96 rows 14.7   tiles of 128 256 rows 27     64 x 11008   direct 128 rows 22.3   tiles 256 rows 27
+//   128 x 11008      direct 256 39.0       tiles 256 28.7             200 x 11008   direct 384 51.4        tiles 256 28.5
+//   200 x 4096, 11008 columns: direct 128 42.1, tiles 256 61.2;  64 x 11008 gated: direct 256 41.6, tiles 256 31.5
+// so that the least of them is taken, and of two the same the tiles of 128.
 static I8Plan plan_gemm(int num_cus, const vx_i8_args& a, bool gated) {
     const int g = gated ? 1 : 0;
-    const bool near = a.xs < (1u << 24) && a.ws[0] < (1u << 24) && a.ws[1] < (1u << 24);  // a tile's rows within 32 bits
-    if (a.xf || a.T <= 128 || !near) {
-        // 16 tt tokens by 16 nt channels
-        struct Direct { int kernel; uint32_t tt, nt[2]; };
-        static const Direct kDirect[4] = {{K_vx_i8_direct_x, 1, {1, 1}}, {K_vx_i8_direct_t1, 1, {1, 1}}, {K_vx_i8_direct_t2, 2, {2, 1}},
-                                          {K_vx_i8_direct_t4, 4, {2, 1}}};
-        const Direct& d = kDirect[a.xf ? 0 : a.T <= 16 ? 1 : a.T <= 32 ? 2 : 3];
-        const uint32_t sums = std::min(d.tt * d.nt[g], gated ? 4u : 8u) * (gated ? 2 : 1);
-        return {d.kernel + g, 16 * d.tt, 16 * d.nt[g], 512, a.x_bytes + sums * 8192, 0};
+    const uint32_t both = gated ? 2 : 1;
+    if (a.xf) {
+        // a workgroup a CU; waves share rows where there are fewer of them than waves, 4096 bytes a step
+        const uint32_t waves = (uint32_t)num_cus * 16;
+        uint32_t split = 1;
+        while (split < 16 && (uint64_t)a.N * split * 2 <= waves && split * 4096u < a.K) split *= 2;
+        const uint32_t per = 16 / split, grid = std::min((uint32_t)num_cus, (a.N - 1) / per + 1);
+        return {K_vx_i8_stream_t1 + 2 * (a.T > 2 ? 2 : (int)a.T - 1) + g, a.T, (a.N - 1) / grid + 1, 1024, a.x_bytes + 1024u, 0, split};
     }
-    // tiles of 256 where they fill the card
-    const uint32_t cn = gated ? 128 : 256;
-    const uint64_t wide = (uint64_t)((a.T + 255) / 256) * ((a.N + cn - 1) / cn);
-    const uint32_t side = wide * 2 > (uint64_t)num_cus ? 256 : 128;
-    return {(side == 256 ? K_vx_i8_tile256 : K_vx_i8_tile128) + g, side, gated ? side / 2 : side, 2 * side, 0, (uint32_t)num_cus * (side == 256 ? 1 : 2)};
+    struct Kernel { int kernel; uint32_t tokens, channels[2], block, at_once; };  // at_once: 0, or workgroups a CU that have several tiles
+    static const Kernel kKernels[6] = {{K_vx_i8_direct_t1, 16, {16, 16}, 512, 0}, {K_vx_i8_direct_t2, 32, {32, 16}, 512, 0},
+                                       {K_vx_i8_direct_t4, 64, {32, 16}, 512, 0}, {K_vx_i8_direct_t4_wide, 64, {64, 32}, 512, 0},
+                                       {K_vx_i8_tile128, 128, {128, 64}, 256, 2}, {K_vx_i8_tile256, 256, {256, 128}, 512, 1}};
+    auto cost = [&](const Kernel& k) {
+        const uint64_t groups = (uint64_t)((a.T - 1) / k.tokens + 1) * ((a.N - 1) / k.channels[g] + 1);
+        return (groups + num_cus - 1) / num_cus * (k.tokens + k.channels[g] * both);
+    };
+    int best = a.T <= 16 ? 0 : a.T <= 32 ? 1 : 2;
+    if (best == 2) {
+        const bool near = a.xs < (1u << 24) && a.ws[0] < (1u << 24) && a.ws[1] < (1u << 24);  // a tile's rows within 32 bits
+        for (int i = 3; i < (near ? 6 : 4); ++i)
+            if (cost(kKernels[i]) < cost(kKernels[best]) + (i == 4)) best = i;  // (of two the same: 512 x 11008 tiles of 128 50.8, of 256 59.2)
+    }
+    const Kernel& k = kKernels[best];
+    const uint32_t fragments = k.tokens / 16 * (k.channels[g] / 16);  // (whose sums meet in LDS, eight products' at a time)
+    return {k.kernel + g, k.tokens, k.channels[g], k.block, k.at_once ? 0u : std::min(fragments, gated ? 4u : 8u) * both * 8192u,
+            (uint32_t)num_cus * k.at_once, 1};
 }
 
 static int run_gemm(vx_ctx ctx, vx_stream stream, const vx_mview* out, const vx_i8_rows* xq, const vx_cview* xf, const vx_i8_rows* w,
@@ -143,8 +167,9 @@ static int run_gemm(vx_ctx ctx, vx_stream stream, const vx_mview* out, const vx_
         a.xfs[0] = x.stride[0];
         a.xfs[1] = x.stride[1];
         a.xf_vec = x.vec;
-        a.pitch = (uint32_t)up(a.K, 64) + 16;
-        a.x_bytes = (uint32_t)up(a.T * (uint64_t)a.pitch + 8 * 16 * 4 + 64, 16);
+        a.pitch = (uint32_t)up(a.K, 4096);
+        const uint32_t rows_there = a.T == 3 ? 4 : a.T;  // (a kernel for four reads a fourth, and makes nothing of it)
+        a.x_bytes = (uint32_t)up(rows_there * (uint64_t)a.pitch + VX_I8_OWN_TOKENS * (16 * 4 + 4), 16);
     } else {
         a.x = (const int8_t*)xq->base;
         a.xs = xq->row_stride_bytes;
@@ -153,6 +178,7 @@ static int run_gemm(vx_ctx ctx, vx_stream stream, const vx_mview* out, const vx_
     const I8Plan p = plan_gemm(ctx_cus(ctx), a, gated);
     a.tiles_t = (a.T - 1) / p.tokens + 1;
     a.tiles_n = (a.N - 1) / p.channels + 1;
+    a.split = p.split;
     if ((uint64_t)a.tiles_t * a.tiles_n >= (1u << 22)) return fail(VX_ERR_UNSUPPORTED, "too many outputs (split the call)");
     if (xf && !own && (s = quantize(ctx, stream, &rows, x))) return s;
     const uint32_t tiles = a.tiles_t * a.tiles_n;

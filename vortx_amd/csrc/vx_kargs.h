@@ -224,7 +224,10 @@ typedef struct vx_i8_args {
     uint32_t xf_vec;       /* 1: xfs[1] == 1 and 16-byte aligned rows */
     uint32_t pitch;        /* bytes between x's rows in LDS, of such kernels */
     uint32_t x_bytes;      /* of LDS that x, its maxima and scales take */
+    uint32_t split;        /* waves of such a kernel that share a row of the weights: a power of two up to 16 */
+    uint32_t pad0;
 } vx_i8_args;
+#define VX_I8_OWN_TOKENS 4 /* of such kernels, at most */
 
 /* Attention over the cache. Query row r = j * group + i of a sequence is its
  * j-th query token, i-th query head of the key/value head. */
