@@ -22,10 +22,10 @@
  *    call needs beyond its operands is passed in by the caller
  *    (vx_gemv_q_ws), like the reference's caller-owned
  *    `shapes: &mut TensorLayoutBuffers` (src/linalg/gemm.rs:47-56). The
- *    kernels of the key/value cache and its attention are loaded, a head size
- *    at a time and once for all contexts of a device, by the first call that
- *    uses them (a few milliseconds; vx_attention_ws_size is such a call), and
- *    stay loaded.
+ *    kernels of the key/value cache and its attention (a head size at a time),
+ *    those of pages and rotation and those of 8-bit integers are loaded, once
+ *    for all contexts of a device, by the first call that uses them (a few
+ *    milliseconds; vx_attention_ws_size is such a call), and stay loaded.
  */
 #ifndef VORTX_HIP_H
 #define VORTX_HIP_H
@@ -486,8 +486,8 @@ int vx_rotate(vx_ctx ctx, vx_stream stream, const vx_mview* q_out, const vx_cvie
               const vx_cview* k, const int32_t* positions, const vx_rotation* how);
 
 /* vx_rotate of q and k, k then written into the cache beside v as vx_kv_write
- * does it, in one launch: the same bits in q_out and in the cache as the two
- * calls one after the other. k is only read. q and k have the cache's dim and
+ * does it, in one launch (queries of many tokens in a second): the same bits in
+ * q_out and in the cache as the two calls one after the other. k is only read. q and k have the cache's dim and
  * the same tokens; q and q_out may be NULL: keys alone. */
 int vx_kv_write_rotated(vx_ctx ctx, vx_stream stream, const vx_kv_cache* cache, const vx_mview* q_out, const vx_cview* q,
                         const vx_cview* k, const vx_cview* v, const int32_t* positions, const int32_t* slots,

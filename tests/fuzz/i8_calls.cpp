@@ -87,6 +87,8 @@ int main() {
     x = rows_of(1u << 31, 16), w = up = rows_of(1u << 20, 16), o.layout = matrix(1u << 31, 1u << 20), f.layout = matrix(1u << 31, 16);
     CHECK(refused(vx_gemm_i8(ctx, nullptr, &o, &x, &w), VX_ERR_UNSUPPORTED));
     CHECK(refused(vx_gemm_i8_x(ctx, nullptr, &o, &f, &w, ws, enough), VX_ERR_UNSUPPORTED));
+    x = rows_of(1, 16), w = up = rows_of(1u << 31, 16), o.layout = matrix(1, 1u << 31), f.layout = matrix(1, 16);
+    CHECK(all(VX_ERR_UNSUPPORTED));
     x = rows_of(0, 16), w = up = rows_of(40, 16), o.layout = matrix(0, 40);
     CHECK(vx_gemm_i8(ctx, nullptr, &o, &x, &w) == VX_OK && vx_gemm_i8_gated(ctx, nullptr, &o, &x, &w, &up, 1) == VX_OK && launches == 0);
     // quantizing

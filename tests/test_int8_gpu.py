@@ -308,3 +308,38 @@ def test_empty_and_refused(i8):
                  lambda: vx.Int8Rows(torch.zeros(4, 32, dtype=torch.int8, device=DEV), torch.zeros(4, device=DEV).double())]:
         with pytest.raises(TypeError):
             call()
+
+
+@pytest.mark.parametrize("T", [1, 4, 20, 60, 150])
+@pytest.mark.parametrize("rows,stride", [(70000, 65536), (300, 1 << 24)])
+def test_weights_past_32_bits(i8, T, rows, stride):
+    """Rows of 192 columns whose places pass 2^32 bytes."""
+    note(f"far weights {T} by {rows} rows {stride} bytes apart")
+    rng = np.random.default_rng(T)
+    K, n = 192, 300
+    data = torch.empty(rows, stride, dtype=torch.int8, device=DEV)
+    x, w, sx, sw = _random(rng, T, n, K)
+    data[-n:, :K] = _gpu(w)
+    weights = vx.Int8Rows(data, torch.cat([torch.ones(rows - n, device=DEV), _gpu(sw)]), K)
+    out = torch.empty(T, rows, device=DEV)
+    i8.dispatch(out, _rows(x, sx), weights)
+    _check(out[:, -n:], _exact(x, w, sx, sw))
+    xf = _gpu(_f32_case(rng, T, K))
+    q = vx.Int8Rows.empty(T, K)
+    i8.quantize(q, xf)
+    i8.dispatch(out, xf, weights, workspace=i8.workspace(T, K))
+    _check(out[:, -n:], _exact(q.data[:, :K].cpu().numpy(), w, q.scales.cpu().numpy(), sw))
+
+
+def test_tokens_past_32_bits(i8):
+    rng = np.random.default_rng(8)
+    T, N, K, stride = 300, 50, 200, 1 << 24
+    data = torch.empty(T, stride, dtype=torch.int8, device=DEV)
+    x, w, sx, sw = _random(rng, T, N, K)
+    data[:, :K] = _gpu(x)
+    out = torch.empty(T, N, device=DEV)
+    i8.dispatch(out, vx.Int8Rows(data, _gpu(sx), K), _rows(w, sw))
+    _check(out, _exact(x, w, sx, sw))
+    i8.quantize(vx.Int8Rows(data, torch.empty(T, device=DEV), K), _gpu(x * sx[:, None]))
+    want, _, _ = _codes(x * sx[:, None])
+    assert np.array_equal(data[:, :K].cpu().numpy(), want)

@@ -347,3 +347,81 @@ def test_rotation_refusals(kv):
         with pytest.raises(vx.VortxError):
             call()
     assert _ffi.VX_ROTATE_PAIRS == 1 and _ffi.VX_ROTATE_NORM == 2
+
+
+@pytest.mark.parametrize("types", [(Q8, Q8), (Q8, Q4)])
+def test_slots_past_32_bits_of_bytes(kv, types):
+    note(f"far slots {types}")
+    hk, dim, page, pages, n = 8, 256, 64, 1 << 15, 45
+    g = torch.Generator(device=DEV).manual_seed(3)
+    k, v = (torch.randn(n, hk, dim, generator=g, device=DEV) for _ in range(2))
+    slots, pos = _i32(pages * page - 3 * np.arange(n) - 1), _i32(np.arange(n) * 999)
+    cache, how = vx.KvCache(pages, page, hk, dim, *types), kv.rotation(vx.rotation_freqs(dim), norm=True)
+    assert cache.data.numel() > 2 ** 32
+    got, want = ([torch.empty_like(k) for _ in range(2)] for _ in range(2))
+    turned = torch.empty_like(k)
+    kv.rotate(turned, k, None, None, pos, how)
+    kv.write(cache, turned, v, slots)
+    kv.read(*want, cache, slots)
+    kv.write(cache, v, k, slots)
+    kv.write_rotated(cache, None, None, k, v, pos, slots, how)
+    kv.read(*got, cache, slots)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    many = slots.repeat_interleave(32)[:1400] - (torch.arange(1400, device=DEV) * 97 % 1000 * 512).int()  # (enough to go by fours)
+    many = torch.unique(many).flip(0).contiguous()
+    k, v = (torch.randn(len(many), hk, dim, generator=g, device=DEV) for _ in range(2))
+    pos, turned = _i32(np.arange(len(many))), torch.empty_like(k)
+    kv.rotate(turned, k, None, None, pos, how)
+    got, want = ([torch.empty_like(k) for _ in range(2)] for _ in range(2))
+    kv.write(cache, turned, v, many)
+    kv.read(*want, cache, many)
+    kv.write(cache, v, k, many)
+    kv.write_rotated(cache, None, None, k, v, pos, many, how)
+    kv.read(*got, cache, many)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+def test_more_tokens_than_a_launch_takes(kv):
+    """2^20 of them a launch: the same as two calls."""
+    note("2^20 + 37 tokens")
+    n, cut, dim, page = (1 << 20) + 37, 500001, 64, 64
+    g = torch.Generator(device=DEV).manual_seed(5)
+    q, k, v = (torch.randn(n, 1, dim, generator=g, device=DEV) for _ in range(3))
+    pos, slots = torch.arange(n, dtype=torch.int32, device=DEV), torch.arange(n, dtype=torch.int32, device=DEV).flip(0).contiguous()
+    how = kv.rotation(vx.rotation_freqs(dim), norm=True)
+    a, b = (vx.KvCache(-(-n // page), page, 1, dim) for _ in range(2))
+    a.data.fill_(1), b.data.fill_(1)
+    qa, ka, qb, kb = (torch.empty_like(q) for _ in range(4))
+    kv.rotate(qa, q, ka, k, pos, how)
+    for s in (slice(0, cut), slice(cut, n)):
+        kv.rotate(qb[s], q[s], kb[s], k[s], pos[s], how)
+    assert torch.equal(qa, qb) and torch.equal(ka, kb)
+    qa.zero_()
+    kv.write_rotated(a, qa, q, k, v, pos, slots, how)
+    for s in (slice(0, cut), slice(cut, n)):
+        kv.write(b, kb[s], v[s], slots[s])
+    assert torch.equal(qa, qb) and torch.equal(a.data, b.data)
+
+
+def test_other_streams(kv):
+    """Rows rotated into two caches at once, each on a stream of its own."""
+    note("two streams")
+    g = torch.Generator(device=DEV).manual_seed(6)
+    n, hq, hk, dim = 600, 8, 2, 128
+    q, k, v = (torch.randn(n, h, dim, generator=g, device=DEV) for h in (hq, hk, hk))
+    pos, slots = _i32(np.arange(n) + 5), _i32(np.random.default_rng(1).permutation(n))
+    how = kv.rotation(vx.rotation_freqs(dim), norm=True, q_weight=torch.rand(dim, generator=g, device=DEV))
+    caches, outs = [vx.KvCache(10, 64, hk, dim) for _ in range(3)], [torch.zeros_like(q) for _ in range(3)]
+    for c in caches:
+        c.data.fill_(9)
+    kv.write_rotated(caches[2], outs[2], q, k, v, pos, slots, how)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    for _ in range(10):
+        for s, c, o in zip(streams, caches, outs):
+            with torch.cuda.stream(s):
+                kv.write_rotated(c, o, q, k, v, pos, slots, how)
+    kv.write_rotated(caches[0], outs[0], q, k, v, pos, slots, how, stream=streams[0])
+    torch.cuda.synchronize()
+    for c, o in zip(caches[:2], outs):
+        assert torch.equal(c.data, caches[2].data) and torch.equal(o, outs[2])

@@ -325,8 +325,8 @@ class KvAttention(_Context):
     def write_rotated(self, cache: KvCache, q_out, q, k, v, positions, slots, how: Rotation, stream=None) -> None:
         """:meth:`rotate` of ``q`` into ``q_out`` and of ``k``, which goes into
         the cache's ``slots`` with ``v`` as :meth:`write` puts it there, in one
-        launch (the same bits as the two calls). ``q`` and ``q_out`` None: keys
-        alone."""
+        launch (queries of many tokens in a second; the same bits as the two
+        calls). ``q`` and ``q_out`` None: keys alone."""
         st = _vx._pycall.kv_write_rotated(_WRITE_ROTATED, self._ctx, stream, cache._addr, q_out, q, k, v, positions, slots, *how._call)
         if st is not None:
             if st:

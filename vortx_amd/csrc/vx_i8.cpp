@@ -179,7 +179,7 @@ static int run_gemm(vx_ctx ctx, vx_stream stream, const vx_mview* out, const vx_
     a.tiles_t = (a.T - 1) / p.tokens + 1;
     a.tiles_n = (a.N - 1) / p.channels + 1;
     a.split = p.split;
-    if ((uint64_t)a.tiles_t * a.tiles_n >= (1u << 22)) return fail(VX_ERR_UNSUPPORTED, "too many outputs (split the call)");
+    if (a.N >= (1u << 31) || (uint64_t)a.tiles_t * a.tiles_n >= (1u << 22)) return fail(VX_ERR_UNSUPPORTED, "too many outputs (split the call)");
     if (xf && !own && (s = quantize(ctx, stream, &rows, x))) return s;
     const uint32_t tiles = a.tiles_t * a.tiles_n;
     return launch_struct(ctx, p.kernel, p.grid ? std::min(tiles, p.grid) : tiles, p.block, stream, &a, p.lds);
