@@ -343,3 +343,32 @@ def test_tokens_past_32_bits(i8):
     i8.quantize(vx.Int8Rows(data, torch.empty(T, device=DEV), K), _gpu(x * sx[:, None]))
     want, _, _ = _codes(x * sx[:, None])
     assert np.array_equal(data[:, :K].cpu().numpy(), want)
+
+
+@pytest.mark.parametrize("gated", [False, True])
+@pytest.mark.parametrize("T,N,K", [(17, 200, 1030), (100, 4096, 11008), (33, 65, 5000), (128, 1000, 4096), (129, 129, 2049), (300, 500, 8191),
+                                   (1000, 130, 16385), (64, 3, 131071), (70, 4097, 1100), (1024, 256, 2048), (20, 31, 1024)])
+def test_parts_of_long_rows(i8, T, N, K, gated):
+    """Sums of parts of K, joined: the bits of the product of vx_i8_quantize's rows, with any contents of the workspace."""
+    note(f"parts {T} x {N} x {K} gated {gated}")
+    rng = np.random.default_rng(T + N + K)
+    x = _gpu(_f32_case(rng, T, K))
+    x[T // 2, K - 1] = float("nan")
+    w, up = (vx.Int8Rows.empty(N, K) for _ in range(2))
+    for r in (w, up):
+        r.data.copy_(torch.randint(-128, 128, r.data.shape, dtype=torch.int8, device=DEV))
+        r.scales.copy_(torch.rand(N, device=DEV) + 0.01)
+    q = vx.Int8Rows.empty(T, K)
+    q.data.fill_(77)
+    i8.quantize(q, x)
+    ws = i8.workspace(T, K)
+    want, got = torch.empty(T, N, device=DEV), torch.full((N, T + 1), 7.0, device=DEV)
+    call = (lambda o, r, **k: i8.dispatch_gated(o, r, w, up, "silu", **k)) if gated else (lambda o, r, **k: i8.dispatch(o, r, w, **k))
+    call(want, q)
+    for fill, out in ((255, torch.empty(T, N, device=DEV)), (0, got.t()[:T])):
+        ws.fill_(fill)
+        call(out, x, workspace=ws)
+        assert torch.equal(out.nan_to_num(3.0), want.nan_to_num(3.0))
+    assert (got[:, T] == 7.0).all() and want[T // 2].isnan().all() and not want[0].isnan().any()
+    if not gated:
+        _check(want[:2], _exact(q.data[:2, :K].cpu().numpy(), w.data[:, :K].cpu().numpy(), q.scales[:2].cpu().numpy(), w.scales.cpu().numpy()))

@@ -457,7 +457,7 @@ VX_I8_STREAM(vx_i8_stream_t4_gated, 4, true, 1)
 // 4096 206 us, 1790 (gated 423, 1750): bound by the matrix cores and the loads, which
 // each take 1.4 of a stage's 1.7 us, and by the stores, which all CUs make at the same
 // time, 16 us a tile of each CU.
-template <int MT, int MN, int WT, int WN, bool GATED>
+template <int MT, int MN, int WT, int WN, bool GATED, bool PART = false>
 struct vx_i8_tile {
     static_assert(MT == MN, "units of one size");
     static constexpr int WAVES = WT * WN, THREADS = 64 * WAVES;
@@ -470,7 +470,9 @@ struct vx_i8_tile {
     static __device__ __forceinline__ uint32_t at(uint32_t r, uint32_t c) { return r * 128 + ((c ^ (r >> 1)) & 7) * 16; }
 
     const vx_i8_args& a;
-    const uint32_t tid, lane, m, kg, wave, S, last;
+    const uint32_t tid, lane, m, kg, wave;
+    uint32_t K, S, last;  // columns (of the part), stages, where the last one begins
+    uint32_t part_of;
     uint32_t off_w[PIECES], off_x[PIECES];  // within the operands' first stage
     i4v base_w[2], base_x;
     uint32_t t0, n0, lds0;
@@ -481,20 +483,29 @@ struct vx_i8_tile {
     }
     __device__ __forceinline__ vx_i8_tile(const vx_i8_args& a_, uint8_t* lds)
         : a(a_), tid(threadIdx.x), lane(tid & 63), m(lane & 15), kg(lane >> 4), wave(__builtin_amdgcn_readfirstlane(tid >> 6)),
-          S((a_.K + 127) / 128), last(128 * (S - 1)),
+          K(a_.K), S((a_.K + 127) / 128), last(128 * (S - 1)), part_of(0),
           lds0(__builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)lds)) {}
 
     // The loads of tile `id` of all in their order.
     __device__ __forceinline__ void place(uint32_t id) {
         // in bands of eight tiles of tokens: the 32 tiles that an XCD works on at a time are 8 by 4,
         // so that its L2 takes 12 operands of a tile from farther away, where 16 by 2 takes 18
-        const uint32_t tile = vx_xcd_order(id, a.tiles_t * a.tiles_n), band = tile / (8 * a.tiles_n), in = tile - band * 8 * a.tiles_n;
+        uint32_t tile = vx_xcd_order(id, a.tiles_t * a.tiles_n * (PART ? a.split : 1u)), k0 = 0;
+        if constexpr (PART) {  // (an XCD has whole parts where it can: its L2 then takes each column of x and of the weights once)
+            part_of = tile / (a.tiles_t * a.tiles_n);
+            tile -= part_of * a.tiles_t * a.tiles_n;
+            k0 = part_of * a.chunk;
+            K = min(a.K - k0, a.chunk);
+            S = (K + 127) / 128;
+            last = 128 * (S - 1);
+        }
+        const uint32_t band = tile / (8 * a.tiles_n), in = tile - band * 8 * a.tiles_n;
         const uint32_t high = min(8u, a.tiles_t - 8 * band);
         t0 = (8 * band + in % high) * MT;
         n0 = in / high * (GATED ? MN / 2 : MN);
-        base_w[0] = buffer(a.w[0] + (uint64_t)n0 * a.ws[0]);
-        base_w[1] = GATED ? buffer(a.w[1] + (uint64_t)n0 * a.ws[1]) : base_w[0];
-        base_x = buffer(a.x + (uint64_t)t0 * a.xs);
+        base_w[0] = buffer(a.w[0] + (uint64_t)n0 * a.ws[0] + k0);
+        base_w[1] = GATED ? buffer(a.w[1] + (uint64_t)n0 * a.ws[1] + k0) : base_w[0];
+        base_x = buffer(a.x + (uint64_t)t0 * a.xs + k0);
 #pragma unroll
         for (int p = 0; p < PIECES; ++p) {
             const uint32_t r = wave * 32 + 8 * p + lane / 8, c = piece(p);
@@ -517,12 +528,12 @@ struct vx_i8_tile {
     __device__ __forceinline__ void request(uint32_t u, uint32_t slot) {
         const uint32_t s = u / 2;
         if (s >= S) return;
-        const bool end = s + 1 == S && a.K % 128;
+        const bool end = s + 1 == S && K % 128;
         uint32_t from[PIECES];
 #pragma unroll
         for (int p = 0; p < PIECES; ++p) {
             const uint32_t k = 16 * piece(p);
-            from[p] = (u & 1 ? off_x[p] : off_w[p]) + (end ? (last + k < a.K ? last : 0u - k) : 128 * s);
+            from[p] = (u & 1 ? off_x[p] : off_w[p]) + (end ? (last + k < K ? last : 0u - k) : 128 * s);
         }
         load(from, u & 1 ? base_x : base_w[0], u & 1 ? base_x : base_w[1], slot, 0);
     }
@@ -546,7 +557,7 @@ struct vx_i8_tile {
         };
         // x past K in the last stage becomes zeros
         auto clear = [&](uint32_t slot) {
-            const uint32_t have = a.K - last;
+            const uint32_t have = K - last;
             if (have == 128) return;
             for (uint32_t i = tid; i < MT * 8; i += THREADS) {
                 const uint32_t r = i / 8, c = i % 8;
@@ -612,8 +623,19 @@ struct vx_i8_tile {
                 }
                 multiply(1);
             }
-            // the results, under the first loads of the next tile (after the scales: loads end in order)
             const uint32_t tt = t0 + wt + m, nn = n0 + (GATED ? wn / 2 : wn) + 4 * kg;
+            if constexpr (PART) {
+                const uint32_t pitch = (a.N + 3) / 4 * 4;
+#pragma unroll
+                for (int j = 0; j < FT; ++j)
+#pragma unroll
+                    for (int i = 0; i < FN; ++i) {
+                        const uint32_t t = tt + 16 * j, n = nn + 16 * (GATED ? i / 2 : i), g = part_of * (GATED ? 2 : 1) + (GATED ? i & 1 : 0);
+                        if (t < a.T && n < a.N) *(i4v*)(a.parts + ((uint64_t)g * a.T + t) * pitch + n) = acc[i][j];
+                    }
+                return;
+            }
+            // the results, under the first loads of the next tile (after the scales: loads end in order)
             float sx[FT];
             f4v sw[FN];
 #pragma unroll
@@ -641,13 +663,38 @@ struct vx_i8_tile {
         }
     }
 };
-#define VX_I8_TILE(name, MT, MN, WT, WN, GATED)                                                  \
-    extern "C" __global__ __launch_bounds__(64 * WT * WN) void name(vx_i8_args a) {              \
-        using tile = vx_i8_tile<MT, MN, WT, WN, GATED>;                                          \
+#define VX_I8_TILE(name, threads, ...)                                                           \
+    extern "C" __global__ __launch_bounds__(threads) void name(vx_i8_args a) {                   \
+        using tile = vx_i8_tile<__VA_ARGS__>;                                                    \
+        static_assert(tile::THREADS == threads, "waves of 64");                                  \
         __shared__ __align__(1024) uint8_t lds[tile::UNIT * tile::UNITS];                        \
         tile(a, lds).run(lds);                                                                   \
     }
-VX_I8_TILE(vx_i8_tile256, 256, 256, 2, 4, false)
-VX_I8_TILE(vx_i8_tile256_gated, 256, 256, 2, 4, true)
-VX_I8_TILE(vx_i8_tile128, 128, 128, 2, 2, false)
-VX_I8_TILE(vx_i8_tile128_gated, 128, 128, 2, 2, true)
+VX_I8_TILE(vx_i8_tile256, 512, 256, 256, 2, 4, false)
+VX_I8_TILE(vx_i8_tile256_gated, 512, 256, 256, 2, 4, true)
+VX_I8_TILE(vx_i8_tile128, 256, 128, 128, 2, 2, false)
+VX_I8_TILE(vx_i8_tile128_gated, 256, 128, 128, 2, 2, true)
+
+// ---------------------------------------------------------------- a long K, few tiles
+// Tiles of 128 over parts of K, whose sums a second launch joins: few tokens by few
+// channels would otherwise leave CUs idle, or have all of them load the same rows.
+VX_I8_TILE(vx_i8_part128, 256, 128, 128, 2, 2, false, true)
+VX_I8_TILE(vx_i8_part128_gated, 256, 128, 128, 2, 2, true, true)
+
+template <bool GATED>
+__device__ __forceinline__ void vx_i8_join_rows(const vx_i8_args& a) {
+    constexpr uint32_t G = GATED ? 2 : 1;
+    const uint32_t fours = (a.N + 3) / 4;
+    const uint64_t id = (uint64_t)blockIdx.x * 256 + threadIdx.x, step = G * (uint64_t)a.T * fours;
+    const uint32_t t = (uint32_t)(id / fours), n = 4 * (uint32_t)(id % fours);
+    if (t >= a.T) return;
+    const i4v* p = (const i4v*)a.parts + id;
+    i4v s[2] = {};
+#pragma unroll 4
+    for (uint32_t q = 0; q < a.split; ++q)
+#pragma unroll
+        for (uint32_t g = 0; g < G; ++g) s[g] += p[q * step + g * (uint64_t)a.T * fours];
+    vx_i8_finish4<GATED>(a, t, n, a.xscale[t], s[0], s[1], vx_i8_scales4(a.wscale[0], n, a.N), GATED ? vx_i8_scales4(a.wscale[1], n, a.N) : f4v{});
+}
+extern "C" __global__ __launch_bounds__(256) void vx_i8_join(vx_i8_args a) { vx_i8_join_rows<false>(a); }
+extern "C" __global__ __launch_bounds__(256) void vx_i8_join_gated(vx_i8_args a) { vx_i8_join_rows<true>(a); }

@@ -69,13 +69,19 @@ static bool own_x(uint32_t T, uint32_t K) {
     return T == 1 ? fours <= 16 : T <= VX_I8_OWN_TOKENS && fours * T <= 4;
 }
 
-static uint64_t ws_bytes(uint32_t T, uint32_t K) { return own_x(T, K) ? 0 : up(K, 128) * T + up(4ull * T, 16); }
+// x's rows and their scales, and behind them sums of parts of K (plan_gemm): 512 workgroups' tiles of 128 by 128.
+static uint64_t rows_bytes(uint32_t T, uint32_t K) { return own_x(T, K) ? 0 : up(K, 128) * T + up(4ull * T, 16); }
+constexpr uint32_t VX_I8_PARTS_TOKENS = 1024, VX_I8_PARTS_COLS = 1024;
+static uint64_t parts_bytes(uint32_t T, uint32_t K) {
+    return T <= 16 || T > VX_I8_PARTS_TOKENS || K < VX_I8_PARTS_COLS ? 0 : std::min(T, 128u) * (512ull * 128 * 4);
+}
+static uint64_t ws_bytes(uint32_t T, uint32_t K) { return rows_bytes(T, K) + parts_bytes(T, K); }
 
 struct I8Plan {
     int kernel;
     uint32_t tokens, channels;  // of a workgroup
     uint32_t block, lds, grid;  // grid: most workgroups, each then has several tiles (0: one each)
-    uint32_t split;
+    uint32_t split, chunk;
 };
 // What a kernel takes is close to what a CU has to load, the rows of x and of the weights of all its workgroups, at
 // some 37 GB/s from L2 (the kernels that go over tiles at 47, where the matrix cores are as long). Us, at 4096 columns:
@@ -92,7 +98,7 @@ static I8Plan plan_gemm(int num_cus, const vx_i8_args& a, bool gated) {
         uint32_t split = 1;
         while (split < 16 && (uint64_t)a.N * split * 2 <= waves && split * 4096u < a.K) split *= 2;
         const uint32_t per = 16 / split, grid = std::min((uint32_t)num_cus, (a.N - 1) / per + 1);
-        return {K_vx_i8_stream_t1 + 2 * (a.T > 2 ? 2 : (int)a.T - 1) + g, a.T, (a.N - 1) / grid + 1, 1024, a.x_bytes + 1024u, 0, split};
+        return {K_vx_i8_stream_t1 + 2 * (a.T > 2 ? 2 : (int)a.T - 1) + g, a.T, (a.N - 1) / grid + 1, 1024, a.x_bytes + 1024u, 0, split, 0};
     }
     struct Kernel { int kernel; uint32_t tokens, channels[2], block, at_once; };  // at_once: 0, or workgroups a CU that have several tiles
     static const Kernel kKernels[6] = {{K_vx_i8_direct_t1, 16, {16, 16}, 512, 0}, {K_vx_i8_direct_t2, 32, {32, 16}, 512, 0},
@@ -102,16 +108,30 @@ static I8Plan plan_gemm(int num_cus, const vx_i8_args& a, bool gated) {
         const uint64_t groups = (uint64_t)((a.T - 1) / k.tokens + 1) * ((a.N - 1) / k.channels[g] + 1);
         return (groups + num_cus - 1) / num_cus * (k.tokens + k.channels[g] * both);
     };
+    const bool near = a.xs < (1u << 24) && a.ws[0] < (1u << 24) && a.ws[1] < (1u << 24);  // a tile's rows within 32 bits
     int best = a.T <= 16 ? 0 : a.T <= 32 ? 1 : 2;
     if (best == 2) {
-        const bool near = a.xs < (1u << 24) && a.ws[0] < (1u << 24) && a.ws[1] < (1u << 24);  // a tile's rows within 32 bits
         for (int i = 3; i < (near ? 6 : 4); ++i)
             if (cost(kKernels[i]) < cost(kKernels[best]) + (i == 4)) best = i;  // (of two the same: 512 x 11008 tiles of 128 50.8, of 256 59.2)
+    }
+    if (a.parts && near) {
+        // Tiles of 128 over parts of K and a launch that joins their sums, against all of K: in bytes that a CU has to load,
+        // where sums go to memory and back at half a CU's share of its rate and a launch takes as long as 150 KB.
+        const uint64_t tiles = ((a.T - 1) / 128 + 1ull) * ((a.N - 1) / kKernels[4].channels[g] + 1), stages = (a.K + 127) / 128;
+        uint64_t least = cost(kKernels[best]) * a.K;
+        uint32_t parts = 0, chunk = 0;
+        for (uint32_t n = 2; n <= 16 && tiles * n <= 2ull * num_cus && stages >= 4ull * n; ++n) {
+            const uint64_t each = (stages + n - 1) / n * 128;
+            if ((n - 1) * each >= a.K || n * (uint64_t)both * a.T * up(a.N, 4) * 4 > parts_bytes(a.T, a.K)) continue;
+            const uint64_t bytes = (tiles * n + num_cus - 1) / num_cus * 256 * each + 16ull * n * both * a.T * a.N / num_cus + 150000;
+            if (bytes < least) least = bytes, parts = n, chunk = (uint32_t)each;
+        }
+        if (parts) return {K_vx_i8_part128 + g, 128, kKernels[4].channels[g], 256, 0, 0, parts, chunk};
     }
     const Kernel& k = kKernels[best];
     const uint32_t fragments = k.tokens / 16 * (k.channels[g] / 16);  // (whose sums meet in LDS, eight products' at a time)
     return {k.kernel + g, k.tokens, k.channels[g], k.block, k.at_once ? 0u : std::min(fragments, gated ? 4u : 8u) * both * 8192u,
-            (uint32_t)num_cus * k.at_once, 1};
+            (uint32_t)num_cus * k.at_once, 1, 0};
 }
 
 static int run_gemm(vx_ctx ctx, vx_stream stream, const vx_mview* out, const vx_i8_rows* xq, const vx_cview* xf, const vx_i8_rows* w,
@@ -160,6 +180,7 @@ static int run_gemm(vx_ctx ctx, vx_stream stream, const vx_mview* out, const vx_
     if (xf && !own) {
         const uint64_t stride = up(a.K, 128);
         rows = vx_i8_rows{ws, (float*)((char*)ws + stride * a.T), stride, a.T, a.K};
+        if (parts_bytes(a.T, a.K)) a.parts = (int32_t*)((char*)ws + rows_bytes(a.T, a.K));
         xq = &rows;
     }
     if (own) {
@@ -179,9 +200,14 @@ static int run_gemm(vx_ctx ctx, vx_stream stream, const vx_mview* out, const vx_
     a.tiles_t = (a.T - 1) / p.tokens + 1;
     a.tiles_n = (a.N - 1) / p.channels + 1;
     a.split = p.split;
+    a.chunk = p.chunk;
     if (a.N >= (1u << 31) || (uint64_t)a.tiles_t * a.tiles_n >= (1u << 22)) return fail(VX_ERR_UNSUPPORTED, "too many outputs (split the call)");
     if (xf && !own && (s = quantize(ctx, stream, &rows, x))) return s;
-    const uint32_t tiles = a.tiles_t * a.tiles_n;
+    const uint32_t tiles = a.tiles_t * a.tiles_n * (p.chunk ? p.split : 1u);
+    if (p.chunk) {
+        if ((s = launch_struct(ctx, p.kernel, tiles, p.block, stream, &a))) return s;
+        return launch_struct(ctx, K_vx_i8_join + (gated ? 1 : 0), (uint32_t)((a.T * up(a.N, 4) / 4 + 255) / 256), 256, stream, &a);
+    }
     return launch_struct(ctx, p.kernel, p.grid ? std::min(tiles, p.grid) : tiles, p.block, stream, &a, p.lds);
 }
 

@@ -224,8 +224,10 @@ typedef struct vx_i8_args {
     uint32_t xf_vec;       /* 1: xfs[1] == 1 and 16-byte aligned rows */
     uint32_t pitch;        /* bytes between x's rows in LDS, of such kernels */
     uint32_t x_bytes;      /* of LDS that x, its maxima and scales take */
-    uint32_t split;        /* waves of such a kernel that share a row of the weights: a power of two up to 16 */
-    uint32_t pad0;
+    uint32_t split;        /* waves of such a kernel that share a row of the weights: a power of two up to 16;
+                            * of kernels for parts of K: how many, chunk columns each (a multiple of 128) */
+    uint32_t chunk;
+    int32_t* parts;        /* their sums, [split][gate, up][T][N up to a multiple of 4], 16-byte aligned */
 } vx_i8_args;
 #define VX_I8_OWN_TOKENS 4 /* of such kernels, at most */
 
