@@ -107,7 +107,7 @@ def _f32_case(rng, T, K):
     return x
 
 
-@pytest.mark.parametrize("rows,cols", [(1, 1), (1, 4), (3, 7), (5, 1023), (4, 1024), (7, 4096), (2, 4099), (3, 5000), (2, 16384), (2, 16390),
+@pytest.mark.parametrize("rows,cols", [(1, 1), (1, 4), (3, 7), (5, 1023), (4, 1024), (7, 4096), (2, 4099), (3, 5000), (2, 16384), (2, 16390), (520, 16390), (600, 4097),
                                        (1, 40003), (700, 130), (0, 5), (3, 0)])
 def test_quantize(i8, rows, cols):
     note(f"quantize {rows} x {cols}")

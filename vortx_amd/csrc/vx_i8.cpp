@@ -53,9 +53,10 @@ static int quantize(vx_ctx ctx, vx_stream stream, const vx_i8_rows* out, const M
     a.scales = out->scales;
     a.rows = out->rows;
     a.cols = out->cols;
-    // rows of up to 4096 stay in 16 registers a thread, longer ones in 64
-    const int k = !x.vec ? K_vx_i8_quantize_any : out->cols <= 4096 ? K_vx_i8_quantize_c4 : K_vx_i8_quantize_c16;
-    return launch_struct(ctx, k, std::min(out->rows, 1u << 20), 256, stream, &a);
+    // rows of up to 4096 stay in 16 registers a thread; longer ones, where there are few, with 1024 threads, or in 64 registers
+    const bool few = out->rows <= 2u * ctx_cus(ctx);
+    const int k = !x.vec ? K_vx_i8_quantize_any : out->cols <= 4096 ? K_vx_i8_quantize_c4 : few ? K_vx_i8_quantize_long : K_vx_i8_quantize_c16;
+    return launch_struct(ctx, k, std::min(out->rows, 1u << 20), k == K_vx_i8_quantize_long ? 1024 : 256, stream, &a);
 }
 
 static uint64_t up(uint64_t n, uint64_t to) { return (n + to - 1) / to * to; }
@@ -117,6 +118,8 @@ static I8Plan plan_gemm(int num_cus, const vx_i8_args& a, bool gated) {
     if (a.parts && near) {
         // Tiles of 128 over parts of K and a launch that joins their sums, against all of K: in bytes that a CU has to load,
         // where sums go to memory and back at half a CU's share of its rate and a launch takes as long as 150 KB.
+        // With / without, x quantized before, us: 100 x 4096 by 11008 columns 25.5 / 36.3, 64 tokens 22.4 / 38, 256 34 / 52, 32
+        // 20.8 / 27; where a part is not worth it (64 x 4096 by 4096 columns, 17.5) nothing changes.
         const uint64_t tiles = ((a.T - 1) / 128 + 1ull) * ((a.N - 1) / kKernels[4].channels[g] + 1), stages = (a.K + 127) / 128;
         uint64_t least = cost(kKernels[best]) * a.K;
         uint32_t parts = 0, chunk = 0;
