@@ -91,6 +91,15 @@ int main() {
     CHECK(all(VX_ERR_UNSUPPORTED));
     x = rows_of(0, 16), w = up = rows_of(40, 16), o.layout = matrix(0, 40);
     CHECK(vx_gemm_i8(ctx, nullptr, &o, &x, &w) == VX_OK && vx_gemm_i8_gated(ctx, nullptr, &o, &x, &w, &up, 1) == VX_OK && launches == 0);
+    // a workspace for so many tokens and columns does for fewer
+    const uint32_t ts[] = {0, 1, 2, 4, 5, 16, 17, 127, 128, 129, 1024, 1025, 5000}, ks[] = {1, 100, 1023, 1024, 4096, 4097, 8192, 65536, 65537, 131071};
+    for (size_t i = 0; i < 13; ++i)
+        for (size_t j = 0; j < 10; ++j) {
+            uint64_t here = 0, more = 0;
+            CHECK(vx_gemm_i8_ws_size(ts[i], ks[j], &here) == VX_OK);
+            if (i + 1 < 13) CHECK(vx_gemm_i8_ws_size(ts[i + 1], ks[j], &more) == VX_OK && more >= here);
+            if (j + 1 < 10) CHECK(vx_gemm_i8_ws_size(ts[i], ks[j + 1], &more) == VX_OK && more >= here);
+        }
     // quantizing
     w = rows_of(5, 100), f.layout = matrix(5, 100);
     CHECK(refused(vx_i8_quantize(nullptr, nullptr, &w, &f), VX_ERR_INVALID));
@@ -112,9 +121,12 @@ int main() {
                     CHECK(vx_gemm_i8(ctx, nullptr, &o, &x, &w) == VX_OK && launches == 1);
                     CHECK(vx_gemm_i8_gated(ctx, nullptr, &o, &x, &w, &up, 3) == VX_OK && launches == 2);
                     CHECK(vx_gemm_i8_ws_size(T, K, &bytes) == VX_OK);
-                    const int each = bytes ? 2 : 1;
-                    CHECK(vx_gemm_i8_x(ctx, nullptr, &o, &f, &w, bytes ? ws : nullptr, bytes) == VX_OK && launches == 2 + each);
-                    CHECK(vx_gemm_i8_gated_x(ctx, nullptr, &o, &f, &w, &up, 2, bytes ? ws : nullptr, bytes) == VX_OK && launches == 2 + 2 * each);
+                    for (int gated = 0; gated < 2; ++gated) {  // by itself, quantized before, or that and its parts joined after
+                        launches = 0;
+                        CHECK((gated ? vx_gemm_i8_gated_x(ctx, nullptr, &o, &f, &w, &up, 2, bytes ? ws : nullptr, bytes)
+                                     : vx_gemm_i8_x(ctx, nullptr, &o, &f, &w, bytes ? ws : nullptr, bytes)) == VX_OK);
+                        CHECK(bytes ? launches == 2 || (launches == 3 && T > 16 && K >= 1024) : launches == 1);
+                    }
                 }
     for (const auto& e : names)
         if (!e.first.compare(0, 5, "vx_i8") && !launched.count(e.second)) std::printf("%s is never launched\n", e.first.c_str()), ++failures;

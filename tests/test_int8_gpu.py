@@ -347,7 +347,8 @@ def test_tokens_past_32_bits(i8):
 
 @pytest.mark.parametrize("gated", [False, True])
 @pytest.mark.parametrize("T,N,K", [(17, 200, 1030), (100, 4096, 11008), (33, 65, 5000), (128, 1000, 4096), (129, 129, 2049), (300, 500, 8191),
-                                   (1000, 130, 16385), (64, 3, 131071), (70, 4097, 1100), (1024, 256, 2048), (20, 31, 1024)])
+                                   (1000, 130, 16385), (64, 3, 131071), (70, 4097, 1100), (1024, 256, 2048), (20, 31, 1024), (2000, 200, 4100),
+                                   (5000, 100, 1500)])
 def test_parts_of_long_rows(i8, T, N, K, gated):
     """Sums of parts of K, joined: the bits of the product of vx_i8_quantize's rows, with any contents of the workspace."""
     note(f"parts {T} x {N} x {K} gated {gated}")
@@ -370,5 +371,9 @@ def test_parts_of_long_rows(i8, T, N, K, gated):
         call(out, x, workspace=ws)
         assert torch.equal(out.nan_to_num(3.0), want.nan_to_num(3.0))
     assert (got[:, T] == 7.0).all() and want[T // 2].isnan().all() and not want[0].isnan().any()
+    if T <= 1000:  # (a workspace for more tokens and columns)
+        out = torch.empty(T, N, device=DEV)
+        call(out, x, workspace=i8.workspace(T + 1100, K + 50))
+        assert torch.equal(out.nan_to_num(3.0), want.nan_to_num(3.0))
     if not gated:
         _check(want[:2], _exact(q.data[:2, :K].cpu().numpy(), w.data[:, :K].cpu().numpy(), q.scales[:2].cpu().numpy(), w.scales.cpu().numpy()))

@@ -70,11 +70,12 @@ static bool own_x(uint32_t T, uint32_t K) {
     return T == 1 ? fours <= 16 : T <= VX_I8_OWN_TOKENS && fours * T <= 4;
 }
 
-// x's rows and their scales, and behind them sums of parts of K (plan_gemm): 512 workgroups' tiles of 128 by 128.
+// x's rows and their scales, and behind them sums of parts of K (plan_gemm): 512 workgroups' tiles of 128 by 128. (Never less
+// for more tokens or columns: a workspace is for up to so many.)
 static uint64_t rows_bytes(uint32_t T, uint32_t K) { return own_x(T, K) ? 0 : up(K, 128) * T + up(4ull * T, 16); }
-constexpr uint32_t VX_I8_PARTS_TOKENS = 1024, VX_I8_PARTS_COLS = 1024;
+constexpr uint32_t VX_I8_PARTS_COLS = 1024;
 static uint64_t parts_bytes(uint32_t T, uint32_t K) {
-    return T <= 16 || T > VX_I8_PARTS_TOKENS || K < VX_I8_PARTS_COLS ? 0 : std::min(T, 128u) * (512ull * 128 * 4);
+    return T <= 16 || K < VX_I8_PARTS_COLS ? 0 : std::min(T, 128u) * (512ull * 128 * 4);
 }
 static uint64_t ws_bytes(uint32_t T, uint32_t K) { return rows_bytes(T, K) + parts_bytes(T, K); }
 
