@@ -425,3 +425,40 @@ def test_other_streams(kv):
     torch.cuda.synchronize()
     for c, o in zip(caches[:2], outs):
         assert torch.equal(c.data, caches[2].data) and torch.equal(o, outs[2])
+
+
+def test_calls_through_ctypes_are_the_same(kv, monkeypatch):
+    """What the fast calls do not take goes through ctypes: the same results and refusals."""
+    note("ctypes")
+    g = torch.Generator(device=DEV).manual_seed(9)
+    n, hq, hk, dim = 20, 4, 2, 64
+    q, k, v = (torch.randn(n, h, dim, generator=g, device=DEV) for h in (hq, hk, hk))
+    how = kv.rotation(vx.rotation_freqs(dim), norm=True, q_weight=torch.rand(hq, dim, generator=g, device=DEV))
+    i8, w, x = vx.Int8Gemm(0), torch.randn(30, 100, generator=g, device=DEV), torch.randn(9, 100, generator=g, device=DEV)
+
+    def everything():
+        pages, step = vx.KvPages(8, 16, 2, 4), vx.KvStep(2, n)
+        kv.resize(pages, _i32([13, 6]), step)
+        cache = vx.KvCache(8, 16, hk, dim)
+        cache.data.zero_()
+        qo, ko, qw, out, gated = torch.empty_like(q), torch.empty_like(k), torch.empty_like(q), torch.empty(9, 30, device=DEV), torch.empty(9, 30, device=DEV)
+        kv.rotate(qo, q, ko, k, step.positions, how)
+        kv.write_rotated(cache, qw, q, k, v, step.positions, step.slots, how)
+        rows, xq = vx.Int8Rows.empty(30, 100), vx.Int8Rows.empty(9, 100)
+        rows.data.zero_(), xq.data.zero_()
+        i8.quantize(rows, w), i8.quantize(xq, x)
+        i8.dispatch(out, x, rows, workspace=i8.workspace(9, 100))
+        i8.dispatch_gated(gated, xq, rows, rows, "relu")
+        for call in [lambda: kv.resize(pages, _i32([1]), step), lambda: kv.rotate(qo, q, ko, k[:3], step.positions, how),
+                     lambda: kv.write_rotated(cache, None, None, k, v, step.positions[:3], step.slots, how), lambda: i8.dispatch(out, x, rows),
+                     lambda: i8.quantize(rows, x)]:
+            with pytest.raises(vx.VortxError):
+                call()
+        return [pages.table, pages.lens, pages.free_count, step.starts, step.slots, step.positions, cache.data, qo, ko, qw, rows.data, rows.scales,
+                xq.data, out, gated]
+
+    fast = everything()
+    for name in ("rotate", "kv_write_rotated", "kv_resize", "i8_quantize", "gemm_i8"):
+        monkeypatch.setattr(vx._pycall, name, lambda *a: None)
+    for a, b in zip(fast, everything()):
+        assert torch.equal(a, b)
