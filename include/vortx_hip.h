@@ -659,7 +659,12 @@ int vx_gemm_i8_x(vx_ctx ctx, vx_stream stream, const vx_mview* out, const vx_cvi
 int vx_gemm_i8_ws_size(uint32_t tokens, uint32_t cols, uint64_t* bytes);
 
 /* Activations of vx_gemm_i8_gated: g / (1 + e^-g); g / 2 (1 + tanh(sqrt(2 / pi)
- * (g + 0.044715 g^3))); g / 2 erfc(-g / sqrt(2)); max(g, 0). */
+ * (g + 0.044715 g^3))); g / 2 erfc(-g / sqrt(2)); max(g, 0). Of any gate g: far
+ * above 0 they are g, far below 0 (minus infinity too: a product past f32's range)
+ * 0, of NaN NaN. What is made of g is off, relatively, by 6 2^-24 at most for
+ * the first and 6 (1 + 2 |g + 0.044715 g^3|) 2^-24 for the second; the third is the
+ * device's erfc (16 steps) of an argument that is 2^-23 off. Below f32's normal
+ * numbers it is 2^-149 more, and the third may be 0 from 2^-126 |g| on. */
 typedef enum vx_act { VX_ACT_SILU = 0, VX_ACT_GELU_TANH = 1, VX_ACT_GELU = 2, VX_ACT_RELU = 3 } vx_act;
 
 /* The gated half of a feed-forward block, out = act(x gate^T) * (x up^T), both

@@ -356,9 +356,12 @@ struct vx_i8_stream {
             }
         }
         if (share == 0 && lane < a.T && row < a.N) {
-            float v = vx_i8_value(s[0], x, vx_i8_scaled(sw[0]));
-            if constexpr (GATED) v = vx_act(a.act, v) * vx_i8_value(s[1], x, vx_i8_scaled(sw[1]));
-            a.out[lane * a.os[0] + row * a.os[1]] = v;
+            float v[1] = {vx_i8_value(s[0], x, vx_i8_scaled(sw[0]))};
+            if constexpr (GATED) {
+                vx_act(a.act, v);
+                v[0] *= vx_i8_value(s[1], x, vx_i8_scaled(sw[1]));
+            }
+            a.out[lane * a.os[0] + row * a.os[1]] = v[0];
         }
     }
 
