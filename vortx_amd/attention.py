@@ -118,7 +118,7 @@ class KvPages:
         self.free, self.free_count = torch.arange(pages - 1, -1, -1, **i32), torch.full((1,), pages, **i32)
         self._c = _ffi.VxKvPages(_ptr(self.table), _ptr(self.lens), _ptr(self.free), _ptr(self.free_count), seqs, cols, cols,
                                  page_tokens, pages, 0)
-        self._addr = C.addressof(self._c)
+        self._at = C.addressof(self._c)  # (not a cache's address)
 
 
 class KvStep:
@@ -249,7 +249,7 @@ class KvAttention(_Context):
         tokens of all sequences."""
         if step.seqs != pages.seqs:
             raise VortxError(_ffi.VX_ERR_SHAPE, f"the step is for {step.seqs} sequences, the pages for {pages.seqs}")
-        st = _vx._pycall.kv_resize(_RESIZE, self._ctx, stream, pages._addr, pages.seqs, want, *step._call)
+        st = _vx._pycall.kv_resize(_RESIZE, self._ctx, stream, pages._at, pages.seqs, want, *step._call)
         if st is not None:
             if st:
                 check(st)

@@ -364,31 +364,31 @@ PyObject* py_i8_quantize(PyObject*, PyObject* const* a, Py_ssize_t n) {
     return run([&] { return f(ctx, st, rows, &x); });
 }
 
-// gemm_i8(fn, ctx, stream, out, x, w, up | None, act, workspace | None): fn a vx_gemm_i8 or vx_gemm_i8_gated with x the
-// address of a vx_i8_rows, or their _x forms with x a tensor; w and up addresses
+// gemm_i8(fn, ctx, stream, out, rows | None, x, w, up | None, act, workspace | None): fn a vx_gemm_i8 or vx_gemm_i8_gated
+// of rows, the address of a vx_i8_rows, or without them their _x forms of x, a tensor (whatever x is otherwise); w and up addresses
 PyObject* py_gemm_i8(PyObject*, PyObject* const* a, Py_ssize_t n) {
-    if (n != 9) return other_path();
+    if (n != 10) return other_path();
     void* fn = addr(a[0]);
     vx_ctx ctx = (vx_ctx)addr(a[1]);
-    const vx_i8_rows *w = (const vx_i8_rows*)addr(a[5]), *u = nullptr;
-    const bool rows = PyLong_CheckExact(a[4]), gated = a[6] != Py_None;
-    if (gated && !(u = (const vx_i8_rows*)addr(a[6]))) return other_path();
+    const vx_i8_rows *w = (const vx_i8_rows*)addr(a[6]), *u = nullptr;
+    const bool rows = a[4] != Py_None, gated = a[7] != Py_None;
+    if (gated && !(u = (const vx_i8_rows*)addr(a[7]))) return other_path();
     vx_stream st;
     vx_mview o;
     vx_cview x;
     uint64_t act = 0, wp = 0, wn = 0;
     const vx_i8_rows* xq = rows ? (const vx_i8_rows*)addr(a[4]) : nullptr;
-    if (!fn || !w || (rows && !xq) || PyErr_Occurred() || !view_of(a[3], false, &o) || (!rows && !view_of(a[4], false, &x)) ||
-        !as_u64(a[7], UINT32_MAX, &act) || !stream_of(a[2], &st))
+    if (!fn || !w || (rows && !xq) || PyErr_Occurred() || !view_of(a[3], false, &o) || (!rows && !view_of(a[5], false, &x)) ||
+        !as_u64(a[8], UINT32_MAX, &act) || !stream_of(a[2], &st))
         return other_path();
     if (rows)
         return run([&] {
             return gated ? ((decltype(&vx_gemm_i8_gated))fn)(ctx, st, &o, xq, w, u, (uint32_t)act) : ((decltype(&vx_gemm_i8))fn)(ctx, st, &o, xq, w);
         });
-    if (a[8] != Py_None) {
-        if (!is_gpu_tensor(a[8])) return other_path();
-        Ref c(PyObject_CallMethodNoArgs(a[8], s_is_contiguous));
-        if (c.o != Py_True || !call_u64(a[8], s_data_ptr, UINT64_MAX, &wp) || !attr_u64(a[8], s_nbytes, UINT64_MAX, &wn)) return other_path();
+    if (a[9] != Py_None) {
+        if (!is_gpu_tensor(a[9])) return other_path();
+        Ref c(PyObject_CallMethodNoArgs(a[9], s_is_contiguous));
+        if (c.o != Py_True || !call_u64(a[9], s_data_ptr, UINT64_MAX, &wp) || !attr_u64(a[9], s_nbytes, UINT64_MAX, &wn)) return other_path();
     }
     void* ws = (void*)(uintptr_t)wp;
     return run([&] {

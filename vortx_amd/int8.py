@@ -57,7 +57,7 @@ class Int8Rows:
             raise VortxError(_ffi.VX_ERR_INVALID, f"rows of 16 bytes' multiples need {need} bytes, the buffer holds {room}")
         self.data, self.scales, self.rows, self.cols = data, scales, rows, cols
         self._c = _ffi.VxI8Rows(data.data_ptr() or None, scales.data_ptr() or None, stride, rows, cols)
-        self._addr = C.addressof(self._c)
+        self._at = C.addressof(self._c)
 
     @staticmethod
     def empty(rows: int, cols: int, device="cuda:0") -> "Int8Rows":
@@ -71,13 +71,20 @@ class Int8Rows:
         return self.data[:, :self.cols].float() * self.scales[:, None]
 
 
+def _rows(name, v):
+    """Calls take an Int8Rows by its address: nothing else has one that they could read."""
+    if not isinstance(v, Int8Rows):
+        raise TypeError(f"{name} must be Int8Rows")
+
+
 class Int8Gemm(_Context):
     """Products of :class:`Int8Rows`."""
 
     def quantize(self, out: Int8Rows, x, stream=None) -> None:
         """The rows of ``x`` (f32 [rows, cols] view) as integers with a scale
         each, max|x| / 127 (vx_i8_quantize)."""
-        st = _vx._pycall.i8_quantize(_QUANTIZE, self._ctx, stream, out._addr, x)
+        _rows("out", out)
+        st = _vx._pycall.i8_quantize(_QUANTIZE, self._ctx, stream, out._at, x)
         if st is not None:
             if st:
                 check(st)
@@ -113,14 +120,14 @@ class Int8Gemm(_Context):
         "gelu_tanh", "gelu", "relu"; ``x`` as in :meth:`dispatch`."""
         if act not in _ACTS:
             raise VortxError(_ffi.VX_ERR_INVALID, f"act is {act!r}: one of {', '.join(_ACTS)} is expected")
-        if up is None:
-            raise TypeError("up must be Int8Rows")
+        _rows("up", up)
         self._run(out, x, gate, up, _ACTS[act], workspace, stream)
 
     def _run(self, out, x, w, up, act, workspace, stream):
+        _rows("weights", w)
         rows = isinstance(x, Int8Rows)
         fn = (_ROWS if rows else _X) if up is None else (_GATED if rows else _GATED_X)
-        st = _vx._pycall.gemm_i8(fn, self._ctx, stream, out, x._addr if rows else x, w._addr, None if up is None else up._addr, act,
+        st = _vx._pycall.gemm_i8(fn, self._ctx, stream, out, x._at if rows else None, x, w._at, None if up is None else up._at, act,
                                  workspace)
         if st is not None:
             if st:
