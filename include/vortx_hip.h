@@ -637,7 +637,7 @@ typedef struct vx_i8_rows {
  * rint(x * (127 / m)), within -127..127, each operation one f32 rounding (ties
  * to even). Where m < 2^-100 scale and integers are 0. A row with a NaN or an
  * infinity has the scale NaN, which every product with it becomes. Bytes past
- * cols stay as they are. */
+ * cols stay as they are. 2^31 columns and more are refused (VX_ERR_UNSUPPORTED). */
 int vx_i8_quantize(vx_ctx ctx, vx_stream stream, const vx_i8_rows* out, const vx_cview* x);
 
 /* out[t, n] = x.scales[t] * w.scales[n] * sum_k x[t, k] w[n, k]: out is a [T, N]

@@ -228,6 +228,8 @@ int vx_i8_quantize(vx_ctx ctx, vx_stream stream, const vx_i8_rows* out, const vx
     if (s) return s;
     if ((s = vx::matrix_view(x->base, &x->layout, &m, "x", false))) return s;
     if (m.rows != out->rows || m.cols != out->cols) return vx::fail(VX_ERR_SHAPE, "x and out have different shapes");
+    // (the kernels' counters go on to a step past a row's end, in 32 bits)
+    if (m.cols > 0x7FFFFFFFu) return vx::fail(VX_ERR_UNSUPPORTED, "rows of 2^31 columns and more");
     return vx::quantize(ctx, stream, out, m);
 }
 
