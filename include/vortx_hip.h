@@ -478,10 +478,10 @@ typedef struct vx_rotation {
 } vx_rotation;
 
 /* q_out = q and k_out = k, [tokens, heads, dim] f32 views of any strides with
- * dims up to 256, normed and rotated (one launch for up to 2^20 tokens). positions: device array
- * [tokens] (NULL if nothing is rotated). k_out and k may be NULL: queries
- * alone. An output is its input's view itself (in place) or lies apart from
- * all inputs. */
+ * dims up to 256 and fewer than 2^31 heads, normed and rotated (one launch for
+ * up to 2^20 tokens). positions: device array [tokens] (NULL if nothing is
+ * rotated). k_out and k may be NULL: queries alone. An output is its input's view
+ * itself (in place) or lies apart from all inputs. */
 int vx_rotate(vx_ctx ctx, vx_stream stream, const vx_mview* q_out, const vx_cview* q, const vx_mview* k_out,
               const vx_cview* k, const int32_t* positions, const vx_rotation* how);
 

@@ -184,6 +184,8 @@ static int plan_rotation(const vx_mview* const (&outs)[2], const vx_cview* const
         if ((s = rows_view(ins[i]->base, &ins[i]->layout, dim, &r, names[i][0], false))) return s;
         if (!first && r.tokens != a->tokens) return fail(VX_ERR_SHAPE, "q and k have different tokens");
         first = false;
+        // (the kernels' counters go on to two steps past a run of heads, in 32 bits)
+        if (r.heads > 0x7FFFFFFFu) return fail(VX_ERR_UNSUPPORTED, "2^31 heads and more");
         a->tokens = r.tokens;
         p.heads = r.heads;
         p.x = (const float*)r.ptr;
