@@ -655,7 +655,8 @@ int vx_gemm_i8(vx_ctx ctx, vx_stream stream, const vx_mview* out, const vx_i8_ro
 int vx_gemm_i8_x(vx_ctx ctx, vx_stream stream, const vx_mview* out, const vx_cview* x, const vx_i8_rows* w,
                  void* workspace, uint64_t workspace_bytes);
 
-/* Bytes of workspace for up to `tokens` rows of up to `cols` f32 values (0: none). */
+/* Bytes of workspace for up to `tokens` rows of up to `cols` f32 values (0: none; more
+ * columns than a product takes count as 131071). */
 int vx_gemm_i8_ws_size(uint32_t tokens, uint32_t cols, uint64_t* bytes);
 
 /* Activations of vx_gemm_i8_gated: g / (1 + e^-g); g / 2 (1 + tanh(sqrt(2 / pi)

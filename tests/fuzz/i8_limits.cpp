@@ -22,6 +22,19 @@ int main() {
                 const int s = vx_i8_quantize(ctx, nullptr, &out, &x);
                 CHECK(cols > 0x7FFFFFFFu ? s == VX_ERR_UNSUPPORTED && launches == 0 && *vx_last_error_message() : s == VX_OK && launches == (rows ? 1 : 0));
             }
+    // A workspace for so many tokens and columns does for fewer, to the ends of both.
+    const uint32_t ends[] = {1, 4, 17, 128, 131071, 131072, 1u << 20, 0x7FFFFFFFu, 0xFFFFFF7Fu, 0xFFFFFF81u, 0xFFFFFFFFu};
+    for (size_t i = 0; i < 11; ++i)
+        for (size_t j = 0; j < 11; ++j) {
+            uint64_t here = 0, more = 0;
+            CHECK(vx_gemm_i8_ws_size(ends[i], ends[j], &here) == VX_OK);
+            if (i + 1 < 11) {
+                CHECK(vx_gemm_i8_ws_size(ends[i + 1], ends[j], &more) == VX_OK && more >= here);
+            }
+            if (j + 1 < 11) {
+                CHECK(vx_gemm_i8_ws_size(ends[i], ends[j + 1], &more) == VX_OK && more >= here);
+            }
+        }
     CHECK(vx_destroy(ctx) == VX_OK);
     if (!failures) std::printf("fine\n");
     return failures != 0;

@@ -77,7 +77,10 @@ constexpr uint32_t VX_I8_PARTS_COLS = 1024;
 static uint64_t parts_bytes(uint32_t T, uint32_t K) {
     return T <= 16 || K < VX_I8_PARTS_COLS ? 0 : std::min(T, 128u) * (512ull * 128 * 4);
 }
-static uint64_t ws_bytes(uint32_t T, uint32_t K) { return rows_bytes(T, K) + parts_bytes(T, K); }
+static uint64_t ws_bytes(uint32_t T, uint32_t K) {
+    K = std::min(K, VX_I8_MOST_COLS);  // (no product has more; sums of both ends would pass 64 bits)
+    return rows_bytes(T, K) + parts_bytes(T, K);
+}
 
 struct I8Plan {
     int kernel;
