@@ -81,10 +81,9 @@ how = attention.Rotation(0, 0, 0, (), _ffi.VxRotation())
 kv.write(cache, h, h, slots, stream=st); only("_WRITE")
 kv.read(h, h, cache, slots, stream=st); only("_READ")
 kv.write_rotated(cache, h, h, h, h, None, slots, how, stream=st); only("_WRITE_ROTATED")
-zeros = torch.zeros
-for n in ("zeros", "full", "arange"):
-    setattr(torch, n, lambda *a, **k: zeros(1))
-pages = attention.KvPages(4, 16, 2, 2)
+pages = attention.KvPages.__new__(attention.KvPages)
+pages._c = _ffi.VxKvPages(4096, 4096, 4096, 4096, 2, 2, 2, 16, 4, 0)
+pages._at = C.addressof(pages._c)
 for bad in (rows(), pages, how, st):
     for call in (lambda: kv.write(bad, h, h, slots, stream=st), lambda: kv.read(h, h, bad, slots, stream=st),
                  lambda: kv.write_rotated(bad, h, h, h, h, None, slots, how, stream=st)):

@@ -102,6 +102,14 @@ def _row_stride(t) -> int:
     return t.stride(0) if t.shape[0] > 1 else t.shape[1]
 
 
+def _i32_on(device):
+    """What torch makes int32 numbers with that kernels can reach."""
+    import torch
+    if torch.device(device).type != "cuda":
+        raise TypeError(f"device is {device}: the GPU is expected")
+    return dict(dtype=torch.int32, device=device)
+
+
 class KvPages:
     """Which of ``pages`` pages of ``page_tokens`` tokens ``seqs`` sequences
     hold, at most ``cols`` each (vx_kv_pages): int32 GPU tensors ``table``
@@ -112,7 +120,7 @@ class KvPages:
     def __init__(self, pages: int, page_tokens: int, seqs: int, cols: int, device="cuda:0"):
         import torch
         _u32(pages=pages, page_tokens=page_tokens, seqs=seqs, cols=cols)
-        i32 = dict(dtype=torch.int32, device=device)
+        i32 = _i32_on(device)
         self.pages, self.page_tokens, self.seqs, self.cols = pages, page_tokens, seqs, cols
         self.table, self.lens = torch.zeros(seqs, cols, **i32), torch.zeros(seqs, **i32)
         self.free, self.free_count = torch.arange(pages - 1, -1, -1, **i32), torch.full((1,), pages, **i32)
@@ -129,7 +137,7 @@ class KvStep:
     def __init__(self, seqs: int, tokens: int, device="cuda:0"):
         import torch
         _u32(seqs=seqs, tokens=tokens)
-        i32 = dict(dtype=torch.int32, device=device)
+        i32 = _i32_on(device)
         self.seqs, self.tokens = seqs, tokens
         self.starts = torch.zeros(seqs + 1, **i32)
         self.slots, self.positions = torch.full((tokens,), -1, **i32), torch.zeros(tokens, **i32)
