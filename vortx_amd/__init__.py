@@ -188,6 +188,17 @@ def _stream(stream) -> int:
     return stream.cuda_stream if hasattr(stream, "cuda_stream") else int(stream)
 
 
+class _ByAddress:
+    """An object that calls take by the addresses in it: its tensors' contents
+    change, but none of its fields is set twice, as another tensor in its place
+    would leave calls with the address of freed memory."""
+
+    def __setattr__(self, name, value):
+        if name in self.__dict__:
+            raise AttributeError(f"{type(self).__name__}.{name} is fixed, calls have its address: copy into it, or make a new {type(self).__name__}")
+        object.__setattr__(self, name, value)
+
+
 # ------------------------------------------------------------------ gemm
 class _Context:
     def __init__(self, device: int = 0):

@@ -34,7 +34,7 @@ from dataclasses import dataclass
 
 import vortx_amd as _vx
 
-from . import _ADDR, _Context, _ffi, _stream, _view_of
+from . import _ADDR, _ByAddress, _Context, _ffi, _stream, _view_of
 from ._ffi import VX_Q8_0, VortxError, check, lib
 
 _WRITE, _READ, _ATTEND, _TREE = (_ADDR[n] for n in ("vx_kv_write", "vx_kv_read", "vx_attention", "vx_attention_tree"))
@@ -110,7 +110,7 @@ def _i32_on(device):
     return dict(dtype=torch.int32, device=device)
 
 
-class KvPages:
+class KvPages(_ByAddress):
     """Which of ``pages`` pages of ``page_tokens`` tokens ``seqs`` sequences
     hold, at most ``cols`` each (vx_kv_pages): int32 GPU tensors ``table``
     [seqs, cols], ``lens`` [seqs], and the stack of free pages, the first
@@ -129,7 +129,7 @@ class KvPages:
         self._at = C.addressof(self._c)  # (not a cache's address)
 
 
-class KvStep:
+class KvStep(_ByAddress):
     """What :meth:`KvAttention.resize` says of a step's new tokens, up to
     ``tokens`` of them: int32 GPU tensors ``starts`` [seqs + 1] (of a batch),
     ``slots`` and ``positions`` [tokens]."""
@@ -152,7 +152,7 @@ def rotation_freqs(rotated: int, base: float = 10000.0, scale: float = 1.0, devi
 
 
 @dataclass
-class Rotation:
+class Rotation(_ByAddress):
     """How queries and keys are normed and rotated (:meth:`KvAttention.rotation`).
     It keeps the tensors it was made of alive; their contents may change."""
     dim: int       # of the heads that it is for (0: any that its rotated dims fit into)

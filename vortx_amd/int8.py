@@ -20,7 +20,7 @@ import ctypes as C
 
 import vortx_amd as _vx
 
-from . import _ADDR, _Context, _ffi, _stream, _view_of
+from . import _ADDR, _ByAddress, _Context, _ffi, _stream, _view_of
 from ._ffi import VortxError, check, lib
 
 _QUANTIZE, _ROWS, _X, _GATED, _GATED_X = (_ADDR[n] for n in ("vx_i8_quantize", "vx_gemm_i8", "vx_gemm_i8_x", "vx_gemm_i8_gated",
@@ -28,7 +28,7 @@ _QUANTIZE, _ROWS, _X, _GATED, _GATED_X = (_ADDR[n] for n in ("vx_i8_quantize", "
 _ACTS = {"silu": 0, "gelu_tanh": 1, "gelu": 2, "relu": 3}
 
 
-class Int8Rows:
+class Int8Rows(_ByAddress):
     """``rows`` x ``cols`` integers, ``data`` (int8 GPU tensor [rows, at least
     cols], neighbours in a row next to each other, rows a multiple of 16 bytes
     apart and 16-byte aligned), with ``scales`` (f32 [rows]) for the values
