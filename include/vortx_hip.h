@@ -642,9 +642,10 @@ int vx_i8_quantize(vx_ctx ctx, vx_stream stream, const vx_i8_rows* out, const vx
 
 /* out[t, n] = x.scales[t] * w.scales[n] * sum_k x[t, k] w[n, k]: out is a [T, N]
  * f32 view of any strides, x [T, K] and w [N, K]. The sum is exact (int32; K up
- * to 131071, else VX_ERR_UNSUPPORTED, as K = 0 is), what is made of it is within
- * 1.5 of f32's steps, and the same bits whatever T and whatever x's form. out lies apart from the
- * inputs. */
+ * to 131071, else VX_ERR_UNSUPPORTED, as K = 0 is), what is made of it is off by 3
+ * 2^-24 at most, relatively (2.5 of f32's steps; 1.5 where the sum is below 2^24;
+ * 2^-150 more below f32's normal numbers), and the same bits whatever T and whatever
+ * x's form. out lies apart from the inputs. */
 int vx_gemm_i8(vx_ctx ctx, vx_stream stream, const vx_mview* out, const vx_i8_rows* x, const vx_i8_rows* w);
 
 /* The same of x as an f32 [T, K] view, whose rows become integers as

@@ -38,8 +38,10 @@ __device__ __forceinline__ uint32_t vx_max4(uint32_t m, f4v x) {
     return max(max(m, max(vx_abs_bits(x.x), vx_abs_bits(x.y))), max(vx_abs_bits(x.z), vx_abs_bits(x.w)));
 }
 
-// sum * sx * sw with three roundings of half a step each, for scales of any size:
-// mantissas are multiplied, the powers of two added and put on at the end.
+// sum * sx * sw for scales of any size: mantissas are multiplied, the powers of two
+// added and put on at the end. Three roundings, of the sum (if 2^24 or more), of the
+// mantissas' product and of the result, 2^-24 each, relatively: the first two may be
+// a step of the result each, 2.5 in all (1.95 measured, 1.4 with sums below 2^24).
 struct vx_i8_scaled {
     float m;
     int e;
