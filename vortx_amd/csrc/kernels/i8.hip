@@ -90,7 +90,7 @@ __device__ __forceinline__ void vx_lds_barrier() { asm volatile("s_waitcnt lgkmc
 // TT x 16 tokens by NT x 16 channels (of each matrix) a workgroup of eight waves,
 // which have K's pieces of 64 U bytes in turn, straight from memory to the matrix
 // cores; their sums meet in LDS at the end. Bound by what a CU takes from L2 and
-// memory, about 37 GB/s: 11008 x 4096 by 16 tokens 15.0 us, 64 22.5, 128 28.6; 32
+// memory, about 37 GB/s: 11008 x 4096 by 16 tokens 16.1 us, 64 22.3, 128 28.7; 32
 // tokens gated 26.2.
 template <int TT, int NT, int U, bool GATED>
 struct vx_i8_direct {
@@ -217,8 +217,8 @@ VX_I8_DIRECT(vx_i8_direct_t4_wide_gated, 4, 2, 1, true)
 // each workgroup for itself, under its first loads, which saves the launch that would
 // do it. Bound by HBM, the weights' bytes, and what a launch takes to begin; a step is
 // kept short, because with 100 instructions more a kilobyte their issue was the bound.
-// One token by 32000 x 4096 26.1 us, 5.0 TB/s; by 11008 x 4096 11.5 (gated 18.1; a row a
-// wave and step of 8 KB, loads under conditions: 13.4 and 24); two tokens 12.5, four 15.2.
+// One token by 32000 x 4096 25.6 us, 5.1 TB/s; by 11008 x 4096 11.5 (gated 18.2; a row a
+// wave and step of 8 KB, loads under conditions: 13.4 and 24); two tokens 12.6, four 15.9.
 template <int TT, bool GATED, int DEPTH>
 struct vx_i8_stream {
     static constexpr int G = GATED ? 2 : 1;
@@ -461,10 +461,15 @@ VX_I8_STREAM(vx_i8_stream_t4_gated, 4, true, 1)
 // brought from memory straight into LDS, and five units go round: two are multiplied
 // while three are on their way. The 16-byte pieces of a row are stored in an order that
 // goes by the row, so that the lanes of a fragment (16 rows, one piece each) meet all
-// banks. 4096 x 4096 x 11008 (tokens, channels, k) 163 us, 2270 TOP/s; 4096 x 11008 x
-// 4096 206 us, 1790 (gated 423, 1750): bound by the matrix cores and the loads, which
-// each take 1.4 of a stage's 1.7 us, and by the stores, which all CUs make at the same
-// time, 16 us a tile of each CU.
+// banks. 4096 x 4096 x 11008 (tokens, channels, k) 158 us, 2330 TOP/s; 4096 x 11008 x
+// 4096 205 us, 1800 (gated 414, 1785). A stage takes 1.7 us: the loads from memory take
+// 1.4 of it by themselves (46 GB/s a CU), all else 1.3, of which the matrix instructions
+// are 2048 cycles, 0.9 to 1.0, so that neither is the bound alone: it is how much of the
+// one lies under the other. Counted over the last product, the matrix cores are busy 37 %
+// of the cycles (45 % of those in which their CU has work: 688 tiles are 2.7 rounds), LDS
+// with reads 14 %, without a bank conflict; a wave waits for data or the others 38 % of its time,
+// and to issue 39 %. Beside the stages the stores, which all CUs make at the same time, 16 us
+// a tile of each CU.
 template <int MT, int MN, int WT, int WN, bool GATED, bool PART = false>
 struct vx_i8_tile {
     static_assert(MT == MN, "units of one size");

@@ -150,10 +150,12 @@ struct vx_held {
 
 // The whole step in one workgroup of a.threads, as many sequences at a time. It is
 // bound by a chain: lengths, their sums, stack or table, what follows from it (32
-// sequences, a token each, 4.1 us traced; 200 with 320000 new tokens 12.3, and 4.8 for
-// the slots after it). What sequences give back has to be on the stack before any
-// takes from it. A thread moves the pages and tokens of its own sequence where all
-// have few, otherwise all threads share them out.
+// sequences, a token each, 4.2 us traced; 200 with 320000 new tokens 12.1, and 5.0 for
+// the slots after it). It puts what sequences give back on the stack before any takes
+// from it. (Sums alone would do: page i that is taken is page i that is given back, as
+// long as there are such, and then comes the stack as it was. Many workgroups could
+// share out a long step so.) A thread moves the pages and tokens of its own sequence
+// where all have few, otherwise all threads share them out.
 constexpr uint32_t VX_OWN_PAGES = 4, VX_OWN_TOKENS = 8;
 extern "C" __global__ __launch_bounds__(1024) void vx_pages_resize(vx_pages_args a) {
     __shared__ uint32_t part[4][16];

@@ -63,8 +63,9 @@ static uint64_t up(uint64_t n, uint64_t to) { return (n + to - 1) / to * to; }
 
 // x that a product quantizes itself (one launch, each workgroup for itself): one token of up to 65536 values, or up to
 // four whose values stay in the workgroup's registers, 16 a thread (4096 values and up to four tokens, 8192 and two). By
-// itself / by a launch before it, 11008 x 4096, us: four tokens 16.8 / 17.2, five as four would be 17.3; 4096 x 11008,
-// four tokens 21.2 / 19.
+// itself / by a launch before it, in a graph, us: 11008 x 4096, two tokens 12.6 / 14.5, four 15.9 / 14.8 (gated 19.6 / 22.4
+// and 22.4 / 22.7); 4096 x 4096, two 7.9 / 8.6, three 9.2 / 8.5, four 9.9 / 8.7; 4096 x 11008, four 21.7 / 16.5. Three and
+// four stay with it although one launch more takes them 1 us less: they need no workspace.
 static bool own_x(uint32_t T, uint32_t K) {
     const uint64_t fours = (K + 4095ull) / 4096;
     return T == 1 ? fours <= 16 : T <= VX_I8_OWN_TOKENS && fours * T <= 4;

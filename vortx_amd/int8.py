@@ -112,7 +112,8 @@ class Int8Gemm(_Context):
     def dispatch(self, out, x, w: Int8Rows, workspace=None, stream=None) -> None:
         """``out`` [T, N] = ``x`` [T, K] times the transpose of ``w`` [N, K].
         ``x``: :class:`Int8Rows`, or an f32 view, whose rows are quantized first
-        (for one to four tokens within the product, else into ``workspace``)."""
+        (for one to four tokens within the product, else into ``workspace``,
+        which is for f32 views alone: rows that are integers need none)."""
         self._run(out, x, w, None, 0, workspace, stream)
 
     def dispatch_gated(self, out, x, gate: Int8Rows, up: Int8Rows, act: str = "silu", workspace=None, stream=None) -> None:
